@@ -12,11 +12,11 @@ import ctypes
 from . import _lib
 from ._lib import (SUCCESS, COMPILATION_FAILED, NO_DATA_PTR_PROVIDED, CALLED_BEFORE_COMPILATION,
                    INVALID_ID, INVALID_BACKEND, INVALID_CPX_DIM, INVALID_DTYPE, INVALID_KTYPE, UNDEFINED_ERROR,
-                   FP32, FP64, BF16, UNDEFINED_DTYPE,
-                   ZERO, RELU, ADD, COPY, MADD, UNDEFINED_KTYPE, CPX_ZERO, CPX_MADD,
+                   FP32, FP64, BF16, INT8, UNDEFINED_DTYPE,
+                   ZERO, RELU, ADD, COPY, MADD, UNDEFINED_KTYPE, CPX_ZERO, CPX_MADD, SILU,
                    DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J,
                    DTYPE_BYTES, EinsumIrError, hip_lib, check)
-from .loops import binary_loops, unary_dims, dim_types, row_major_strides  # noqa: F401
+from .loops import binary_loops, contraction_i8_loops, unary_dims, dim_types, row_major_strides  # noqa: F401
 
 
 def _ptr(x):
@@ -104,6 +104,62 @@ class PermutePlan(_Plan):
     def execute(self, inp, out, stream=None):
         check(hip_lib().etir_hip_permute_execute(self._handle, _ptr(inp), _ptr(out),
                                                  _stream_ptr(stream)))
+
+
+class ContractionI8Plan(_Plan):
+    """Product of 8-bit integers with scales (etir_hip_contraction_i8_create):
+
+        out = last(scale_left * scale_right * sum_k left * right + bias)
+
+    contraction_i8_loops gives the arguments for an einsum string.  A scale or
+    bias without strides is not read."""
+
+    def __init__(self, dim_types, sizes, strides_left, strides_right, strides_out, strides_scale_left=None,
+                 strides_scale_right=None, strides_bias=None, dtype_out=FP32, ktype_last_touch=UNDEFINED_KTYPE):
+        super().__init__()
+        opt = lambda s: None if s is None else _lib.i64_array(s)  # noqa: E731
+        check(hip_lib().etir_hip_contraction_i8_create(
+            len(sizes), _lib.i32_array(dim_types), _lib.i64_array(sizes), _lib.i64_array(strides_left),
+            _lib.i64_array(strides_right), opt(strides_scale_left), opt(strides_scale_right), opt(strides_bias),
+            _lib.i64_array(strides_out), dtype_out, ktype_last_touch, ctypes.byref(self._handle)))
+
+    def execute(self, left, right, out, scale_left=None, scale_right=None, bias=None, stream=None):
+        check(hip_lib().etir_hip_contraction_i8_execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left),
+                                                        _ptr(scale_right), _ptr(bias), _ptr(out),
+                                                        _stream_ptr(stream)))
+
+
+class NormQuantPlan(_Plan):
+    """RMS norm with the residual's addition, rows rounded to 8 bits
+    (etir_hip_norm_quant_create).  ld_*: elements from row to row, cols unless
+    given; dtype_weight: dtype unless given."""
+
+    def __init__(self, rows, cols, dtype=BF16, dtype_weight=None, eps=1e-6, ld_in=None, ld_residual=None,
+                 ld_total=None, ld_q=None, ld_values=None):
+        super().__init__()
+        ld = [cols if v is None else v for v in (ld_in, ld_residual, ld_total, ld_q, ld_values)]
+        check(hip_lib().etir_hip_norm_quant_create(rows, cols, *ld, dtype, dtype if dtype_weight is None else dtype_weight,
+                                                   eps, ctypes.byref(self._handle)))
+
+    def execute(self, x, q, scale, residual=None, weight=None, total=None, values=None, stream=None):
+        check(hip_lib().etir_hip_norm_quant_execute(self._handle, _ptr(x), _ptr(residual), _ptr(weight), _ptr(total),
+                                                    _ptr(q), _ptr(scale), _ptr(values), _stream_ptr(stream)))
+
+
+class ActQuantPlan(_Plan):
+    """Activation f(x) or f(gate) * x, rows rounded to 8 bits
+    (etir_hip_act_quant_create).  ktype: UNDEFINED_KTYPE (none), RELU or SILU;
+    ld_*: elements from row to row, cols unless given."""
+
+    def __init__(self, rows, cols, dtype=BF16, ktype=UNDEFINED_KTYPE, ld_in=None, ld_gate=None, ld_q=None,
+                 ld_values=None):
+        super().__init__()
+        ld = [cols if v is None else v for v in (ld_in, ld_gate, ld_q, ld_values)]
+        check(hip_lib().etir_hip_act_quant_create(rows, cols, *ld, dtype, ktype, ctypes.byref(self._handle)))
+
+    def execute(self, x, q, scale, gate=None, values=None, stream=None):
+        check(hip_lib().etir_hip_act_quant_execute(self._handle, _ptr(x), _ptr(gate), _ptr(q), _ptr(scale),
+                                                   _ptr(values), _stream_ptr(stream)))
 
 
 def synchronize(stream=None):

@@ -23,9 +23,10 @@ INVALID_DTYPE = 9
 INVALID_KTYPE = 10
 UNDEFINED_ERROR = 99
 
-FP32, FP64, BF16, UNDEFINED_DTYPE = 0, 1, 2, 99
+FP32, FP64, BF16, INT8, UNDEFINED_DTYPE = 0, 1, 2, 3, 99
 ZERO, RELU, ADD, COPY, MADD, UNDEFINED_KTYPE = 0, 1, 2, 3, 4, 99
 CPX_ZERO, CPX_MADD = 6, 8
+SILU = 20
 DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J = 0, 1, 2, 3, 4, 5, 6
 
 DTYPE_BYTES = {FP32: 4, FP64: 8, BF16: 2}
@@ -45,6 +46,15 @@ _HIP_SIGS = {
                                                ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.POINTER(_vp)]),
     "etir_hip_permute_execute": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
+    "etir_hip_contraction_i8_create": (ctypes.c_int, [ctypes.c_int64, _i32p, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p,
+                                                      _i64p, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(_vp)]),
+    "etir_hip_contraction_i8_execute": (ctypes.c_int, [_vp] * 8),
+    "etir_hip_norm_quant_create": (ctypes.c_int, [ctypes.c_int64] * 7 + [ctypes.c_int32, ctypes.c_int32, ctypes.c_float,
+                                                                        ctypes.POINTER(_vp)]),
+    "etir_hip_norm_quant_execute": (ctypes.c_int, [_vp] * 9),
+    "etir_hip_act_quant_create": (ctypes.c_int, [ctypes.c_int64] * 6 + [ctypes.c_int32, ctypes.c_int32,
+                                                                       ctypes.POINTER(_vp)]),
+    "etir_hip_act_quant_execute": (ctypes.c_int, [_vp] * 7),
     "etir_hip_plan_destroy": (ctypes.c_int, [_vp]),
     "etir_hip_plan_describe": (ctypes.c_int, [_vp, ctypes.c_char_p, ctypes.c_int64]),
     "etir_hip_plan_flops": (ctypes.c_int64, [_vp]),

@@ -1,7 +1,7 @@
 // extern "C" entry points of libeinsum_ir_hip.so (declared in
 // include/einsum_ir_hip.h).  Thin: argument checks, plan ownership, error
 // strings; planning and kernels live in contract_plan.cpp / permute.hip.
-#include "etir_internal.h"
+#include "i8_internal.h"
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -144,6 +144,12 @@ int etir_hip_plan_describe( etir_plan_t plan, char * buf, int64_t len ) {
   if( plan->kind == 1 ) {
     l_s = plan->cont.desc;
   }
+  else if( plan->kind == 3 ) {
+    l_s = plan->i8->desc;
+  }
+  else if( plan->kind > 3 ) {
+    l_s = plan->quant->desc;
+  }
   else {
     static char const * l_modes[] = { "fill", "transpose", "copy_vec", "gather", "tiled", "reg4", "rows", "pair" };
     etir::PermutePlan const & p = plan->perm;
@@ -183,6 +189,7 @@ int etir_hip_plan_describe( etir_plan_t plan, char * buf, int64_t len ) {
 }
 
 int64_t etir_hip_plan_flops( etir_plan_t plan ) {
+  if( plan != nullptr && plan->kind == 3 ) return plan->i8->flops;
   if( plan == nullptr || plan->kind != 1 ) return 0;
   return plan->cont.flops;
 }
@@ -190,6 +197,8 @@ int64_t etir_hip_plan_flops( etir_plan_t plan ) {
 int64_t etir_hip_plan_bytes( etir_plan_t plan ) {
   if( plan == nullptr ) return 0;
   if( plan->kind == 1 ) return plan->cont.bytes;
+  if( plan->kind == 3 ) return plan->i8->bytes;
+  if( plan->kind > 3 ) return plan->quant->bytes;
   etir::PermutePlan const & p = plan->perm;
   int64_t l_rw = ( p.ktype == ETIR_KTYPE_ZERO ) ? 1 : ( p.ktype == ETIR_KTYPE_ADD ? 3 : 2 );
   return l_rw * p.elem_bytes * p.num_elements;

@@ -469,13 +469,18 @@ int  launch_contraction( ContractionPlan const & plan,
                          hipStream_t             stream,
                          bool                    ordered );
 
+struct I8Plan;
+struct QuantPlan;
+
 }  // namespace etir
 
 struct etir_plan_s {
-  int32_t kind = 0;              // 1 contraction, 2 permutation
+  int32_t kind = 0;              // 1 contraction, 2 permutation, 3 8-bit contraction, 4 norm_quant, 5 act_quant
   int32_t device = 0;
   etir::ContractionPlan cont;
   etir::PermutePlan     perm;
+  std::shared_ptr< etir::I8Plan >    i8;
+  std::shared_ptr< etir::QuantPlan > quant;
 };
 
 #endif

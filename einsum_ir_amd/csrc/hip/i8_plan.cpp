@@ -1,0 +1,431 @@
+// Planner and C entry points of the 8-bit layer operators
+// (etir_hip_contraction_i8_*, etir_hip_norm_quant_*, etir_hip_act_quant_*,
+// include/einsum_ir_hip.h).
+//
+// A product's loops are sorted by type and fused where they are contiguous in
+// every tensor, as the contraction planner does (contract_plan.cpp); the
+// general kernel takes what is left as it is.
+#include "i8_internal.h"
+#include <algorithm>
+#include <limits>
+#include <vector>
+
+namespace etir {
+
+namespace {
+
+// largest K: 128 * 128 * K stays below 2^31
+constexpr int64_t kI8MaxK = 131071;
+
+struct Loop {
+  int64_t size;
+  int64_t s[I8_TENSORS];
+};
+
+bool contiguous( Loop const & outer, Loop const & inner ) {
+  for( int l_t = 0; l_t < I8_TENSORS; l_t++ ) {
+    if( outer.s[l_t] != inner.s[l_t] * inner.size ) return false;
+  }
+  return true;
+}
+
+// sorts by the stride in `slot` (outermost first) and fuses
+void order_and_fuse( std::vector< Loop > & loops, int slot ) {
+  std::stable_sort( loops.begin(), loops.end(),
+                    [slot]( Loop const & x, Loop const & y ) { return x.s[slot] > y.s[slot]; } );
+  std::vector< Loop > l_out;
+  for( Loop const & l_l : loops ) {
+    if( !l_out.empty() && contiguous( l_out.back(), l_l ) ) {
+      Loop l_f = l_l;
+      l_f.size *= l_out.back().size;
+      l_out.back() = l_f;
+    }
+    else l_out.push_back( l_l );
+  }
+  loops = l_out;
+}
+
+int to_loops( std::vector< Loop > const & loops, I8Loops & out ) {
+  if( loops.size() > std::size_t( kI8MaxLoops ) ) {
+    return fail( ETIR_COMPILATION_FAILED, "contraction_i8: too many loops of one type that cannot be fused" );
+  }
+  out.n = int32_t( loops.size() );
+  for( int l_i = 0; l_i < out.n; l_i++ ) {
+    out.size[l_i] = int32_t( loops[l_i].size );
+    std::copy_n( loops[l_i].s, int( I8_TENSORS ), out.stride[l_i] );
+  }
+  return ETIR_SUCCESS;
+}
+
+int64_t smallest( std::vector< Loop > const & loops, int slot ) {
+  int64_t l_s = std::numeric_limits< int64_t >::max();
+  for( Loop const & l_l : loops ) l_s = std::min( l_s, l_l.s[slot] );
+  return l_s;
+}
+
+std::string sizes_of( I8Loops const & l ) {
+  std::string l_s = "[";
+  for( int l_i = 0; l_i < l.n; l_i++ ) l_s += ( l_i ? "," : "" ) + std::to_string( l.size[l_i] );
+  return l_s + "]";
+}
+
+}  // namespace
+
+int plan_i8( int64_t         num_loops,
+             int32_t const * dim_types,
+             int64_t const * sizes,
+             int64_t const * strides_left,
+             int64_t const * strides_right,
+             int64_t const * strides_scale_left,
+             int64_t const * strides_scale_right,
+             int64_t const * strides_bias,
+             int64_t const * strides_out,
+             int32_t         dtype_out,
+             int32_t         ktype_last_touch,
+             I8Plan        & plan ) {
+  if( num_loops < 0 || ( num_loops > 0 && ( dim_types == nullptr || sizes == nullptr || strides_left == nullptr
+                                            || strides_right == nullptr || strides_out == nullptr ) ) ) {
+    return fail( ETIR_COMPILATION_FAILED, "contraction_i8: invalid loop arrays" );
+  }
+  if( dtype_out != ETIR_FP32 && dtype_out != ETIR_BF16 ) {
+    return fail( ETIR_INVALID_DTYPE, "contraction_i8: the output is FP32 or BF16" );
+  }
+  if( ktype_last_touch != ETIR_KTYPE_UNDEFINED && ktype_last_touch != ETIR_KTYPE_RELU ) {
+    return fail( ETIR_INVALID_KTYPE, "contraction_i8: the last touch is RELU or UNDEFINED" );
+  }
+
+  std::vector< Loop > l_loops[4];              // by ETIR_DIM_C/M/N/K
+  int64_t l_total[4] = { 1, 1, 1, 1 };
+  int64_t const l_limit[4] = { std::numeric_limits< int32_t >::max(), std::numeric_limits< int32_t >::max(),
+                               std::numeric_limits< int32_t >::max(), kI8MaxK };
+  for( int64_t l_i = 0; l_i < num_loops; l_i++ ) {
+    int32_t const l_ty = dim_types[l_i];
+    if( l_ty == ETIR_DIM_I || l_ty == ETIR_DIM_J ) continue;
+    if( l_ty < ETIR_DIM_C || l_ty > ETIR_DIM_K ) {
+      return fail( ETIR_COMPILATION_FAILED, "contraction_i8: unsupported dimension type" );
+    }
+    int64_t const l_sz = sizes[l_i];
+    if( l_sz < 0 ) return fail( ETIR_COMPILATION_FAILED, "contraction_i8: negative loop size" );
+    if( l_sz != 0 && l_total[l_ty] > l_limit[l_ty] / l_sz ) {
+      return fail( ETIR_COMPILATION_FAILED, l_ty == ETIR_DIM_K
+                   ? "contraction_i8: K over 131071 could exceed a 32-bit sum"
+                   : "contraction_i8: more than 2^31 - 1 indices of one type" );
+    }
+    l_total[l_ty] *= l_sz;
+    if( l_sz < 2 ) continue;
+    Loop l_l{};
+    l_l.size = l_sz;
+    l_l.s[I8_A] = strides_left[l_i];
+    l_l.s[I8_B] = strides_right[l_i];
+    l_l.s[I8_OUT] = strides_out[l_i];
+    if( strides_scale_left != nullptr ) l_l.s[I8_SA] = strides_scale_left[l_i];
+    if( strides_scale_right != nullptr ) l_l.s[I8_SB] = strides_scale_right[l_i];
+    if( strides_bias != nullptr ) l_l.s[I8_BIAS] = strides_bias[l_i];
+    for( int64_t l_s : l_l.s ) {
+      if( l_s < 0 ) return fail( ETIR_COMPILATION_FAILED, "contraction_i8: negative stride" );
+    }
+    bool const l_left = l_ty == ETIR_DIM_C || l_ty == ETIR_DIM_M;
+    bool const l_right = l_ty == ETIR_DIM_C || l_ty == ETIR_DIM_N;
+    if( ( !l_left && l_l.s[I8_SA] != 0 ) || ( !l_right && ( l_l.s[I8_SB] != 0 || l_l.s[I8_BIAS] != 0 ) ) ) {
+      return fail( ETIR_COMPILATION_FAILED,
+                   "contraction_i8: scale_left runs over C and M loops, scale_right and bias over C and N loops" );
+    }
+    // strides of a tensor along a loop that it does not have are not read
+    if( l_ty == ETIR_DIM_M ) l_l.s[I8_B] = 0;
+    if( l_ty == ETIR_DIM_N ) l_l.s[I8_A] = 0;
+    if( l_ty == ETIR_DIM_K ) l_l.s[I8_OUT] = 0;
+    else if( l_l.s[I8_OUT] == 0 ) {
+      return fail( ETIR_COMPILATION_FAILED, "contraction_i8: output elements have to lie apart" );
+    }
+    l_loops[l_ty].push_back( l_l );
+  }
+
+  // the columns are the side with the output's smaller stride
+  plan.swapped = smallest( l_loops[ETIR_DIM_M], I8_OUT ) < smallest( l_loops[ETIR_DIM_N], I8_OUT );
+  if( plan.swapped ) {
+    std::swap( l_loops[ETIR_DIM_M], l_loops[ETIR_DIM_N] );
+    std::swap( l_total[ETIR_DIM_M], l_total[ETIR_DIM_N] );
+    for( auto & l_ty : l_loops ) for( Loop & l_l : l_ty ) {
+      std::swap( l_l.s[I8_A], l_l.s[I8_B] );
+      std::swap( l_l.s[I8_SA], l_l.s[I8_SB] );
+    }
+  }
+  plan.has_sa = strides_scale_left != nullptr;
+  plan.has_sb = strides_scale_right != nullptr;
+  if( plan.swapped ) std::swap( plan.has_sa, plan.has_sb );
+  plan.has_bias = strides_bias != nullptr;
+
+  I8GeneralArgs & a = plan.args;
+  I8Loops * const l_to[4] = { &a.c, &a.m, &a.n, &a.k };
+  for( int l_ty = 0; l_ty < 4; l_ty++ ) {
+    order_and_fuse( l_loops[l_ty], l_ty == ETIR_DIM_K ? int( I8_A ) : int( I8_OUT ) );
+    int const l_err = to_loops( l_loops[l_ty], *l_to[l_ty] );
+    if( l_err != ETIR_SUCCESS ) return l_err;
+  }
+  a.C = l_total[ETIR_DIM_C];
+  a.M = l_total[ETIR_DIM_M];
+  a.N = l_total[ETIR_DIM_N];
+  a.K = l_total[ETIR_DIM_K];
+  a.out_bf16 = dtype_out == ETIR_BF16;
+  a.relu = ktype_last_touch == ETIR_KTYPE_RELU;
+  a.bias_rows = plan.swapped;
+  a.tiles_m = int32_t( ( a.M + 63 ) / 64 );
+  a.tiles_n = int32_t( ( a.N + 63 ) / 64 );
+  // a grid's threads are counted in 32 bits
+  double const l_grid = double( a.tiles_m ) * a.tiles_n * double( a.C );
+  if( l_grid >= 4294967296.0 / 256 ) {
+    return fail( ETIR_COMPILATION_FAILED, "contraction_i8: grid too large" );
+  }
+  plan.flops = 2 * a.C * a.M * a.N * a.K;
+  int64_t const l_rows = plan.swapped ? a.N : a.M, l_cols = plan.swapped ? a.M : a.N;
+  plan.bytes = a.C * ( a.M + a.N ) * a.K + ( dtype_out == ETIR_BF16 ? 2 : 4 ) * a.C * a.M * a.N
+             + ( strides_scale_left != nullptr ? 4 * a.C * l_rows : 0 )
+             + ( ( strides_scale_right != nullptr ? 4 : 0 ) + ( strides_bias != nullptr ? 4 : 0 ) ) * a.C * l_cols;
+  plan.desc = "contraction_i8 general C=" + sizes_of( a.c ) + " rows=" + sizes_of( a.m ) + " cols=" + sizes_of( a.n )
+            + " K=" + sizes_of( a.k ) + ( plan.swapped ? " swapped" : "" )
+            + ( a.out_bf16 ? " out=bf16" : " out=fp32" );
+  return ETIR_SUCCESS;
+}
+
+int launch_i8( I8Plan const & plan,
+               void const   * left,
+               void const   * right,
+               void const   * scale_left,
+               void const   * scale_right,
+               void const   * bias,
+               void         * out,
+               hipStream_t    stream ) {
+  I8GeneralArgs a = plan.args;
+  if( a.C == 0 || a.M == 0 || a.N == 0 ) return ETIR_SUCCESS;
+  a.a  = static_cast< int8_t const * >( plan.swapped ? right : left );
+  a.b  = static_cast< int8_t const * >( plan.swapped ? left : right );
+  a.sa = plan.has_sa ? static_cast< float const * >( plan.swapped ? scale_right : scale_left ) : nullptr;
+  a.sb = plan.has_sb ? static_cast< float const * >( plan.swapped ? scale_left : scale_right ) : nullptr;
+  a.bias = plan.has_bias ? static_cast< float const * >( bias ) : nullptr;
+  a.out = out;
+  if( out == nullptr || ( a.K > 0 && ( a.a == nullptr || a.b == nullptr ) ) ) {
+    return fail( ETIR_NO_DATA_PTR_PROVIDED, "contraction_i8: null tensor pointer" );
+  }
+  if( ( plan.has_sa && a.sa == nullptr ) || ( plan.has_sb && a.sb == nullptr )
+      || ( plan.has_bias && a.bias == nullptr ) ) {
+    return fail( ETIR_NO_DATA_PTR_PROVIDED, "contraction_i8: null scale or bias, but its strides were given" );
+  }
+  return launch_i8_general( a, stream );
+}
+
+namespace {
+
+// arguments that both row operators share
+int check_rows( char const * what, int64_t rows, int64_t cols, int64_t ld_q, int64_t ld_values, int32_t dtype ) {
+  std::string const l_w( what );
+  if( dtype != ETIR_BF16 && dtype != ETIR_FP32 ) {
+    return fail( ETIR_INVALID_DTYPE, l_w + ": the rows are BF16 or FP32" );
+  }
+  int64_t const l_max = std::numeric_limits< int32_t >::max();
+  if( rows < 0 || cols < 0 || rows > l_max || cols > l_max ) {
+    return fail( ETIR_COMPILATION_FAILED, l_w + ": rows and cols are 0 to 2^31 - 1" );
+  }
+  if( rows > 1 && ( ld_q < cols || ld_values < cols ) ) {
+    return fail( ETIR_COMPILATION_FAILED, l_w + ": rows of an output overlap" );
+  }
+  return ETIR_SUCCESS;
+}
+
+// Runs fn; what it throws (only memory can run out) becomes an error code.
+template< class Fn >
+int guarded( Fn && fn ) {
+  try {
+    return fn();
+  }
+  catch( ... ) {
+    return fail( ETIR_UNDEFINED_ERROR, "out of memory" );   // short enough to need none
+  }
+}
+
+// a new plan of the given kind on the current device
+int new_plan( int32_t kind, etir_plan_t * plan ) {
+  int l_device = 0;
+  ETIR_HIP_CHECK( hipGetDevice( &l_device ) );
+  etir_plan_s * l_plan = new etir_plan_s();
+  l_plan->kind = kind;
+  l_plan->device = l_device;
+  *plan = l_plan;
+  return ETIR_SUCCESS;
+}
+
+}  // namespace
+
+}  // namespace etir
+
+using etir::fail;
+
+extern "C" {
+
+int etir_hip_contraction_i8_create( int64_t         num_loops,
+                                    int32_t const * dim_types,
+                                    int64_t const * sizes,
+                                    int64_t const * strides_left,
+                                    int64_t const * strides_right,
+                                    int64_t const * strides_scale_left,
+                                    int64_t const * strides_scale_right,
+                                    int64_t const * strides_bias,
+                                    int64_t const * strides_out,
+                                    int32_t         dtype_out,
+                                    int32_t         ktype_last_touch,
+                                    etir_plan_t   * plan ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr ) return fail( ETIR_UNDEFINED_ERROR, "plan output pointer is null" );
+    *plan = nullptr;
+    auto l_i8 = std::make_shared< etir::I8Plan >();
+    int l_err = etir::plan_i8( num_loops, dim_types, sizes, strides_left, strides_right, strides_scale_left,
+                               strides_scale_right, strides_bias, strides_out, dtype_out, ktype_last_touch, *l_i8 );
+    if( l_err == ETIR_SUCCESS ) l_err = etir::new_plan( 3, plan );
+    if( l_err == ETIR_SUCCESS ) ( *plan )->i8 = l_i8;
+    return l_err;
+  } );
+}
+
+int etir_hip_contraction_i8_execute( etir_plan_t  plan,
+                                     void const * left,
+                                     void const * right,
+                                     void const * scale_left,
+                                     void const * scale_right,
+                                     void const * bias,
+                                     void       * out,
+                                     void       * stream ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr || plan->kind != 3 ) {
+      return fail( ETIR_CALLED_BEFORE_COMPILATION, "not a plan of an 8-bit contraction" );
+    }
+    return etir::launch_i8( *plan->i8, left, right, scale_left, scale_right, bias, out,
+                            reinterpret_cast< hipStream_t >( stream ) );
+  } );
+}
+
+int etir_hip_norm_quant_create( int64_t       rows,
+                                int64_t       cols,
+                                int64_t       ld_in,
+                                int64_t       ld_residual,
+                                int64_t       ld_total,
+                                int64_t       ld_q,
+                                int64_t       ld_values,
+                                int32_t       dtype,
+                                int32_t       dtype_weight,
+                                float         eps,
+                                etir_plan_t * plan ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr ) return fail( ETIR_UNDEFINED_ERROR, "plan output pointer is null" );
+    *plan = nullptr;
+    int l_err = etir::check_rows( "norm_quant", rows, cols, ld_q, ld_values, dtype );
+    if( l_err != ETIR_SUCCESS ) return l_err;
+    if( dtype_weight != ETIR_BF16 && dtype_weight != ETIR_FP32 ) {
+      return fail( ETIR_INVALID_DTYPE, "norm_quant: the weight is BF16 or FP32" );
+    }
+    if( ld_in < 0 || ld_residual < 0 || ( rows > 1 && ld_total < cols ) ) {
+      return fail( ETIR_COMPILATION_FAILED, "norm_quant: negative row stride, or rows of total overlap" );
+    }
+    if( !( eps >= 0.0f ) || eps > std::numeric_limits< float >::max() ) {
+      return fail( ETIR_COMPILATION_FAILED, "norm_quant: eps is finite and at least 0" );
+    }
+    auto l_q = std::make_shared< etir::QuantPlan >();
+    l_q->norm = true;
+    l_q->rows = rows;
+    l_q->cols = cols;
+    l_q->dtype = dtype;
+    l_q->dtype_weight = dtype_weight;
+    l_q->eps = eps;
+    l_q->ld_in = ld_in;
+    l_q->ld_second = ld_residual;
+    l_q->ld_total = ld_total;
+    l_q->ld_q = ld_q;
+    l_q->ld_values = ld_values;
+    etir::describe_quant( *l_q );
+    l_err = etir::new_plan( 4, plan );
+    if( l_err == ETIR_SUCCESS ) ( *plan )->quant = l_q;
+    return l_err;
+  } );
+}
+
+int etir_hip_norm_quant_execute( etir_plan_t  plan,
+                                 void const * in,
+                                 void const * residual,
+                                 void const * weight,
+                                 void       * total,
+                                 void       * q,
+                                 void       * scale,
+                                 void       * values,
+                                 void       * stream ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr || plan->kind != 4 ) {
+      return fail( ETIR_CALLED_BEFORE_COMPILATION, "not a norm_quant plan" );
+    }
+    etir::QuantPlan const & p = *plan->quant;
+    etir::QuantArgs a{};
+    a.in = in;
+    a.second = residual;
+    a.weight = weight;
+    a.total = total;
+    a.q = static_cast< int8_t * >( q );
+    a.scale = static_cast< float * >( scale );
+    a.values = values;
+    return etir::launch_quant( p, a, reinterpret_cast< hipStream_t >( stream ) );
+  } );
+}
+
+int etir_hip_act_quant_create( int64_t       rows,
+                               int64_t       cols,
+                               int64_t       ld_in,
+                               int64_t       ld_gate,
+                               int64_t       ld_q,
+                               int64_t       ld_values,
+                               int32_t       dtype,
+                               int32_t       ktype,
+                               etir_plan_t * plan ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr ) return fail( ETIR_UNDEFINED_ERROR, "plan output pointer is null" );
+    *plan = nullptr;
+    int l_err = etir::check_rows( "act_quant", rows, cols, ld_q, ld_values, dtype );
+    if( l_err != ETIR_SUCCESS ) return l_err;
+    if( ld_in < 0 || ld_gate < 0 ) return fail( ETIR_COMPILATION_FAILED, "act_quant: negative row stride" );
+    if( ktype != ETIR_KTYPE_UNDEFINED && ktype != ETIR_KTYPE_RELU && ktype != ETIR_KTYPE_SILU ) {
+      return fail( ETIR_INVALID_KTYPE, "act_quant: the activation is RELU, SILU or UNDEFINED" );
+    }
+    auto l_q = std::make_shared< etir::QuantPlan >();
+    l_q->rows = rows;
+    l_q->cols = cols;
+    l_q->dtype = dtype;
+    l_q->ktype = ktype;
+    l_q->ld_in = ld_in;
+    l_q->ld_second = ld_gate;
+    l_q->ld_q = ld_q;
+    l_q->ld_values = ld_values;
+    etir::describe_quant( *l_q );
+    l_err = etir::new_plan( 5, plan );
+    if( l_err == ETIR_SUCCESS ) ( *plan )->quant = l_q;
+    return l_err;
+  } );
+}
+
+int etir_hip_act_quant_execute( etir_plan_t  plan,
+                                void const * in,
+                                void const * gate,
+                                void       * q,
+                                void       * scale,
+                                void       * values,
+                                void       * stream ) {
+  return etir::guarded( [&]() -> int {
+    if( plan == nullptr || plan->kind != 5 ) {
+      return fail( ETIR_CALLED_BEFORE_COMPILATION, "not an act_quant plan" );
+    }
+    etir::QuantPlan const & p = *plan->quant;
+    etir::QuantArgs a{};
+    a.in = in;
+    a.second = gate;
+    a.q = static_cast< int8_t * >( q );
+    a.scale = static_cast< float * >( scale );
+    a.values = values;
+    return etir::launch_quant( p, a, reinterpret_cast< hipStream_t >( stream ) );
+  } );
+}
+
+}  // extern "C"

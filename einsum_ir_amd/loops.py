@@ -84,6 +84,27 @@ def binary_loops(expr, sizes, sizes_outer_left=None, sizes_outer_right=None,
     }
 
 
+def contraction_i8_loops(expr, sizes, scale_left=None, scale_right=None, bias=None, sizes_outer_left=None,
+                         sizes_outer_right=None, sizes_outer_out=None):
+    """Arguments of ContractionI8Plan for an einsum string: the loops of
+    binary_loops with the row-major strides of the scales and the bias, whose
+    dimensions are given as strings (``scale_left="bt"``; None: not there)."""
+    lp = binary_loops(expr, sizes, sizes_outer_left, sizes_outer_right, sizes_outer_out)
+    (left, right), _ = _split(expr)
+    for name, dims, of in (("scale_left", scale_left, left), ("scale_right", scale_right, right), ("bias", bias, right)):
+        if dims is not None and not set(dims) <= set(of):
+            raise ValueError(f"{name} has dimensions that its operand lacks: {dims!r} of {of!r}")
+
+    def strides(dims):
+        if dims is None:
+            return None
+        s = row_major_strides(dims, sizes)
+        return [s.get(d, 0) for d in lp["dims"]]
+    return {k: lp[k] for k in ("dim_types", "sizes", "strides_left", "strides_right", "strides_out")} | {
+        "strides_scale_left": strides(scale_left), "strides_scale_right": strides(scale_right),
+        "strides_bias": strides(bias)}
+
+
 def unary_dims(expr, sizes):
     """Sizes, input strides (reordered to output order) and output strides of a
     permutation ``"abcd->dbca"`` with row-major tensors."""

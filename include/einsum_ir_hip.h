@@ -46,10 +46,13 @@ extern "C" {
 #define ETIR_UNDEFINED_ERROR           99
 
 /* data types: einsum_ir::data_t (reference src/constants.h:48-52) plus the
- * additive value BF16 (the reference has no bf16; 2 is unused there). */
+ * additive values BF16 and INT8 (the reference has neither; 2 and 3 are unused
+ * there).  INT8 names the operands of etir_hip_contraction_i8_*; no other call
+ * takes it. */
 #define ETIR_FP32                       0
 #define ETIR_FP64                       1
 #define ETIR_BF16                       2
+#define ETIR_INT8                       3
 #define ETIR_UNDEFINED_DTYPE           99
 
 /* kernel types: einsum_ir::kernel_t (reference src/constants.h:61-77) */
@@ -60,6 +63,7 @@ extern "C" {
 #define ETIR_KTYPE_MADD                 4
 #define ETIR_KTYPE_CPX_ZERO             6
 #define ETIR_KTYPE_CPX_MADD             8
+#define ETIR_KTYPE_SILU                20   /* additive: x / (1 + exp(-x)), etir_hip_act_quant_create only */
 #define ETIR_KTYPE_UNDEFINED           99
 
 /* dimension types: einsum_ir::dim_t (reference src/constants.h:9-18) */
@@ -217,7 +221,127 @@ int etir_hip_permute_execute( etir_plan_t  plan,
                               void       * out,
                               void       * stream );
 
-/* Releases a contraction or permutation plan and its device tables. */
+/*
+ * 8-bit layer operators.  No counterpart in the reference, whose contractions
+ * are fp32 and fp64: a linear layer that answers in 8 bits is
+ *   norm_quant -> contraction_i8 -> act_quant -> contraction_i8
+ * with the residual added by the next layer's norm_quant.  The plans own no
+ * device memory: executions overlap freely and may be captured into graphs.
+ *
+ * Product of 8-bit integers with a scale for each left row (token) and each
+ * right row (channel):
+ *   out[c,m,n] = last( scale_left[c,m] * scale_right[c,n]
+ *                      * sum_k left[c,m,k] * right[c,n,k] + bias[c,n] )
+ * The arguments follow etir_hip_contraction_create: loops of type
+ * ETIR_DIM_C/M/N/K (I and J are accepted and not iterated) with element strides
+ * in every tensor.  left and right hold ETIR_INT8, the scales and the bias fp32,
+ * the output dtype_out (ETIR_FP32 or ETIR_BF16); last touch RELU or UNDEFINED.
+ * The stride list of a scale or of the bias may be NULL: that tensor is then
+ * not read (a scale of 1, a bias of 0).  Strides of scale_left on N and K
+ * loops, of scale_right and bias on M and K loops have to be 0.  The sum is a
+ * 32-bit integer and exact; K is at most 131071.  Scales and bias are applied
+ * in fp32, with one rounding to bf16 at the end.
+ *
+ * Strides are at least 0 and may be anything otherwise; the output's elements
+ * have to lie apart.  Fast: both operands unit-stride along one K loop, and
+ * M, N and C loops that fuse to one each.  A product of any size 0 in C, M or N
+ * does nothing; without K the sums are 0.  At most 6 loops of one type that
+ * cannot be fused.
+ */
+int etir_hip_contraction_i8_create( int64_t         num_loops,
+                                    int32_t const * dim_types,
+                                    int64_t const * sizes,
+                                    int64_t const * strides_left,
+                                    int64_t const * strides_right,
+                                    int64_t const * strides_scale_left,
+                                    int64_t const * strides_scale_right,
+                                    int64_t const * strides_bias,
+                                    int64_t const * strides_out,
+                                    int32_t         dtype_out,
+                                    int32_t         ktype_last_touch,
+                                    etir_plan_t   * plan );
+
+/* Enqueues one product on `stream`.  A scale or bias pointer is needed where
+ * its strides were given.  The output may not overlap an input. */
+int etir_hip_contraction_i8_execute( etir_plan_t  plan,
+                                     void const * left,
+                                     void const * right,
+                                     void const * scale_left,
+                                     void const * scale_right,
+                                     void const * bias,
+                                     void       * out,
+                                     void       * stream );
+
+/*
+ * RMS norm with the residual's addition, rows rounded to 8 bits.  For each of
+ * `rows` rows of `cols` elements, in fp32 (the mean square in fp64):
+ *   s = in + residual                total  = s, rounded to dtype
+ *   t = s * weight                   a      = max |t|
+ *   q = rint( t * (127 / a) )        scale  = a / (127 * sqrt( mean(s^2) + eps ))
+ *   values = q * scale, rounded to dtype
+ * q does not depend on the order of the sum.  A row of zeros has q = 0 and
+ * scale = 0; a row with an infinity, a NaN or a product s * weight beyond fp32
+ * has q = 0 and scale = NaN.
+ * dtype (in, residual, total, values) and dtype_weight: ETIR_BF16 or ETIR_FP32;
+ * q: int8; scale: fp32, `rows` of them.  Elements of a row are adjacent, row i
+ * starts at i * ld_*; ld_in and ld_residual may be less than cols (0: one row
+ * for all), the output's ld_* not.  eps is at least 0.
+ */
+int etir_hip_norm_quant_create( int64_t       rows,
+                                int64_t       cols,
+                                int64_t       ld_in,
+                                int64_t       ld_residual,
+                                int64_t       ld_total,
+                                int64_t       ld_q,
+                                int64_t       ld_values,
+                                int32_t       dtype,
+                                int32_t       dtype_weight,
+                                float         eps,
+                                etir_plan_t * plan );
+
+/* Enqueues one norm on `stream`.  residual (none), weight (1), total and values
+ * (not wanted) may be NULL.  total may be in or residual itself (same pointer
+ * and row stride); no other output may overlap an input. */
+int etir_hip_norm_quant_execute( etir_plan_t  plan,
+                                 void const * in,
+                                 void const * residual,
+                                 void const * weight,
+                                 void       * total,
+                                 void       * q,
+                                 void       * scale,
+                                 void       * values,
+                                 void       * stream );
+
+/*
+ * Activation, gated where a gate is given, rows rounded to 8 bits:
+ *   y = f( in )  or  f( gate ) * in  (fp32)      a     = max |y|
+ *   q = rint( y * (127 / a) )                    scale = a / 127
+ *   values = q * scale, rounded to dtype
+ * f: ktype UNDEFINED (identity), RELU or SILU.  Rows of zeros, of infinities and
+ * of NaN, types and row strides as for etir_hip_norm_quant_create.  With no
+ * activation it lays out weights: one row, and so one scale, a channel.
+ */
+int etir_hip_act_quant_create( int64_t       rows,
+                               int64_t       cols,
+                               int64_t       ld_in,
+                               int64_t       ld_gate,
+                               int64_t       ld_q,
+                               int64_t       ld_values,
+                               int32_t       dtype,
+                               int32_t       ktype,
+                               etir_plan_t * plan );
+
+/* Enqueues one activation on `stream`; gate and values may be NULL.  No output
+ * may overlap an input. */
+int etir_hip_act_quant_execute( etir_plan_t  plan,
+                                void const * in,
+                                void const * gate,
+                                void       * q,
+                                void       * scale,
+                                void       * values,
+                                void       * stream );
+
+/* Releases a plan of any kind and its device tables. */
 int etir_hip_plan_destroy( etir_plan_t plan );
 
 /*
@@ -231,12 +355,12 @@ int etir_hip_plan_describe( etir_plan_t plan,
 
 /* Number of floating point operations of one execution of a contraction plan
  * (2*C*M*N*K; same definition as the bench harness, reference
- * src/bench_binary.cpp:46-50), 0 for permutation plans. */
+ * src/bench_binary.cpp:46-50), 0 for plans of permutations, norms and activations. */
 int64_t etir_hip_plan_flops( etir_plan_t plan );
 
 /* Algorithmic HBM bytes of one execution (every input element read once, every
  * output element written once, plus a read of the output where the touch
- * kernels need it). */
+ * kernels need it).  Norms and activations: with every optional tensor. */
 int64_t etir_hip_plan_bytes( etir_plan_t plan );
 
 /* Reason for the last failure of an etir_hip_* call on this thread. */
