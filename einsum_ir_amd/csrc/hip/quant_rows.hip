@@ -9,8 +9,9 @@
 // mean square is summed in fp64 (squares of fp32 stay in range), which costs
 // nothing beside the row's bytes.
 //
-// One workgroup takes a row; two passes over it, the first for the sum and the
-// maximum, the second for the outputs.
+// Bound by the row's bytes: every input is read once and kept in registers, as
+// fp32, while the row's maximum (and mean square) is found; 16 bytes a lane and
+// load, at any address.  A row longer than the registers hold is read twice.
 #include "i8_internal.h"
 #include "contract_kernel.h"
 #include <algorithm>
@@ -50,73 +51,244 @@ struct RowScale {
   __device__ float q( float y ) const { return finite ? rintf( ( y * pre ) * inv ) : 0.0f; }
 };
 
-template< class T, bool NORM >
-__global__ __launch_bounds__( 256 )
-void quant_rows_kernel( QuantArgs a ) {
-  __shared__ double   l_sums[4];
-  __shared__ uint32_t l_tops[4];
-  int const l_t = threadIdx.x;
-  for( int64_t l_row = blockIdx.x; l_row < a.rows; l_row += gridDim.x ) {
-  T const * l_in = static_cast< T const * >( a.in ) + l_row * a.ld_in;
-  T const * l_second = a.second ? static_cast< T const * >( a.second ) + l_row * a.ld_second : nullptr;
+// V elements of a row at any address: 16 bytes
+template< class T > struct Vec;
+template<> struct Vec< float > {
+  static constexpr int V = 4;
+  typedef float    t __attribute__( ( ext_vector_type( 4 ), aligned( 4 ) ) );
+  typedef uint32_t q __attribute__( ( aligned( 1 ) ) );
+  __device__ static void unpack( t v, float * f ) {
+#pragma unroll
+    for( int l_i = 0; l_i < V; l_i++ ) f[l_i] = v[l_i];
+  }
+  __device__ static t pack( float const * f ) { return t{ f[0], f[1], f[2], f[3] }; }
+};
+template<> struct Vec< uint16_t > {
+  static constexpr int V = 8;
+  typedef uint32_t t __attribute__( ( ext_vector_type( 4 ), aligned( 2 ) ) );
+  typedef uint64_t q __attribute__( ( aligned( 1 ) ) );
+  __device__ static void unpack( t v, float * f ) {
+#pragma unroll
+    for( int l_i = 0; l_i < V; l_i += 2 ) {
+      f[l_i]     = __uint_as_float( v[l_i / 2] << 16 );
+      f[l_i + 1] = __uint_as_float( v[l_i / 2] & 0xffff0000u );
+    }
+  }
+  __device__ static t pack( float const * f ) {
+    typedef __bf16 b2 __attribute__( ( ext_vector_type( 2 ) ) );
+    t l_v;
+#pragma unroll
+    for( int l_i = 0; l_i < 4; l_i++ ) {
+      l_v[l_i] = __builtin_bit_cast( uint32_t, b2{ static_cast< __bf16 >( f[2 * l_i] ), static_cast< __bf16 >( f[2 * l_i + 1] ) } );
+    }
+    return l_v;
+  }
+};
 
-  // the row's element i before rounding (norm: s in *sum)
-  auto value = [&]( int64_t i, float * sum ) -> float {
-    float l_v = to_f32( l_in[i] );
-    if constexpr( NORM ) {
-      if( l_second ) l_v += to_f32( l_second[i] );
-      *sum = l_v;
-      if( a.weight ) {
-        l_v *= a.weight_f32 ? static_cast< float const * >( a.weight )[i]
-                            : kern::bf16_to_f32( static_cast< uint16_t const * >( a.weight )[i] );
+// elements i .. i + V - 1 of a row, zeros from n on
+template< class T >
+__device__ inline void load_v( T const * row, int64_t i, int64_t n, float * f ) {
+  if( i + Vec< T >::V <= n ) {
+    Vec< T >::unpack( *reinterpret_cast< typename Vec< T >::t const * >( row + i ), f );
+    return;
+  }
+#pragma unroll
+  for( int l_e = 0; l_e < Vec< T >::V; l_e++ ) f[l_e] = i + l_e < n ? to_f32( row[i + l_e] ) : 0.0f;
+}
+
+template< class T >
+__device__ inline void store_v( T * row, int64_t i, int64_t n, float const * f ) {
+  if( i + Vec< T >::V <= n ) {
+    *reinterpret_cast< typename Vec< T >::t * >( row + i ) = Vec< T >::pack( f );
+    return;
+  }
+#pragma unroll
+  for( int l_e = 0; l_e < Vec< T >::V; l_e++ ) {
+    if( i + l_e < n ) row[i + l_e] = from_f32< T >( f[l_e] );
+  }
+}
+
+// THREADS threads a row, 256 or THREADS a workgroup.  CHUNKS > 0: the row fits
+// CHUNKS vectors a thread; 0: it is read twice.
+template< class T, bool NORM, int THREADS, int CHUNKS >
+__global__ __launch_bounds__( THREADS < 256 ? 256 : THREADS )
+void quant_rows_kernel( QuantArgs a ) {
+  constexpr int V     = Vec< T >::V;
+  constexpr int ROWS  = THREADS < 256 ? 256 / THREADS : 1;   // rows a workgroup
+  constexpr int WAVES = THREADS / 64;                        // waves a row
+  constexpr int HELD  = CHUNKS > 0 ? CHUNKS : 1;
+  __shared__ double   l_sums[WAVES];
+  __shared__ uint32_t l_tops[WAVES];
+  int const l_t = threadIdx.x % THREADS;
+
+  // rows of one workgroup's waves are apart only where a wave holds a whole
+  // row, so every thread of a workgroup meets the same barriers
+  for( int64_t l_row = int64_t( blockIdx.x ) * ROWS + threadIdx.x / THREADS; l_row < a.rows;
+       l_row += int64_t( gridDim.x ) * ROWS ) {
+    T const * l_in = static_cast< T const * >( a.in ) + l_row * a.ld_in;
+    T const * l_second = a.second ? static_cast< T const * >( a.second ) + l_row * a.ld_second : nullptr;
+
+    // V elements before rounding; norm: s in l_s
+    auto value = [&]( int64_t i, float * y, float * s ) {
+      load_v( l_in, i, a.cols, y );
+      float l_f[V];
+      if constexpr( NORM ) {
+        if( l_second ) {
+          load_v( l_second, i, a.cols, l_f );
+#pragma unroll
+          for( int l_e = 0; l_e < V; l_e++ ) y[l_e] += l_f[l_e];
+        }
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) s[l_e] = y[l_e];
+        if( a.weight ) {
+          if( a.weight_f32 ) {
+#pragma unroll
+            for( int l_h = 0; l_h < V; l_h += 4 ) load_v( static_cast< float const * >( a.weight ), i + l_h, a.cols, l_f + l_h );
+          }
+          else if constexpr( V == 8 ) load_v( static_cast< uint16_t const * >( a.weight ), i, a.cols, l_f );
+          else {
+#pragma unroll
+            for( int l_e = 0; l_e < V; l_e++ ) {
+              l_f[l_e] = i + l_e < a.cols ? to_f32( static_cast< uint16_t const * >( a.weight )[i + l_e] ) : 0.0f;
+            }
+          }
+#pragma unroll
+          for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= l_f[l_e];
+        }
       }
-      return l_v;
+      else if( l_second ) {
+        load_v( l_second, i, a.cols, l_f );
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= activate( l_f[l_e], a.ktype );
+      }
+      else {
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] = activate( y[l_e], a.ktype );
+      }
+    };
+
+    float l_y[HELD][V];
+    double l_sum = 0.0;
+    uint32_t l_top = 0;
+    auto first = [&]( int64_t i, float * y ) {
+      float l_s[V];
+      value( i, y, l_s );
+#pragma unroll
+      for( int l_e = 0; l_e < V; l_e++ ) {
+        if constexpr( NORM ) l_sum += double( l_s[l_e] ) * double( l_s[l_e] );
+        l_top = max( l_top, __float_as_uint( y[l_e] ) & 0x7fffffffu );
+      }
+      // the thread that read these elements writes them, after it read them
+      // for the last time, so total may be in or residual itself
+      if constexpr( NORM && CHUNKS > 0 ) {
+        if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, i, a.cols, l_s );
+      }
+    };
+    if constexpr( CHUNKS > 0 ) {
+#pragma unroll
+      for( int l_c = 0; l_c < CHUNKS; l_c++ ) {
+        int64_t const l_i = int64_t( l_c * THREADS + l_t ) * V;
+        if( l_i < a.cols ) first( l_i, l_y[l_c] );
+      }
     }
     else {
-      return l_second ? activate( to_f32( l_second[i] ), a.ktype ) * l_v : activate( l_v, a.ktype );
+      for( int64_t l_i = int64_t( l_t ) * V; l_i < a.cols; l_i += THREADS * V ) first( l_i, l_y[0] );
     }
-  };
 
-  double l_sum = 0.0;
-  uint32_t l_top = 0;
-  for( int64_t l_i = l_t; l_i < a.cols; l_i += 256 ) {
-    float l_s = 0.0f;
-    float const l_y = value( l_i, &l_s );
-    l_sum += double( l_s ) * double( l_s );
-    l_top = max( l_top, __float_as_uint( l_y ) & 0x7fffffffu );
-  }
-  for( int l_d = 32; l_d > 0; l_d /= 2 ) {
-    l_sum += __shfl_xor( l_sum, l_d );
-    l_top = max( l_top, uint32_t( __shfl_xor( int( l_top ), l_d ) ) );
-  }
-  if( l_t % 64 == 0 ) {
-    l_sums[l_t / 64] = l_sum;
-    l_tops[l_t / 64] = l_top;
-  }
-  __syncthreads();
-  l_sum = ( l_sums[0] + l_sums[1] ) + ( l_sums[2] + l_sums[3] );
-  l_top = max( max( l_tops[0], l_tops[1] ), max( l_tops[2], l_tops[3] ) );
+#pragma unroll
+    for( int l_d = 32; l_d > 0; l_d /= 2 ) {
+      if constexpr( NORM ) l_sum += __shfl_xor( l_sum, l_d );
+      l_top = max( l_top, uint32_t( __shfl_xor( int( l_top ), l_d ) ) );
+    }
+    if constexpr( WAVES > 1 ) {
+      if( l_t % 64 == 0 ) {
+        l_sums[l_t / 64] = l_sum;
+        l_tops[l_t / 64] = l_top;
+      }
+      __syncthreads();
+      l_sum = 0.0;
+#pragma unroll
+      for( int l_w = 0; l_w < WAVES; l_w++ ) {
+        if constexpr( NORM ) l_sum += l_sums[l_w];
+        l_top = max( l_top, l_tops[l_w] );
+      }
+    }
 
-  RowScale const l_r( l_top );
-  float l_scale = l_r.a / 127.0f;
-  if constexpr( NORM ) {
-    if( l_top != 0u ) l_scale = float( double( l_r.a ) / ( 127.0 * sqrt( l_sum / double( a.cols ) + double( a.eps ) ) ) );
-  }
-  if( !l_r.finite ) l_scale = __uint_as_float( 0x7fc00000u );
-  if( l_t == 0 ) a.scale[l_row] = l_scale;
-
-  // an element's inputs are read by the thread that writes its outputs, so
-  // total may be in or residual itself
-  for( int64_t l_i = l_t; l_i < a.cols; l_i += 256 ) {
-    float l_s = 0.0f;
-    float const l_q = l_r.q( value( l_i, &l_s ) );
-    a.q[l_row * a.ld_q + l_i] = int8_t( int( l_q ) );
+    RowScale const l_r( l_top );
+    float l_scale = l_r.a / 127.0f;
     if constexpr( NORM ) {
-      if( a.total ) static_cast< T * >( a.total )[l_row * a.ld_total + l_i] = from_f32< T >( l_s );
+      if( l_top != 0u ) l_scale = float( double( l_r.a ) / ( 127.0 * sqrt( l_sum / double( a.cols ) + double( a.eps ) ) ) );
     }
-    if( a.values ) static_cast< T * >( a.values )[l_row * a.ld_values + l_i] = from_f32< T >( l_q * l_scale );
+    if( !l_r.finite ) l_scale = __uint_as_float( 0x7fc00000u );
+    if( l_t == 0 ) a.scale[l_row] = l_scale;
+
+    auto last = [&]( int64_t i, float const * y ) {
+      float l_q[V];
+      typename std::conditional< V == 8, uint64_t, uint32_t >::type l_bits = 0;
+#pragma unroll
+      for( int l_e = 0; l_e < V; l_e++ ) {
+        l_q[l_e] = l_r.q( y[l_e] );
+        l_bits |= decltype( l_bits )( uint8_t( int( l_q[l_e] ) ) ) << ( 8 * l_e );
+      }
+      int8_t * l_to = a.q + l_row * a.ld_q + i;
+      if( i + V <= a.cols ) *reinterpret_cast< typename Vec< T >::q * >( l_to ) = l_bits;
+      else {
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) if( i + l_e < a.cols ) l_to[l_e] = int8_t( l_bits >> ( 8 * l_e ) );
+      }
+      if( a.values ) {
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) l_q[l_e] *= l_scale;
+        store_v( static_cast< T * >( a.values ) + l_row * a.ld_values, i, a.cols, l_q );
+      }
+    };
+    if constexpr( CHUNKS > 0 ) {
+#pragma unroll
+      for( int l_c = 0; l_c < CHUNKS; l_c++ ) {
+        int64_t const l_i = int64_t( l_c * THREADS + l_t ) * V;
+        if( l_i < a.cols ) last( l_i, l_y[l_c] );
+      }
+    }
+    else {
+      for( int64_t l_i = int64_t( l_t ) * V; l_i < a.cols; l_i += THREADS * V ) {
+        float l_s[V];
+        value( l_i, l_y[0], l_s );
+        if constexpr( NORM ) {
+          if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, l_i, a.cols, l_s );
+        }
+        last( l_i, l_y[0] );
+      }
+    }
+    if constexpr( WAVES > 1 ) __syncthreads();
   }
-  __syncthreads();
+}
+
+template< class T, bool NORM, int THREADS, int CHUNKS >
+void launch_shape( QuantArgs const & a, hipStream_t stream ) {
+  constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+  // a grid's threads are counted in 32 bits, so workgroups loop over rows
+  int64_t const l_grid = std::min< int64_t >( ( a.rows + ROWS - 1 ) / ROWS, 1 << 20 );
+  hipLaunchKernelGGL( ( quant_rows_kernel< T, NORM, THREADS, CHUNKS > ), dim3( uint32_t( l_grid ) ),
+                      dim3( THREADS < 256 ? 256 : THREADS ), 0, stream, a );
+}
+
+// Threads a row by its vectors of 16 bytes: a wave where one vector a lane
+// holds the row (no exchange between waves), else as few waves as hold it in
+// two vectors a lane.  1024 threads have 128 registers each: four vectors fit
+// them in fp32 (16 elements), not in bf16 (32).
+template< class T, bool NORM >
+void launch_rows( QuantArgs const & a, hipStream_t stream ) {
+  int64_t const l_vecs = ( a.cols + Vec< T >::V - 1 ) / Vec< T >::V;
+  if( l_vecs <= 64 )        launch_shape< T, NORM, 64, 1 >( a, stream );
+  else if( l_vecs <= 256 )  launch_shape< T, NORM, 256, 1 >( a, stream );
+  else if( l_vecs <= 512 )  launch_shape< T, NORM, 256, 2 >( a, stream );
+  else if( l_vecs <= 1024 ) launch_shape< T, NORM, 512, 2 >( a, stream );
+  else if( l_vecs <= 2048 ) launch_shape< T, NORM, 1024, 2 >( a, stream );
+  else {
+    if constexpr( Vec< T >::V == 4 ) {
+      if( l_vecs <= 4096 ) return launch_shape< T, NORM, 1024, 4 >( a, stream );
+    }
+    launch_shape< T, NORM, 1024, 0 >( a, stream );
   }
 }
 
@@ -146,13 +318,8 @@ int launch_quant( QuantPlan const & plan, QuantArgs const & args, hipStream_t st
   a.eps = plan.eps;
   a.weight_f32 = plan.dtype_weight == ETIR_FP32;
   a.ktype = plan.ktype;
-  // a grid's threads are counted in 32 bits, so workgroups loop over rows
-  dim3 const l_grid( static_cast< uint32_t >( std::min< int64_t >( plan.rows, 1 << 20 ) ) ), l_block( 256 );
-  bool const l_bf16 = plan.dtype == ETIR_BF16;
-  if( l_bf16 && plan.norm )  hipLaunchKernelGGL( ( quant_rows_kernel< uint16_t, true > ), l_grid, l_block, 0, stream, a );
-  if( l_bf16 && !plan.norm ) hipLaunchKernelGGL( ( quant_rows_kernel< uint16_t, false > ), l_grid, l_block, 0, stream, a );
-  if( !l_bf16 && plan.norm ) hipLaunchKernelGGL( ( quant_rows_kernel< float, true > ), l_grid, l_block, 0, stream, a );
-  if( !l_bf16 && !plan.norm ) hipLaunchKernelGGL( ( quant_rows_kernel< float, false > ), l_grid, l_block, 0, stream, a );
+  if( plan.dtype == ETIR_BF16 ) plan.norm ? launch_rows< uint16_t, true >( a, stream ) : launch_rows< uint16_t, false >( a, stream );
+  else                          plan.norm ? launch_rows< float, true >( a, stream ) : launch_rows< float, false >( a, stream );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
     return fail( ETIR_UNDEFINED_ERROR, std::string( "quant_rows launch failed: " ) + hipGetErrorString( l_e ) );
