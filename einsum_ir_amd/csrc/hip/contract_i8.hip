@@ -138,8 +138,7 @@ void contract_i8_general_kernel( I8GeneralArgs a ) {
   for( int l_i = 0; l_i < 16; l_i++ ) {
     int const l_m = l_wm + 8 * ( l_i / 4 ) + 4 * ( l_lane / 32 ) + l_i % 4;
     if( l_m >= l_rows ) continue;
-    float l_v = float( l_acc[l_i] ) * l_sa[l_m] * l_sb[l_n] + ( l_bias_m[l_m] + l_bias_n[l_n] );
-    if( a.relu && l_v < 0.0f ) l_v = 0.0f;     // a NaN stays
+    float const l_v = i8_finish( l_acc[l_i], l_sa[l_m], l_sb[l_n], l_bias_m[l_m] + l_bias_n[l_n], a.relu );
     int64_t const l_o = l_out_m[l_m] + l_out_n[l_n];
     if( a.out_bf16 ) static_cast< uint16_t * >( a.out )[l_o] = kern::f32_to_bf16_rne( l_v );
     else             static_cast< float * >( a.out )[l_o] = l_v;

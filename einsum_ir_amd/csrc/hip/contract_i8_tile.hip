@@ -1,0 +1,458 @@
+// gfx950 product of 8-bit integers, tiles staged through LDS:
+//
+//   out[c][m][n] = last( sa[c][m] sb[c][n] sum_k A[c][m][k] B[c][n][k] + bias )
+//
+// A workgroup computes a BM x BN tile with v_mfma_i32_32x32x32_i8, WM x WN waves
+// a K group and KG groups, which take the blocks of 128 k in turn and add their
+// sums in LDS at the end (integers: in any order the same).
+//
+// LDS holds 128 k of a row in 128 bytes, 16-byte piece g of row r at place
+// g ^ swz(r), so that the fragment reads (16 bytes a lane, 32 rows) touch every
+// bank equally.  Where rows are 16-byte aligned the pieces go there directly
+// (buffer_load ... lds, 8 rows an instruction, whole 128-byte lines); else
+// through registers, from any byte address.  Two buffers: the loads of block
+// t + 1 fly while block t is multiplied, one barrier a block.
+//
+// The channels' side is the first operand of the matrix instruction, so a lane
+// holds 4 neighbouring columns of the output; the tile goes out through LDS in
+// rows of 16-byte stores.
+#include "i8_internal.h"
+#include "contract_dma.h"
+
+namespace etir {
+namespace {
+
+using kern::i32x4;
+typedef int32_t i32x16 __attribute__( ( ext_vector_type( 16 ) ) );
+typedef float f32x4 __attribute__( ( ext_vector_type( 4 ) ) );
+
+constexpr int kBk = 128;      // k of a block
+
+// how an operand's pieces get into LDS
+enum Load : int {
+  LOAD_DMA    = 0,    // directly: rows and K at multiples of 16 bytes
+  LOAD_DWORDS = 1,    // through registers: at multiples of 4
+  LOAD_BYTES  = 2     // through registers: anywhere
+};
+
+struct TileArgs {
+  I8Args a;
+  int32_t tiles_m, tiles_n;
+  int32_t blocks;             // blocks of 128 k
+  int32_t vec_out;            // output rows take 16-byte stores
+};
+
+// ROWS rows of an operand by WAVES waves, one K group's side of the tile
+template< int ROWS, int WAVES, int LOAD >
+struct Side {
+  static constexpr bool DMA   = LOAD == LOAD_DMA;
+  static constexpr int PIECES = ROWS / 8;             // of 8 rows x 128 bytes
+  static constexpr int EACH   = PIECES / WAVES;       // a wave's pieces
+  static_assert( PIECES % WAVES == 0, "pieces have to divide over the waves" );
+
+  uint32_t m_off[DMA ? EACH : 1];       // bytes from the tile's first row to the lane's 16 bytes of block 0
+  i32x4    m_rsrc;
+  int8_t const * m_row[DMA ? 1 : EACH];
+  I8Vec< LOAD == LOAD_BYTES > m_reg[DMA ? 1 : EACH];
+  int      m_k[2];                      // the lane's k of a block in even and odd pieces
+  uint32_t m_first;                     // the wave's first piece
+
+  __device__ inline void init( int8_t const * tile, int64_t stride, int32_t rows, int wave, int lane ) {
+    m_first = wave * EACH;
+    if constexpr( DMA ) m_rsrc = kern::make_rsrc( tile, kern::kDmaOob );
+#pragma unroll
+    for( int l_i = 0; l_i < 2; l_i++ ) m_k[l_i] = 16 * ( ( lane % 8 ) ^ int( kern::swz_k( 8 * l_i + lane / 8 ) ) );
+#pragma unroll
+    for( int l_i = 0; l_i < EACH; l_i++ ) {
+      // rows past the tensor read its last one and are not stored
+      int32_t const l_r = min( int32_t( 8 * ( m_first + l_i ) + lane / 8 ), rows - 1 );
+      if constexpr( DMA ) m_off[l_i] = uint32_t( l_r * int32_t( stride ) + k_of( l_i ) );
+      else                m_row[l_i] = tile + l_r * stride;
+    }
+  }
+  __device__ inline int k_of( int i ) const { return m_k[( m_first + i ) % 2]; }
+
+  // starts the load of the wave's piece I of the block at k0; DMA: into lds
+  template< int I >
+  __device__ __attribute__( ( always_inline ) ) inline void issue( uint32_t lds, int32_t k0, int32_t K ) {
+    if constexpr( DMA ) {
+      uint32_t l_off = m_off[I];
+      // K is a multiple of 16, so a lane's k are inside or outside; outside: zeros
+      if( k0 + kBk > K && k0 + k_of( I ) >= K ) l_off = kern::kDmaOob;
+      kern::set_m0( lds + ( m_first + I ) * 1024 );
+      kern::dma16_so< 0 >( m_rsrc, l_off, uint32_t( k0 ) );
+    }
+    else {
+      m_reg[I].load( m_row[I] + i8_piece( k0 + k_of( I ), K ).at );
+    }
+  }
+
+  // piece I from registers into lds
+  template< int I >
+  __device__ __attribute__( ( always_inline ) ) inline void put( char * lds, int32_t k0, int32_t K, int lane ) {
+    i32x4 l_v = m_reg[I].value();
+    if( k0 + kBk > K ) {
+      int const l_skip = i8_piece( k0 + k_of( I ), K ).skip;
+#pragma unroll
+      for( int l_d = 0; l_d < 4; l_d++ ) l_v[l_d] &= int32_t( i8_mask( l_skip, l_d ) );
+    }
+    *reinterpret_cast< i32x4 * >( lds + ( m_first + I ) * 1024 + 16 * lane ) = l_v;
+  }
+};
+
+// Stores 32 rows x COLS columns of a wave's slab from row m1, column n1 of the
+// output: 16 bytes a lane where the output's rows take them at multiples of 4
+// bytes, else an element a lane; non-temporal, the output is not read here
+// again (4072 x 2048 x 2048: 23.2 -> 21.2 us).
+template< int COLS, int PITCH, class T >
+__device__ inline void store_slab( TileArgs const & t, float const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
+  I8Args const & a = t.a;
+  constexpr int V = 16 / sizeof( T );
+  constexpr int LANES = COLS / V;            // lanes a row
+  typedef T v __attribute__( ( ext_vector_type( V ) ) );
+  typedef v v_dword __attribute__( ( aligned( 4 ) ) );
+  T * const l_out = static_cast< T * >( a.out ) + out0;
+  if( t.vec_out ) {
+#pragma unroll
+    for( int l_p = 0; l_p < 32 * LANES / 64; l_p++ ) {
+      int const l_r = l_p * ( 64 / LANES ) + lane / LANES, l_c = lane % LANES * V;
+      v l_v;
+#pragma unroll
+      for( int l_e = 0; l_e < V; l_e += 4 ) {
+        f32x4 const l_f = *reinterpret_cast< f32x4 const * >( slab + l_r * PITCH + l_c + l_e );
+#pragma unroll
+        for( int l_d = 0; l_d < 4; l_d++ ) l_v[l_e + l_d] = static_cast< T >( l_f[l_d] );
+      }
+      if( m1 + l_r >= a.M ) continue;
+      T * const l_o = l_out + ( m1 + l_r ) * a.o_row + n1 + l_c;
+      if( n1 + l_c + V <= a.N ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_dword * >( l_o ) );
+      else {
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) if( n1 + l_c + l_e < a.N ) l_o[l_e] = l_v[l_e];
+      }
+    }
+  }
+  else {
+#pragma unroll 4
+    for( int l_p = 0; l_p < 32 * COLS / 64; l_p++ ) {
+      int const l_r = ( l_p * 64 + lane ) / COLS, l_c = ( l_p * 64 + lane ) % COLS;
+      T const l_v = static_cast< T >( slab[l_r * PITCH + l_c] );
+      if( m1 + l_r < a.M && n1 + l_c < a.N ) l_out[( m1 + l_r ) * a.o_row + ( n1 + l_c ) * a.o_col] = l_v;
+    }
+  }
+}
+
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, int LOAD >
+__global__ __launch_bounds__( 64 * WM * WN * KG )
+void contract_i8_tile_kernel( TileArgs t ) {
+  constexpr bool DMA = LOAD == LOAD_DMA;
+  constexpr int WAVES = WM * WN;                       // of a K group
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks a wave
+  constexpr int STAGE = ( BM + BN ) * kBk;
+  constexpr int PITCH = BN / WN + 4;                   // output slab: floats a row
+  constexpr int SLABS = WAVES * 32 * PITCH * 4;
+  constexpr int PARTS = KG > 1 ? ( KG - 1 ) * BM * BN * 4 : 0;
+  constexpr int BYTES = STAGES * KG * STAGE > SLABS + PARTS ? STAGES * KG * STAGE : SLABS + PARTS;
+  __shared__ __align__( 16 ) char l_lds[BYTES];
+  __shared__ __align__( 16 ) float l_sb[BN], l_bias[BN];
+
+  I8Args const & a = t.a;
+  int const l_lane = threadIdx.x % 64;
+  int const l_w = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
+  int const l_group = l_w / WAVES, l_wave = l_w % WAVES;
+  int const l_wm = l_wave / WN * ( BM / WM ), l_wn = l_wave % WN * ( BN / WN );
+
+  // Neighbouring tiles on one XCD (workgroups go to the 8 XCDs in turn), and
+  // there in bands of 8 tile rows, so that its cache serves both operands.
+  uint32_t l_id = blockIdx.x;
+  uint32_t const l_each = gridDim.x / 8;
+  if( l_id < 8 * l_each ) l_id = l_id % 8 * l_each + l_id / 8;
+  int32_t const l_per_c = t.tiles_m * t.tiles_n;
+  int32_t const l_c = l_id / l_per_c;
+  int32_t const l_r = l_id % l_per_c;
+  int32_t const l_band = l_r / ( 8 * t.tiles_n ) * 8;
+  int32_t const l_high = min( 8, t.tiles_m - l_band );
+  int32_t const l_m0 = ( l_band + l_r % ( 8 * t.tiles_n ) % l_high ) * BM;
+  int32_t const l_n0 = ( l_r % ( 8 * t.tiles_n ) / l_high ) * BN;
+
+  Side< BM, WAVES, LOAD > l_a;
+  Side< BN, WAVES, LOAD > l_b;
+  l_a.init( a.a + l_c * a.c[I8_A] + l_m0 * a.a_row, a.a_row, a.M - l_m0, l_wave, l_lane );
+  l_b.init( a.b + l_c * a.c[I8_B] + l_n0 * a.b_col, a.b_col, a.N - l_n0, l_wave, l_lane );
+
+  // scales and bias, needed after the loop
+  constexpr int CH = ( BN + 64 * WAVES * KG - 1 ) / ( 64 * WAVES * KG );
+  float l_sb_r[CH], l_bias_r[CH], l_sa[TM], l_bias_m[TM];
+#pragma unroll
+  for( int l_i = 0; l_i < CH; l_i++ ) {
+    int32_t const l_n = min( l_n0 + l_i * 64 * WAVES * KG + int( threadIdx.x ), a.N - 1 );
+    l_sb_r[l_i] = a.sb ? a.sb[l_c * a.c[I8_SB] + l_n * a.sb_col] : 1.0f;
+    l_bias_r[l_i] = a.bias ? a.bias[l_c * a.c[I8_BIAS] + l_n * a.bias_col] : 0.0f;
+  }
+  int const l_row = l_lane % 32;
+#pragma unroll
+  for( int l_j = 0; l_j < TM; l_j++ ) {
+    int32_t const l_m = min( l_m0 + l_wm + 32 * l_j + l_row, a.M - 1 );
+    l_sa[l_j] = a.sa ? a.sa[l_c * a.c[I8_SA] + l_m * a.sa_row] : 1.0f;
+    l_bias_m[l_j] = a.bias ? a.bias[l_c * a.c[I8_BIAS] + l_m * a.bias_row] : 0.0f;
+  }
+
+  // this group's buffers
+  char * const l_buf = l_lds + l_group * STAGES * STAGE;
+  uint32_t const l_buf_at = kern::lds_addr( l_buf );
+  int const l_steps = ( t.blocks + KG - 1 ) / KG;
+  // first k of the group's step s; past the last block nothing is in range and
+  // zeros are loaded
+  auto k_of_step = [&]( int s ) -> int32_t { return min( s * KG + l_group, t.blocks ) * kBk; };
+  // pieces FROM to TO - 1 of the wave's, both sides counted through
+  constexpr int EACH_A = Side< BM, WAVES, LOAD >::EACH, EACH = EACH_A + Side< BN, WAVES, LOAD >::EACH;
+  auto issue = [&]( auto ic, int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
+    constexpr int l_i = decltype( ic )::value;
+    uint32_t const l_to = l_buf_at + stage * STAGE;
+    if constexpr( l_i < EACH_A ) l_a.template issue< l_i >( l_to, k0, a.K );
+    else                         l_b.template issue< l_i - EACH_A >( l_to + BM * kBk, k0, a.K );
+  };
+  auto put = [&]( int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
+    kern::static_for< DMA ? 0 : EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
+      constexpr int l_i = decltype( ic )::value;
+      char * const l_to = l_buf + stage * STAGE;
+      if constexpr( l_i < EACH_A ) l_a.template put< l_i >( l_to, k0, a.K, l_lane );
+      else                         l_b.template put< l_i - EACH_A >( l_to + BM * kBk, k0, a.K, l_lane );
+    } );
+  };
+  // pieces of block 1 (two buffers) that are issued in front of the loop
+  constexpr int EARLY = ( EACH + 1 ) / 2;
+  kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, k_of_step( 0 ) ); } );
+  if constexpr( STAGES > 2 ) {
+    kern::static_for< STAGES - 2 >( [&]( auto sc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_s = decltype( sc )::value + 1;
+      kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, l_s, k_of_step( l_s ) ); } );
+    } );
+  }
+  else if constexpr( DMA ) {
+    kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
+    kern::wait_vmcnt< EARLY >();
+    kern::barrier_lds();
+  }
+  else {
+    put( 0, k_of_step( 0 ) );
+    kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
+    put( 1, k_of_step( 1 ) );
+    kern::wait_lgkmcnt0();
+    kern::barrier_lds();
+  }
+
+  // Fragments of 32 k: TM of rows, then TN of columns.
+  constexpr int FRAGS = TM + TN, MFMAS = TM * TN;
+  constexpr int HELD = STAGES > 2 ? 4 : 2;
+  i32x4 l_f[HELD][FRAGS];
+  uint32_t const l_swz = kern::swz_k( l_row );       // of 32-row blocks: the same
+  auto read = [&]( auto fc, i32x4 * f, int stage, int q ) __attribute__( ( always_inline ) ) {
+    constexpr int l_i = decltype( fc )::value;
+    int const l_first = l_i < TM ? l_wm + 32 * l_i : BM + l_wn + 32 * ( l_i - TM );
+    f[l_i] = *reinterpret_cast< i32x4 const * >( l_buf + stage * STAGE + l_first * kBk + l_row * kBk
+                                                 + ( ( ( 2 * q + l_lane / 32 ) ^ l_swz ) << 4 ) );
+  };
+  i32x16 l_acc[TN][TM];
+#pragma unroll
+  for( int l_i = 0; l_i < TN * TM; l_i++ ) l_acc[l_i / TM][l_i % TM] = i32x16{ 0 };
+  auto multiply = [&]( auto mc, i32x4 const * f ) __attribute__( ( always_inline ) ) {
+    constexpr int l_i = decltype( mc )::value / TM, l_j = decltype( mc )::value % TM;
+    l_acc[l_i][l_j] = __builtin_amdgcn_mfma_i32_32x32x32_i8( f[TM + l_i], f[l_j], l_acc[l_i][l_j], 0, 0, 0 );
+  };
+
+  // Two buffers: one block of 128 k in 4 parts of 32.  During a part's matrix instructions
+  // the next part's fragments are read; the barrier stands in front of the last
+  // part, when every wave has read all of this block and the next one has
+  // landed, and the block after that is loaded over this one from there on,
+  // half of it in the last part, half in the next block's first.
+  auto step = [&]( auto stage_c, int s ) __attribute__( ( always_inline ) ) {
+    constexpr int l_st = decltype( stage_c )::value;
+    kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_q = decltype( qc )::value;
+      if constexpr( l_q == 3 ) {
+        if constexpr( DMA ) kern::wait_vmcnt< 0 >();
+        kern::wait_lgkmcnt0();
+        kern::barrier_lds();
+      }
+      int32_t const l_k0 = k_of_step( s + ( l_q == 3 || !DMA ? 2 : 1 ) );
+      if constexpr( !DMA && l_q == 3 ) put( l_st, l_k0 );
+      kern::static_for< MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) {
+        constexpr int l_m = decltype( mc )::value;
+        multiply( mc, l_f[l_q % 2] );
+        // the next part's fragments over the first half of the instructions
+        constexpr int l_slots = ( MFMAS + 1 ) / 2;
+        if constexpr( l_m < l_slots ) {
+          constexpr int l_from = FRAGS * l_m / l_slots, l_to = FRAGS * ( l_m + 1 ) / l_slots;
+          kern::static_for< l_to - l_from >( [&]( auto fc ) __attribute__( ( always_inline ) ) {
+            read( std::integral_constant< int, l_from + decltype( fc )::value >(), l_f[( l_q + 1 ) % 2],
+                  l_q == 3 ? 1 - l_st : l_st, ( l_q + 1 ) % 4 );
+          } );
+        }
+        if constexpr( DMA && ( l_q == 3 || l_q == 0 ) ) {
+          constexpr int l_p0 = l_q == 3 ? 0 : EARLY, l_n = l_q == 3 ? EARLY : EACH - EARLY;
+          constexpr int l_from = l_p0 + l_n * l_m / MFMAS, l_to = l_p0 + l_n * ( l_m + 1 ) / MFMAS;
+          kern::static_for< l_to - l_from >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
+            issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_q == 3 ? l_st : 1 - l_st, l_k0 );
+          } );
+        }
+        if constexpr( !DMA && l_q == 0 && l_m == 0 ) {
+          kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, l_k0 ); } );
+        }
+        __builtin_amdgcn_sched_barrier( 0 );
+      } );
+    } );
+  };
+  // More buffers, for small tiles, which wait for memory and not for the matrix
+  // cores: blocks are issued STAGES - 1 ahead, also past the last one, so that
+  // a wave's loads in flight are the same number in every step.
+  auto deep = [&]( auto stage_c, int s ) __attribute__( ( always_inline ) ) {
+    constexpr int l_st = decltype( stage_c )::value;
+    // this block is in LDS, and every wave has read the last one
+    kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+    kern::wait_lgkmcnt0();
+    kern::barrier_lds();
+    kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_q = decltype( qc )::value;
+      kern::static_for< FRAGS >( [&]( auto fc ) __attribute__( ( always_inline ) ) { read( fc, l_f[l_q % HELD], l_st, l_q ); } );
+    } );
+    __builtin_amdgcn_sched_barrier( 0 );
+    int32_t const l_k0 = k_of_step( s + STAGES - 1 );
+    kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
+      issue( ic, ( l_st + STAGES - 1 ) % STAGES, l_k0 );
+    } );
+    __builtin_amdgcn_sched_barrier( 0 );
+    kern::static_for< 4 * MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_m = decltype( mc )::value;
+      multiply( std::integral_constant< int, l_m % MFMAS >(), l_f[l_m / MFMAS % HELD] );
+    } );
+  };
+  if constexpr( STAGES == 2 ) {
+    kern::static_for< FRAGS >( [&]( auto fc ) __attribute__( ( always_inline ) ) { read( fc, l_f[0], 0, 0 ); } );
+    for( int l_s = 0; l_s < l_steps; l_s += 2 ) {
+      step( std::integral_constant< int, 0 >(), l_s );
+      if( l_s + 1 < l_steps ) step( std::integral_constant< int, 1 >(), l_s + 1 );
+    }
+  }
+  else {
+    for( int l_s = 0; l_s < l_steps; l_s += STAGES ) {
+      kern::static_for< STAGES >( [&]( auto sc ) __attribute__( ( always_inline ) ) {
+        constexpr int l_st = decltype( sc )::value;
+        if( l_s + l_st < l_steps ) deep( sc, l_s + l_st );
+      } );
+    }
+  }
+  if constexpr( DMA ) kern::wait_vmcnt< 0 >();
+#pragma unroll
+  for( int l_i = 0; l_i < CH; l_i++ ) {
+    int const l_n = l_i * 64 * WAVES * KG + threadIdx.x;
+    if( l_n < BN ) {
+      l_sb[l_n] = l_sb_r[l_i];
+      l_bias[l_n] = l_bias_r[l_i];
+    }
+  }
+  __syncthreads();           // nothing is on its way into LDS, all fragments are read, the scales are there
+
+  // the other groups' sums to the first one
+  if constexpr( KG > 1 ) {
+    i32x4 * const l_part = reinterpret_cast< i32x4 * >( l_lds + SLABS );
+    if( l_group > 0 ) {
+#pragma unroll
+      for( int l_i = 0; l_i < TN * TM * 4; l_i++ ) {
+        i32x16 const & l_v = l_acc[l_i / 4 / TM][l_i / 4 % TM];
+        int const l_e = 4 * ( l_i % 4 );
+        l_part[( ( ( l_group - 1 ) * WAVES + l_wave ) * TN * TM * 4 + l_i ) * 64 + l_lane]
+            = i32x4{ l_v[l_e], l_v[l_e + 1], l_v[l_e + 2], l_v[l_e + 3] };
+      }
+    }
+    __syncthreads();
+    if( l_group > 0 ) return;
+    for( int l_g = 0; l_g < KG - 1; l_g++ ) {
+#pragma unroll
+      for( int l_i = 0; l_i < TN * TM * 4; l_i++ ) {
+        i32x4 const l_v = l_part[( ( l_g * WAVES + l_wave ) * TN * TM * 4 + l_i ) * 64 + l_lane];
+#pragma unroll
+        for( int l_e = 0; l_e < 4; l_e++ ) l_acc[l_i / 4 / TM][l_i / 4 % TM][4 * ( l_i % 4 ) + l_e] += l_v[l_e];
+      }
+    }
+  }
+
+  // 32 rows at a time through this wave's slab
+  float * const l_slab = reinterpret_cast< float * >( l_lds ) + l_wave * 32 * PITCH;
+  int64_t const l_out0 = l_c * a.c[I8_OUT];
+#pragma unroll
+  for( int l_j = 0; l_j < TM; l_j++ ) {
+#pragma unroll
+    for( int l_i = 0; l_i < TN; l_i++ ) {
+#pragma unroll
+      for( int l_q = 0; l_q < 4; l_q++ ) {
+        int const l_n = 32 * l_i + 8 * l_q + 4 * ( l_lane / 32 );
+        f32x4 const l_sb4 = *reinterpret_cast< f32x4 const * >( l_sb + l_wn + l_n );
+        f32x4 l_b4 = *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
+        if( a.bias_row != 0 ) l_b4 = f32x4{ l_bias_m[l_j], l_bias_m[l_j], l_bias_m[l_j], l_bias_m[l_j] };
+        f32x4 l_v;
+#pragma unroll
+        for( int l_e = 0; l_e < 4; l_e++ ) {
+          l_v[l_e] = i8_finish( l_acc[l_i][l_j][4 * l_q + l_e], l_sa[l_j], l_sb4[l_e], l_b4[l_e], a.relu );
+        }
+        *reinterpret_cast< f32x4 * >( l_slab + l_row * PITCH + l_n ) = l_v;
+      }
+    }
+    // the slab is this wave's own, and its LDS operations are in order
+    __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
+    constexpr int COLS = BN / WN;
+    int32_t const l_n1 = l_n0 + l_wn, l_m1 = l_m0 + l_wm + 32 * l_j;
+    if( a.out_bf16 ) store_slab< COLS, PITCH, __bf16 >( t, l_slab, l_out0, l_m1, l_n1, l_lane );
+    else             store_slab< COLS, PITCH, float >( t, l_slab, l_out0, l_m1, l_n1, l_lane );
+    __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
+  }
+}
+
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, int LOAD >
+int launch_shape( TileArgs t, hipStream_t stream ) {
+  I8Args const & a = t.a;
+  t.tiles_m = ( a.M + BM - 1 ) / BM;
+  t.tiles_n = ( a.N + BN - 1 ) / BN;
+  t.blocks = ( a.K + kBk - 1 ) / kBk;
+  uint32_t const l_grid = uint32_t( int64_t( t.tiles_m ) * t.tiles_n * a.C );
+  hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, LOAD > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
+                      0, stream, t );
+  hipError_t const l_e = hipGetLastError();
+  if( l_e != hipSuccess ) {
+    return fail( ETIR_UNDEFINED_ERROR, std::string( "contraction_i8 launch failed: " ) + hipGetErrorString( l_e ) );
+  }
+  return ETIR_SUCCESS;
+}
+
+}  // namespace
+
+int launch_i8_tile( I8Args const & a, I8Kernel kernel, hipStream_t stream ) {
+  TileArgs t{};
+  t.a = a;
+  int64_t const l_item = a.out_bf16 ? 2 : 4;
+  t.vec_out = a.o_col == 1 && uintptr_t( a.out ) % 4 == 0 && a.o_row * l_item % 4 == 0 && a.c[I8_OUT] * l_item % 4 == 0;
+  bool const l_dwords = i8_aligned( a, 4 );
+  switch( kernel ) {
+    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, LOAD_DMA >( t, stream );
+    case I8Kernel::REG_32x32:
+      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 32, 32, 1, 1, 4, 2, LOAD_BYTES >( t, stream );
+    case I8Kernel::REG_64x64:
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 64, 64, 2, 2, 1, 2, LOAD_BYTES >( t, stream );
+    case I8Kernel::REG_64x64_K2:
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 64, 64, 2, 2, 2, 2, LOAD_BYTES >( t, stream );
+    case I8Kernel::REG_128x128:
+      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 128, 128, 2, 2, 1, 2, LOAD_BYTES >( t, stream );
+    default: return fail( ETIR_COMPILATION_FAILED, "contraction_i8: unknown tile" );
+  }
+}
+
+}  // namespace etir

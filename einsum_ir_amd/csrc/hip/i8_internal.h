@@ -42,15 +42,112 @@ struct I8GeneralArgs {
   int32_t bias_rows;       // the bias runs over rows (A and B have changed places)
 };
 
-enum class I8Kernel : int32_t {
-  GENERAL = 0      // any strides, 64 x 64 tiles (contract_i8.hip)
+// One loop of each type at most, both operands unit-stride along K, K >= 16.
+struct I8Args {
+  int8_t const * a;
+  int8_t const * b;
+  float const  * sa;       // null: 1
+  float const  * sb;       // null: 1
+  float const  * bias;     // null: 0
+  void         * out;
+  int32_t C, M, N, K;
+  // strides from row (of A), column (row of B) and batch index to the next
+  int64_t a_row, b_col;
+  int64_t o_row, o_col;
+  int64_t sa_row, sb_col;
+  int64_t bias_row, bias_col;
+  int64_t c[I8_TENSORS];
+  int32_t out_bf16;
+  int32_t relu;
 };
+
+// The kernels.  TILE_*: through LDS (contract_i8_tile.hip); their rows come in
+// directly where they lie at multiples of 16 bytes, else through registers.
+enum class I8Kernel : int32_t {
+  GENERAL,            // any strides, 64 x 64 tiles (contract_i8.hip)
+  FEW_16,             // a side of up to 16, K over the waves (contract_i8_few.hip)
+  FEW_32,             // a side of up to 32
+  TILE_32x32,
+  TILE_64x32,
+  TILE_64x64,
+  TILE_128x128,
+  TILE_256x128,
+  TILE_256x256,
+  REG_32x32,          // through registers
+  REG_64x64,
+  REG_64x64_K2,       // with K over two groups of waves
+  REG_128x128
+};
+
+// rows of both operands, and K, at multiples of n bytes
+inline bool i8_aligned( I8Args const & a, int64_t n ) {
+  return a.K % n == 0 && uintptr_t( a.a ) % n == 0 && uintptr_t( a.b ) % n == 0 && a.a_row % n == 0
+      && a.b_col % n == 0 && a.c[I8_A] % n == 0 && a.c[I8_B] % n == 0;
+}
+// 16, 4 or 1
+inline int32_t i8_alignment( I8Args const & a ) {
+  return i8_aligned( a, 16 ) ? 16 : i8_aligned( a, 4 ) ? 4 : 1;
+}
+
+// 16 k of a row where K ends inside them: the row's last 16 are loaded in
+// their place, and those that belong to an earlier piece count as zeros on one
+// operand's side.
+struct I8Piece {
+  int32_t at;      // first k to load, at least 0 (K >= 16)
+  int32_t skip;    // leading bytes that count as zeros, 16: all
+};
+__device__ inline I8Piece i8_piece( int32_t k, int32_t K ) {
+  return { min( k, K - 16 ), k < K ? max( k - ( K - 16 ), 0 ) : 16 };
+}
+// 16 bytes of a row on their way.  BYTES: at any address, read as the five
+// aligned dwords that hold them (of which only those with a byte of the 16 are
+// read) and shifted into place: 16-byte loads off a 4-byte boundary run at a
+// third of the rate of aligned ones (2.3 TB/s of 7.5 from the cache, 5.4 so).
+// Else: at a multiple of 4.
+template< bool BYTES >
+struct I8Vec {
+  typedef int32_t v4 __attribute__( ( ext_vector_type( 4 ) ) );
+  typedef v4 v4_dword __attribute__( ( aligned( 4 ) ) );
+  v4      m_v;
+  int32_t m_w;
+  int32_t m_shift;
+  __device__ __attribute__( ( always_inline ) ) inline void load( int8_t const * p ) {
+    if constexpr( BYTES ) {
+      uintptr_t const l_p = reinterpret_cast< uintptr_t >( p );
+      m_v = *reinterpret_cast< v4_dword const * >( l_p & ~uintptr_t( 3 ) );
+      m_w = *reinterpret_cast< int32_t const * >( ( l_p + 15 ) & ~uintptr_t( 3 ) );
+      m_shift = int32_t( l_p & 3 );
+    }
+    else m_v = *reinterpret_cast< v4_dword const * >( p );
+  }
+  __device__ __attribute__( ( always_inline ) ) inline v4 value() const {
+    if constexpr( !BYTES ) return m_v;
+    else return v4{ int32_t( __builtin_amdgcn_alignbyte( m_v[1], m_v[0], m_shift ) ),
+                    int32_t( __builtin_amdgcn_alignbyte( m_v[2], m_v[1], m_shift ) ),
+                    int32_t( __builtin_amdgcn_alignbyte( m_v[3], m_v[2], m_shift ) ),
+                    int32_t( __builtin_amdgcn_alignbyte( m_w, m_v[3], m_shift ) ) };
+  }
+};
+
+// the bytes of dword d (0 to 3) of a piece that count
+__device__ inline uint32_t i8_mask( int32_t skip, int32_t d ) {
+  int32_t const l_z = skip - 4 * d;
+  return l_z <= 0 ? 0xffffffffu : l_z >= 4 ? 0u : 0xffffffffu << ( 8 * l_z );
+}
+
+// scale, bias and last touch of one sum
+__device__ inline float i8_finish( int32_t sum, float sa, float sb, float bias, int32_t relu ) {
+  float const l_v = float( sum ) * sa * sb + bias;
+  return relu && l_v < 0.0f ? 0.0f : l_v;       // a NaN stays
+}
 
 struct I8Plan {
   I8Kernel kernel = I8Kernel::GENERAL;
+  int32_t  alignment = 0;              // of the operands' rows that the kernel was chosen for
   bool     swapped = false;            // A = right tensor, B = left tensor
   bool     has_sa = false, has_sb = false, has_bias = false;
   I8GeneralArgs args{};                // pointers set at execution
+  I8Args   affine{};                   // kernels other than GENERAL; pointers set at execution
   int64_t  flops = 0;
   int64_t  bytes = 0;
   std::string desc;
@@ -78,6 +175,8 @@ int launch_i8( I8Plan const & plan,
                hipStream_t    stream );
 
 int launch_i8_general( I8GeneralArgs const & a, hipStream_t stream );
+int launch_i8_few( I8Args const & a, hipStream_t stream );
+int launch_i8_tile( I8Args const & a, I8Kernel kernel, hipStream_t stream );
 
 // ---------------------------------------------------------------------------
 // rows rounded to 8-bit integers with one scale a row

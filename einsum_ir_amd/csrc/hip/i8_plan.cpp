@@ -69,6 +69,117 @@ std::string sizes_of( I8Loops const & l ) {
   return l_s + "]";
 }
 
+// What choose_kernel knows of a kernel: a workgroup's rows and columns (FEW: of
+// the few and the many side), its threads, the k it takes in a step, and the
+// time of a workgroup alone on its compute unit as measured over 170 products
+// with rows at multiples of 16 bytes, 50 at 4, 80 at others (1 to 8192 rows,
+// 16 to 16384 columns, K 64 to 12288): fixed + step * steps.  The times that
+// follow are off by 10 to 20 % (root mean square), but alike for neighbours: the
+// kernel chosen is 1 to 2 % slower than the best of all on average, 2.4 times
+// as fast as 64 x 64 tiles everywhere at few tokens, 1.9 times at many.
+struct Candidate {
+  I8Kernel     kernel;
+  char const * name;
+  int32_t      alignment;          // 16: these rows only; 4, 1: of such rows or better
+  int32_t      rows, cols, threads, step_k;
+  float        fixed_us, step_us;
+};
+Candidate const kCandidates[] = {
+  { I8Kernel::FEW_16,       "few 16",       4,  16,  16,  512, 2048, 0.0f, 0.87f },
+  { I8Kernel::FEW_32,       "few 32",       4,  32,  16,  512, 2048, 0.0f, 1.30f },
+  { I8Kernel::TILE_32x32,   "tile 32x32",   16, 32,  32,  256, 512,  2.1f, 0.34f },
+  { I8Kernel::TILE_64x32,   "tile 64x32",   16, 64,  32,  256, 256,  2.0f, 0.28f },
+  { I8Kernel::TILE_64x64,   "tile 64x64",   16, 64,  64,  256, 128,  1.4f, 0.23f },
+  { I8Kernel::TILE_128x128, "tile 128x128", 16, 128, 128, 512, 128,  3.2f, 0.44f },
+  { I8Kernel::TILE_256x128, "tile 256x128", 16, 256, 128, 512, 128,  5.1f, 0.72f },
+  { I8Kernel::TILE_256x256, "tile 256x256", 16, 256, 256, 512, 128,  8.4f, 1.09f },
+  { I8Kernel::REG_32x32,    "regs 32x32",   4,  32,  32,  256, 512,  3.0f, 0.51f },
+  { I8Kernel::REG_64x64,    "regs 64x64",   4,  64,  64,  256, 128,  1.9f, 0.33f },
+  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 4, 64,  64,  512, 256,  3.0f, 0.45f },
+  { I8Kernel::REG_128x128,  "regs 128x128", 4,  128, 128, 256, 128,  5.8f, 0.63f },
+  { I8Kernel::FEW_16,       "few 16",       1,  16,  16,  512, 2048, 0.0f, 1.40f },
+  { I8Kernel::FEW_32,       "few 32",       1,  32,  16,  512, 2048, 0.0f, 3.18f },
+  { I8Kernel::REG_32x32,    "regs 32x32",   1,  32,  32,  256, 512,  3.8f, 0.93f },
+  { I8Kernel::REG_64x64,    "regs 64x64",   1,  64,  64,  256, 128,  2.3f, 0.55f },
+  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 1, 64,  64,  512, 256,  3.4f, 0.81f },
+  { I8Kernel::REG_128x128,  "regs 128x128", 1,  128, 128, 256, 128,  7.0f, 1.07f }
+};
+
+int64_t ceil_div( int64_t x, int64_t y ) { return ( x + y - 1 ) / y; }
+
+// The kernel that should take the least time on 256 compute units: tiles in
+// rounds of one workgroup each, at least 1.15 times the tensors' bytes at 5.3
+// TB/s.  The first of equals is the one with the smaller tiles.
+Candidate const * choose_candidate( I8Args const & a, int32_t alignment ) {
+  Candidate const * l_best = nullptr;
+  double l_least = 0.0;
+  double const l_bytes = double( a.C ) * ( ( double( a.M ) + a.N ) * a.K + double( a.out_bf16 ? 2 : 4 ) * a.M * a.N );
+  for( Candidate const & l_c : kCandidates ) {
+    // the rows of alignment 4 and 1 have their own entries, and those of 16 the few-sided kernels' of 4
+    bool const l_few = l_c.kernel == I8Kernel::FEW_16 || l_c.kernel == I8Kernel::FEW_32;
+    if( l_few ? ( l_c.alignment == 1 ) != ( alignment == 1 ) : l_c.alignment != alignment ) continue;
+    double l_groups, l_us;
+    if( l_few ) {
+      if( std::min( a.M, a.N ) > l_c.rows ) continue;
+      l_groups = double( ceil_div( std::max( a.M, a.N ), l_c.cols ) ) * a.C;
+    }
+    else {
+      // a tile's rows are addressed by 31 bits from its first one
+      if( std::max( l_c.rows * a.a_row, l_c.cols * a.b_col ) + a.K >= ( int64_t( 1 ) << 31 ) ) continue;
+      l_groups = double( ceil_div( a.M, l_c.rows ) ) * ceil_div( a.N, l_c.cols ) * a.C;
+      double const l_steps = double( ceil_div( a.K, l_c.step_k ) );
+      l_us = std::max( double( ceil_div( int64_t( l_groups ), 256 ) ) * ( l_c.fixed_us + l_steps * l_c.step_us ),
+                       1.15 * l_bytes / 5.3e6 );
+    }
+    if( l_few ) {
+      // latency, or what the rows' 64-byte pieces take in the caches
+      l_us = std::max( double( ceil_div( a.K, l_c.step_k ) ) * l_c.step_us,
+                       l_groups * a.K * 1e-6 * ( 3.1 + 0.12 * std::min( a.M, a.N ) ) * ( l_c.alignment == 1 ? 1.6 : 1.0 ) );
+    }
+    // a grid's threads are counted in 32 bits
+    if( l_groups * l_c.threads >= 4294967296.0 ) continue;
+    if( l_best == nullptr || l_us < l_least ) {
+      l_best = &l_c;
+      l_least = l_us;
+    }
+  }
+  return l_best;
+}
+
+// The kernel for a product whose loops are in plan.args; its name.
+char const * choose_kernel( I8Plan & plan ) {
+  I8GeneralArgs const & a = plan.args;
+  bool const l_unit_k = a.k.n == 0 || ( a.k.n == 1 && a.k.stride[0][I8_A] == 1 && a.k.stride[0][I8_B] == 1 );
+  if( a.c.n > 1 || a.m.n > 1 || a.n.n > 1 || !l_unit_k || a.K < 16 || a.C == 0 || a.M == 0 || a.N == 0 ) return "general";
+  I8Args & f = plan.affine;
+  f.C = int32_t( a.C );
+  f.M = int32_t( a.M );
+  f.N = int32_t( a.N );
+  f.K = int32_t( a.K );
+  // without a loop every stride is 0
+  f.a_row = a.m.stride[0][I8_A];
+  f.o_row = a.m.stride[0][I8_OUT];
+  f.sa_row = a.m.stride[0][I8_SA];
+  f.bias_row = a.m.stride[0][I8_BIAS];
+  f.b_col = a.n.stride[0][I8_B];
+  f.o_col = a.n.n == 0 ? 1 : a.n.stride[0][I8_OUT];
+  f.sb_col = a.n.stride[0][I8_SB];
+  f.bias_col = a.n.stride[0][I8_BIAS];
+  std::copy_n( a.c.stride[0], int( I8_TENSORS ), f.c );
+  f.out_bf16 = a.out_bf16;
+  f.relu = a.relu;
+  plan.alignment = i8_alignment( f );
+  Candidate const * l_c = choose_candidate( f, plan.alignment );
+  if( l_c == nullptr ) return "general";
+  plan.kernel = l_c->kernel;
+  return l_c->name;
+}
+
+int launch_affine( I8Kernel kernel, I8Args const & a, hipStream_t stream ) {
+  if( kernel == I8Kernel::FEW_16 || kernel == I8Kernel::FEW_32 ) return launch_i8_few( a, stream );
+  return launch_i8_tile( a, kernel, stream );
+}
+
 }  // namespace
 
 int plan_i8( int64_t         num_loops,
@@ -181,7 +292,7 @@ int plan_i8( int64_t         num_loops,
   plan.bytes = a.C * ( a.M + a.N ) * a.K + ( dtype_out == ETIR_BF16 ? 2 : 4 ) * a.C * a.M * a.N
              + ( strides_scale_left != nullptr ? 4 * a.C * l_rows : 0 )
              + ( ( strides_scale_right != nullptr ? 4 : 0 ) + ( strides_bias != nullptr ? 4 : 0 ) ) * a.C * l_cols;
-  plan.desc = "contraction_i8 general C=" + sizes_of( a.c ) + " rows=" + sizes_of( a.m ) + " cols=" + sizes_of( a.n )
+  plan.desc = std::string( "contraction_i8 " ) + choose_kernel( plan ) + " C=" + sizes_of( a.c ) + " rows=" + sizes_of( a.m ) + " cols=" + sizes_of( a.n )
             + " K=" + sizes_of( a.k ) + ( plan.swapped ? " swapped" : "" )
             + ( a.out_bf16 ? " out=bf16" : " out=fp32" );
   return ETIR_SUCCESS;
@@ -210,7 +321,19 @@ int launch_i8( I8Plan const & plan,
       || ( plan.has_bias && a.bias == nullptr ) ) {
     return fail( ETIR_NO_DATA_PTR_PROVIDED, "contraction_i8: null scale or bias, but its strides were given" );
   }
-  return launch_i8_general( a, stream );
+  if( plan.kernel == I8Kernel::GENERAL ) return launch_i8_general( a, stream );
+  I8Args f = plan.affine;
+  f.a = a.a;
+  f.b = a.b;
+  f.sa = a.sa;
+  f.sb = a.sb;
+  f.bias = a.bias;
+  f.out = a.out;
+  // pointers may be less aligned than the strides
+  int32_t const l_alignment = i8_alignment( f );
+  if( l_alignment >= plan.alignment ) return launch_affine( plan.kernel, f, stream );
+  Candidate const * l_c = choose_candidate( f, l_alignment );
+  return l_c == nullptr ? launch_i8_general( a, stream ) : launch_affine( l_c->kernel, f, stream );
 }
 
 namespace {

@@ -262,3 +262,30 @@ def test_refuses_missing_tensors(torch_cuda):
     with pytest.raises(eir.EinsumIrError) as e:
         eir.check(eir.hip_lib().etir_hip_contraction_i8_execute(other.handle, *[f.data_ptr()] * 6, None))
     assert e.value.code == eir.CALLED_BEFORE_COMPILATION
+
+
+# a size for each kernel that a product may take, with tiles cut off on both
+# sides, one K block and several, K ending inside a block
+KERNELS = [("few 16", 5, 1040, 140), ("few 16", 5, 997, 140), ("few 16", 5, 1044, 140), ("few 32", 29, 2064, 140),
+           ("few 32", 29, 515, 140), ("few 32", 29, 1044, 140), ("tile 32x32", 70, 1040, 200),
+           ("tile 64x32", 130, 1040, 2050), ("tile 64x64", 70, 96, 200), ("tile 64x64", 1500, 2064, 1300),
+           ("tile 128x128", 1500, 4112, 2050), ("tile 128x128", 3000, 96, 700), ("tile 256x128", 3000, 96, 1300),
+           ("tile 256x256", 2100, 1040, 4300), ("regs 32x32", 70, 1044, 200), ("regs 32x32", 70, 1041, 140),
+           ("regs 64x64", 70, 515, 140), ("regs 64x64", 130, 1044, 2050), ("regs 64x64 k2", 130, 997, 2050),
+           ("regs 64x64 k2", 130, 2052, 2050), ("regs 128x128", 1000, 515, 2050), ("regs 128x128", 1000, 1044, 2050)]
+
+
+@pytest.mark.parametrize("name,m,k,n", KERNELS)
+@pytest.mark.parametrize("swap", [False, True])
+def test_every_kernel(torch_cuda, name, m, k, n, swap):
+    """The size takes the kernel that it is here for, bias along both sides of the tile."""
+    desc, _ = run(torch_cuda, "tk,ok->ot" if swap else "tk,ok->to", dict(t=m, k=k, o=n),
+                  eir.BF16 if n % 4 else eir.FP32, relu=True, seed=m)
+    assert desc.startswith(f"contraction_i8 {name} C="), desc
+
+
+@pytest.mark.parametrize("k", [16, 112, 128, 129, 256, 260, 383, 384, 500, 512, 640, 1024, 1025, 1100])
+@pytest.mark.parametrize("m,n", [(200, 70), (900, 1000), (3000, 600), (4000, 2400)])
+def test_ends_of_k(torch_cuda, m, n, k):
+    """K of fewer blocks than buffers, of as many, and ending at any place of a block."""
+    run(torch_cuda, "tk,ok->to", dict(t=m, k=k, o=n), eir.BF16, seed=k)
