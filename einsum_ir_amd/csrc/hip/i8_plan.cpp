@@ -345,8 +345,8 @@ int check_rows( char const * what, int64_t rows, int64_t cols, int64_t ld_q, int
     return fail( ETIR_INVALID_DTYPE, l_w + ": the rows are BF16 or FP32" );
   }
   int64_t const l_max = std::numeric_limits< int32_t >::max();
-  if( rows < 0 || cols < 0 || rows > l_max || cols > l_max ) {
-    return fail( ETIR_COMPILATION_FAILED, l_w + ": rows and cols are 0 to 2^31 - 1" );
+  if( rows < 0 || cols < 0 || rows > l_max || cols > l_max / 2 ) {
+    return fail( ETIR_COMPILATION_FAILED, l_w + ": rows are 0 to 2^31 - 1, cols 0 to 2^30 - 1" );
   }
   if( rows > 1 && ( ld_q < cols || ld_values < cols ) ) {
     return fail( ETIR_COMPILATION_FAILED, l_w + ": rows of an output overlap" );

@@ -56,7 +56,7 @@ template< class T > struct Vec;
 template<> struct Vec< float > {
   static constexpr int V = 4;
   typedef float    t __attribute__( ( ext_vector_type( 4 ), aligned( 4 ) ) );
-  typedef uint32_t q __attribute__( ( aligned( 1 ) ) );
+  typedef uint32_t q;
   __device__ static void unpack( t v, float * f ) {
 #pragma unroll
     for( int l_i = 0; l_i < V; l_i++ ) f[l_i] = v[l_i];
@@ -66,7 +66,7 @@ template<> struct Vec< float > {
 template<> struct Vec< uint16_t > {
   static constexpr int V = 8;
   typedef uint32_t t __attribute__( ( ext_vector_type( 4 ), aligned( 2 ) ) );
-  typedef uint64_t q __attribute__( ( aligned( 1 ) ) );
+  typedef uint64_t q __attribute__( ( aligned( 4 ) ) );
   __device__ static void unpack( t v, float * f ) {
 #pragma unroll
     for( int l_i = 0; l_i < V; l_i += 2 ) {
@@ -85,79 +85,97 @@ template<> struct Vec< uint16_t > {
   }
 };
 
-// elements i .. i + V - 1 of a row, zeros from n on
+// A vector of a row of n elements: those of i .. i + V - 1 that the row has.
+// It is read from `at`, where all V are inside the row (so that no lane waits
+// for element-wise loads of its own); what does not belong to it counts as
+// zeros and is not written.  n < V: read element by element, at = 0.
+template< int V >
+struct Place {
+  int32_t i, at;
+  __device__ Place( int32_t i_, int32_t n ) : i( i_ ), at( max( min( i_, n - V ), 0 ) ) {}
+  __device__ bool whole( int32_t n ) const { return at == i && n >= V; }
+  __device__ bool has( int e, int32_t n ) const { return at + e >= i && at + e < i + V && at + e < n; }
+};
+
 template< class T >
-__device__ inline void load_v( T const * row, int64_t i, int64_t n, float * f ) {
-  if( i + Vec< T >::V <= n ) {
-    Vec< T >::unpack( *reinterpret_cast< typename Vec< T >::t const * >( row + i ), f );
+__device__ inline void load_v( T const * row, int32_t at, int32_t n, float * f ) {
+  if( n >= Vec< T >::V ) {
+    Vec< T >::unpack( *reinterpret_cast< typename Vec< T >::t const * >( row + at ), f );
     return;
   }
 #pragma unroll
-  for( int l_e = 0; l_e < Vec< T >::V; l_e++ ) f[l_e] = i + l_e < n ? to_f32( row[i + l_e] ) : 0.0f;
+  for( int l_e = 0; l_e < Vec< T >::V; l_e++ ) f[l_e] = l_e < n ? to_f32( row[l_e] ) : 0.0f;
 }
 
+// Non-temporal: these rows are written whole and not read here again (norm of
+// 16384 x 8192 bf16: 271 -> 256 us; non-temporal loads: 307).
 template< class T >
-__device__ inline void store_v( T * row, int64_t i, int64_t n, float const * f ) {
-  if( i + Vec< T >::V <= n ) {
-    *reinterpret_cast< typename Vec< T >::t * >( row + i ) = Vec< T >::pack( f );
+__device__ inline void store_v( T * row, Place< Vec< T >::V > p, int32_t n, float const * f ) {
+  if( p.whole( n ) ) {
+    __builtin_nontemporal_store( Vec< T >::pack( f ), reinterpret_cast< typename Vec< T >::t * >( row + p.at ) );
     return;
   }
 #pragma unroll
   for( int l_e = 0; l_e < Vec< T >::V; l_e++ ) {
-    if( i + l_e < n ) row[i + l_e] = from_f32< T >( f[l_e] );
+    if( p.has( l_e, n ) ) row[p.at + l_e] = from_f32< T >( f[l_e] );
   }
 }
 
-// THREADS threads a row, 256 or THREADS a workgroup.  CHUNKS > 0: the row fits
+// THREADS threads a row; a workgroup takes 4 rows of a wave each, or one row.  CHUNKS > 0: the row fits
 // CHUNKS vectors a thread; 0: it is read twice.
 template< class T, bool NORM, int THREADS, int CHUNKS >
-__global__ __launch_bounds__( THREADS < 256 ? 256 : THREADS )
+__global__ __launch_bounds__( THREADS == 64 ? 256 : THREADS )
 void quant_rows_kernel( QuantArgs a ) {
   constexpr int V     = Vec< T >::V;
-  constexpr int ROWS  = THREADS < 256 ? 256 / THREADS : 1;   // rows a workgroup
+  constexpr int ROWS  = THREADS == 64 ? 4 : 1;               // rows a workgroup
   constexpr int WAVES = THREADS / 64;                        // waves a row
   constexpr int HELD  = CHUNKS > 0 ? CHUNKS : 1;
   __shared__ double   l_sums[WAVES];
   __shared__ uint32_t l_tops[WAVES];
   int const l_t = threadIdx.x % THREADS;
+  int const l_sub = __builtin_amdgcn_readfirstlane( threadIdx.x / THREADS );
+  int32_t const l_cols = int32_t( a.cols );
 
   // rows of one workgroup's waves are apart only where a wave holds a whole
   // row, so every thread of a workgroup meets the same barriers
-  for( int64_t l_row = int64_t( blockIdx.x ) * ROWS + threadIdx.x / THREADS; l_row < a.rows;
+  for( int64_t l_row = int64_t( blockIdx.x ) * ROWS + l_sub; l_row < a.rows;
        l_row += int64_t( gridDim.x ) * ROWS ) {
     T const * l_in = static_cast< T const * >( a.in ) + l_row * a.ld_in;
+    // Vectors start where those of q lie at multiples of 4 bytes: off them 16
+    // bytes move at a third of the rate.  Where all rows are one after the
+    // other that is a multiple of 4 elements in every tensor.
+    int const l_shift = int( ( reinterpret_cast< uintptr_t >( a.q ) + l_row * a.ld_q ) & 3 );
     T const * l_second = a.second ? static_cast< T const * >( a.second ) + l_row * a.ld_second : nullptr;
 
     // V elements before rounding; norm: s in l_s
-    auto value = [&]( int64_t i, float * y, float * s ) {
-      load_v( l_in, i, a.cols, y );
+    auto value = [&]( Place< V > const & p, float * y, float * s ) {
+      load_v( l_in, p.at, l_cols, y );
       float l_f[V];
       if constexpr( NORM ) {
         if( l_second ) {
-          load_v( l_second, i, a.cols, l_f );
+          load_v( l_second, p.at, l_cols, l_f );
 #pragma unroll
           for( int l_e = 0; l_e < V; l_e++ ) y[l_e] += l_f[l_e];
         }
 #pragma unroll
         for( int l_e = 0; l_e < V; l_e++ ) s[l_e] = y[l_e];
         if( a.weight ) {
-          if( a.weight_f32 ) {
-#pragma unroll
-            for( int l_h = 0; l_h < V; l_h += 4 ) load_v( static_cast< float const * >( a.weight ), i + l_h, a.cols, l_f + l_h );
-          }
-          else if constexpr( V == 8 ) load_v( static_cast< uint16_t const * >( a.weight ), i, a.cols, l_f );
-          else {
+          if( a.weight_f32 != ( V == 4 ) ) {
+            // the weight's type is not the row's
 #pragma unroll
             for( int l_e = 0; l_e < V; l_e++ ) {
-              l_f[l_e] = i + l_e < a.cols ? to_f32( static_cast< uint16_t const * >( a.weight )[i + l_e] ) : 0.0f;
+              int32_t const l_i = min( p.at + l_e, l_cols - 1 );
+              l_f[l_e] = V == 8 ? static_cast< float const * >( a.weight )[l_i]
+                                : to_f32( static_cast< uint16_t const * >( a.weight )[l_i] );
             }
           }
+          else load_v( static_cast< T const * >( a.weight ), p.at, l_cols, l_f );
 #pragma unroll
           for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= l_f[l_e];
         }
       }
       else if( l_second ) {
-        load_v( l_second, i, a.cols, l_f );
+        load_v( l_second, p.at, l_cols, l_f );
 #pragma unroll
         for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= activate( l_f[l_e], a.ktype );
       }
@@ -165,34 +183,44 @@ void quant_rows_kernel( QuantArgs a ) {
 #pragma unroll
         for( int l_e = 0; l_e < V; l_e++ ) y[l_e] = activate( y[l_e], a.ktype );
       }
+      if( !p.whole( l_cols ) ) {
+#pragma unroll
+        for( int l_e = 0; l_e < V; l_e++ ) {
+          if( p.has( l_e, l_cols ) ) continue;
+          y[l_e] = 0.0f;
+          if constexpr( NORM ) s[l_e] = 0.0f;
+        }
+      }
     };
 
     float l_y[HELD][V];
     double l_sum = 0.0;
     uint32_t l_top = 0;
-    auto first = [&]( int64_t i, float * y ) {
+    auto first = [&]( int32_t i, float * y ) {
       float l_s[V];
-      value( i, y, l_s );
+      Place< V > const l_p( i, l_cols );
+      value( l_p, y, l_s );
 #pragma unroll
       for( int l_e = 0; l_e < V; l_e++ ) {
         if constexpr( NORM ) l_sum += double( l_s[l_e] ) * double( l_s[l_e] );
         l_top = max( l_top, __float_as_uint( y[l_e] ) & 0x7fffffffu );
       }
-      // the thread that read these elements writes them, after it read them
-      // for the last time, so total may be in or residual itself
+      // Total may be in or residual itself: an element is written by the thread
+      // whose vector it belongs to, after it was read there for the last time;
+      // a vector beside it that reads it too does not count it.
       if constexpr( NORM && CHUNKS > 0 ) {
-        if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, i, a.cols, l_s );
+        if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, l_p, l_cols, l_s );
       }
     };
     if constexpr( CHUNKS > 0 ) {
 #pragma unroll
       for( int l_c = 0; l_c < CHUNKS; l_c++ ) {
-        int64_t const l_i = int64_t( l_c * THREADS + l_t ) * V;
-        if( l_i < a.cols ) first( l_i, l_y[l_c] );
+        int32_t const l_i = ( l_c * THREADS + l_t ) * V - l_shift;
+        if( l_i < l_cols ) first( l_i, l_y[l_c] );
       }
     }
     else {
-      for( int64_t l_i = int64_t( l_t ) * V; l_i < a.cols; l_i += THREADS * V ) first( l_i, l_y[0] );
+      for( int32_t l_i = l_t * V - l_shift; l_i < l_cols; l_i += THREADS * V ) first( l_i, l_y[0] );
     }
 
 #pragma unroll
@@ -222,7 +250,8 @@ void quant_rows_kernel( QuantArgs a ) {
     if( !l_r.finite ) l_scale = __uint_as_float( 0x7fc00000u );
     if( l_t == 0 ) a.scale[l_row] = l_scale;
 
-    auto last = [&]( int64_t i, float const * y ) {
+    auto last = [&]( int32_t i, float const * y ) {
+      Place< V > const l_p( i, l_cols );
       float l_q[V];
       typename std::conditional< V == 8, uint64_t, uint32_t >::type l_bits = 0;
 #pragma unroll
@@ -230,31 +259,32 @@ void quant_rows_kernel( QuantArgs a ) {
         l_q[l_e] = l_r.q( y[l_e] );
         l_bits |= decltype( l_bits )( uint8_t( int( l_q[l_e] ) ) ) << ( 8 * l_e );
       }
-      int8_t * l_to = a.q + l_row * a.ld_q + i;
-      if( i + V <= a.cols ) *reinterpret_cast< typename Vec< T >::q * >( l_to ) = l_bits;
+      int8_t * l_to = a.q + l_row * a.ld_q + l_p.at;
+      if( l_p.whole( l_cols ) ) *reinterpret_cast< typename Vec< T >::q * >( l_to ) = l_bits;
       else {
 #pragma unroll
-        for( int l_e = 0; l_e < V; l_e++ ) if( i + l_e < a.cols ) l_to[l_e] = int8_t( l_bits >> ( 8 * l_e ) );
+        for( int l_e = 0; l_e < V; l_e++ ) if( l_p.has( l_e, l_cols ) ) l_to[l_e] = int8_t( l_bits >> ( 8 * l_e ) );
       }
       if( a.values ) {
 #pragma unroll
         for( int l_e = 0; l_e < V; l_e++ ) l_q[l_e] *= l_scale;
-        store_v( static_cast< T * >( a.values ) + l_row * a.ld_values, i, a.cols, l_q );
+        store_v( static_cast< T * >( a.values ) + l_row * a.ld_values, l_p, l_cols, l_q );
       }
     };
     if constexpr( CHUNKS > 0 ) {
 #pragma unroll
       for( int l_c = 0; l_c < CHUNKS; l_c++ ) {
-        int64_t const l_i = int64_t( l_c * THREADS + l_t ) * V;
-        if( l_i < a.cols ) last( l_i, l_y[l_c] );
+        int32_t const l_i = ( l_c * THREADS + l_t ) * V - l_shift;
+        if( l_i < l_cols ) last( l_i, l_y[l_c] );
       }
     }
     else {
-      for( int64_t l_i = int64_t( l_t ) * V; l_i < a.cols; l_i += THREADS * V ) {
+      for( int32_t l_i = l_t * V - l_shift; l_i < l_cols; l_i += THREADS * V ) {
         float l_s[V];
-        value( l_i, l_y[0], l_s );
+        Place< V > const l_p( l_i, l_cols );
+        value( l_p, l_y[0], l_s );
         if constexpr( NORM ) {
-          if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, l_i, a.cols, l_s );
+          if( a.total ) store_v( static_cast< T * >( a.total ) + l_row * a.ld_total, l_p, l_cols, l_s );
         }
         last( l_i, l_y[0] );
       }
@@ -265,24 +295,29 @@ void quant_rows_kernel( QuantArgs a ) {
 
 template< class T, bool NORM, int THREADS, int CHUNKS >
 void launch_shape( QuantArgs const & a, hipStream_t stream ) {
-  constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+  constexpr int ROWS = THREADS == 64 ? 4 : 1;
   // a grid's threads are counted in 32 bits, so workgroups loop over rows
   int64_t const l_grid = std::min< int64_t >( ( a.rows + ROWS - 1 ) / ROWS, 1 << 20 );
   hipLaunchKernelGGL( ( quant_rows_kernel< T, NORM, THREADS, CHUNKS > ), dim3( uint32_t( l_grid ) ),
-                      dim3( THREADS < 256 ? 256 : THREADS ), 0, stream, a );
+                      dim3( ROWS * THREADS ), 0, stream, a );
 }
 
 // Threads a row by its vectors of 16 bytes: a wave where one vector a lane
-// holds the row (no exchange between waves), else as few waves as hold it in
-// two vectors a lane.  1024 threads have 128 registers each: four vectors fit
-// them in fp32 (16 elements), not in bf16 (32).
+// holds the row (no exchange between waves), else few waves with two vectors a
+// lane, which leaves most of a compute unit's registers to other rows: 4072
+// rows of 256 vectors take 14.7 us so and 16.4 with one vector; 3000 of 126
+// take 10.7 with two vectors in a wave and 8.6 with one in two waves.
 template< class T, bool NORM >
 void launch_rows( QuantArgs const & a, hipStream_t stream ) {
-  int64_t const l_vecs = ( a.cols + Vec< T >::V - 1 ) / Vec< T >::V;
+  // a row of q that starts off a multiple of 4 bytes shifts its vectors
+  bool const l_even = reinterpret_cast< uintptr_t >( a.q ) % 4 == 0 && ( a.ld_q % 4 == 0 || a.rows == 1 );
+  int64_t const l_vecs = ( a.cols + ( l_even ? 0 : 3 ) + Vec< T >::V - 1 ) / Vec< T >::V;
   if( l_vecs <= 64 )        launch_shape< T, NORM, 64, 1 >( a, stream );
-  else if( l_vecs <= 256 )  launch_shape< T, NORM, 256, 1 >( a, stream );
+  else if( l_vecs <= 128 )  launch_shape< T, NORM, 128, 1 >( a, stream );
+  else if( l_vecs <= 256 )  launch_shape< T, NORM, 128, 2 >( a, stream );
   else if( l_vecs <= 512 )  launch_shape< T, NORM, 256, 2 >( a, stream );
   else if( l_vecs <= 1024 ) launch_shape< T, NORM, 512, 2 >( a, stream );
+  else if( l_vecs <= 1536 ) launch_shape< T, NORM, 768, 2 >( a, stream );
   else if( l_vecs <= 2048 ) launch_shape< T, NORM, 1024, 2 >( a, stream );
   else {
     if constexpr( Vec< T >::V == 4 ) {
