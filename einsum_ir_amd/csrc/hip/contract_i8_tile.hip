@@ -100,29 +100,27 @@ struct Side {
   }
 };
 
-// Stores 32 rows x COLS columns of a wave's slab from row m1, column n1 of the
-// output: 16 bytes a lane where the output's rows take them at multiples of 4
-// bytes, else an element a lane; non-temporal, the output is not read here
+// elements from row to row of a wave's output slab in LDS
+template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T ) );
+
+// Stores ROWS rows x COLS columns of a wave's slab from row m1, column n1 of
+// the output on: 16 bytes a lane where the output's rows take them at multiples
+// of 4 bytes, else an element a lane; non-temporal, the output is not read here
 // again (4072 x 2048 x 2048: 23.2 -> 21.2 us).
-template< int COLS, int PITCH, class T >
-__device__ inline void store_slab( TileArgs const & t, float const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
+template< int ROWS, int COLS, class T >
+__device__ inline void store_slab( TileArgs const & t, T const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
   I8Args const & a = t.a;
   constexpr int V = 16 / sizeof( T );
   constexpr int LANES = COLS / V;            // lanes a row
+  constexpr int PITCH = kPitch< T, COLS >;
   typedef T v __attribute__( ( ext_vector_type( V ) ) );
   typedef v v_dword __attribute__( ( aligned( 4 ) ) );
   T * const l_out = static_cast< T * >( a.out ) + out0;
   if( t.vec_out ) {
 #pragma unroll
-    for( int l_p = 0; l_p < 32 * LANES / 64; l_p++ ) {
+    for( int l_p = 0; l_p < ROWS * LANES / 64; l_p++ ) {
       int const l_r = l_p * ( 64 / LANES ) + lane / LANES, l_c = lane % LANES * V;
-      v l_v;
-#pragma unroll
-      for( int l_e = 0; l_e < V; l_e += 4 ) {
-        f32x4 const l_f = *reinterpret_cast< f32x4 const * >( slab + l_r * PITCH + l_c + l_e );
-#pragma unroll
-        for( int l_d = 0; l_d < 4; l_d++ ) l_v[l_e + l_d] = static_cast< T >( l_f[l_d] );
-      }
+      v const l_v = *reinterpret_cast< v const * >( slab + l_r * PITCH + l_c );
       if( m1 + l_r >= a.M ) continue;
       T * const l_o = l_out + ( m1 + l_r ) * a.o_row + n1 + l_c;
       if( n1 + l_c + V <= a.N ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_dword * >( l_o ) );
@@ -134,23 +132,26 @@ __device__ inline void store_slab( TileArgs const & t, float const * slab, int64
   }
   else {
 #pragma unroll 4
-    for( int l_p = 0; l_p < 32 * COLS / 64; l_p++ ) {
+    for( int l_p = 0; l_p < ROWS * COLS / 64; l_p++ ) {
       int const l_r = ( l_p * 64 + lane ) / COLS, l_c = ( l_p * 64 + lane ) % COLS;
-      T const l_v = static_cast< T >( slab[l_r * PITCH + l_c] );
+      T const l_v = slab[l_r * PITCH + l_c];
       if( m1 + l_r < a.M && n1 + l_c < a.N ) l_out[( m1 + l_r ) * a.o_row + ( n1 + l_c ) * a.o_col] = l_v;
     }
   }
 }
 
-template< int BM, int BN, int WM, int WN, int KG, int STAGES, int LOAD >
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
 __global__ __launch_bounds__( 64 * WM * WN * KG )
 void contract_i8_tile_kernel( TileArgs t ) {
   constexpr bool DMA = LOAD == LOAD_DMA;
   constexpr int WAVES = WM * WN;                       // of a K group
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks a wave
   constexpr int STAGE = ( BM + BN ) * kBk;
-  constexpr int PITCH = BN / WN + 4;                   // output slab: floats a row
-  constexpr int SLABS = WAVES * 32 * PITCH * 4;
+  constexpr int COLS = BN / WN;
+  // a wave's output slab: fp32 32 rows, bf16 all of its rows
+  constexpr int SLAB_F32 = 32 * kPitch< float, COLS > * 4, SLAB_BF16 = 32 * TM * kPitch< __bf16, COLS > * 2;
+  constexpr int SLAB = SLAB_F32 > SLAB_BF16 ? SLAB_F32 : SLAB_BF16;
+  constexpr int SLABS = WAVES * SLAB;
   constexpr int PARTS = KG > 1 ? ( KG - 1 ) * BM * BN * 4 : 0;
   constexpr int BYTES = STAGES * KG * STAGE > SLABS + PARTS ? STAGES * KG * STAGE : SLABS + PARTS;
   __shared__ __align__( 16 ) char l_lds[BYTES];
@@ -228,6 +229,10 @@ void contract_i8_tile_kernel( TileArgs t ) {
       constexpr int l_s = decltype( sc )::value + 1;
       kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, l_s, k_of_step( l_s ) ); } );
     } );
+    if constexpr( !DEEP ) {
+      kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+      kern::barrier_lds();
+    }
   }
   else if constexpr( DMA ) {
     kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
@@ -237,14 +242,13 @@ void contract_i8_tile_kernel( TileArgs t ) {
   else {
     put( 0, k_of_step( 0 ) );
     kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
-    put( 1, k_of_step( 1 ) );
     kern::wait_lgkmcnt0();
     kern::barrier_lds();
   }
 
   // Fragments of 32 k: TM of rows, then TN of columns.
   constexpr int FRAGS = TM + TN, MFMAS = TM * TN;
-  constexpr int HELD = STAGES > 2 ? 4 : 2;
+  constexpr int HELD = DEEP ? 4 : 2;
   i32x4 l_f[HELD][FRAGS];
   uint32_t const l_swz = kern::swz_k( l_row );       // of 32-row blocks: the same
   auto read = [&]( auto fc, i32x4 * f, int stage, int q ) __attribute__( ( always_inline ) ) {
@@ -266,17 +270,16 @@ void contract_i8_tile_kernel( TileArgs t ) {
   // part, when every wave has read all of this block and the next one has
   // landed, and the block after that is loaded over this one from there on,
   // half of it in the last part, half in the next block's first.
-  auto step = [&]( auto stage_c, int s ) __attribute__( ( always_inline ) ) {
-    constexpr int l_st = decltype( stage_c )::value;
+  auto step = [&]( int l_st, int l_next, int l_free, int s ) __attribute__( ( always_inline ) ) {
     kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
       constexpr int l_q = decltype( qc )::value;
       if constexpr( l_q == 3 ) {
-        if constexpr( DMA ) kern::wait_vmcnt< 0 >();
+        if constexpr( DMA ) kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+        else                put( l_next, k_of_step( s + 1 ) );
         kern::wait_lgkmcnt0();
         kern::barrier_lds();
       }
-      int32_t const l_k0 = k_of_step( s + ( l_q == 3 || !DMA ? 2 : 1 ) );
-      if constexpr( !DMA && l_q == 3 ) put( l_st, l_k0 );
+      int32_t const l_k0 = k_of_step( s + ( STAGES > 2 ? STAGES - 1 : l_q == 3 ? 2 : 1 ) );
       kern::static_for< MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) {
         constexpr int l_m = decltype( mc )::value;
         multiply( mc, l_f[l_q % 2] );
@@ -286,17 +289,23 @@ void contract_i8_tile_kernel( TileArgs t ) {
           constexpr int l_from = FRAGS * l_m / l_slots, l_to = FRAGS * ( l_m + 1 ) / l_slots;
           kern::static_for< l_to - l_from >( [&]( auto fc ) __attribute__( ( always_inline ) ) {
             read( std::integral_constant< int, l_from + decltype( fc )::value >(), l_f[( l_q + 1 ) % 2],
-                  l_q == 3 ? 1 - l_st : l_st, ( l_q + 1 ) % 4 );
+                  l_q == 3 ? l_next : l_st, ( l_q + 1 ) % 4 );
           } );
         }
-        if constexpr( DMA && ( l_q == 3 || l_q == 0 ) ) {
+        if constexpr( STAGES > 2 && l_q < 3 ) {
+          constexpr int l_at = l_q * MFMAS + l_m, l_from = EACH * l_at / ( 3 * MFMAS ), l_to = EACH * ( l_at + 1 ) / ( 3 * MFMAS );
+          kern::static_for< l_to - l_from >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
+            issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_free, l_k0 );
+          } );
+        }
+        if constexpr( STAGES == 2 && DMA && ( l_q == 3 || l_q == 0 ) ) {
           constexpr int l_p0 = l_q == 3 ? 0 : EARLY, l_n = l_q == 3 ? EARLY : EACH - EARLY;
           constexpr int l_from = l_p0 + l_n * l_m / MFMAS, l_to = l_p0 + l_n * ( l_m + 1 ) / MFMAS;
           kern::static_for< l_to - l_from >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
-            issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_q == 3 ? l_st : 1 - l_st, l_k0 );
+            issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_q == 3 ? l_st : l_next, l_k0 );
           } );
         }
-        if constexpr( !DMA && l_q == 0 && l_m == 0 ) {
+        if constexpr( !DMA && l_q == 3 && l_m == 0 ) {
           kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, l_k0 ); } );
         }
         __builtin_amdgcn_sched_barrier( 0 );
@@ -327,11 +336,14 @@ void contract_i8_tile_kernel( TileArgs t ) {
       multiply( std::integral_constant< int, l_m % MFMAS >(), l_f[l_m / MFMAS % HELD] );
     } );
   };
-  if constexpr( STAGES == 2 ) {
+  if constexpr( !DEEP ) {
     kern::static_for< FRAGS >( [&]( auto fc ) __attribute__( ( always_inline ) ) { read( fc, l_f[0], 0, 0 ); } );
-    for( int l_s = 0; l_s < l_steps; l_s += 2 ) {
-      step( std::integral_constant< int, 0 >(), l_s );
-      if( l_s + 1 < l_steps ) step( std::integral_constant< int, 1 >(), l_s + 1 );
+    int l_st = 0, l_free = STAGES - 1;
+    for( int l_s = 0; l_s < l_steps; l_s++ ) {
+      int const l_next = l_st == STAGES - 1 ? 0 : l_st + 1;
+      step( l_st, l_next, l_free, l_s );
+      l_free = l_st;
+      l_st = l_next;
     }
   }
   else {
@@ -377,45 +389,58 @@ void contract_i8_tile_kernel( TileArgs t ) {
     }
   }
 
-  // 32 rows at a time through this wave's slab
-  float * const l_slab = reinterpret_cast< float * >( l_lds ) + l_wave * 32 * PITCH;
+  // PASS blocks of 32 rows at a time through this wave's slab
   int64_t const l_out0 = l_c * a.c[I8_OUT];
+  auto finish = [&]( auto zero, auto pass ) __attribute__( ( always_inline ) ) {
+    typedef decltype( zero ) T;
+    typedef T t4 __attribute__( ( ext_vector_type( 4 ) ) );
+    constexpr int PASS = decltype( pass )::value;
+    T * const l_slab = reinterpret_cast< T * >( l_lds + l_wave * SLAB );
 #pragma unroll
-  for( int l_j = 0; l_j < TM; l_j++ ) {
+    for( int l_j0 = 0; l_j0 < TM; l_j0 += PASS ) {
 #pragma unroll
-    for( int l_i = 0; l_i < TN; l_i++ ) {
+      for( int l_i = 0; l_i < TN; l_i++ ) {
 #pragma unroll
-      for( int l_q = 0; l_q < 4; l_q++ ) {
-        int const l_n = 32 * l_i + 8 * l_q + 4 * ( l_lane / 32 );
-        f32x4 const l_sb4 = *reinterpret_cast< f32x4 const * >( l_sb + l_wn + l_n );
-        f32x4 l_b4 = *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
-        if( a.bias_row != 0 ) l_b4 = f32x4{ l_bias_m[l_j], l_bias_m[l_j], l_bias_m[l_j], l_bias_m[l_j] };
-        f32x4 l_v;
+        for( int l_q = 0; l_q < 4; l_q++ ) {
+          int const l_n = 32 * l_i + 8 * l_q + 4 * ( l_lane / 32 );
+          f32x4 const l_sb4 = *reinterpret_cast< f32x4 const * >( l_sb + l_wn + l_n );
+          f32x4 l_b4 = { 0.0f, 0.0f, 0.0f, 0.0f };
+          if( a.bias ) l_b4 = *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
 #pragma unroll
-        for( int l_e = 0; l_e < 4; l_e++ ) {
-          l_v[l_e] = i8_finish( l_acc[l_i][l_j][4 * l_q + l_e], l_sa[l_j], l_sb4[l_e], l_b4[l_e], a.relu );
+          for( int l_j = l_j0; l_j < l_j0 + PASS; l_j++ ) {
+            float l_v[4];
+#pragma unroll
+            for( int l_e = 0; l_e < 4; l_e++ ) {
+              l_v[l_e] = i8_finish( l_acc[l_i][l_j][4 * l_q + l_e], l_sa[l_j], l_sb4[l_e],
+                                    a.bias_row != 0 ? l_bias_m[l_j] : l_b4[l_e], 0 );
+            }
+            if( a.relu ) {
+#pragma unroll
+              for( int l_e = 0; l_e < 4; l_e++ ) l_v[l_e] = l_v[l_e] < 0.0f ? 0.0f : l_v[l_e];
+            }
+            *reinterpret_cast< t4 * >( l_slab + ( 32 * ( l_j - l_j0 ) + l_row ) * kPitch< T, COLS > + l_n )
+                = t4{ static_cast< T >( l_v[0] ), static_cast< T >( l_v[1] ), static_cast< T >( l_v[2] ), static_cast< T >( l_v[3] ) };
+          }
         }
-        *reinterpret_cast< f32x4 * >( l_slab + l_row * PITCH + l_n ) = l_v;
       }
+      // the slab is this wave's own, and its LDS operations are in order
+      __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
+      store_slab< 32 * PASS, COLS, T >( t, l_slab, l_out0, l_m0 + l_wm + 32 * l_j0, l_n0 + l_wn, l_lane );
+      __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
     }
-    // the slab is this wave's own, and its LDS operations are in order
-    __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
-    constexpr int COLS = BN / WN;
-    int32_t const l_n1 = l_n0 + l_wn, l_m1 = l_m0 + l_wm + 32 * l_j;
-    if( a.out_bf16 ) store_slab< COLS, PITCH, __bf16 >( t, l_slab, l_out0, l_m1, l_n1, l_lane );
-    else             store_slab< COLS, PITCH, float >( t, l_slab, l_out0, l_m1, l_n1, l_lane );
-    __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
-  }
+  };
+  if( a.out_bf16 ) finish( __bf16( 0.0f ), std::integral_constant< int, TM >() );
+  else             finish( 0.0f, std::integral_constant< int, 1 >() );
 }
 
-template< int BM, int BN, int WM, int WN, int KG, int STAGES, int LOAD >
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
 int launch_shape( TileArgs t, hipStream_t stream ) {
   I8Args const & a = t.a;
   t.tiles_m = ( a.M + BM - 1 ) / BM;
   t.tiles_n = ( a.N + BN - 1 ) / BN;
   t.blocks = ( a.K + kBk - 1 ) / kBk;
   uint32_t const l_grid = uint32_t( int64_t( t.tiles_m ) * t.tiles_n * a.C );
-  hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, LOAD > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
+  hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, DEEP, LOAD > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
                       0, stream, t );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
@@ -433,24 +458,25 @@ int launch_i8_tile( I8Args const & a, I8Kernel kernel, hipStream_t stream ) {
   t.vec_out = a.o_col == 1 && uintptr_t( a.out ) % 4 == 0 && a.o_row * l_item % 4 == 0 && a.c[I8_OUT] * l_item % 4 == 0;
   bool const l_dwords = i8_aligned( a, 4 );
   switch( kernel ) {
-    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, true, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, true, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_128x64:  return launch_shape< 128, 64, 2, 2, 1, 3, false, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, false, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, false, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, false, LOAD_DMA >( t, stream );
     case I8Kernel::REG_32x32:
-      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 32, 32, 1, 1, 4, 2, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_BYTES >( t, stream );
     case I8Kernel::REG_64x64:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 64, 64, 2, 2, 1, 2, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_BYTES >( t, stream );
     case I8Kernel::REG_64x64_K2:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 64, 64, 2, 2, 2, 2, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_BYTES >( t, stream );
     case I8Kernel::REG_128x128:
-      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 128, 128, 2, 2, 1, 2, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_DWORDS >( t, stream )
+                      : launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_BYTES >( t, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction_i8: unknown tile" );
   }
 }

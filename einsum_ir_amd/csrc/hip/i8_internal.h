@@ -70,6 +70,7 @@ enum class I8Kernel : int32_t {
   TILE_32x32,
   TILE_64x32,
   TILE_64x64,
+  TILE_128x64,
   TILE_128x128,
   TILE_256x128,
   TILE_256x256,

@@ -90,6 +90,7 @@ Candidate const kCandidates[] = {
   { I8Kernel::TILE_32x32,   "tile 32x32",   16, 32,  32,  256, 512,  2.1f, 0.34f },
   { I8Kernel::TILE_64x32,   "tile 64x32",   16, 64,  32,  256, 256,  2.0f, 0.28f },
   { I8Kernel::TILE_64x64,   "tile 64x64",   16, 64,  64,  256, 128,  1.4f, 0.23f },
+  { I8Kernel::TILE_128x64,  "tile 128x64",  16, 128, 64,  256, 128,  2.3f, 0.34f },
   { I8Kernel::TILE_128x128, "tile 128x128", 16, 128, 128, 512, 128,  3.2f, 0.44f },
   { I8Kernel::TILE_256x128, "tile 256x128", 16, 256, 128, 512, 128,  5.1f, 0.72f },
   { I8Kernel::TILE_256x256, "tile 256x256", 16, 256, 256, 512, 128,  8.4f, 1.09f },
