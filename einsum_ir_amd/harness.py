@@ -5,6 +5,7 @@
     python -m einsum_ir_amd.harness expression einsum_string dimension_sizes contraction_path
                                                [dtype [store_lock [print_tree]]]
     python -m einsum_ir_amd.harness tree       einsum_tree dimension_sizes [dtype]
+    python -m einsum_ir_amd.harness mlp_i8     tokens,width,hidden,blocks,classes [activation [dtype]]
 
 Arguments and printed reports follow the reference's bench_binary
 (reference src/bench_binary.cpp:212-408), bench_unary (src/bench_unary.cpp:55-336),
@@ -19,6 +20,11 @@ times are device times of the HIP stream (one warm-up, then repetitions for
 ~0.2 s; the reference times one evaluation on the host clock); the loop order
 of bench_binary is accepted and ignored (one kernel grid runs every loop);
 print_tree is not provided.
+
+mlp_i8 has no counterpart in the reference: a residual MLP answered in 8 bits
+(einsum_ir_amd.mlp_i8; activation RELU, SILU or GATED_SILU, dtype BF16 or FP32),
+randn inputs and weights, compared with the same network in float64 without any
+rounding to 8 bits.
 """
 import re
 import sys
@@ -406,10 +412,62 @@ def bench_tree(argv):
     return 0 if ok else 1
 
 
+def mlp_float64(torch, blocks, norm, head, x, act, gated, eps=1e-6):
+    """The network of einsum_ir_amd.mlp_i8 in float64, nothing rounded to 8 bits."""
+    f = {"RELU": torch.relu, "SILU": torch.nn.functional.silu}[act]
+    rms = lambda v, w: v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) * w.double()  # noqa: E731
+    x = x.double()
+    for b in blocks:
+        h = rms(x, b["norm"]) @ b["up"].double().T.contiguous()
+        if gated:
+            g, h = h.chunk(2, dim=1)
+            h = f(g) * h
+        else:
+            h = f(h)
+        x = x + h @ b["down"].double().T.contiguous()
+    return rms(x, norm) @ head.double().T.contiguous()
+
+
+def bench_mlp_i8(argv):
+    import torch
+    from .mlp_i8 import MlpI8
+    sizes = [int(v) for v in argv[0].split(",")]
+    act = argv[1] if len(argv) > 1 else "RELU"
+    dtype = argv[2] if len(argv) > 2 else "BF16"
+    if len(sizes) != 5 or act not in ("RELU", "SILU", "GATED_SILU") or dtype not in ("BF16", "FP32"):
+        print("five sizes, activation RELU, SILU or GATED_SILU, dtype BF16 or FP32 expected", file=sys.stderr)
+        return 1
+    tokens, width, hidden, num, classes = sizes
+    gated, act = act.startswith("GATED_"), act.replace("GATED_", "")
+    td = _torch_dtype(torch, dtype)
+    rand = lambda o, i: (torch.randn(o, i, device="cuda") / i ** 0.5).to(td)  # noqa: E731
+    blocks = [dict(norm=torch.ones(width, device="cuda"), up=rand(hidden * (2 if gated else 1), width),
+                   down=rand(width, hidden)) for _ in range(num)]
+    norm, head = torch.ones(width, device="cuda"), rand(classes, width)
+    x = torch.randn(tokens, width, device="cuda").to(td)
+    t0 = time.perf_counter()
+    net = MlpI8(blocks, norm, head, dtype=_DT[dtype], ktype={"RELU": _lib.RELU, "SILU": _lib.SILU}[act], gated=gated)
+    net(x)
+    torch.cuda.synchronize()
+    t_compile = time.perf_counter() - t0
+    t = _timed(torch, lambda: net(x))
+    flops = net.num_ops(tokens)
+    ref = mlp_float64(torch, blocks, norm, head, x, act, gated)
+    err = float((net(x).double() - ref).norm() / ref.norm())
+    print("einsum_ir:")
+    print(f"  #ops:           {flops}")
+    print(f"  time (compile): {t_compile}")
+    print(f"  time (eval):    {t}")
+    print(f"  gops (eval):    {flops / t * 1e-9}")
+    print(f"  error (float64, nothing rounded to 8 bits): {err}")
+    print(f"CSV_DATA: einsum_ir,\"mlp_i8\",\"{argv[0]}\",{flops},{t_compile},{t},{flops / t * 1e-9},{err}")
+    return 0 if err < 0.1 else 1
+
+
 def main(argv=None):
     argv = list(sys.argv[1:] if argv is None else argv)
     cmds = {"binary": (bench_binary, 2), "unary": (bench_unary, 2), "expression": (bench_expression, 3),
-            "tree": (bench_tree, 2)}
+            "tree": (bench_tree, 2), "mlp_i8": (bench_mlp_i8, 1)}
     if not argv or argv[0] not in cmds or len(argv) - 1 < cmds[argv[0]][1]:
         print(__doc__, file=sys.stderr)
         return 1

@@ -1,0 +1,131 @@
+"""A residual multi-layer perceptron answered in 8 bits, from the 8-bit layer
+operators (NormQuantPlan, ContractionI8Plan, ActQuantPlan).  No counterpart in
+the reference, whose bench_mlp (reference src/bench_mlp.cpp:85-307) runs its
+layers in fp32.
+
+    x += delta                      norm_quant: the residual's addition,
+    n  = rms_norm(x) * norm                     the norm and its 8-bit rows
+    h  = n up^T + up_bias           contraction_i8
+    a  = f(h), or f(gate) * h       act_quant, 8-bit rows
+    delta = a down^T + down_bias    contraction_i8
+
+for each block, then a last norm and the product with the head's weights.  Every
+product reads 8-bit rows with a scale for each token and 8-bit weights with a
+scale for each channel; the hidden states between are bf16 or fp32.
+"""
+
+from . import ActQuantPlan, BF16, ContractionI8Plan, FP32, NormQuantPlan, RELU, contraction_i8_loops
+
+
+class LinearI8:
+    """Weights [channels, width] laid out once as 8-bit rows with a scale a channel."""
+
+    def __init__(self, torch, weight, bias=None, stream=None):
+        if weight.dim() != 2 or weight.dtype not in (torch.bfloat16, torch.float32) or not weight.is_cuda:
+            raise ValueError("weights are [channels, width] tensors of bf16 or fp32 on the GPU")
+        if bias is not None and (tuple(bias.shape) != (weight.shape[0],) or bias.dtype != torch.float32
+                                 or not bias.is_cuda):
+            raise ValueError("a bias holds one fp32 value a channel, on the GPU")
+        weight = weight.contiguous()
+        self.channels, self.width = weight.shape
+        self.q = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
+        self.scale = torch.empty(self.channels, device=weight.device)
+        self.bias = None if bias is None else bias.contiguous()
+        plan = ActQuantPlan(self.channels, self.width, dtype=BF16 if weight.dtype == torch.bfloat16 else FP32)
+        plan.execute(weight, self.q, self.scale, stream=stream)
+
+    def plan(self, tokens, dtype):
+        """The product of this layer with 8-bit rows of so many tokens."""
+        return ContractionI8Plan(**contraction_i8_loops(
+            "tk,ok->to", dict(t=tokens, k=self.width, o=self.channels), scale_left="t", scale_right="o",
+            bias=None if self.bias is None else "o"), dtype_out=dtype)
+
+
+class MlpI8:
+    """blocks: dicts of the tensors ``norm`` [width], ``up`` [hidden, width] (gated: [2 hidden, width], the gates'
+    rows first), ``down`` [width, hidden] and, where there are such, ``up_bias`` and ``down_bias``; ``norm`` [width] and
+    ``head`` [classes, width] end the network.  Weights are bf16 or fp32 and rounded to 8 bits here; norms have the
+    type of the hidden states (dtype), biases fp32.  ktype: UNDEFINED_KTYPE, RELU or SILU.
+
+    Calls enqueue on the given stream (None: torch's current one when they are made).  A first call with a number of
+    tokens makes its plans and buffers; later ones allocate nothing and can be captured.  The logits are a buffer of
+    this object, written by the next call with as many tokens."""
+
+    def __init__(self, blocks, norm, head, dtype=BF16, ktype=RELU, gated=False, eps=1e-6, stream=None):
+        import torch
+        if dtype not in (BF16, FP32):
+            raise ValueError("hidden states are BF16 or FP32")
+        self._torch, self.dtype, self.ktype, self.gated, self.eps, self.stream = torch, dtype, ktype, gated, eps, stream
+        s, td = self._stream(), self._torch_dtype()
+        with torch.cuda.stream(s):
+            self.blocks = [dict(norm=b["norm"].to(td).contiguous(),
+                                up=LinearI8(torch, b["up"], b.get("up_bias"), s),
+                                down=LinearI8(torch, b["down"], b.get("down_bias"), s)) for b in blocks]
+            self.norm = norm.to(td).contiguous()
+            self.head = LinearI8(torch, head, None, s)
+        self.width = self.head.width
+        for b in self.blocks:
+            hidden = b["up"].channels // (2 if gated else 1)
+            if (b["up"].width != self.width or b["down"].channels != self.width or b["down"].width != hidden
+                    or b["norm"].numel() != self.width or (gated and b["up"].channels % 2)):
+                raise ValueError("the blocks' tensors do not fit each other")
+        if self.norm.numel() != self.width:
+            raise ValueError("the last norm does not fit the head")
+        self._by_tokens = {}
+
+    def _stream(self):
+        return self.stream if self.stream is not None else self._torch.cuda.current_stream()
+
+    def _torch_dtype(self):
+        return self._torch.bfloat16 if self.dtype == BF16 else self._torch.float32
+
+    def _prepare(self, tokens):
+        torch, td = self._torch, self._torch_dtype()
+        dev = self.head.q.device
+        empty = lambda *shape, **kw: torch.empty(shape, device=dev, **kw)  # noqa: E731
+        wide = max([b["down"].width for b in self.blocks], default=0)
+        p = dict(norm=NormQuantPlan(tokens, self.width, dtype=self.dtype, eps=self.eps),
+                 q=empty(tokens, self.width, dtype=torch.int8), q_scale=empty(tokens),
+                 a=empty(tokens * wide, dtype=torch.int8), a_scale=empty(tokens),
+                 h=empty(tokens * wide * (2 if self.gated else 1), dtype=td),
+                 total=empty(tokens, self.width, dtype=td), delta=empty(tokens, self.width, dtype=td),
+                 logits=empty(tokens, self.head.channels, dtype=td), head=self.head.plan(tokens, self.dtype), blocks=[])
+        for b in self.blocks:
+            f, n = b["down"].width, b["up"].channels
+            p["blocks"].append((b["up"].plan(tokens, self.dtype),
+                                ActQuantPlan(tokens, f, dtype=self.dtype, ktype=self.ktype, ld_in=n, ld_gate=n),
+                                b["down"].plan(tokens, self.dtype)))
+        return p
+
+    def __call__(self, x):
+        """Logits [tokens, classes] of hidden states x [tokens, width]."""
+        torch, td = self._torch, self._torch_dtype()
+        if x.dim() != 2 or x.shape[1] != self.width or x.dtype != td or not x.is_cuda or not x.is_contiguous():
+            raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {td} on the GPU")
+        tokens = x.shape[0]
+        p = self._by_tokens.get(tokens)
+        if p is None:
+            p = self._by_tokens[tokens] = self._prepare(tokens)
+        s = self._stream()
+        state, delta = x, None
+        for b, (up, act, down) in zip(self.blocks, p["blocks"]):
+            p["norm"].execute(state, p["q"], p["q_scale"], residual=delta, weight=b["norm"],
+                              total=None if delta is None else p["total"], stream=s)
+            up.execute(p["q"], b["up"].q, p["h"], scale_left=p["q_scale"], scale_right=b["up"].scale,
+                       bias=b["up"].bias, stream=s)
+            f = b["down"].width
+            act.execute(p["h"][f:] if self.gated else p["h"], p["a"], p["a_scale"],
+                        gate=p["h"] if self.gated else None, stream=s)
+            if delta is not None:
+                state = p["total"]
+            down.execute(p["a"], b["down"].q, p["delta"], scale_left=p["a_scale"], scale_right=b["down"].scale,
+                         bias=b["down"].bias, stream=s)
+            delta = p["delta"]
+        p["norm"].execute(state, p["q"], p["q_scale"], residual=delta, weight=self.norm, stream=s)
+        p["head"].execute(p["q"], self.head.q, p["logits"], scale_left=p["q_scale"], scale_right=self.head.scale, stream=s)
+        return p["logits"]
+
+    def num_ops(self, tokens):
+        """Operations of the products of one call."""
+        per = sum(b[k].channels * b[k].width for b in self.blocks for k in ("up", "down"))
+        return 2 * tokens * (per + self.head.channels * self.head.width)
