@@ -21,9 +21,7 @@ from .loops import binary_loops, contraction_i8_loops, unary_dims, dim_types, ro
 
 def _ptr(x):
     """Device pointer of a torch tensor, an int, or None."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
     return x.data_ptr()
 
@@ -123,10 +121,13 @@ class ContractionI8Plan(_Plan):
             _lib.i64_array(strides_right), opt(strides_scale_left), opt(strides_scale_right), opt(strides_bias),
             _lib.i64_array(strides_out), dtype_out, ktype_last_touch, ctypes.byref(self._handle)))
 
+        self._execute = hip_lib().etir_hip_contraction_i8_execute
+
     def execute(self, left, right, out, scale_left=None, scale_right=None, bias=None, stream=None):
-        check(hip_lib().etir_hip_contraction_i8_execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left),
-                                                        _ptr(scale_right), _ptr(bias), _ptr(out),
-                                                        _stream_ptr(stream)))
+        err = self._execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left), _ptr(scale_right), _ptr(bias),
+                            _ptr(out), _stream_ptr(stream))
+        if err:
+            check(err)
 
 
 class NormQuantPlan(_Plan):
@@ -141,9 +142,13 @@ class NormQuantPlan(_Plan):
         check(hip_lib().etir_hip_norm_quant_create(rows, cols, *ld, dtype, dtype if dtype_weight is None else dtype_weight,
                                                    eps, ctypes.byref(self._handle)))
 
+        self._execute = hip_lib().etir_hip_norm_quant_execute
+
     def execute(self, x, q, scale, residual=None, weight=None, total=None, values=None, stream=None):
-        check(hip_lib().etir_hip_norm_quant_execute(self._handle, _ptr(x), _ptr(residual), _ptr(weight), _ptr(total),
-                                                    _ptr(q), _ptr(scale), _ptr(values), _stream_ptr(stream)))
+        err = self._execute(self._handle, _ptr(x), _ptr(residual), _ptr(weight), _ptr(total), _ptr(q), _ptr(scale),
+                            _ptr(values), _stream_ptr(stream))
+        if err:
+            check(err)
 
 
 class ActQuantPlan(_Plan):
@@ -157,9 +162,13 @@ class ActQuantPlan(_Plan):
         ld = [cols if v is None else v for v in (ld_in, ld_gate, ld_q, ld_values)]
         check(hip_lib().etir_hip_act_quant_create(rows, cols, *ld, dtype, ktype, ctypes.byref(self._handle)))
 
+        self._execute = hip_lib().etir_hip_act_quant_execute
+
     def execute(self, x, q, scale, gate=None, values=None, stream=None):
-        check(hip_lib().etir_hip_act_quant_execute(self._handle, _ptr(x), _ptr(gate), _ptr(q), _ptr(scale),
-                                                   _ptr(values), _stream_ptr(stream)))
+        err = self._execute(self._handle, _ptr(x), _ptr(gate), _ptr(q), _ptr(scale), _ptr(values),
+                            _stream_ptr(stream))
+        if err:
+            check(err)
 
 
 def synchronize(stream=None):

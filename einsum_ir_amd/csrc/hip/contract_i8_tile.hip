@@ -35,13 +35,6 @@ enum Load : int {
   LOAD_BYTES  = 2     // through registers: anywhere
 };
 
-struct TileArgs {
-  I8Args a;
-  int32_t tiles_m, tiles_n;
-  int32_t blocks;             // blocks of 128 k
-  int32_t vec_out;            // output rows take 16-byte stores
-};
-
 // ROWS rows of an operand by WAVES waves, one K group's side of the tile
 template< int ROWS, int WAVES, int LOAD >
 struct Side {
@@ -57,7 +50,7 @@ struct Side {
   int      m_k[2];                      // the lane's k of a block in even and odd pieces
   uint32_t m_first;                     // the wave's first piece
 
-  __device__ inline void init( int8_t const * tile, int64_t stride, int32_t rows, int wave, int lane ) {
+  __device__ inline void init( int8_t const * tile, int32_t stride, int32_t rows, int wave, int lane ) {
     m_first = wave * EACH;
     if constexpr( DMA ) m_rsrc = kern::make_rsrc( tile, kern::kDmaOob );
 #pragma unroll
@@ -66,8 +59,8 @@ struct Side {
     for( int l_i = 0; l_i < EACH; l_i++ ) {
       // rows past the tensor read its last one and are not stored
       int32_t const l_r = min( int32_t( 8 * ( m_first + l_i ) + lane / 8 ), rows - 1 );
-      if constexpr( DMA ) m_off[l_i] = uint32_t( l_r * int32_t( stride ) + k_of( l_i ) );
-      else                m_row[l_i] = tile + l_r * stride;
+      if constexpr( DMA ) m_off[l_i] = uint32_t( l_r * stride + k_of( l_i ) );
+      else                m_row[l_i] = tile + int64_t( l_r ) * stride;
     }
   }
   __device__ inline int k_of( int i ) const { return m_k[( m_first + i ) % 2]; }
@@ -108,21 +101,20 @@ template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T 
 // of 4 bytes, else an element a lane; non-temporal, the output is not read here
 // again (4072 x 2048 x 2048: 23.2 -> 21.2 us).
 template< int ROWS, int COLS, class T >
-__device__ inline void store_slab( TileArgs const & t, T const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
-  I8Args const & a = t.a;
+__device__ inline void store_slab( I8Args const & a, T const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
   constexpr int V = 16 / sizeof( T );
   constexpr int LANES = COLS / V;            // lanes a row
   constexpr int PITCH = kPitch< T, COLS >;
   typedef T v __attribute__( ( ext_vector_type( V ) ) );
   typedef v v_dword __attribute__( ( aligned( 4 ) ) );
   T * const l_out = static_cast< T * >( a.out ) + out0;
-  if( t.vec_out ) {
+  if( a.has( I8Args::VEC_OUT ) ) {
 #pragma unroll
     for( int l_p = 0; l_p < ROWS * LANES / 64; l_p++ ) {
       int const l_r = l_p * ( 64 / LANES ) + lane / LANES, l_c = lane % LANES * V;
       v const l_v = *reinterpret_cast< v const * >( slab + l_r * PITCH + l_c );
       if( m1 + l_r >= a.M ) continue;
-      T * const l_o = l_out + ( m1 + l_r ) * a.o_row + n1 + l_c;
+      T * const l_o = l_out + int64_t( m1 + l_r ) * a.o_row + n1 + l_c;
       if( n1 + l_c + V <= a.N ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_dword * >( l_o ) );
       else {
 #pragma unroll
@@ -135,14 +127,14 @@ __device__ inline void store_slab( TileArgs const & t, T const * slab, int64_t o
     for( int l_p = 0; l_p < ROWS * COLS / 64; l_p++ ) {
       int const l_r = ( l_p * 64 + lane ) / COLS, l_c = ( l_p * 64 + lane ) % COLS;
       T const l_v = slab[l_r * PITCH + l_c];
-      if( m1 + l_r < a.M && n1 + l_c < a.N ) l_out[( m1 + l_r ) * a.o_row + ( n1 + l_c ) * a.o_col] = l_v;
+      if( m1 + l_r < a.M && n1 + l_c < a.N ) l_out[int64_t( m1 + l_r ) * a.o_row + int64_t( n1 + l_c ) * a.o_col] = l_v;
     }
   }
 }
 
 template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
 __global__ __launch_bounds__( 64 * WM * WN * KG )
-void contract_i8_tile_kernel( TileArgs t ) {
+void contract_i8_tile_kernel( I8Args a ) {
   constexpr bool DMA = LOAD == LOAD_DMA;
   constexpr int WAVES = WM * WN;                       // of a K group
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks a wave
@@ -157,7 +149,9 @@ void contract_i8_tile_kernel( TileArgs t ) {
   __shared__ __align__( 16 ) char l_lds[BYTES];
   __shared__ __align__( 16 ) float l_sb[BN], l_bias[BN];
 
-  I8Args const & a = t.a;
+  int32_t const l_k = a.K();
+  int32_t const l_blocks = ( l_k + kBk - 1 ) / kBk;
+  int32_t const l_tiles_m = ( a.M + BM - 1 ) / BM, l_tiles_n = ( a.N + BN - 1 ) / BN;
   int const l_lane = threadIdx.x % 64;
   int const l_w = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
   int const l_group = l_w / WAVES, l_wave = l_w % WAVES;
@@ -165,60 +159,59 @@ void contract_i8_tile_kernel( TileArgs t ) {
 
   // Neighbouring tiles on one XCD (workgroups go to the 8 XCDs in turn), and
   // there in bands of 8 tile rows, so that its cache serves both operands.
-  uint32_t l_id = blockIdx.x;
-  uint32_t const l_each = gridDim.x / 8;
-  if( l_id < 8 * l_each ) l_id = l_id % 8 * l_each + l_id / 8;
-  int32_t const l_per_c = t.tiles_m * t.tiles_n;
-  int32_t const l_c = l_id / l_per_c;
-  int32_t const l_r = l_id % l_per_c;
-  int32_t const l_band = l_r / ( 8 * t.tiles_n ) * 8;
-  int32_t const l_high = min( 8, t.tiles_m - l_band );
-  int32_t const l_m0 = ( l_band + l_r % ( 8 * t.tiles_n ) % l_high ) * BM;
-  int32_t const l_n0 = ( l_r % ( 8 * t.tiles_n ) / l_high ) * BN;
+  int32_t const l_per_c = l_tiles_m * l_tiles_n, l_each = l_per_c / 8;
+  int64_t const l_c = blockIdx.x / l_per_c;
+  int32_t l_r = blockIdx.x % l_per_c;
+  if( l_r < 8 * l_each ) l_r = l_r % 8 * l_each + l_r / 8;
+  int32_t const l_band = l_r / ( 8 * l_tiles_n ) * 8;
+  int32_t const l_high = min( 8, l_tiles_m - l_band );
+  int32_t const l_m0 = ( l_band + l_r % ( 8 * l_tiles_n ) % l_high ) * BM;
+  int32_t const l_n0 = ( l_r % ( 8 * l_tiles_n ) / l_high ) * BN;
 
   Side< BM, WAVES, LOAD > l_a;
   Side< BN, WAVES, LOAD > l_b;
-  l_a.init( a.a + l_c * a.c[I8_A] + l_m0 * a.a_row, a.a_row, a.M - l_m0, l_wave, l_lane );
-  l_b.init( a.b + l_c * a.c[I8_B] + l_n0 * a.b_col, a.b_col, a.N - l_n0, l_wave, l_lane );
+  l_a.init( a.a + l_c * a.c[I8_A] + int64_t( l_m0 ) * a.a_row, a.a_row, a.M - l_m0, l_wave, l_lane );
+  l_b.init( a.b + l_c * a.c[I8_B] + int64_t( l_n0 ) * a.b_col, a.b_col, a.N - l_n0, l_wave, l_lane );
 
   // scales and bias, needed after the loop
+  bool const l_bias_rows = a.has( I8Args::BIAS_ROWS );
   constexpr int CH = ( BN + 64 * WAVES * KG - 1 ) / ( 64 * WAVES * KG );
   float l_sb_r[CH], l_bias_r[CH], l_sa[TM], l_bias_m[TM];
 #pragma unroll
   for( int l_i = 0; l_i < CH; l_i++ ) {
     int32_t const l_n = min( l_n0 + l_i * 64 * WAVES * KG + int( threadIdx.x ), a.N - 1 );
-    l_sb_r[l_i] = a.sb ? a.sb[l_c * a.c[I8_SB] + l_n * a.sb_col] : 1.0f;
-    l_bias_r[l_i] = a.bias ? a.bias[l_c * a.c[I8_BIAS] + l_n * a.bias_col] : 0.0f;
+    l_sb_r[l_i] = a.sb ? a.sb[l_c * a.c[I8_SB] + int64_t( l_n ) * a.sb_col] : 1.0f;
+    l_bias_r[l_i] = a.bias && !l_bias_rows ? a.bias[l_c * a.c[I8_BIAS] + int64_t( l_n ) * a.bias_step] : 0.0f;
   }
   int const l_row = l_lane % 32;
 #pragma unroll
   for( int l_j = 0; l_j < TM; l_j++ ) {
     int32_t const l_m = min( l_m0 + l_wm + 32 * l_j + l_row, a.M - 1 );
-    l_sa[l_j] = a.sa ? a.sa[l_c * a.c[I8_SA] + l_m * a.sa_row] : 1.0f;
-    l_bias_m[l_j] = a.bias ? a.bias[l_c * a.c[I8_BIAS] + l_m * a.bias_row] : 0.0f;
+    l_sa[l_j] = a.sa ? a.sa[l_c * a.c[I8_SA] + int64_t( l_m ) * a.sa_row] : 1.0f;
+    l_bias_m[l_j] = a.bias && l_bias_rows ? a.bias[l_c * a.c[I8_BIAS] + int64_t( l_m ) * a.bias_step] : 0.0f;
   }
 
   // this group's buffers
   char * const l_buf = l_lds + l_group * STAGES * STAGE;
   uint32_t const l_buf_at = kern::lds_addr( l_buf );
-  int const l_steps = ( t.blocks + KG - 1 ) / KG;
+  int const l_steps = ( l_blocks + KG - 1 ) / KG;
   // first k of the group's step s; past the last block nothing is in range and
   // zeros are loaded
-  auto k_of_step = [&]( int s ) -> int32_t { return min( s * KG + l_group, t.blocks ) * kBk; };
+  auto k_of_step = [&]( int s ) -> int32_t { return min( s * KG + l_group, l_blocks ) * kBk; };
   // pieces FROM to TO - 1 of the wave's, both sides counted through
   constexpr int EACH_A = Side< BM, WAVES, LOAD >::EACH, EACH = EACH_A + Side< BN, WAVES, LOAD >::EACH;
   auto issue = [&]( auto ic, int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
     constexpr int l_i = decltype( ic )::value;
     uint32_t const l_to = l_buf_at + stage * STAGE;
-    if constexpr( l_i < EACH_A ) l_a.template issue< l_i >( l_to, k0, a.K );
-    else                         l_b.template issue< l_i - EACH_A >( l_to + BM * kBk, k0, a.K );
+    if constexpr( l_i < EACH_A ) l_a.template issue< l_i >( l_to, k0, l_k );
+    else                         l_b.template issue< l_i - EACH_A >( l_to + BM * kBk, k0, l_k );
   };
   auto put = [&]( int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
     kern::static_for< DMA ? 0 : EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
       constexpr int l_i = decltype( ic )::value;
       char * const l_to = l_buf + stage * STAGE;
-      if constexpr( l_i < EACH_A ) l_a.template put< l_i >( l_to, k0, a.K, l_lane );
-      else                         l_b.template put< l_i - EACH_A >( l_to + BM * kBk, k0, a.K, l_lane );
+      if constexpr( l_i < EACH_A ) l_a.template put< l_i >( l_to, k0, l_k, l_lane );
+      else                         l_b.template put< l_i - EACH_A >( l_to + BM * kBk, k0, l_k, l_lane );
     } );
   };
   // pieces of block 1 (two buffers) that are issued in front of the loop
@@ -405,16 +398,16 @@ void contract_i8_tile_kernel( TileArgs t ) {
           int const l_n = 32 * l_i + 8 * l_q + 4 * ( l_lane / 32 );
           f32x4 const l_sb4 = *reinterpret_cast< f32x4 const * >( l_sb + l_wn + l_n );
           f32x4 l_b4 = { 0.0f, 0.0f, 0.0f, 0.0f };
-          if( a.bias ) l_b4 = *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
+          if( a.bias && !l_bias_rows ) l_b4 = *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
 #pragma unroll
           for( int l_j = l_j0; l_j < l_j0 + PASS; l_j++ ) {
             float l_v[4];
 #pragma unroll
             for( int l_e = 0; l_e < 4; l_e++ ) {
               l_v[l_e] = i8_finish( l_acc[l_i][l_j][4 * l_q + l_e], l_sa[l_j], l_sb4[l_e],
-                                    a.bias_row != 0 ? l_bias_m[l_j] : l_b4[l_e], 0 );
+                                    l_bias_rows ? l_bias_m[l_j] : l_b4[l_e], 0 );
             }
-            if( a.relu ) {
+            if( a.has( I8Args::RELU ) ) {
 #pragma unroll
               for( int l_e = 0; l_e < 4; l_e++ ) l_v[l_e] = l_v[l_e] < 0.0f ? 0.0f : l_v[l_e];
             }
@@ -425,23 +418,19 @@ void contract_i8_tile_kernel( TileArgs t ) {
       }
       // the slab is this wave's own, and its LDS operations are in order
       __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
-      store_slab< 32 * PASS, COLS, T >( t, l_slab, l_out0, l_m0 + l_wm + 32 * l_j0, l_n0 + l_wn, l_lane );
+      store_slab< 32 * PASS, COLS, T >( a, l_slab, l_out0, l_m0 + l_wm + 32 * l_j0, l_n0 + l_wn, l_lane );
       __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
     }
   };
-  if( a.out_bf16 ) finish( __bf16( 0.0f ), std::integral_constant< int, TM >() );
+  if( a.has( I8Args::OUT_BF16 ) ) finish( __bf16( 0.0f ), std::integral_constant< int, TM >() );
   else             finish( 0.0f, std::integral_constant< int, 1 >() );
 }
 
 template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
-int launch_shape( TileArgs t, hipStream_t stream ) {
-  I8Args const & a = t.a;
-  t.tiles_m = ( a.M + BM - 1 ) / BM;
-  t.tiles_n = ( a.N + BN - 1 ) / BN;
-  t.blocks = ( a.K + kBk - 1 ) / kBk;
-  uint32_t const l_grid = uint32_t( int64_t( t.tiles_m ) * t.tiles_n * a.C );
+int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
+  uint32_t const l_grid = uint32_t( ( int64_t( a.M ) + BM - 1 ) / BM * ( ( int64_t( a.N ) + BN - 1 ) / BN ) * C );
   hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, DEEP, LOAD > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
-                      0, stream, t );
+                      0, stream, a );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
     return fail( ETIR_UNDEFINED_ERROR, std::string( "contraction_i8 launch failed: " ) + hipGetErrorString( l_e ) );
@@ -451,32 +440,33 @@ int launch_shape( TileArgs t, hipStream_t stream ) {
 
 }  // namespace
 
-int launch_i8_tile( I8Args const & a, I8Kernel kernel, hipStream_t stream ) {
-  TileArgs t{};
-  t.a = a;
-  int64_t const l_item = a.out_bf16 ? 2 : 4;
-  t.vec_out = a.o_col == 1 && uintptr_t( a.out ) % 4 == 0 && a.o_row * l_item % 4 == 0 && a.c[I8_OUT] * l_item % 4 == 0;
+int launch_i8_tile( I8Args const & args, int64_t C, I8Kernel kernel, hipStream_t stream ) {
+  I8Args a = args;
+  int64_t const l_item = a.has( I8Args::OUT_BF16 ) ? 2 : 4;
+  if( a.o_col == 1 && uintptr_t( a.out ) % 4 == 0 && a.o_row * l_item % 4 == 0 && a.c[I8_OUT] * l_item % 4 == 0 ) {
+    a.k_flags |= I8Args::VEC_OUT;
+  }
   bool const l_dwords = i8_aligned( a, 4 );
   switch( kernel ) {
-    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, true, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, true, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_128x64:  return launch_shape< 128, 64, 2, 2, 1, 3, false, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, false, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, false, LOAD_DMA >( t, stream );
-    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, false, LOAD_DMA >( t, stream );
+    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, true, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, true, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_128x64:  return launch_shape< 128, 64, 2, 2, 1, 3, false, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, false, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, false, LOAD_DMA >( a, C, stream );
+    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, false, LOAD_DMA >( a, C, stream );
     case I8Kernel::REG_32x32:
-      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_DWORDS >( a, C, stream )
+                      : launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_BYTES >( a, C, stream );
     case I8Kernel::REG_64x64:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_DWORDS >( a, C, stream )
+                      : launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_BYTES >( a, C, stream );
     case I8Kernel::REG_64x64_K2:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_DWORDS >( a, C, stream )
+                      : launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_BYTES >( a, C, stream );
     case I8Kernel::REG_128x128:
-      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_DWORDS >( t, stream )
-                      : launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_BYTES >( t, stream );
+      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_DWORDS >( a, C, stream )
+                      : launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_BYTES >( a, C, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction_i8: unknown tile" );
   }
 }

@@ -43,6 +43,8 @@ struct I8GeneralArgs {
 };
 
 // One loop of each type at most, both operands unit-stride along K, K >= 16.
+// All strides fit 32 bits.  112 bytes: a launch with more than that in kernel
+// arguments takes 3.6 us of the host, one with up to 112 bytes 2.9 us.
 struct I8Args {
   int8_t const * a;
   int8_t const * b;
@@ -50,16 +52,21 @@ struct I8Args {
   float const  * sb;       // null: 1
   float const  * bias;     // null: 0
   void         * out;
-  int32_t C, M, N, K;
+  int32_t M, N;
+  uint32_t k_flags;        // K (17 bits) and flags
   // strides from row (of A), column (row of B) and batch index to the next
-  int64_t a_row, b_col;
-  int64_t o_row, o_col;
-  int64_t sa_row, sb_col;
-  int64_t bias_row, bias_col;
-  int64_t c[I8_TENSORS];
-  int32_t out_bf16;
-  int32_t relu;
+  int32_t a_row, b_col;
+  int32_t o_row, o_col;
+  int32_t sa_row, sb_col;
+  int32_t bias_step;       // along rows (BIAS_ROWS) or columns
+  int32_t c[I8_TENSORS];
+
+  enum : uint32_t { K_MASK = ( 1u << 20 ) - 1, OUT_BF16 = 1u << 20, RELU = 1u << 21, BIAS_ROWS = 1u << 22,
+                    VEC_OUT = 1u << 23 };   // VEC_OUT: output rows take 16-byte stores (tiles)
+  __host__ __device__ int32_t K() const { return int32_t( k_flags & K_MASK ); }
+  __host__ __device__ bool has( uint32_t flag ) const { return ( k_flags & flag ) != 0; }
 };
+static_assert( sizeof( I8Args ) == 112, "kernel arguments" );
 
 // The kernels.  TILE_*: through LDS (contract_i8_tile.hip); their rows come in
 // directly where they lie at multiples of 16 bytes, else through registers.
@@ -82,7 +89,7 @@ enum class I8Kernel : int32_t {
 
 // rows of both operands, and K, at multiples of n bytes
 inline bool i8_aligned( I8Args const & a, int64_t n ) {
-  return a.K % n == 0 && uintptr_t( a.a ) % n == 0 && uintptr_t( a.b ) % n == 0 && a.a_row % n == 0
+  return a.K() % n == 0 && uintptr_t( a.a ) % n == 0 && uintptr_t( a.b ) % n == 0 && a.a_row % n == 0
       && a.b_col % n == 0 && a.c[I8_A] % n == 0 && a.c[I8_B] % n == 0;
 }
 // 16, 4 or 1
@@ -176,8 +183,8 @@ int launch_i8( I8Plan const & plan,
                hipStream_t    stream );
 
 int launch_i8_general( I8GeneralArgs const & a, hipStream_t stream );
-int launch_i8_few( I8Args const & a, hipStream_t stream );
-int launch_i8_tile( I8Args const & a, I8Kernel kernel, hipStream_t stream );
+int launch_i8_few( I8Args const & a, int64_t C, hipStream_t stream );
+int launch_i8_tile( I8Args const & a, int64_t C, I8Kernel kernel, hipStream_t stream );
 
 // ---------------------------------------------------------------------------
 // rows rounded to 8-bit integers with one scale a row
@@ -197,6 +204,7 @@ struct QuantPlan {
 void describe_quant( QuantPlan & plan );
 
 // One row: y = norm or activation of the inputs, q = rint( y * 127 / max|y| ).
+// (112 bytes, as above.)
 struct QuantArgs {
   void const * in;
   void const * second;      // residual (norm) or gate (activation); null: none
@@ -205,12 +213,12 @@ struct QuantArgs {
   int8_t     * q;
   float      * scale;
   void       * values;      // q * scale; null: not wanted
-  int64_t rows, cols;
   int64_t ld_in, ld_second, ld_total, ld_q, ld_values;
+  int32_t rows, cols;
   float   eps;
-  int32_t weight_f32;
-  int32_t ktype;
+  int32_t mode;             // norm: 1 where the weight is fp32; activation: the kernel type
 };
+static_assert( sizeof( QuantArgs ) == 112, "kernel arguments" );
 
 int launch_quant( QuantPlan const & plan, QuantArgs const & a, hipStream_t stream );
 

@@ -111,10 +111,11 @@ int64_t ceil_div( int64_t x, int64_t y ) { return ( x + y - 1 ) / y; }
 // The kernel that should take the least time on 256 compute units: tiles in
 // rounds of one workgroup each, at least 1.15 times the tensors' bytes at 5.3
 // TB/s.  The first of equals is the one with the smaller tiles.
-Candidate const * choose_candidate( I8Args const & a, int32_t alignment ) {
+Candidate const * choose_candidate( I8Args const & a, int64_t C, int32_t alignment ) {
   Candidate const * l_best = nullptr;
   double l_least = 0.0;
-  double const l_bytes = double( a.C ) * ( ( double( a.M ) + a.N ) * a.K + double( a.out_bf16 ? 2 : 4 ) * a.M * a.N );
+  int32_t const l_k = a.K();
+  double const l_bytes = double( C ) * ( ( double( a.M ) + a.N ) * l_k + double( a.has( I8Args::OUT_BF16 ) ? 2 : 4 ) * a.M * a.N );
   for( Candidate const & l_c : kCandidates ) {
     // the rows of alignment 4 and 1 have their own entries, and those of 16 the few-sided kernels' of 4
     bool const l_few = l_c.kernel == I8Kernel::FEW_16 || l_c.kernel == I8Kernel::FEW_32;
@@ -122,20 +123,20 @@ Candidate const * choose_candidate( I8Args const & a, int32_t alignment ) {
     double l_groups, l_us;
     if( l_few ) {
       if( std::min( a.M, a.N ) > l_c.rows ) continue;
-      l_groups = double( ceil_div( std::max( a.M, a.N ), l_c.cols ) ) * a.C;
+      l_groups = double( ceil_div( std::max( a.M, a.N ), l_c.cols ) ) * C;
     }
     else {
       // a tile's rows are addressed by 31 bits from its first one
-      if( std::max( l_c.rows * a.a_row, l_c.cols * a.b_col ) + a.K >= ( int64_t( 1 ) << 31 ) ) continue;
-      l_groups = double( ceil_div( a.M, l_c.rows ) ) * ceil_div( a.N, l_c.cols ) * a.C;
-      double const l_steps = double( ceil_div( a.K, l_c.step_k ) );
+      if( std::max( int64_t( l_c.rows ) * a.a_row, int64_t( l_c.cols ) * a.b_col ) + l_k >= ( int64_t( 1 ) << 31 ) ) continue;
+      l_groups = double( ceil_div( a.M, l_c.rows ) ) * ceil_div( a.N, l_c.cols ) * C;
+      double const l_steps = double( ceil_div( l_k, l_c.step_k ) );
       l_us = std::max( double( ceil_div( int64_t( l_groups ), 256 ) ) * ( l_c.fixed_us + l_steps * l_c.step_us ),
                        1.15 * l_bytes / 5.3e6 );
     }
     if( l_few ) {
       // latency, or what the rows' 64-byte pieces take in the caches
-      l_us = std::max( double( ceil_div( a.K, l_c.step_k ) ) * l_c.step_us,
-                       l_groups * a.K * 1e-6 * ( 3.1 + 0.12 * std::min( a.M, a.N ) ) * ( l_c.alignment == 1 ? 1.6 : 1.0 ) );
+      l_us = std::max( double( ceil_div( l_k, l_c.step_k ) ) * l_c.step_us,
+                       l_groups * l_k * 1e-6 * ( 3.1 + 0.12 * std::min( a.M, a.N ) ) * ( l_c.alignment == 1 ? 1.6 : 1.0 ) );
     }
     // a grid's threads are counted in 32 bits
     if( l_groups * l_c.threads >= 4294967296.0 ) continue;
@@ -152,33 +153,34 @@ char const * choose_kernel( I8Plan & plan ) {
   I8GeneralArgs const & a = plan.args;
   bool const l_unit_k = a.k.n == 0 || ( a.k.n == 1 && a.k.stride[0][I8_A] == 1 && a.k.stride[0][I8_B] == 1 );
   if( a.c.n > 1 || a.m.n > 1 || a.n.n > 1 || !l_unit_k || a.K < 16 || a.C == 0 || a.M == 0 || a.N == 0 ) return "general";
+  // strides of 32 bits
+  for( I8Loops const * l_l : { &a.c, &a.m, &a.n } ) {
+    for( int64_t l_s : l_l->stride[0] ) if( l_s > std::numeric_limits< int32_t >::max() ) return "general";
+  }
   I8Args & f = plan.affine;
-  f.C = int32_t( a.C );
   f.M = int32_t( a.M );
   f.N = int32_t( a.N );
-  f.K = int32_t( a.K );
+  f.k_flags = uint32_t( a.K ) | ( a.out_bf16 ? I8Args::OUT_BF16 : 0u ) | ( a.relu ? I8Args::RELU : 0u )
+            | ( a.bias_rows ? I8Args::BIAS_ROWS : 0u );
   // without a loop every stride is 0
-  f.a_row = a.m.stride[0][I8_A];
-  f.o_row = a.m.stride[0][I8_OUT];
-  f.sa_row = a.m.stride[0][I8_SA];
-  f.bias_row = a.m.stride[0][I8_BIAS];
-  f.b_col = a.n.stride[0][I8_B];
-  f.o_col = a.n.n == 0 ? 1 : a.n.stride[0][I8_OUT];
-  f.sb_col = a.n.stride[0][I8_SB];
-  f.bias_col = a.n.stride[0][I8_BIAS];
+  f.a_row = int32_t( a.m.stride[0][I8_A] );
+  f.o_row = int32_t( a.m.stride[0][I8_OUT] );
+  f.sa_row = int32_t( a.m.stride[0][I8_SA] );
+  f.b_col = int32_t( a.n.stride[0][I8_B] );
+  f.o_col = a.n.n == 0 ? 1 : int32_t( a.n.stride[0][I8_OUT] );
+  f.sb_col = int32_t( a.n.stride[0][I8_SB] );
+  f.bias_step = int32_t( ( a.bias_rows ? a.m : a.n ).stride[0][I8_BIAS] );
   std::copy_n( a.c.stride[0], int( I8_TENSORS ), f.c );
-  f.out_bf16 = a.out_bf16;
-  f.relu = a.relu;
   plan.alignment = i8_alignment( f );
-  Candidate const * l_c = choose_candidate( f, plan.alignment );
+  Candidate const * l_c = choose_candidate( f, a.C, plan.alignment );
   if( l_c == nullptr ) return "general";
   plan.kernel = l_c->kernel;
   return l_c->name;
 }
 
-int launch_affine( I8Kernel kernel, I8Args const & a, hipStream_t stream ) {
-  if( kernel == I8Kernel::FEW_16 || kernel == I8Kernel::FEW_32 ) return launch_i8_few( a, stream );
-  return launch_i8_tile( a, kernel, stream );
+int launch_affine( I8Kernel kernel, I8Args const & a, int64_t C, hipStream_t stream ) {
+  if( kernel == I8Kernel::FEW_16 || kernel == I8Kernel::FEW_32 ) return launch_i8_few( a, C, stream );
+  return launch_i8_tile( a, C, kernel, stream );
 }
 
 }  // namespace
@@ -332,9 +334,9 @@ int launch_i8( I8Plan const & plan,
   f.out = a.out;
   // pointers may be less aligned than the strides
   int32_t const l_alignment = i8_alignment( f );
-  if( l_alignment >= plan.alignment ) return launch_affine( plan.kernel, f, stream );
-  Candidate const * l_c = choose_candidate( f, l_alignment );
-  return l_c == nullptr ? launch_i8_general( a, stream ) : launch_affine( l_c->kernel, f, stream );
+  if( l_alignment >= plan.alignment ) return launch_affine( plan.kernel, f, a.C, stream );
+  Candidate const * l_c = choose_candidate( f, a.C, l_alignment );
+  return l_c == nullptr ? launch_i8_general( a, stream ) : launch_affine( l_c->kernel, f, a.C, stream );
 }
 
 namespace {

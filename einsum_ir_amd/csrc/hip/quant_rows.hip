@@ -141,6 +141,11 @@ __device__ inline void store_v( T * row, Place< Vec< T >::V > p, int32_t n, floa
   }
 }
 
+// Workgroups of a launch at most (a grid's threads are counted in 32 bits): they
+// loop over rows.  A constant, since a kernel that reads its grid's size is
+// given 256 bytes of further arguments, which cost 0.7 us of the host.
+constexpr int64_t kMaxGroups = 1 << 20;
+
 // THREADS threads a row; a workgroup takes 4 rows of a wave each, or one row.  CHUNKS > 0: the row fits
 // CHUNKS vectors a thread; 0: it is read twice.
 template< class T, bool NORM, int THREADS, int CHUNKS >
@@ -154,12 +159,12 @@ void quant_rows_kernel( QuantArgs a ) {
   __shared__ uint32_t l_tops[WAVES];
   int const l_t = threadIdx.x % THREADS;
   int const l_sub = __builtin_amdgcn_readfirstlane( threadIdx.x / THREADS );
-  int32_t const l_cols = int32_t( a.cols );
+  int32_t const l_cols = a.cols;
 
   // rows of one workgroup's waves are apart only where a wave holds a whole
   // row, so every thread of a workgroup meets the same barriers
   for( int64_t l_row = int64_t( blockIdx.x ) * ROWS + l_sub; l_row < a.rows;
-       l_row += int64_t( gridDim.x ) * ROWS ) {
+       l_row += kMaxGroups * ROWS ) {
     T const * l_in = static_cast< T const * >( a.in ) + l_row * a.ld_in;
     // Vectors start where those of q lie at multiples of 4 bytes: off them 16
     // bytes move at a third of the rate.  Where all rows are one after the
@@ -180,7 +185,7 @@ void quant_rows_kernel( QuantArgs a ) {
 #pragma unroll
         for( int l_e = 0; l_e < V; l_e++ ) s[l_e] = y[l_e];
         if( a.weight ) {
-          if( a.weight_f32 != ( V == 4 ) ) {
+          if( ( a.mode != 0 ) != ( V == 4 ) ) {
             // the weight's type is not the row's
 #pragma unroll
             for( int l_e = 0; l_e < V; l_e++ ) {
@@ -197,11 +202,11 @@ void quant_rows_kernel( QuantArgs a ) {
       else if( l_second ) {
         load_v( l_second, p.at, l_cols, l_f );
 #pragma unroll
-        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= activate( l_f[l_e], a.ktype );
+        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] *= activate( l_f[l_e], a.mode );
       }
       else {
 #pragma unroll
-        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] = activate( y[l_e], a.ktype );
+        for( int l_e = 0; l_e < V; l_e++ ) y[l_e] = activate( y[l_e], a.mode );
       }
       if( !p.whole( l_cols ) ) {
 #pragma unroll
@@ -336,8 +341,7 @@ void quant_rows_kernel( QuantArgs a ) {
 template< class T, bool NORM, int THREADS, int CHUNKS >
 void launch_shape( QuantArgs const & a, hipStream_t stream ) {
   constexpr int ROWS = THREADS == 64 ? 4 : 1;
-  // a grid's threads are counted in 32 bits, so workgroups loop over rows
-  int64_t const l_grid = std::min< int64_t >( ( a.rows + ROWS - 1 ) / ROWS, 1 << 20 );
+  int64_t const l_grid = std::min( ( int64_t( a.rows ) + ROWS - 1 ) / ROWS, kMaxGroups );
   hipLaunchKernelGGL( ( quant_rows_kernel< T, NORM, THREADS, CHUNKS > ), dim3( uint32_t( l_grid ) ),
                       dim3( ROWS * THREADS ), 0, stream, a );
 }
@@ -383,16 +387,15 @@ int launch_quant( QuantPlan const & plan, QuantArgs const & args, hipStream_t st
   if( a.scale == nullptr || ( plan.cols > 0 && ( a.in == nullptr || a.q == nullptr ) ) ) {
     return fail( ETIR_NO_DATA_PTR_PROVIDED, plan.norm ? "norm_quant: null tensor pointer" : "act_quant: null tensor pointer" );
   }
-  a.rows = plan.rows;
-  a.cols = plan.cols;
+  a.rows = int32_t( plan.rows );
+  a.cols = int32_t( plan.cols );
   a.ld_in = plan.ld_in;
   a.ld_second = plan.ld_second;
   a.ld_total = plan.ld_total;
   a.ld_q = plan.ld_q;
   a.ld_values = plan.ld_values;
   a.eps = plan.eps;
-  a.weight_f32 = plan.dtype_weight == ETIR_FP32;
-  a.ktype = plan.ktype;
+  a.mode = plan.norm ? int32_t( plan.dtype_weight == ETIR_FP32 ) : plan.ktype;
   if( plan.dtype == ETIR_BF16 ) plan.norm ? launch_rows< uint16_t, true >( a, stream ) : launch_rows< uint16_t, false >( a, stream );
   else                          plan.norm ? launch_rows< float, true >( a, stream ) : launch_rows< float, false >( a, stream );
   hipError_t const l_e = hipGetLastError();

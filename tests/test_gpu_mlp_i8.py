@@ -70,7 +70,7 @@ def test_mlp(torch_cuda, tokens, width, hidden, classes, act, gated, dtype):
     from einsum_ir_amd.mlp_i8 import MlpI8
     td = torch.bfloat16 if dtype == eir.BF16 else torch.float32
     blocks, norm, head = _net(torch, width, hidden, classes, 2, gated, td, bias=not gated)
-    x = torch.randn(tokens, width, device="cuda").to(td)
+    x = torch.randn(tokens, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(tokens)).to(td)
     net = MlpI8(blocks, norm, head, dtype=dtype, ktype={"RELU": eir.RELU, "SILU": eir.SILU}[act], gated=gated)
     got = net(x).double()
     f = {"RELU": torch.relu, "SILU": torch.nn.functional.silu}[act]
@@ -85,6 +85,19 @@ def test_mlp(torch_cuda, tokens, width, hidden, classes, act, gated, dtype):
     full = harness.mlp_float64(torch, blocks, norm.to(td), head, x, act, gated)
     err = float((got - full).norm() / full.norm())
     assert err <= 0.1, err
+
+
+def test_repeats_bit_for_bit(torch_cuda):
+    """Integer sums and maxima have no order: the same call gives the same bits."""
+    torch = torch_cuda
+    from einsum_ir_amd.mlp_i8 import MlpI8
+    blocks, norm, head = _net(torch, 500, 777, 33, 2, True, torch.float32, bias=False)
+    net = MlpI8(blocks, norm, head, dtype=eir.FP32, ktype=eir.SILU, gated=True)
+    for tokens in (1, 5, 200):
+        x = torch.randn(tokens, 500, device="cuda")
+        first = net(x).clone()
+        for _ in range(10):
+            assert torch.equal(net(x), first)
 
 
 def test_numbers_of_tokens_and_graph(torch_cuda):
