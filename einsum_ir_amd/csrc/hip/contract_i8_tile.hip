@@ -97,16 +97,19 @@ struct Side {
 template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T ) );
 
 // Stores ROWS rows x COLS columns of a wave's slab from row m1, column n1 of
-// the output on: 16 bytes a lane where the output's rows take them at multiples
-// of 4 bytes, else an element a lane; non-temporal, the output is not read here
-// again (4072 x 2048 x 2048: 23.2 -> 21.2 us).
+// the output on: 16 bytes a lane where the columns are adjacent, else an element
+// a lane; non-temporal, the output is not read here again (4072 x 2048 x 2048:
+// 23.2 -> 21.2 us).  bf16 rows of an odd stride start between two dwords, where
+// these stores are slow but better than an element a lane (2395 x 80 x 7693:
+// 23.3 us against 27.7; vectors shifted by one element to lie on dwords, with
+// single stores at the slab's edges, 27.7).
 template< int ROWS, int COLS, class T >
 __device__ inline void store_slab( I8Args const & a, T const * slab, int64_t out0, int32_t m1, int32_t n1, int lane ) {
   constexpr int V = 16 / sizeof( T );
   constexpr int LANES = COLS / V;            // lanes a row
   constexpr int PITCH = kPitch< T, COLS >;
   typedef T v __attribute__( ( ext_vector_type( V ) ) );
-  typedef v v_dword __attribute__( ( aligned( 4 ) ) );
+  typedef v v_any __attribute__( ( aligned( sizeof( T ) ) ) );
   T * const l_out = static_cast< T * >( a.out ) + out0;
   if( a.has( I8Args::VEC_OUT ) ) {
 #pragma unroll
@@ -115,10 +118,11 @@ __device__ inline void store_slab( I8Args const & a, T const * slab, int64_t out
       v const l_v = *reinterpret_cast< v const * >( slab + l_r * PITCH + l_c );
       if( m1 + l_r >= a.M ) continue;
       T * const l_o = l_out + int64_t( m1 + l_r ) * a.o_row + n1 + l_c;
-      if( n1 + l_c + V <= a.N ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_dword * >( l_o ) );
+      int32_t const l_left = a.N - n1 - l_c;       // columns from this lane's first on
+      if( l_left >= V ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_any * >( l_o ) );
       else {
 #pragma unroll
-        for( int l_e = 0; l_e < V; l_e++ ) if( n1 + l_c + l_e < a.N ) l_o[l_e] = l_v[l_e];
+        for( int l_e = 0; l_e < V; l_e++ ) if( l_e < l_left ) l_o[l_e] = l_v[l_e];
       }
     }
   }
@@ -442,10 +446,7 @@ int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
 
 int launch_i8_tile( I8Args const & args, int64_t C, I8Kernel kernel, hipStream_t stream ) {
   I8Args a = args;
-  int64_t const l_item = a.has( I8Args::OUT_BF16 ) ? 2 : 4;
-  if( a.o_col == 1 && uintptr_t( a.out ) % 4 == 0 && a.o_row * l_item % 4 == 0 && a.c[I8_OUT] * l_item % 4 == 0 ) {
-    a.k_flags |= I8Args::VEC_OUT;
-  }
+  if( a.o_col == 1 ) a.k_flags |= I8Args::VEC_OUT;
   bool const l_dwords = i8_aligned( a, 4 );
   switch( kernel ) {
     case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, LOAD_DMA >( a, C, stream );

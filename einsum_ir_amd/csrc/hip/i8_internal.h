@@ -62,7 +62,7 @@ struct I8Args {
   int32_t c[I8_TENSORS];
 
   enum : uint32_t { K_MASK = ( 1u << 20 ) - 1, OUT_BF16 = 1u << 20, RELU = 1u << 21, BIAS_ROWS = 1u << 22,
-                    VEC_OUT = 1u << 23 };   // VEC_OUT: output rows take 16-byte stores (tiles)
+                    VEC_OUT = 1u << 23 };   // VEC_OUT: the output's columns are adjacent (tiles)
   __host__ __device__ int32_t K() const { return int32_t( k_flags & K_MASK ); }
   __host__ __device__ bool has( uint32_t flag ) const { return ( k_flags & flag ) != 0; }
 };

@@ -86,7 +86,7 @@ struct Candidate {
 };
 Candidate const kCandidates[] = {
   { I8Kernel::FEW_16,       "few 16",       4,  16,  16,  512, 2048, 0.0f, 0.87f },
-  { I8Kernel::FEW_32,       "few 32",       4,  32,  16,  512, 2048, 0.0f, 1.30f },
+  { I8Kernel::FEW_32,       "few 32",       4,  32,  16,  512, 2048, 0.0f, 1.75f },
   { I8Kernel::TILE_32x32,   "tile 32x32",   16, 32,  32,  256, 512,  2.1f, 0.34f },
   { I8Kernel::TILE_64x32,   "tile 64x32",   16, 64,  32,  256, 256,  2.0f, 0.28f },
   { I8Kernel::TILE_64x64,   "tile 64x64",   16, 64,  64,  256, 128,  1.4f, 0.23f },
