@@ -4,7 +4,10 @@
 //   out[c][many][few] = last( s s sum_k MANY[c][many][k] FEW[c][few][k] + bias )
 //
 // Bound by the bytes of the many side, each read once.  A workgroup takes
-// 16 rows of it and all of the few side (16 FB rows), and its waves split K:
+// 16 rows of it and all of the few side (16 FB rows), and its waves split K;
+// with up to 4 few rows it may take 4 rows and put a quarter of K each into the
+// 16 rows of a fragment instead, of which those products count whose quarters
+// are the same (PARTS 4: four times the workgroups for a short many side):
 // that keeps all of a workgroup's bytes in flight at once where there are few
 // workgroups, and needs no memory between workgroups.  Operands go from global
 // memory straight into the fragments of v_mfma_i32_16x16x64_i8 (16 k of a row a
@@ -23,28 +26,29 @@ typedef int32_t i32x4 __attribute__( ( ext_vector_type( 4 ) ) );
 constexpr int kSteps = 4;      // steps of 64 k whose loads are in flight together
 constexpr int kPiece = 64 * kSteps;
 constexpr int kWaves = 8;      // of a workgroup, over K
-constexpr int kMany  = 16;     // rows of the many side a workgroup
 
-template< int FB, bool BYTES >
+template< int FB, int PARTS, bool BYTES >
 __global__ __launch_bounds__( 64 * kWaves )
 void contract_i8_few_kernel( I8Args a ) {     // A: the many side
-  constexpr int FEW = 16 * FB;
-  constexpr int PITCH = kMany + 4;                       // 16-byte writes of 16 few rows over all banks
-  __shared__ __align__( 16 ) int32_t l_part[kWaves][FEW * PITCH];
+  constexpr int MANY = 16 / PARTS, FEW = 16 * FB / PARTS;   // rows of a workgroup
+  constexpr int PITCH = MANY + 4;                           // 16-byte writes of the few rows over all banks
+  __shared__ __align__( 16 ) int32_t l_part[kWaves * PARTS][FEW * PITCH];
 
   int const l_lane = threadIdx.x % 64;
   int const l_wave = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
   int32_t const l_k = a.K();
-  int32_t const l_tiles = ( a.M + kMany - 1 ) / kMany, l_pieces = ( l_k + kPiece - 1 ) / kPiece;
+  int32_t const l_tiles = ( a.M + MANY - 1 ) / MANY;
+  int32_t const l_pieces = ( l_k + kPiece * PARTS - 1 ) / ( kPiece * PARTS );      // of a part of K
   int64_t const l_c = blockIdx.x / l_tiles;
-  int32_t const l_m0 = ( blockIdx.x % l_tiles ) * kMany;
-  int const l_kl = 16 * ( l_lane / 16 );
+  int32_t const l_m0 = ( blockIdx.x % l_tiles ) * MANY;
+  int const l_row = l_lane % MANY, l_part_k = l_lane % 16 / MANY;
+  int32_t const l_kl = 16 * ( l_lane / 16 ) + l_part_k * l_pieces * kPiece;
 
-  int8_t const * const l_pm = a.a + l_c * a.c[I8_A] + int64_t( min( l_m0 + l_lane % 16, a.M - 1 ) ) * a.a_row;
+  int8_t const * const l_pm = a.a + l_c * a.c[I8_A] + int64_t( min( l_m0 + l_row, a.M - 1 ) ) * a.a_row;
   int8_t const * l_pf[FB];
 #pragma unroll
   for( int l_i = 0; l_i < FB; l_i++ ) {
-    l_pf[l_i] = a.b + l_c * a.c[I8_B] + int64_t( min( 16 * l_i + l_lane % 16, a.N - 1 ) ) * a.b_col;
+    l_pf[l_i] = a.b + l_c * a.c[I8_B] + int64_t( min( 16 * l_i + l_row, a.N - 1 ) ) * a.b_col;
   }
 
   i32x4 l_acc[FB];
@@ -82,26 +86,30 @@ void contract_i8_few_kernel( I8Args a ) {     // A: the many side
   int32_t const l_rot = int32_t( blockIdx.x % uint32_t( l_pieces ) );
   for( int32_t l_i = l_wave; l_i < l_pieces; l_i += kWaves ) {
     int32_t const l_p = l_i + l_rot < l_pieces ? l_i + l_rot : l_i + l_rot - l_pieces;
-    if( ( l_p + 1 ) * kPiece <= l_k ) step( l_p * kPiece, std::false_type() );
+    if( ( l_p + 1 + ( PARTS - 1 ) * l_pieces ) * kPiece <= l_k ) step( l_p * kPiece, std::false_type() );
     else                              step( l_p * kPiece, std::true_type() );
   }
 
-  // the accumulators hold many rows 4 (lane / 16) + 0..3 of few row lane % 16
+  // the accumulators hold rows 4 (lane / 16) + 0..3 of A against row lane % 16
+  // of B; with parts those of the same part count
+  if( PARTS == 1 || l_lane / 16 == l_part_k ) {
 #pragma unroll
-  for( int l_j = 0; l_j < FB; l_j++ ) {
-    *reinterpret_cast< i32x4 * >( &l_part[l_wave][( 16 * l_j + l_lane % 16 ) * PITCH + 4 * ( l_lane / 16 )] ) = l_acc[l_j];
+    for( int l_j = 0; l_j < FB; l_j++ ) {
+      *reinterpret_cast< i32x4 * >( &l_part[l_wave * PARTS + ( PARTS > 1 ? l_part_k : 0 )]
+                                           [( 16 * l_j + l_row ) * PITCH + ( PARTS > 1 ? 0 : 4 * ( l_lane / 16 ) )] ) = l_acc[l_j];
+    }
   }
   __syncthreads();
 
   bool const l_along_many = a.o_row <= a.o_col;     // neighbouring lanes on neighbouring outputs
-  for( int l_e = threadIdx.x; l_e < kMany * FEW; l_e += 64 * kWaves ) {
-    int const l_m = l_along_many ? l_e % kMany : l_e / FEW;
-    int const l_f = l_along_many ? l_e / kMany : l_e % FEW;
+  for( int l_e = threadIdx.x; l_e < MANY * FEW; l_e += 64 * kWaves ) {
+    int const l_m = l_along_many ? l_e % MANY : l_e / FEW;
+    int const l_f = l_along_many ? l_e / MANY : l_e % FEW;
     int32_t const l_mg = l_m0 + l_m;
     if( l_mg >= a.M || l_f >= a.N ) continue;
     int32_t l_sum = 0;
 #pragma unroll
-    for( int l_w = 0; l_w < kWaves; l_w++ ) l_sum += l_part[l_w][l_f * PITCH + l_m];
+    for( int l_w = 0; l_w < kWaves * PARTS; l_w++ ) l_sum += l_part[l_w][l_f * PITCH + l_m];
     float const l_sm = a.sa ? a.sa[l_c * a.c[I8_SA] + int64_t( l_mg ) * a.sa_row] : 1.0f;
     float const l_sf = a.sb ? a.sb[l_c * a.c[I8_SB] + int64_t( l_f ) * a.sb_col] : 1.0f;
     float const l_b = a.bias ? a.bias[l_c * a.c[I8_BIAS] + int64_t( a.has( I8Args::BIAS_ROWS ) ? l_mg : l_f ) * a.bias_step] : 0.0f;
@@ -112,9 +120,10 @@ void contract_i8_few_kernel( I8Args a ) {     // A: the many side
   }
 }
 
-template< int FB, bool BYTES >
+template< int FB, int PARTS, bool BYTES >
 int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
-  hipLaunchKernelGGL( ( contract_i8_few_kernel< FB, BYTES > ), dim3( uint32_t( ( a.M + kMany - 1 ) / kMany * C ) ),
+  constexpr int MANY = 16 / PARTS;
+  hipLaunchKernelGGL( ( contract_i8_few_kernel< FB, PARTS, BYTES > ), dim3( uint32_t( ( a.M + MANY - 1 ) / MANY * C ) ),
                       dim3( 64 * kWaves ), 0, stream, a );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
@@ -125,7 +134,7 @@ int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
 
 }  // namespace
 
-int launch_i8_few( I8Args const & args, int64_t C, hipStream_t stream ) {
+int launch_i8_few( I8Args const & args, int64_t C, I8Kernel kernel, hipStream_t stream ) {
   I8Args a = args;
   if( a.M <= a.N ) {
     // the few side is A: A and B change places
@@ -140,8 +149,14 @@ int launch_i8_few( I8Args const & args, int64_t C, hipStream_t stream ) {
     a.k_flags ^= I8Args::BIAS_ROWS;
   }
   bool const l_bytes = !i8_aligned( a, 4 );
-  if( a.N <= 16 ) return l_bytes ? launch_shape< 1, true >( a, C, stream ) : launch_shape< 1, false >( a, C, stream );
-  return l_bytes ? launch_shape< 2, true >( a, C, stream ) : launch_shape< 2, false >( a, C, stream );
+  switch( kernel ) {
+    case I8Kernel::FEW_4:
+      return l_bytes ? launch_shape< 1, 4, true >( a, C, stream ) : launch_shape< 1, 4, false >( a, C, stream );
+    case I8Kernel::FEW_16:
+      return l_bytes ? launch_shape< 1, 1, true >( a, C, stream ) : launch_shape< 1, 1, false >( a, C, stream );
+    default:
+      return l_bytes ? launch_shape< 2, 1, true >( a, C, stream ) : launch_shape< 2, 1, false >( a, C, stream );
+  }
 }
 
 }  // namespace etir

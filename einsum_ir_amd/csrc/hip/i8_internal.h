@@ -72,7 +72,8 @@ static_assert( sizeof( I8Args ) == 112, "kernel arguments" );
 // directly where they lie at multiples of 16 bytes, else through registers.
 enum class I8Kernel : int32_t {
   GENERAL,            // any strides, 64 x 64 tiles (contract_i8.hip)
-  FEW_16,             // a side of up to 16, K over the waves (contract_i8_few.hip)
+  FEW_4,              // a side of up to 4, K over the waves and in 4 parts (contract_i8_few.hip)
+  FEW_16,             // a side of up to 16, K over the waves
   FEW_32,             // a side of up to 32
   TILE_32x32,
   TILE_64x32,
@@ -183,7 +184,7 @@ int launch_i8( I8Plan const & plan,
                hipStream_t    stream );
 
 int launch_i8_general( I8GeneralArgs const & a, hipStream_t stream );
-int launch_i8_few( I8Args const & a, int64_t C, hipStream_t stream );
+int launch_i8_few( I8Args const & a, int64_t C, I8Kernel kernel, hipStream_t stream );
 int launch_i8_tile( I8Args const & a, int64_t C, I8Kernel kernel, hipStream_t stream );
 
 // ---------------------------------------------------------------------------
