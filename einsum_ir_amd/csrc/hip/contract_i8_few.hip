@@ -48,7 +48,7 @@ void contract_i8_few_kernel( I8Args a ) {     // A: the many side
   int8_t const * l_pf[FB];
 #pragma unroll
   for( int l_i = 0; l_i < FB; l_i++ ) {
-    l_pf[l_i] = a.b + l_c * a.c[I8_B] + int64_t( min( 16 * l_i + l_row, a.N - 1 ) ) * a.b_col;
+    l_pf[l_i] = a.b + l_c * a.c[I8_B] + int64_t( min( MANY * l_i + l_row, a.N - 1 ) ) * a.b_col;
   }
 
   i32x4 l_acc[FB];
@@ -96,7 +96,7 @@ void contract_i8_few_kernel( I8Args a ) {     // A: the many side
 #pragma unroll
     for( int l_j = 0; l_j < FB; l_j++ ) {
       *reinterpret_cast< i32x4 * >( &l_part[l_wave * PARTS + ( PARTS > 1 ? l_part_k : 0 )]
-                                           [( 16 * l_j + l_row ) * PITCH + ( PARTS > 1 ? 0 : 4 * ( l_lane / 16 ) )] ) = l_acc[l_j];
+                                           [( MANY * l_j + l_row ) * PITCH + ( PARTS > 1 ? 0 : 4 * ( l_lane / 16 ) )] ) = l_acc[l_j];
     }
   }
   __syncthreads();
@@ -152,6 +152,10 @@ int launch_i8_few( I8Args const & args, int64_t C, I8Kernel kernel, hipStream_t 
   switch( kernel ) {
     case I8Kernel::FEW_4:
       return l_bytes ? launch_shape< 1, 4, true >( a, C, stream ) : launch_shape< 1, 4, false >( a, C, stream );
+    case I8Kernel::FEW_8_PARTS:
+      return l_bytes ? launch_shape< 2, 4, true >( a, C, stream ) : launch_shape< 2, 4, false >( a, C, stream );
+    case I8Kernel::FEW_16_PARTS:
+      return l_bytes ? launch_shape< 4, 4, true >( a, C, stream ) : launch_shape< 4, 4, false >( a, C, stream );
     case I8Kernel::FEW_16:
       return l_bytes ? launch_shape< 1, 1, true >( a, C, stream ) : launch_shape< 1, 1, false >( a, C, stream );
     default:

@@ -73,6 +73,8 @@ static_assert( sizeof( I8Args ) == 112, "kernel arguments" );
 enum class I8Kernel : int32_t {
   GENERAL,            // any strides, 64 x 64 tiles (contract_i8.hip)
   FEW_4,              // a side of up to 4, K over the waves and in 4 parts (contract_i8_few.hip)
+  FEW_8_PARTS,        // the same, a side of up to 8
+  FEW_16_PARTS,       // a side of up to 16
   FEW_16,             // a side of up to 16, K over the waves
   FEW_32,             // a side of up to 32
   TILE_32x32,

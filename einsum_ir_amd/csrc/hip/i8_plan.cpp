@@ -72,44 +72,49 @@ std::string sizes_of( I8Loops const & l ) {
 // What choose_kernel knows of a kernel.  Tiles: a workgroup's rows and columns,
 // its threads, the k it takes in a step, and the time of a workgroup alone on
 // its compute unit, fixed + step * steps.  Few-sided kernels (rows, cols: of the
-// few and the many side): fixed + step * K / 1024 where nothing else bounds
-// them, and at least (row_us + few_us * few rows) for every 10^6 k of all
-// workgroups, which their 64-byte pieces of rows take in the caches, and 0.4 ns
-// for each workgroup.
+// few and the many side): fixed + (step + step_few * few rows) * K / 1024 where
+// nothing else bounds them, and at least (row + few * few rows) for every 10^6 k
+// of all workgroups, which their 64-byte pieces of rows take in the caches, and
+// 0.4 ns for each workgroup.
 // Measured over 170 products with rows at multiples of 16 bytes, 50 at 4, 80 at
-// others (1 to 8192 rows, 16 to 16384 columns, K 64 to 12288), few 4 over 48.
-// The times that follow are off by 10 to 20 % (root mean square), but alike for
-// neighbours: the kernel chosen is 1 % slower than the best of all on average
+// others (1 to 8192 rows, 16 to 16384 columns, K 64 to 12288), K in parts over
+// 100.  The times that follow are off by 10 to 20 % (root mean square), but alike
+// for neighbours: the kernel chosen is 1 % slower than the best of all on average
 // (64 x 64 tiles everywhere: 36 %).
 struct Candidate {
   I8Kernel     kernel;
   char const * name;
   int32_t      alignment;          // 16: these rows only; 4, 1: of such rows (few: 4 or 16)
   int32_t      rows, cols, threads, step_k;
-  float        fixed_us, step_us, row_us, few_us;
+  float        fixed_us, step_us;
+  float        step_few_us, row_us, few_us;      // few-sided kernels
 };
 Candidate const kCandidates[] = {
-  { I8Kernel::FEW_4,        "few 4",         4,  4,   4,   512, 1024, 0.35f, 0.10f, 0.63f, 0.07f },
-  { I8Kernel::FEW_16,       "few 16",        4,  16,  16,  512, 1024, 0.0f,  0.50f, 3.1f,  0.12f },
-  { I8Kernel::FEW_32,       "few 32",        4,  32,  16,  512, 1024, 0.0f,  0.85f, 3.1f,  0.12f },
-  { I8Kernel::TILE_32x32,   "tile 32x32",    16, 32,  32,  256, 512,  2.1f,  0.34f, 0.0f,  0.0f },
-  { I8Kernel::TILE_64x32,   "tile 64x32",    16, 64,  32,  256, 256,  2.0f,  0.28f, 0.0f,  0.0f },
-  { I8Kernel::TILE_64x64,   "tile 64x64",    16, 64,  64,  256, 128,  1.4f,  0.23f, 0.0f,  0.0f },
-  { I8Kernel::TILE_128x64,  "tile 128x64",   16, 128, 64,  256, 128,  2.3f,  0.34f, 0.0f,  0.0f },
-  { I8Kernel::TILE_128x128, "tile 128x128",  16, 128, 128, 512, 128,  3.2f,  0.44f, 0.0f,  0.0f },
-  { I8Kernel::TILE_256x128, "tile 256x128",  16, 256, 128, 512, 128,  5.1f,  0.72f, 0.0f,  0.0f },
-  { I8Kernel::TILE_256x256, "tile 256x256",  16, 256, 256, 512, 128,  8.4f,  1.09f, 0.0f,  0.0f },
-  { I8Kernel::REG_32x32,    "regs 32x32",    4,  32,  32,  256, 512,  3.0f,  0.51f, 0.0f,  0.0f },
-  { I8Kernel::REG_64x64,    "regs 64x64",    4,  64,  64,  256, 128,  1.9f,  0.33f, 0.0f,  0.0f },
-  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 4,  64,  64,  512, 256,  3.0f,  0.45f, 0.0f,  0.0f },
-  { I8Kernel::REG_128x128,  "regs 128x128",  4,  128, 128, 256, 128,  5.8f,  0.63f, 0.0f,  0.0f },
-  { I8Kernel::FEW_4,        "few 4",         1,  4,   4,   512, 1024, 0.50f, 0.25f, 1.0f,  0.11f },
-  { I8Kernel::FEW_16,       "few 16",        1,  16,  16,  512, 1024, 0.0f,  0.75f, 5.0f,  0.19f },
-  { I8Kernel::FEW_32,       "few 32",        1,  32,  16,  512, 1024, 0.0f,  1.55f, 5.0f,  0.19f },
-  { I8Kernel::REG_32x32,    "regs 32x32",    1,  32,  32,  256, 512,  3.8f,  0.93f, 0.0f,  0.0f },
-  { I8Kernel::REG_64x64,    "regs 64x64",    1,  64,  64,  256, 128,  2.3f,  0.55f, 0.0f,  0.0f },
-  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 1,  64,  64,  512, 256,  3.4f,  0.81f, 0.0f,  0.0f },
-  { I8Kernel::REG_128x128,  "regs 128x128",  1,  128, 128, 256, 128,  7.0f,  1.07f, 0.0f,  0.0f }
+  { I8Kernel::FEW_4,        "few 4",         4,  4,   4,   512, 1024, 0.35f, 0.10f, 0.0f,   0.63f, 0.07f },
+  { I8Kernel::FEW_8_PARTS,  "few 8 parts",   4,  8,   4,   512, 1024, 0.35f, 0.31f, 0.0f,   0.63f, 0.09f },
+  { I8Kernel::FEW_16_PARTS, "few 16 parts",  4,  16,  4,   512, 1024, 0.45f, 0.54f, 0.0f,   0.63f, 0.10f },
+  { I8Kernel::FEW_16,       "few 16",        4,  16,  16,  512, 1024, 0.0f,  0.48f, 0.022f, 3.1f,  0.12f },
+  { I8Kernel::FEW_32,       "few 32",        4,  32,  16,  512, 1024, 0.0f,  0.48f, 0.022f, 3.1f,  0.12f },
+  { I8Kernel::TILE_32x32,   "tile 32x32",    16, 32,  32,  256, 512,  2.1f,  0.34f },
+  { I8Kernel::TILE_64x32,   "tile 64x32",    16, 64,  32,  256, 256,  2.0f,  0.28f },
+  { I8Kernel::TILE_64x64,   "tile 64x64",    16, 64,  64,  256, 128,  1.4f,  0.23f },
+  { I8Kernel::TILE_128x64,  "tile 128x64",   16, 128, 64,  256, 128,  2.3f,  0.34f },
+  { I8Kernel::TILE_128x128, "tile 128x128",  16, 128, 128, 512, 128,  3.2f,  0.44f },
+  { I8Kernel::TILE_256x128, "tile 256x128",  16, 256, 128, 512, 128,  5.1f,  0.72f },
+  { I8Kernel::TILE_256x256, "tile 256x256",  16, 256, 256, 512, 128,  8.4f,  1.09f },
+  { I8Kernel::REG_32x32,    "regs 32x32",    4,  32,  32,  256, 512,  3.0f,  0.51f },
+  { I8Kernel::REG_64x64,    "regs 64x64",    4,  64,  64,  256, 128,  1.9f,  0.33f },
+  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 4,  64,  64,  512, 256,  3.0f,  0.45f },
+  { I8Kernel::REG_128x128,  "regs 128x128",  4,  128, 128, 256, 128,  5.8f,  0.63f },
+  { I8Kernel::FEW_4,        "few 4",         1,  4,   4,   512, 1024, 0.50f, 0.25f, 0.0f,   1.0f,  0.11f },
+  { I8Kernel::FEW_8_PARTS,  "few 8 parts",   1,  8,   4,   512, 1024, 0.50f, 0.50f, 0.0f,   1.0f,  0.14f },
+  { I8Kernel::FEW_16_PARTS, "few 16 parts",  1,  16,  4,   512, 1024, 0.60f, 0.86f, 0.0f,   1.0f,  0.16f },
+  { I8Kernel::FEW_16,       "few 16",        1,  16,  16,  512, 1024, 0.0f,  0.75f, 0.035f, 5.0f,  0.19f },
+  { I8Kernel::FEW_32,       "few 32",        1,  32,  16,  512, 1024, 0.0f,  0.75f, 0.035f, 5.0f,  0.19f },
+  { I8Kernel::REG_32x32,    "regs 32x32",    1,  32,  32,  256, 512,  3.8f,  0.93f },
+  { I8Kernel::REG_64x64,    "regs 64x64",    1,  64,  64,  256, 128,  2.3f,  0.55f },
+  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 1,  64,  64,  512, 256,  3.4f,  0.81f },
+  { I8Kernel::REG_128x128,  "regs 128x128",  1,  128, 128, 256, 128,  7.0f,  1.07f }
 };
 
 int64_t ceil_div( int64_t x, int64_t y ) { return ( x + y - 1 ) / y; }
@@ -140,8 +145,9 @@ Candidate const * choose_candidate( I8Args const & a, int64_t C, int32_t alignme
                        1.15 * l_bytes / 5.3e6 );
     }
     if( l_few ) {
-      l_us = std::max( l_c.fixed_us + double( l_k ) / l_c.step_k * l_c.step_us,
-                       l_groups * ( l_k * 1e-6 * ( l_c.row_us + l_c.few_us * std::min( a.M, a.N ) ) + 0.4e-3 ) );
+      int32_t const l_rows = std::min( a.M, a.N );
+      l_us = std::max( l_c.fixed_us + double( l_k ) / l_c.step_k * ( l_c.step_us + l_c.step_few_us * l_rows ),
+                       l_groups * ( l_k * 1e-6 * ( l_c.row_us + l_c.few_us * l_rows ) + 0.4e-3 ) );
     }
     // a grid's threads are counted in 32 bits
     if( l_groups * l_c.threads >= 4294967296.0 ) continue;

@@ -266,7 +266,9 @@ def test_refuses_missing_tensors(torch_cuda):
 
 # a size for each kernel that a product may take, with tiles cut off on both
 # sides, one K block and several, K ending inside a block
-KERNELS = [("few 4", 1, 4096, 500), ("few 4", 4, 5012, 130), ("few 4", 3, 4607, 301), ("few 16", 5, 1040, 140), ("few 16", 5, 997, 140), ("few 16", 5, 1044, 140), ("few 32", 29, 2064, 140),
+KERNELS = [("few 4", 1, 4096, 500), ("few 4", 4, 5012, 130), ("few 4", 3, 4607, 301),
+           ("few 8 parts", 8, 4096, 500), ("few 8 parts", 5, 5012, 130), ("few 8 parts", 7, 4607, 301),
+           ("few 16 parts", 16, 8192, 500), ("few 16 parts", 9, 5012, 130), ("few 16 parts", 13, 4607, 301), ("few 16", 5, 1040, 140), ("few 16", 5, 997, 140), ("few 16", 5, 1044, 140), ("few 32", 29, 2064, 140),
            ("few 32", 29, 515, 140), ("few 32", 29, 1044, 140), ("tile 32x32", 70, 1040, 200),
            ("tile 64x32", 130, 1040, 2050), ("tile 64x64", 70, 96, 200), ("tile 64x64", 600, 2064, 1300), ("tile 128x64", 1400, 2064, 1300),
            ("tile 128x128", 1500, 4112, 2050), ("tile 128x128", 3000, 96, 700), ("tile 256x128", 4072, 2048, 2048),
@@ -285,7 +287,7 @@ def test_every_kernel(torch_cuda, name, m, k, n, swap):
 
 
 @pytest.mark.parametrize("k", [1008, 1024, 1040, 2064, 4096, 4111, 6147, 8192, 9001])
-@pytest.mark.parametrize("m,n", [(1, 37), (2, 203), (3, 1030), (4, 64), (64, 4)])
+@pytest.mark.parametrize("m,n", [(1, 37), (2, 203), (3, 1030), (4, 64), (64, 4), (6, 90), (8, 513), (9, 70), (16, 200)])
 def test_parts_of_k(torch_cuda, m, n, k):
     """K in 4 parts of whole and cut pieces, parts with nothing in them."""
     run(torch_cuda, "tk,ok->to", dict(t=m, k=k, o=n), eir.BF16, seed=k)
