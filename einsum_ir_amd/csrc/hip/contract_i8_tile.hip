@@ -6,12 +6,14 @@
 // a K group and KG groups, which take the blocks of 128 k in turn and add their
 // sums in LDS at the end (integers: in any order the same).
 //
-// LDS holds 128 k of a row in 128 bytes, 16-byte piece g of row r at place
-// g ^ swz(r), so that the fragment reads (16 bytes a lane, 32 rows) touch every
-// bank equally.  Where rows are 16-byte aligned the pieces go there directly
-// (buffer_load ... lds, 8 rows an instruction, whole 128-byte lines); else
-// through registers, from any byte address.  Two buffers: the loads of block
-// t + 1 fly while block t is multiplied, one barrier a block.
+// Operands go from global memory into LDS directly (buffer_load ... lds).  Rows
+// at multiples of 16 bytes: 128 k of a row in 128 bytes, 16-byte piece g of row r
+// at place g ^ swz(r), so that the fragment reads (16 bytes a lane, 32 rows)
+// touch every bank equally.  Rows anywhere (SHIFT): the dwords that hold the 128
+// k, in 144 bytes; a fragment is read with the dword after it and shifted by its
+// row's first byte, and k from K on count as zeros on one side (2048 a side with
+// K = 2050: 22 us, byte-wise through registers 30, K = 2048 15).  Two to four
+// buffers, one barrier a block.
 //
 // The channels' side is the first operand of the matrix instruction, so a lane
 // holds 4 neighbouring columns of the output; the tile goes out through LDS in
@@ -28,70 +30,75 @@ typedef float f32x4 __attribute__( ( ext_vector_type( 4 ) ) );
 
 constexpr int kBk = 128;      // k of a block
 
-// how an operand's pieces get into LDS
-enum Load : int {
-  LOAD_DMA    = 0,    // directly: rows and K at multiples of 16 bytes
-  LOAD_DWORDS = 1,    // through registers: at multiples of 4
-  LOAD_BYTES  = 2     // through registers: anywhere
-};
-
-// ROWS rows of an operand by WAVES waves, one K group's side of the tile
-template< int ROWS, int WAVES, int LOAD >
+// ROWS rows of an operand by WAVES waves, one K group's side of the tile, loaded
+// 64 pieces of 16 bytes at a time.
+// Rows (and K) at multiples of 16 bytes: 8 pieces a row, piece g of row r at
+// place g ^ swz(r).  SHIFT, rows anywhere: the 9 pieces that hold a row's 128 k
+// from the dword on that the row's first byte lies in, one after the other; the
+// pitch of 144 bytes spreads 16 rows over all banks.
+template< int ROWS, int WAVES, bool SHIFT >
 struct Side {
-  static constexpr bool DMA   = LOAD == LOAD_DMA;
-  static constexpr int PIECES = ROWS / 8;             // of 8 rows x 128 bytes
-  static constexpr int EACH   = PIECES / WAVES;       // a wave's pieces
-  static_assert( PIECES % WAVES == 0, "pieces have to divide over the waves" );
+  static constexpr int PER_ROW = SHIFT ? 9 : 8;
+  static constexpr int PITCH   = 16 * PER_ROW;
+  static constexpr int LOADS   = ( ROWS * PER_ROW + 63 ) / 64;
+  static constexpr int EACH    = ( LOADS + WAVES - 1 ) / WAVES;      // a wave's loads
+  static constexpr int BYTES   = EACH * WAVES * 1024;
+  static_assert( SHIFT || LOADS % WAVES == 0, "loads have to divide over the waves" );
 
-  uint32_t m_off[DMA ? EACH : 1];       // bytes from the tile's first row to the lane's 16 bytes of block 0
+  uint32_t m_off[EACH];       // bytes from the tile's first row to the lane's piece of block 0
   i32x4    m_rsrc;
-  int8_t const * m_row[DMA ? 1 : EACH];
-  I8Vec< LOAD == LOAD_BYTES > m_reg[DMA ? 1 : EACH];
-  int      m_k[2];                      // the lane's k of a block in even and odd pieces
-  uint32_t m_first;                     // the wave's first piece
+  int      m_k[2];            // the lane's k of a block in even and odd loads (not SHIFT)
+  uint32_t m_first;           // the wave's first load
 
-  __device__ inline void init( int8_t const * tile, int32_t stride, int32_t rows, int wave, int lane ) {
+  __device__ inline void init( int8_t const * tile, int32_t stride, int32_t rows, int32_t K, int wave, int lane ) {
     m_first = wave * EACH;
-    if constexpr( DMA ) m_rsrc = kern::make_rsrc( tile, kern::kDmaOob );
+    if constexpr( SHIFT ) {
+      // up to the dword of the last k of the tile's last row
+      uint32_t const l_off = uint32_t( reinterpret_cast< uintptr_t >( tile ) & 3 );
+      m_rsrc = kern::make_rsrc( tile - l_off, ( l_off + uint32_t( min( rows, ROWS ) - 1 ) * uint32_t( stride ) + uint32_t( K ) + 3 ) & ~3u );
 #pragma unroll
-    for( int l_i = 0; l_i < 2; l_i++ ) m_k[l_i] = 16 * ( ( lane % 8 ) ^ int( kern::swz_k( 8 * l_i + lane / 8 ) ) );
+      for( int l_i = 0; l_i < EACH; l_i++ ) {
+        uint32_t const l_piece = ( m_first + l_i ) * 64 + lane, l_r = l_piece / PER_ROW;
+        m_off[l_i] = ( ( l_off + min( l_r, uint32_t( rows - 1 ) ) * uint32_t( stride ) ) & ~3u ) + 16 * ( l_piece % PER_ROW );
+        if( l_r >= ROWS ) m_off[l_i] = kern::kDmaOob;
+      }
+    }
+    else {
+      m_rsrc = kern::make_rsrc( tile, kern::kDmaOob );
 #pragma unroll
-    for( int l_i = 0; l_i < EACH; l_i++ ) {
-      // rows past the tensor read its last one and are not stored
-      int32_t const l_r = min( int32_t( 8 * ( m_first + l_i ) + lane / 8 ), rows - 1 );
-      if constexpr( DMA ) m_off[l_i] = uint32_t( l_r * stride + k_of( l_i ) );
-      else                m_row[l_i] = tile + int64_t( l_r ) * stride;
+      for( int l_i = 0; l_i < 2; l_i++ ) m_k[l_i] = 16 * ( ( lane % 8 ) ^ int( kern::swz_k( 8 * l_i + lane / 8 ) ) );
+#pragma unroll
+      for( int l_i = 0; l_i < EACH; l_i++ ) {
+        // rows past the tensor read its last one and are not stored
+        int32_t const l_r = min( int32_t( 8 * ( m_first + l_i ) + lane / 8 ), rows - 1 );
+        m_off[l_i] = uint32_t( l_r * stride + k_of( l_i ) );
+      }
     }
   }
   __device__ inline int k_of( int i ) const { return m_k[( m_first + i ) % 2]; }
 
-  // starts the load of the wave's piece I of the block at k0; DMA: into lds
+  // starts the wave's load I of the block at k0 into lds
   template< int I >
   __device__ __attribute__( ( always_inline ) ) inline void issue( uint32_t lds, int32_t k0, int32_t K ) {
-    if constexpr( DMA ) {
-      uint32_t l_off = m_off[I];
-      // K is a multiple of 16, so a lane's k are inside or outside; outside: zeros
-      if( k0 + kBk > K && k0 + k_of( I ) >= K ) l_off = kern::kDmaOob;
-      kern::set_m0( lds + ( m_first + I ) * 1024 );
-      kern::dma16_so< 0 >( m_rsrc, l_off, uint32_t( k0 ) );
+    uint32_t l_off = m_off[I], l_k0 = uint32_t( k0 );
+    if constexpr( SHIFT ) {
+      // where the pieces may leave the tensor, the k go into the offset that
+      // the buffer's range check sees
+      if( k0 + PITCH > K ) {
+        l_off += l_k0;
+        l_k0 = 0;
+      }
     }
-    else {
-      m_reg[I].load( m_row[I] + i8_piece( k0 + k_of( I ), K ).at );
-    }
-  }
-
-  // piece I from registers into lds
-  template< int I >
-  __device__ __attribute__( ( always_inline ) ) inline void put( char * lds, int32_t k0, int32_t K, int lane ) {
-    i32x4 l_v = m_reg[I].value();
-    if( k0 + kBk > K ) {
-      int const l_skip = i8_piece( k0 + k_of( I ), K ).skip;
-#pragma unroll
-      for( int l_d = 0; l_d < 4; l_d++ ) l_v[l_d] &= int32_t( i8_mask( l_skip, l_d ) );
-    }
-    *reinterpret_cast< i32x4 * >( lds + ( m_first + I ) * 1024 + 16 * lane ) = l_v;
+    // K is a multiple of 16, so a lane's k are inside or outside; outside: zeros
+    else if( k0 + kBk > K && k0 + k_of( I ) >= K ) l_off = kern::kDmaOob;
+    kern::set_m0( lds + ( m_first + I ) * 1024 );
+    kern::dma16_so< 0 >( m_rsrc, l_off, l_k0 );
   }
 };
+
+// 16 k of a row as read from LDS; SHIFT: the dwords they lie in
+template< bool SHIFT > struct Raw { i32x4 v; };
+template<> struct Raw< true > { i32x4 v; int32_t w; };
 
 // elements from row to row of a wave's output slab in LDS
 template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T ) );
@@ -136,13 +143,14 @@ __device__ inline void store_slab( I8Args const & a, T const * slab, int64_t out
   }
 }
 
-template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, bool SHIFT >
 __global__ __launch_bounds__( 64 * WM * WN * KG )
 void contract_i8_tile_kernel( I8Args a ) {
-  constexpr bool DMA = LOAD == LOAD_DMA;
   constexpr int WAVES = WM * WN;                       // of a K group
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks a wave
-  constexpr int STAGE = ( BM + BN ) * kBk;
+  typedef Side< BM, WAVES, SHIFT > SideA;
+  typedef Side< BN, WAVES, SHIFT > SideB;
+  constexpr int STAGE = SideA::BYTES + SideB::BYTES;
   constexpr int COLS = BN / WN;
   // a wave's output slab: fp32 32 rows, bf16 all of its rows
   constexpr int SLAB_F32 = 32 * kPitch< float, COLS > * 4, SLAB_BF16 = 32 * TM * kPitch< __bf16, COLS > * 2;
@@ -172,10 +180,12 @@ void contract_i8_tile_kernel( I8Args a ) {
   int32_t const l_m0 = ( l_band + l_r % ( 8 * l_tiles_n ) % l_high ) * BM;
   int32_t const l_n0 = ( l_r % ( 8 * l_tiles_n ) / l_high ) * BN;
 
-  Side< BM, WAVES, LOAD > l_a;
-  Side< BN, WAVES, LOAD > l_b;
-  l_a.init( a.a + l_c * a.c[I8_A] + int64_t( l_m0 ) * a.a_row, a.a_row, a.M - l_m0, l_wave, l_lane );
-  l_b.init( a.b + l_c * a.c[I8_B] + int64_t( l_n0 ) * a.b_col, a.b_col, a.N - l_n0, l_wave, l_lane );
+  int8_t const * const l_at_a = a.a + l_c * a.c[I8_A] + int64_t( l_m0 ) * a.a_row;
+  int8_t const * const l_at_b = a.b + l_c * a.c[I8_B] + int64_t( l_n0 ) * a.b_col;
+  SideA l_a;
+  SideB l_b;
+  l_a.init( l_at_a, a.a_row, a.M - l_m0, l_k, l_wave, l_lane );
+  l_b.init( l_at_b, a.b_col, a.N - l_n0, l_k, l_wave, l_lane );
 
   // scales and bias, needed after the loop
   bool const l_bias_rows = a.has( I8Args::BIAS_ROWS );
@@ -202,23 +212,15 @@ void contract_i8_tile_kernel( I8Args a ) {
   // first k of the group's step s; past the last block nothing is in range and
   // zeros are loaded
   auto k_of_step = [&]( int s ) -> int32_t { return min( s * KG + l_group, l_blocks ) * kBk; };
-  // pieces FROM to TO - 1 of the wave's, both sides counted through
-  constexpr int EACH_A = Side< BM, WAVES, LOAD >::EACH, EACH = EACH_A + Side< BN, WAVES, LOAD >::EACH;
+  // the wave's load i, those of both sides counted through
+  constexpr int EACH = SideA::EACH + SideB::EACH;
   auto issue = [&]( auto ic, int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
     constexpr int l_i = decltype( ic )::value;
     uint32_t const l_to = l_buf_at + stage * STAGE;
-    if constexpr( l_i < EACH_A ) l_a.template issue< l_i >( l_to, k0, l_k );
-    else                         l_b.template issue< l_i - EACH_A >( l_to + BM * kBk, k0, l_k );
+    if constexpr( l_i < SideA::EACH ) l_a.template issue< l_i >( l_to, k0, l_k );
+    else                              l_b.template issue< l_i - SideA::EACH >( l_to + SideA::BYTES, k0, l_k );
   };
-  auto put = [&]( int stage, int32_t k0 ) __attribute__( ( always_inline ) ) {
-    kern::static_for< DMA ? 0 : EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
-      constexpr int l_i = decltype( ic )::value;
-      char * const l_to = l_buf + stage * STAGE;
-      if constexpr( l_i < EACH_A ) l_a.template put< l_i >( l_to, k0, l_k, l_lane );
-      else                         l_b.template put< l_i - EACH_A >( l_to + BM * kBk, k0, l_k, l_lane );
-    } );
-  };
-  // pieces of block 1 (two buffers) that are issued in front of the loop
+  // loads of block 1 (two buffers) that are issued in front of the loop
   constexpr int EARLY = ( EACH + 1 ) / 2;
   kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, k_of_step( 0 ) ); } );
   if constexpr( STAGES > 2 ) {
@@ -231,28 +233,48 @@ void contract_i8_tile_kernel( I8Args a ) {
       kern::barrier_lds();
     }
   }
-  else if constexpr( DMA ) {
+  else {
     kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
     kern::wait_vmcnt< EARLY >();
-    kern::barrier_lds();
-  }
-  else {
-    put( 0, k_of_step( 0 ) );
-    kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, k_of_step( 1 ) ); } );
-    kern::wait_lgkmcnt0();
     kern::barrier_lds();
   }
 
   // Fragments of 32 k: TM of rows, then TN of columns.
   constexpr int FRAGS = TM + TN, MFMAS = TM * TN;
   constexpr int HELD = DEEP ? 4 : 2;
-  i32x4 l_f[HELD][FRAGS];
+  Raw< SHIFT > l_f[HELD][FRAGS];
   uint32_t const l_swz = kern::swz_k( l_row );       // of 32-row blocks: the same
-  auto read = [&]( auto fc, i32x4 * f, int stage, int q ) __attribute__( ( always_inline ) ) {
+  auto read = [&]( auto fc, Raw< SHIFT > * f, int stage, int q ) __attribute__( ( always_inline ) ) {
     constexpr int l_i = decltype( fc )::value;
-    int const l_first = l_i < TM ? l_wm + 32 * l_i : BM + l_wn + 32 * ( l_i - TM );
-    f[l_i] = *reinterpret_cast< i32x4 const * >( l_buf + stage * STAGE + l_first * kBk + l_row * kBk
-                                                 + ( ( ( 2 * q + l_lane / 32 ) ^ l_swz ) << 4 ) );
+    int const l_first = l_i < TM ? ( l_wm + 32 * l_i ) * SideA::PITCH : SideA::BYTES + ( l_wn + 32 * ( l_i - TM ) ) * SideB::PITCH;
+    char const * const l_p = l_buf + stage * STAGE + l_first + l_row * SideA::PITCH;
+    if constexpr( SHIFT ) {
+      f[l_i].v = *reinterpret_cast< i32x4 const * >( l_p + 16 * ( 2 * q + l_lane / 32 ) );
+      f[l_i].w = *reinterpret_cast< int32_t const * >( l_p + 16 * ( 2 * q + l_lane / 32 ) + 16 );
+    }
+    else f[l_i].v = *reinterpret_cast< i32x4 const * >( l_p + ( ( ( 2 * q + l_lane / 32 ) ^ l_swz ) << 4 ) );
+  };
+  // SHIFT: the first byte of a row in its dword (of rows 32 apart the same), and
+  // from K on zeros on A's side
+  int const l_shift_a = int( ( reinterpret_cast< uintptr_t >( l_at_a ) + uint32_t( l_row ) * uint32_t( a.a_row ) ) & 3 );
+  int const l_shift_b = int( ( reinterpret_cast< uintptr_t >( l_at_b ) + uint32_t( l_row ) * uint32_t( a.b_col ) ) & 3 );
+  auto ready = [&]( auto fc, Raw< SHIFT > const * f, int32_t k0, int q ) __attribute__( ( always_inline ) ) -> i32x4 {
+    constexpr int l_i = decltype( fc )::value;
+    i32x4 l_v = f[l_i].v;
+    if constexpr( SHIFT ) {
+      int const l_s = l_i < TM ? l_shift_a : l_shift_b;
+      l_v = i32x4{ int32_t( __builtin_amdgcn_alignbyte( l_v[1], l_v[0], l_s ) ), int32_t( __builtin_amdgcn_alignbyte( l_v[2], l_v[1], l_s ) ),
+                   int32_t( __builtin_amdgcn_alignbyte( l_v[3], l_v[2], l_s ) ), int32_t( __builtin_amdgcn_alignbyte( f[l_i].w, l_v[3], l_s ) ) };
+      if( l_i < TM && k0 + kBk > l_k ) {
+        int32_t const l_n = l_k - ( k0 + 32 * q + 16 * ( l_lane / 32 ) );      // bytes that count
+#pragma unroll
+        for( int l_d = 0; l_d < 4; l_d++ ) {
+          int32_t const l_left = l_n - 4 * l_d;
+          l_v[l_d] &= l_left >= 4 ? -1 : l_left <= 0 ? 0 : int32_t( ( 1u << ( 8 * l_left ) ) - 1 );
+        }
+      }
+    }
+    return l_v;
   };
   i32x16 l_acc[TN][TM];
 #pragma unroll
@@ -271,15 +293,18 @@ void contract_i8_tile_kernel( I8Args a ) {
     kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
       constexpr int l_q = decltype( qc )::value;
       if constexpr( l_q == 3 ) {
-        if constexpr( DMA ) kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
-        else                put( l_next, k_of_step( s + 1 ) );
+        kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
         kern::wait_lgkmcnt0();
         kern::barrier_lds();
       }
       int32_t const l_k0 = k_of_step( s + ( STAGES > 2 ? STAGES - 1 : l_q == 3 ? 2 : 1 ) );
+      i32x4 l_g[FRAGS];
+      kern::static_for< FRAGS >( [&]( auto fc ) __attribute__( ( always_inline ) ) {
+        l_g[decltype( fc )::value] = ready( fc, l_f[l_q % 2], k_of_step( s ), l_q );
+      } );
       kern::static_for< MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) {
         constexpr int l_m = decltype( mc )::value;
-        multiply( mc, l_f[l_q % 2] );
+        multiply( mc, l_g );
         // the next part's fragments over the first half of the instructions
         constexpr int l_slots = ( MFMAS + 1 ) / 2;
         if constexpr( l_m < l_slots ) {
@@ -295,15 +320,12 @@ void contract_i8_tile_kernel( I8Args a ) {
             issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_free, l_k0 );
           } );
         }
-        if constexpr( STAGES == 2 && DMA && ( l_q == 3 || l_q == 0 ) ) {
+        if constexpr( STAGES == 2 && ( l_q == 3 || l_q == 0 ) ) {
           constexpr int l_p0 = l_q == 3 ? 0 : EARLY, l_n = l_q == 3 ? EARLY : EACH - EARLY;
           constexpr int l_from = l_p0 + l_n * l_m / MFMAS, l_to = l_p0 + l_n * ( l_m + 1 ) / MFMAS;
           kern::static_for< l_to - l_from >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
             issue( std::integral_constant< int, l_from + decltype( ic )::value >(), l_q == 3 ? l_st : l_next, l_k0 );
           } );
-        }
-        if constexpr( !DMA && l_q == 3 && l_m == 0 ) {
-          kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, l_k0 ); } );
         }
         __builtin_amdgcn_sched_barrier( 0 );
       } );
@@ -328,9 +350,13 @@ void contract_i8_tile_kernel( I8Args a ) {
       issue( ic, ( l_st + STAGES - 1 ) % STAGES, l_k0 );
     } );
     __builtin_amdgcn_sched_barrier( 0 );
-    kern::static_for< 4 * MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) {
-      constexpr int l_m = decltype( mc )::value;
-      multiply( std::integral_constant< int, l_m % MFMAS >(), l_f[l_m / MFMAS % HELD] );
+    kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_q = decltype( qc )::value;
+      i32x4 l_g[FRAGS];
+      kern::static_for< FRAGS >( [&]( auto fc ) __attribute__( ( always_inline ) ) {
+        l_g[decltype( fc )::value] = ready( fc, l_f[l_q % HELD], k_of_step( s ), l_q );
+      } );
+      kern::static_for< MFMAS >( [&]( auto mc ) __attribute__( ( always_inline ) ) { multiply( mc, l_g ); } );
     } );
   };
   if constexpr( !DEEP ) {
@@ -351,7 +377,7 @@ void contract_i8_tile_kernel( I8Args a ) {
       } );
     }
   }
-  if constexpr( DMA ) kern::wait_vmcnt< 0 >();
+  kern::wait_vmcnt< 0 >();
 #pragma unroll
   for( int l_i = 0; l_i < CH; l_i++ ) {
     int const l_n = l_i * 64 * WAVES * KG + threadIdx.x;
@@ -430,10 +456,10 @@ void contract_i8_tile_kernel( I8Args a ) {
   else             finish( 0.0f, std::integral_constant< int, 1 >() );
 }
 
-template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, int LOAD >
+template< int BM, int BN, int WM, int WN, int KG, int STAGES, bool DEEP, bool SHIFT >
 int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
   uint32_t const l_grid = uint32_t( ( int64_t( a.M ) + BM - 1 ) / BM * ( ( int64_t( a.N ) + BN - 1 ) / BN ) * C );
-  hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, DEEP, LOAD > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
+  hipLaunchKernelGGL( ( contract_i8_tile_kernel< BM, BN, WM, WN, KG, STAGES, DEEP, SHIFT > ), dim3( l_grid ), dim3( 64 * WM * WN * KG ),
                       0, stream, a );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
@@ -447,27 +473,18 @@ int launch_shape( I8Args const & a, int64_t C, hipStream_t stream ) {
 int launch_i8_tile( I8Args const & args, int64_t C, I8Kernel kernel, hipStream_t stream ) {
   I8Args a = args;
   if( a.o_col == 1 ) a.k_flags |= I8Args::VEC_OUT;
-  bool const l_dwords = i8_aligned( a, 4 );
   switch( kernel ) {
-    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, true, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, true, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_128x64:  return launch_shape< 128, 64, 2, 2, 1, 3, false, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, false, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, false, LOAD_DMA >( a, C, stream );
-    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, false, LOAD_DMA >( a, C, stream );
-    case I8Kernel::REG_32x32:
-      return l_dwords ? launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_DWORDS >( a, C, stream )
-                      : launch_shape< 32, 32, 1, 1, 4, 2, false, LOAD_BYTES >( a, C, stream );
-    case I8Kernel::REG_64x64:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_DWORDS >( a, C, stream )
-                      : launch_shape< 64, 64, 2, 2, 1, 2, false, LOAD_BYTES >( a, C, stream );
-    case I8Kernel::REG_64x64_K2:
-      return l_dwords ? launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_DWORDS >( a, C, stream )
-                      : launch_shape< 64, 64, 2, 2, 2, 2, false, LOAD_BYTES >( a, C, stream );
-    case I8Kernel::REG_128x128:
-      return l_dwords ? launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_DWORDS >( a, C, stream )
-                      : launch_shape< 128, 128, 2, 2, 1, 2, false, LOAD_BYTES >( a, C, stream );
+    case I8Kernel::TILE_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, false >( a, C, stream );
+    case I8Kernel::TILE_64x32:   return launch_shape< 64, 32, 2, 1, 2, 4, true, false >( a, C, stream );
+    case I8Kernel::TILE_64x64:   return launch_shape< 64, 64, 2, 2, 1, 4, true, false >( a, C, stream );
+    case I8Kernel::TILE_128x64:  return launch_shape< 128, 64, 2, 2, 1, 3, false, false >( a, C, stream );
+    case I8Kernel::TILE_128x128: return launch_shape< 128, 128, 2, 4, 1, 4, false, false >( a, C, stream );
+    case I8Kernel::TILE_256x128: return launch_shape< 256, 128, 4, 2, 1, 3, false, false >( a, C, stream );
+    case I8Kernel::TILE_256x256: return launch_shape< 256, 256, 4, 2, 1, 2, false, false >( a, C, stream );
+    case I8Kernel::SHIFT_32x32:   return launch_shape< 32, 32, 1, 1, 4, 3, true, true >( a, C, stream );
+    case I8Kernel::SHIFT_64x64:   return launch_shape< 64, 64, 2, 2, 1, 3, true, true >( a, C, stream );
+    case I8Kernel::SHIFT_128x128: return launch_shape< 128, 128, 2, 4, 1, 3, false, true >( a, C, stream );
+    case I8Kernel::SHIFT_256x128: return launch_shape< 256, 128, 4, 2, 1, 2, false, true >( a, C, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction_i8: unknown tile" );
   }
 }

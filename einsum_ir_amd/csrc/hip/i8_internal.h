@@ -68,8 +68,8 @@ struct I8Args {
 };
 static_assert( sizeof( I8Args ) == 112, "kernel arguments" );
 
-// The kernels.  TILE_*: through LDS (contract_i8_tile.hip); their rows come in
-// directly where they lie at multiples of 16 bytes, else through registers.
+// The kernels.  TILE_*: through LDS (contract_i8_tile.hip), rows (and K) at
+// multiples of 16 bytes.
 enum class I8Kernel : int32_t {
   GENERAL,            // any strides, 64 x 64 tiles (contract_i8.hip)
   FEW_4,              // a side of up to 4, K over the waves and in 4 parts (contract_i8_few.hip)
@@ -84,10 +84,10 @@ enum class I8Kernel : int32_t {
   TILE_128x128,
   TILE_256x128,
   TILE_256x256,
-  REG_32x32,          // through registers
-  REG_64x64,
-  REG_64x64_K2,       // with K over two groups of waves
-  REG_128x128
+  SHIFT_32x32,        // the same, rows anywhere
+  SHIFT_64x64,
+  SHIFT_128x128,
+  SHIFT_256x128
 };
 
 // rows of both operands, and K, at multiples of n bytes

@@ -76,15 +76,15 @@ std::string sizes_of( I8Loops const & l ) {
 // nothing else bounds them, and at least (row + few * few rows) for every 10^6 k
 // of all workgroups, which their 64-byte pieces of rows take in the caches, and
 // 0.4 ns for each workgroup.
-// Measured over 170 products with rows at multiples of 16 bytes, 50 at 4, 80 at
-// others (1 to 8192 rows, 16 to 16384 columns, K 64 to 12288), K in parts over
-// 100.  The times that follow are off by 10 to 20 % (root mean square), but alike
-// for neighbours: the kernel chosen is 1 % slower than the best of all on average
+// Measured over 170 products with rows at multiples of 16 bytes and 150 at others
+// (1 to 8192 rows, 16 to 16384 columns, K 64 to 12288), K in parts over 100.  The
+// times that follow are off by 10 to 20 % (root mean square), but alike for
+// neighbours: the kernel chosen is 1 % slower than the best of all on average
 // (64 x 64 tiles everywhere: 36 %).
 struct Candidate {
   I8Kernel     kernel;
   char const * name;
-  int32_t      alignment;          // 16: these rows only; 4, 1: of such rows (few: 4 or 16)
+  int32_t      alignment;          // of the rows; tiles: 16 bytes or not (1), few-sided: 4 (or more) or not (1)
   int32_t      rows, cols, threads, step_k;
   float        fixed_us, step_us;
   float        step_few_us, row_us, few_us;      // few-sided kernels
@@ -102,19 +102,15 @@ Candidate const kCandidates[] = {
   { I8Kernel::TILE_128x128, "tile 128x128",  16, 128, 128, 512, 128,  3.2f,  0.44f },
   { I8Kernel::TILE_256x128, "tile 256x128",  16, 256, 128, 512, 128,  5.1f,  0.72f },
   { I8Kernel::TILE_256x256, "tile 256x256",  16, 256, 256, 512, 128,  8.4f,  1.09f },
-  { I8Kernel::REG_32x32,    "regs 32x32",    4,  32,  32,  256, 512,  3.0f,  0.51f },
-  { I8Kernel::REG_64x64,    "regs 64x64",    4,  64,  64,  256, 128,  1.9f,  0.33f },
-  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 4,  64,  64,  512, 256,  3.0f,  0.45f },
-  { I8Kernel::REG_128x128,  "regs 128x128",  4,  128, 128, 256, 128,  5.8f,  0.63f },
   { I8Kernel::FEW_4,        "few 4",         1,  4,   4,   512, 1024, 0.50f, 0.25f, 0.0f,   1.0f,  0.11f },
   { I8Kernel::FEW_8_PARTS,  "few 8 parts",   1,  8,   4,   512, 1024, 0.50f, 0.50f, 0.0f,   1.0f,  0.14f },
   { I8Kernel::FEW_16_PARTS, "few 16 parts",  1,  16,  4,   512, 1024, 0.60f, 0.86f, 0.0f,   1.0f,  0.16f },
   { I8Kernel::FEW_16,       "few 16",        1,  16,  16,  512, 1024, 0.0f,  0.75f, 0.035f, 5.0f,  0.19f },
   { I8Kernel::FEW_32,       "few 32",        1,  32,  16,  512, 1024, 0.0f,  0.75f, 0.035f, 5.0f,  0.19f },
-  { I8Kernel::REG_32x32,    "regs 32x32",    1,  32,  32,  256, 512,  3.8f,  0.93f },
-  { I8Kernel::REG_64x64,    "regs 64x64",    1,  64,  64,  256, 128,  2.3f,  0.55f },
-  { I8Kernel::REG_64x64_K2, "regs 64x64 k2", 1,  64,  64,  512, 256,  3.4f,  0.81f },
-  { I8Kernel::REG_128x128,  "regs 128x128",  1,  128, 128, 256, 128,  7.0f,  1.07f }
+  { I8Kernel::SHIFT_32x32,  "shift 32x32",   1,  32,  32,  256, 512,  2.5f,  0.54f },
+  { I8Kernel::SHIFT_64x64,  "shift 64x64",   1,  64,  64,  256, 128,  1.5f,  0.40f },
+  { I8Kernel::SHIFT_128x128, "shift 128x128", 1, 128, 128, 512, 128,  3.7f,  0.69f },
+  { I8Kernel::SHIFT_256x128, "shift 256x128", 1, 256, 128, 512, 128,  4.7f,  1.05f }
 };
 
 int64_t ceil_div( int64_t x, int64_t y ) { return ( x + y - 1 ) / y; }
@@ -128,9 +124,9 @@ Candidate const * choose_candidate( I8Args const & a, int64_t C, int32_t alignme
   int32_t const l_k = a.K();
   double const l_bytes = double( C ) * ( ( double( a.M ) + a.N ) * l_k + double( a.has( I8Args::OUT_BF16 ) ? 2 : 4 ) * a.M * a.N );
   for( Candidate const & l_c : kCandidates ) {
-    // the rows of alignment 4 and 1 have their own entries, and those of 16 the few-sided kernels' of 4
+    // tiles: rows at multiples of 16 bytes or not; few-sided: of 4 or not
     bool const l_few = l_c.kernel <= I8Kernel::FEW_32;
-    if( l_few ? ( l_c.alignment == 1 ) != ( alignment == 1 ) : l_c.alignment != alignment ) continue;
+    if( l_few ? ( l_c.alignment == 1 ) != ( alignment == 1 ) : ( l_c.alignment == 16 ) != ( alignment == 16 ) ) continue;
     double l_groups, l_us;
     if( l_few ) {
       if( std::min( a.M, a.N ) > l_c.rows ) continue;

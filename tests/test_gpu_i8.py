@@ -272,9 +272,9 @@ KERNELS = [("few 4", 1, 4096, 500), ("few 4", 4, 5012, 130), ("few 4", 3, 4607, 
            ("few 32", 29, 515, 140), ("few 32", 29, 1044, 140), ("tile 32x32", 70, 1040, 200),
            ("tile 64x32", 130, 1040, 2050), ("tile 64x64", 70, 96, 200), ("tile 64x64", 600, 2064, 1300), ("tile 128x64", 1400, 2064, 1300),
            ("tile 128x128", 1500, 4112, 2050), ("tile 128x128", 3000, 96, 700), ("tile 256x128", 4072, 2048, 2048),
-           ("tile 256x256", 2100, 1040, 4300), ("regs 32x32", 70, 1044, 200), ("regs 32x32", 70, 1041, 140),
-           ("regs 64x64", 70, 515, 140), ("regs 64x64", 130, 1044, 2050), ("regs 64x64 k2", 130, 997, 2050),
-           ("regs 64x64 k2", 130, 2052, 2050), ("regs 128x128", 1000, 515, 2050), ("regs 128x128", 1000, 1044, 2050)]
+           ("tile 256x256", 2100, 1040, 4300), ("shift 32x32", 70, 1044, 200), ("shift 32x32", 70, 1041, 140),
+           ("shift 64x64", 70, 515, 140), ("shift 64x64", 600, 1044, 1300), ("shift 256x128", 2100, 2061, 4300),
+           ("shift 128x128", 1000, 515, 4050), ("shift 256x128", 2000, 1044, 2050), ("shift 128x128", 1000, 1044, 4050)]
 
 
 @pytest.mark.parametrize("name,m,k,n", KERNELS)
