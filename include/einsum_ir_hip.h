@@ -244,7 +244,9 @@ int etir_hip_permute_execute( etir_plan_t  plan,
  *
  * Strides are at least 0 and may be anything otherwise; the output's elements
  * have to lie apart.  Fast: both operands unit-stride along one K loop, and
- * M, N and C loops that fuse to one each.  A product of any size 0 in C, M or N
+ * M, N and C loops that fuse to one each, with strides below 2^31; operands
+ * whose rows and K are multiples of 16 bytes run up to twice as fast as others.
+ * A product of any size 0 in C, M or N
  * does nothing; without K the sums are 0.  At most 6 loops of one type that
  * cannot be fused.
  */
@@ -283,7 +285,8 @@ int etir_hip_contraction_i8_execute( etir_plan_t  plan,
  * scale = 0; a row with an infinity, a NaN or a product s * weight beyond fp32
  * has q = 0 and scale = NaN.
  * dtype (in, residual, total, values) and dtype_weight: ETIR_BF16 or ETIR_FP32;
- * q: int8; scale: fp32, `rows` of them.  Elements of a row are adjacent, row i
+ * q: int8; scale: fp32, `rows` of them.  rows is at most 2^31 - 1 and cols
+ * 2^30 - 1.  Elements of a row are adjacent, row i
  * starts at i * ld_*; ld_in and ld_residual may be less than cols (0: one row
  * for all), the output's ld_* not.  eps is at least 0.
  */
