@@ -1,7 +1,7 @@
 """GPU parity of the product of 8-bit integers with scales
 (etir_hip_contraction_i8_*).  No counterpart in the reference.
 
-Checker: the same contraction in float64.  The integer sum is exact, so an
+Oracle: the same contraction in float64.  The integer sum is exact, so an
 output is off by the roundings of the fp32 epilogue alone: the sum to fp32, two
 products and one addition, each within 2^-24 of a value no larger than
 |scaled sum| + |bias|, and half a unit of the output's last place.

@@ -1,7 +1,7 @@
 """GPU parity of the operators that round rows to 8 bits (etir_hip_norm_quant_*,
 etir_hip_act_quant_*).  No counterpart in the reference.
 
-Checker: the formulas in float64.  With y the row before rounding and a its
+Oracle: the formulas in float64.  With y the row before rounding and a its
 largest magnitude, the kernel's y carries at most 2 roundings (norm: sum and
 product) or 8 (SiLU: exponential, sum, quotient, product), its 127 / a two more
 and the product with it one, each 2^-24 relative: q is within 0.5 + 127 * 12 *
