@@ -397,6 +397,9 @@ int launch_quant( QuantPlan const & plan, QuantArgs const & args, hipStream_t st
   }
   a.rows = int32_t( plan.rows );
   a.cols = int32_t( plan.cols );
+  // rows of nothing: the scales are 0 (a vector in front of q's first dword would
+  // take the weight of a column that is not there)
+  if( a.cols == 0 ) a.weight = nullptr;
   a.ld_in = plan.ld_in;
   a.ld_second = plan.ld_second;
   a.ld_total = plan.ld_total;

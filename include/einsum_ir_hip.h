@@ -321,8 +321,9 @@ int etir_hip_norm_quant_execute( etir_plan_t  plan,
  *   q = rint( y * (127 / a) )                    scale = a / 127
  *   values = q * scale, rounded to dtype
  * f: ktype UNDEFINED (identity), RELU or SILU, v / (1 + exp(-v)) (0 below -88.7,
- * where exp(-v) leaves fp32).  Rows of zeros, of infinities and of NaN, types and row strides as for etir_hip_norm_quant_create.  With no
- * activation it lays out weights: one row, and so one scale, a channel.
+ * where exp(-v) leaves fp32).  Rows of zeros, of infinities and of NaN, types
+ * and row strides as for etir_hip_norm_quant_create.  With no activation it lays
+ * out weights: one row, and so one scale, a channel.
  */
 int etir_hip_act_quant_create( int64_t       rows,
                                int64_t       cols,
