@@ -17,8 +17,21 @@ scale for each channel; the hidden states between are bf16 or fp32.
 from . import ActQuantPlan, BF16, ContractionI8Plan, FP32, NormQuantPlan, RELU, contraction_i8_loops
 
 
+def _torch_stream(torch, stream):
+    """A torch stream of a stream, a handle, or None (the current one)."""
+    if stream is None:
+        return torch.cuda.current_stream()
+    if isinstance(stream, int):
+        return torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    return stream
+
+
 class LinearI8:
-    """Weights [channels, width] laid out once as 8-bit rows with a scale a channel."""
+    """Weights [channels, width] laid out once as 8-bit rows with a scale a channel.
+
+    They are laid out on the given stream (None: torch's current one), which waits for the current stream's work
+    before, and the current stream for it after: on both the weight may come straight from its making, be dropped
+    and the rows be used."""
 
     def __init__(self, torch, weight, bias=None, stream=None):
         if weight.dim() != 2 or weight.dtype not in (torch.bfloat16, torch.float32) or not weight.is_cuda:
@@ -26,13 +39,18 @@ class LinearI8:
         if bias is not None and (tuple(bias.shape) != (weight.shape[0],) or bias.dtype != torch.float32
                                  or not bias.is_cuda):
             raise ValueError("a bias holds one fp32 value a channel, on the GPU")
-        weight = weight.contiguous()
         self.channels, self.width = weight.shape
-        self.q = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
-        self.scale = torch.empty(self.channels, device=weight.device)
-        self.bias = None if bias is None else bias.contiguous()
         plan = ActQuantPlan(self.channels, self.width, dtype=BF16 if weight.dtype == torch.bfloat16 else FP32)
-        plan.execute(weight, self.q, self.scale, stream=stream)
+        s, current = _torch_stream(torch, stream), torch.cuda.current_stream()
+        # the copies and buffers come from the stream's own pool, as they are used on it
+        s.wait_stream(current)
+        with torch.cuda.stream(s):
+            weight = weight.contiguous()
+            self.q = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
+            self.scale = torch.empty(self.channels, device=weight.device)
+            self.bias = None if bias is None else bias.contiguous()
+            plan.execute(weight, self.q, self.scale, stream=s)
+        current.wait_stream(s)
 
     def plan(self, tokens, dtype):
         """The product of this layer with 8-bit rows of so many tokens."""
