@@ -73,6 +73,11 @@ class MlpI8:
         import torch
         if dtype not in (BF16, FP32):
             raise ValueError("hidden states are BF16 or FP32")
+        # kernels read the norms through their addresses: all tensors on the head's GPU
+        names = ("norm", "up", "down", "up_bias", "down_bias")
+        for t in [norm, head] + [b.get(n) for b in blocks for n in names]:
+            if t is not None and (not t.is_cuda or t.device != head.device):
+                raise ValueError("the network's tensors are on one GPU")
         self._torch, self.dtype, self.ktype, self.gated, self.eps, self.stream = torch, dtype, ktype, gated, eps, stream
         s, td = self._stream(), self._torch_dtype()
         with torch.cuda.stream(s):
@@ -118,8 +123,8 @@ class MlpI8:
     def __call__(self, x):
         """Logits [tokens, classes] of hidden states x [tokens, width]."""
         torch, td = self._torch, self._torch_dtype()
-        if x.dim() != 2 or x.shape[1] != self.width or x.dtype != td or not x.is_cuda or not x.is_contiguous():
-            raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {td} on the GPU")
+        if x.dim() != 2 or x.shape[1] != self.width or x.dtype != td or x.device != self.head.q.device or not x.is_contiguous():
+            raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {td} on the weights' GPU")
         tokens = x.shape[0]
         p = self._by_tokens.get(tokens)
         if p is None:
