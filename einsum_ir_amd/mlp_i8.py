@@ -65,9 +65,11 @@ class MlpI8:
     ``head`` [classes, width] end the network.  Weights are bf16 or fp32 and rounded to 8 bits here; norms have the
     type of the hidden states (dtype), biases fp32.  ktype: UNDEFINED_KTYPE, RELU or SILU.
 
-    Calls enqueue on the given stream (None: torch's current one when they are made).  A first call with a number of
-    tokens makes its plans and buffers; later ones allocate nothing and can be captured.  The logits are a buffer of
-    this object, written by the next call with as many tokens."""
+    The weights are laid out when the network is made, which waits for it: calls may follow on any stream.  They
+    enqueue on the given stream (None: torch's current one when they are made), where x has to be ready.  A first call
+    on a stream with a number of tokens makes its plans and buffers; later ones allocate nothing and can be captured.
+    Each stream has buffers of its own, so calls on different streams may overlap.  The logits are such a buffer,
+    written by the next call on the stream with as many tokens."""
 
     def __init__(self, blocks, norm, head, dtype=BF16, ktype=RELU, gated=False, eps=1e-6, stream=None):
         import torch
@@ -78,8 +80,10 @@ class MlpI8:
         for t in [norm, head] + [b.get(n) for b in blocks for n in names]:
             if t is not None and (not t.is_cuda or t.device != head.device):
                 raise ValueError("the network's tensors are on one GPU")
-        self._torch, self.dtype, self.ktype, self.gated, self.eps, self.stream = torch, dtype, ktype, gated, eps, stream
+        self._torch, self.dtype, self.ktype, self.gated, self.eps = torch, dtype, ktype, gated, eps
+        self.stream = None if stream is None else _torch_stream(torch, stream)
         s, td = self._stream(), self._torch_dtype()
+        s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             self.blocks = [dict(norm=b["norm"].to(td).contiguous(),
                                 up=LinearI8(torch, b["up"], b.get("up_bias"), s),
@@ -94,7 +98,8 @@ class MlpI8:
                 raise ValueError("the blocks' tensors do not fit each other")
         if self.norm.numel() != self.width:
             raise ValueError("the last norm does not fit the head")
-        self._by_tokens = {}
+        self._calls = {}
+        s.synchronize()
 
     def _stream(self):
         return self.stream if self.stream is not None else self._torch.cuda.current_stream()
@@ -125,11 +130,11 @@ class MlpI8:
         torch, td = self._torch, self._torch_dtype()
         if x.dim() != 2 or x.shape[1] != self.width or x.dtype != td or x.device != self.head.q.device or not x.is_contiguous():
             raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {td} on the weights' GPU")
-        tokens = x.shape[0]
-        p = self._by_tokens.get(tokens)
+        tokens, s = x.shape[0], self._stream()
+        p = self._calls.get((s.cuda_stream, tokens))
         if p is None:
-            p = self._by_tokens[tokens] = self._prepare(tokens)
-        s = self._stream()
+            with torch.cuda.stream(s):      # the buffers come from the pool of the stream that uses them
+                p = self._calls[s.cuda_stream, tokens] = self._prepare(tokens)
         state, delta = x, None
         for b, (up, act, down) in zip(self.blocks, p["blocks"]):
             p["norm"].execute(state, p["q"], p["q_scale"], residual=delta, weight=b["norm"],

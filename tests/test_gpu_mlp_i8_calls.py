@@ -36,3 +36,77 @@ def test_refuses_tensors_off_the_gpu(torch_cuda, where):
         blocks[1][name] = blocks[1][name].cpu()
     with pytest.raises(ValueError):
         MlpI8(blocks, norm, head)
+
+
+def _work(torch, n=3):
+    """Keeps the current stream busy for some ms."""
+    a = torch.full((4096, 4096), 1e-3, device="cuda")
+    for _ in range(n):
+        a = a @ a
+    return a
+
+
+@pytest.mark.parametrize("made_on", ["default", "side"])
+def test_calls_on_two_streams_at_once(torch_cuda, made_on):
+    """Calls with as many tokens on two streams, neither waiting for the other: each has buffers of its own."""
+    torch = torch_cuda
+    x = [torch.randn(40, 256, device="cuda").bfloat16() for _ in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0] if made_on == "side" else torch.cuda.default_stream()):
+        net = _net(torch, 256, 4096, 300, 3)
+    want = []
+    for v in x:
+        want.append(net(v).clone())
+        torch.cuda.synchronize()
+    got, ptrs = [[], []], set()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                y = net(x[i])
+                ptrs.add((i, y.data_ptr()))
+                got[i].append(y.clone())
+    torch.cuda.synchronize()
+    assert len(ptrs) == 2 and len({p for _, p in ptrs}) == 2
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i]), i
+
+
+def test_first_call_beside_work_of_the_current_stream(torch_cuda):
+    """A network with a stream of its own takes no memory that work still pending on the current stream writes."""
+    torch = torch_cuda
+    s = torch.cuda.Stream()
+    net = _net(torch, 256, 4096, 300, 2, stream=s)
+    x = torch.randn(300, 256, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    _work(torch)
+    for _ in range(4):      # freed at once, written when the work is done
+        for size in (300 * 256, 300 * 4096, 300 * 4096 * 2, 300 * 300 * 2):
+            torch.empty(size, dtype=torch.int8, device="cuda").fill_(77)
+    y = net(x)
+    s.synchronize()
+    first = y.clone()
+    torch.cuda.synchronize()
+    again = net(x)
+    s.synchronize()
+    assert torch.equal(first, y) and torch.equal(again, first)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_network_made_from_tensors_in_the_making(torch_cuda, own_stream):
+    """Weights that the current stream is still making, and calls on another stream right after."""
+    torch = torch_cuda
+    from einsum_ir_amd.mlp_i8 import MlpI8
+    blocks, norm, head = _tensors(torch, 256, 1024, 33)
+    x = torch.randn(9, 256, device="cuda").bfloat16()
+    want = MlpI8(blocks, norm, head)(x).clone()
+    torch.cuda.synchronize()
+    _work(torch)
+    late = [{k: None if v is None else v.clone() for k, v in b.items()} for b in blocks]
+    s = torch.cuda.Stream()
+    net = MlpI8(late, norm.clone(), head.clone(), stream=s if own_stream else None)
+    del late
+    with torch.cuda.stream(s):
+        y = net(x)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
