@@ -13,6 +13,7 @@ for each block, then a last norm and the product with the head's weights.  Every
 product reads 8-bit rows with a scale for each token and 8-bit weights with a
 scale for each channel; the hidden states between are bf16 or fp32.
 """
+from collections import OrderedDict
 
 from . import ActQuantPlan, BF16, ContractionI8Plan, FP32, NormQuantPlan, RELU, contraction_i8_loops
 
@@ -66,10 +67,13 @@ class MlpI8:
     type of the hidden states (dtype), biases fp32.  ktype: UNDEFINED_KTYPE, RELU or SILU.
 
     The weights are laid out when the network is made, which waits for it: calls may follow on any stream.  They
-    enqueue on the given stream (None: torch's current one when they are made), where x has to be ready.  A first call
-    on a stream with a number of tokens makes its plans and buffers; later ones allocate nothing and can be captured.
-    Each stream has buffers of its own, so calls on different streams may overlap.  The logits are such a buffer,
-    written by the next call on the stream with as many tokens."""
+    enqueue on the given stream (None: torch's current one when they are made), where x has to be ready.  Each stream
+    has buffers of its own, so calls on different streams may overlap: work buffers for the most tokens that it has
+    seen, and the logits of a number of tokens, which the next call on the stream with as many writes again.  Plans and
+    logits are kept for the last KEPT streams and numbers of tokens.  A call with one of these and no more tokens than
+    before allocates nothing and can be captured; what a captured call uses stays as long as this object."""
+
+    KEPT = 64
 
     def __init__(self, blocks, norm, head, dtype=BF16, ktype=RELU, gated=False, eps=1e-6, stream=None):
         import torch
@@ -90,7 +94,7 @@ class MlpI8:
                                 down=LinearI8(torch, b["down"], b.get("down_bias"), s)) for b in blocks]
             self.norm = norm.to(td).contiguous()
             self.head = LinearI8(torch, head, None, s)
-        self.width = self.head.width
+        self.width, self._td, self._device = self.head.width, td, self.head.q.device
         for b in self.blocks:
             hidden = b["up"].channels // (2 if gated else 1)
             if (b["up"].width != self.width or b["down"].channels != self.width or b["down"].width != hidden
@@ -98,7 +102,9 @@ class MlpI8:
                 raise ValueError("the blocks' tensors do not fit each other")
         if self.norm.numel() != self.width:
             raise ValueError("the last norm does not fit the head")
-        self._calls = {}
+        self._calls = OrderedDict()      # plans and logits by stream and tokens, the last used at the end
+        self._work = {}                  # work buffers by stream
+        self._captured = {}              # what graphs may write
         s.synchronize()
 
     def _stream(self):
@@ -107,17 +113,21 @@ class MlpI8:
     def _torch_dtype(self):
         return self._torch.bfloat16 if self.dtype == BF16 else self._torch.float32
 
-    def _prepare(self, tokens):
-        torch, td = self._torch, self._torch_dtype()
-        dev = self.head.q.device
+    def _work_buffers(self, tokens):
+        """What no caller sees, for up to so many tokens."""
+        torch, td, dev = self._torch, self._td, self._device
         empty = lambda *shape, **kw: torch.empty(shape, device=dev, **kw)  # noqa: E731
         wide = max([b["down"].width for b in self.blocks], default=0)
+        return dict(tokens=tokens, q=empty(tokens, self.width, dtype=torch.int8), q_scale=empty(tokens),
+                    a=empty(tokens * wide, dtype=torch.int8), a_scale=empty(tokens),
+                    h=empty(tokens * wide * (2 if self.gated else 1), dtype=td),
+                    total=empty(tokens, self.width, dtype=td), delta=empty(tokens, self.width, dtype=td))
+
+    def _prepare(self, tokens):
+        """Plans and logits of a number of tokens."""
         p = dict(norm=NormQuantPlan(tokens, self.width, dtype=self.dtype, eps=self.eps),
-                 q=empty(tokens, self.width, dtype=torch.int8), q_scale=empty(tokens),
-                 a=empty(tokens * wide, dtype=torch.int8), a_scale=empty(tokens),
-                 h=empty(tokens * wide * (2 if self.gated else 1), dtype=td),
-                 total=empty(tokens, self.width, dtype=td), delta=empty(tokens, self.width, dtype=td),
-                 logits=empty(tokens, self.head.channels, dtype=td), head=self.head.plan(tokens, self.dtype), blocks=[])
+                 logits=self._torch.empty((tokens, self.head.channels), device=self._device, dtype=self._td),
+                 head=self.head.plan(tokens, self.dtype), blocks=[])
         for b in self.blocks:
             f, n = b["down"].width, b["up"].channels
             p["blocks"].append((b["up"].plan(tokens, self.dtype),
@@ -125,32 +135,52 @@ class MlpI8:
                                 b["down"].plan(tokens, self.dtype)))
         return p
 
+    def _of_call(self, s, tokens):
+        """Plans and logits, and work buffers of a call on s, the current stream."""
+        key = s.cuda_stream, tokens
+        p, w = self._calls.get(key), self._work.get(s.cuda_stream)
+        if p is None:
+            p = self._calls[key] = self._prepare(tokens)
+            if len(self._calls) > self.KEPT:
+                (gone, _), _ = self._calls.popitem(last=False)
+                if all(stream != gone for stream, _ in self._calls):
+                    self._work.pop(gone, None)
+        else:
+            self._calls.move_to_end(key)
+        if w is None or w["tokens"] < tokens:
+            # the smaller ones go back to the stream's pool, in order with its work
+            w = self._work[s.cuda_stream] = self._work_buffers(tokens)
+        if self._torch.cuda.is_current_stream_capturing():
+            self._captured.update({id(p): p, id(w): w})
+        return p, w
+
     def __call__(self, x):
         """Logits [tokens, classes] of hidden states x [tokens, width]."""
-        torch, td = self._torch, self._torch_dtype()
-        if x.dim() != 2 or x.shape[1] != self.width or x.dtype != td or x.device != self.head.q.device or not x.is_contiguous():
-            raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {td} on the weights' GPU")
-        tokens, s = x.shape[0], self._stream()
-        p = self._calls.get((s.cuda_stream, tokens))
-        if p is None:
-            with torch.cuda.stream(s):      # the buffers come from the pool of the stream that uses them
-                p = self._calls[s.cuda_stream, tokens] = self._prepare(tokens)
+        if (x.dim() != 2 or x.shape[1] != self.width or x.dtype != self._td or x.device != self._device
+                or not x.is_contiguous()):
+            raise ValueError(f"x is a contiguous [tokens, {self.width}] tensor of {self._td} on the weights' GPU")
+        s = self._stream()
+        if self.stream is None:
+            p, w = self._of_call(s, x.shape[0])
+        else:
+            with self._torch.cuda.stream(s):      # the buffers come from the pool of the stream that uses them
+                p, w = self._of_call(s, x.shape[0])
         state, delta = x, None
         for b, (up, act, down) in zip(self.blocks, p["blocks"]):
-            p["norm"].execute(state, p["q"], p["q_scale"], residual=delta, weight=b["norm"],
-                              total=None if delta is None else p["total"], stream=s)
-            up.execute(p["q"], b["up"].q, p["h"], scale_left=p["q_scale"], scale_right=b["up"].scale,
+            p["norm"].execute(state, w["q"], w["q_scale"], residual=delta, weight=b["norm"],
+                              total=None if delta is None else w["total"], stream=s)
+            up.execute(w["q"], b["up"].q, w["h"], scale_left=w["q_scale"], scale_right=b["up"].scale,
                        bias=b["up"].bias, stream=s)
             f = b["down"].width
-            act.execute(p["h"][f:] if self.gated else p["h"], p["a"], p["a_scale"],
-                        gate=p["h"] if self.gated else None, stream=s)
+            act.execute(w["h"][f:] if self.gated else w["h"], w["a"], w["a_scale"],
+                        gate=w["h"] if self.gated else None, stream=s)
             if delta is not None:
-                state = p["total"]
-            down.execute(p["a"], b["down"].q, p["delta"], scale_left=p["a_scale"], scale_right=b["down"].scale,
+                state = w["total"]
+            down.execute(w["a"], b["down"].q, w["delta"], scale_left=w["a_scale"], scale_right=b["down"].scale,
                          bias=b["down"].bias, stream=s)
-            delta = p["delta"]
-        p["norm"].execute(state, p["q"], p["q_scale"], residual=delta, weight=self.norm, stream=s)
-        p["head"].execute(p["q"], self.head.q, p["logits"], scale_left=p["q_scale"], scale_right=self.head.scale, stream=s)
+            delta = w["delta"]
+        p["norm"].execute(state, w["q"], w["q_scale"], residual=delta, weight=self.norm, stream=s)
+        p["head"].execute(w["q"], self.head.q, p["logits"], scale_left=w["q_scale"], scale_right=self.head.scale, stream=s)
         return p["logits"]
 
     def num_ops(self, tokens):

@@ -6,6 +6,8 @@ import einsum_ir_amd as eir
 
 pytestmark = pytest.mark.gpu
 
+KEPT = 64       # numbers of tokens whose logits a network keeps
+
 
 def _net(torch, width=64, hidden=96, classes=8, num=2, seed=0, **kw):
     from einsum_ir_amd.mlp_i8 import MlpI8
@@ -110,3 +112,69 @@ def test_network_made_from_tensors_in_the_making(torch_cuda, own_stream):
         y = net(x)
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+def test_memory_of_many_numbers_of_tokens(torch_cuda):
+    """Every number of tokens up to 300: the work buffers of the most, and the logits of the last 64 numbers, each block
+    of memory rounded up to 512 bytes."""
+    torch = torch_cuda
+    width, hidden, classes, most = 256, 1024, 33, 300
+    net = _net(torch, width, hidden, classes)
+    x = torch.randn(most, width, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for tokens in list(range(1, most + 1)) + list(range(most, 0, -1)):
+        net(x[:tokens])
+    torch.cuda.synchronize()
+    per_token = width + 4 + hidden + 4 + 2 * hidden + 2 * 2 * width
+    bound = most * per_token + 7 * 512 + KEPT * (most * classes * 2 + 512)
+    assert torch.cuda.memory_allocated() - before <= bound
+
+
+def test_logits_of_other_calls_stay(torch_cuda):
+    """Calls with other numbers of tokens, larger ones and more of them than are kept, leave a call's logits alone."""
+    torch = torch_cuda
+    net = _net(torch, 256, 512, 33)
+    x = torch.randn(200, 256, device="cuda").bfloat16()
+    y = net(x[:7])
+    first = y.clone()
+    for tokens in list(range(8, 8 + 2 * KEPT)) + [200, 1]:
+        net(x[-tokens:])
+    torch.cuda.synchronize()
+    assert torch.equal(y, first)
+    assert torch.equal(net(x[:7]), first)
+
+
+def test_graph_outlives_larger_calls(torch_cuda):
+    """A captured call replays after calls that need larger buffers and after its numbers of tokens is forgotten."""
+    import ctypes
+    torch = torch_cuda
+    s = torch.cuda.Stream()
+    net = _net(torch, 256, 512, 33, stream=s)
+    x = torch.randn(7, 256, device="cuda").bfloat16()
+    big = torch.randn(300, 256, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    net(x)
+    s.synchronize()
+    lib, graph = eir.hip_lib(), ctypes.c_void_p()
+    eir.check(lib.etir_hip_graph_begin(s.cuda_stream))
+    y = net(x)
+    eir.check(lib.etir_hip_graph_end(s.cuda_stream, ctypes.byref(graph)))
+    for i in range(3):
+        for tokens in [300] + list(range(100, 101 + KEPT)):
+            net(big[:tokens])
+        s.synchronize()
+        with torch.cuda.stream(s):      # takes what memory is free
+            junk = [torch.full((n,), 55, dtype=torch.int8, device="cuda") for n in (7 * 256, 7 * 512, 7 * 1024, 512) * 20]
+        x.copy_(torch.randn(7, 256, device="cuda"))
+        torch.cuda.synchronize()
+        eir.check(lib.etir_hip_graph_launch(graph, s.cuda_stream))
+        s.synchronize()
+        replayed = y.clone()
+        assert all(bool((j == 55).all()) for j in junk), i
+        torch.cuda.synchronize()
+        again = net(x)
+        s.synchronize()
+        assert torch.equal(replayed, again), i
+        del junk
+    eir.check(lib.etir_hip_graph_destroy(graph))
