@@ -23,3 +23,31 @@ def test_rows_of_nothing(torch_cuda, off, dtype, dtype_weight):
     torch.cuda.synchronize()
     assert bool((q == 9).all()) and bool((x == 0).all())
     assert bool((sc[:5] == 0.0).all()) and bool((sc[5:] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype,dtype_weight", [(eir.BF16, eir.FP32), (eir.FP32, eir.BF16)])
+@pytest.mark.parametrize("cols", [1, 3, 5, 7, 64, 301, 2048, 9001, 20003])
+@pytest.mark.parametrize("off", [0, 1])
+def test_weight_of_the_other_type(torch_cuda, off, cols, dtype, dtype_weight):
+    """q within 0.5 + 1e-4 of t * 127 / a and the scale within 2^-20 (2 roundings of t, two of 127 / a, one of their
+    product, each 2^-24); total is a rounding of the sum, bit for bit."""
+    torch = torch_cuda
+    td = {eir.BF16: torch.bfloat16, eir.FP32: torch.float32}
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn((3, cols), device="cuda", generator=g).to(td[dtype])
+    r = torch.randn((3, cols), device="cuda", generator=g).to(td[dtype])
+    w = (1 + 0.3 * torch.randn(cols, device="cuda", generator=g)).to(td[dtype_weight])
+    q = torch.full((3 * cols + 8,), 99, dtype=torch.int8, device="cuda")
+    sc, total = torch.empty(3, device="cuda"), torch.empty_like(x)
+    plan = eir.NormQuantPlan(3, cols, dtype=dtype, dtype_weight=dtype_weight)
+    plan.execute(x, q[off:], sc, residual=r, weight=w, total=total, stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    s = x.double() + r.double()
+    t = s * w.double()
+    a = t.abs().amax(-1, keepdim=True)
+    got = q[off:off + 3 * cols].reshape(3, cols).double()
+    assert float((got - t * 127 / a).abs().max()) <= 0.5 + 1e-4
+    want = a.squeeze(-1) / (127 * torch.sqrt(s.square().mean(-1) + 1e-6))
+    assert bool(((sc.double() - want).abs() <= want * 2.0 ** -20).all())
+    assert torch.equal(total, (x.float() + r.float()).to(td[dtype]))
+    assert bool((q[:off] == 99).all()) and bool((q[off + 3 * cols:] == 99).all())
