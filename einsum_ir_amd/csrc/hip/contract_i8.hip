@@ -22,7 +22,7 @@ typedef i32x4 i32x4_u __attribute__( ( aligned( 1 ) ) );
 
 constexpr int kTile  = 64;
 constexpr int kBk    = 64;
-constexpr int kPitch = kBk + 16;   // 80 bytes a row: 8 rows of 16-byte reads touch all 64 banks twice, none three times
+constexpr int kPitch = kBk + 16;   // 80 bytes a row: 16 rows of 16-byte reads touch each of the 64 banks once
 
 __device__ inline int64_t offset_of( I8Loops const & l, int64_t index, int tensor ) {
   int64_t l_off = 0;

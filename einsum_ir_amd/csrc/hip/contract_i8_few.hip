@@ -5,11 +5,12 @@
 //
 // Bound by the bytes of the many side, each read once.  A workgroup takes
 // 16 rows of it and all of the few side (16 FB rows), and its waves split K;
-// with up to 4 few rows it may take 4 rows and put a quarter of K each into the
-// 16 rows of a fragment instead, of which those products count whose quarters
-// are the same (PARTS 4: four times the workgroups for a short many side):
-// that keeps all of a workgroup's bytes in flight at once where there are few
-// workgroups, and needs no memory between workgroups.  Operands go from global
+// with up to 16 few rows it may take 4 rows of it instead and put a quarter of K
+// each into the 16 rows of a fragment, the few side in fragments of 4 rows, of
+// which those products count whose quarters are the same (PARTS 4: four times
+// the workgroups for a short many side): that keeps all of a workgroup's bytes
+// in flight at once where there are few workgroups, and needs no memory between
+// workgroups.  Operands go from global
 // memory straight into the fragments of v_mfma_i32_16x16x64_i8 (16 k of a row a
 // lane, 4 lanes a row), at any byte address; the partial sums meet in LDS,
 // where their order cannot change an integer sum.  Rows past a side's end read

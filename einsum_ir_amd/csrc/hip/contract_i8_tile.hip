@@ -284,11 +284,13 @@ void contract_i8_tile_kernel( I8Args a ) {
     l_acc[l_i][l_j] = __builtin_amdgcn_mfma_i32_32x32x32_i8( f[TM + l_i], f[l_j], l_acc[l_i][l_j], 0, 0, 0 );
   };
 
-  // Two buffers: one block of 128 k in 4 parts of 32.  During a part's matrix instructions
-  // the next part's fragments are read; the barrier stands in front of the last
-  // part, when every wave has read all of this block and the next one has
-  // landed, and the block after that is loaded over this one from there on,
-  // half of it in the last part, half in the next block's first.
+  // One block of 128 k in 4 parts of 32.  During a part's matrix instructions the
+  // next part's fragments are read; the barrier stands in front of the last part,
+  // when every wave has read all of this block and the next one has landed.  Two
+  // buffers: the block after that is loaded over this one from there on, half of
+  // it in the last part, half in the next block's first.  More: the block
+  // STAGES - 1 ahead is loaded over the last one, spread over the first three
+  // parts.
   auto step = [&]( int l_st, int l_next, int l_free, int s ) __attribute__( ( always_inline ) ) {
     kern::static_for< 4 >( [&]( auto qc ) __attribute__( ( always_inline ) ) {
       constexpr int l_q = decltype( qc )::value;
@@ -331,7 +333,7 @@ void contract_i8_tile_kernel( I8Args a ) {
       } );
     } );
   };
-  // More buffers, for small tiles, which wait for memory and not for the matrix
+  // DEEP, for small tiles, which wait for memory and not for the matrix
   // cores: blocks are issued STAGES - 1 ahead, also past the last one, so that
   // a wave's loads in flight are the same number in every step.
   auto deep = [&]( auto stage_c, int s ) __attribute__( ( always_inline ) ) {

@@ -76,11 +76,12 @@ std::string sizes_of( I8Loops const & l ) {
 // nothing else bounds them, and at least (row + few * few rows) for every 10^6 k
 // of all workgroups, which their 64-byte pieces of rows take in the caches, and
 // 0.4 ns for each workgroup.
-// Measured over 170 products with rows at multiples of 16 bytes and 150 at others
-// (1 to 8192 rows, 16 to 16384 columns, K 64 to 12288), K in parts over 100.  The
-// times that follow are off by 10 to 20 % (root mean square), but alike for
-// neighbours: the kernel chosen is 1 % slower than the best of all on average
-// (64 x 64 tiles everywhere: 36 %).
+// Fitted to 170 products with rows at multiples of 16 bytes and 150 at others (1
+// to 8192 rows, 16 to 16384 columns, K 64 to 12288).  The times that follow are
+// off by 7 to 30 % (root mean square; K in parts up to 46 %), but alike for
+// neighbours: the kernel chosen is 0.7 % slower than the best of all on average
+// over these products, 0.8 % over 150 others (64 x 64 tiles everywhere: 44 and
+// 42 %), and 28 % at most (profiles/i8_choice.txt).
 struct Candidate {
   I8Kernel     kernel;
   char const * name;

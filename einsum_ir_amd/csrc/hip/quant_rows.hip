@@ -33,7 +33,7 @@ __device__ inline float activate( float v, int32_t ktype ) {
     // exp(-v) = 2^t (1 + r ln 2), t + r = -v log2(e), t rounded, r its rest:
     // with the hardware's exponential and reciprocal (1 ulp each) within 8
     // half ulps of v / (1 + exp(-v)), at a third of the instructions of the
-    // library's, which bounded the kernel (gated, 8192 x 8192 bf16: 100 -> 84 us).
+    // library's, which bounded the kernel (gated, 8192 x 8192 bf16: 98 -> 86 us).
     // A quarter of 1 + exp(-v) is inverted, whose reciprocal stays above 2^-126 up
     // to the end of exp's range (the hardware's is 0 below): near there, v < -87.3,
     // the quotient has up to 2 bits less, and below -88.7 exp(-v) is infinite and
@@ -136,7 +136,8 @@ __device__ inline void load_v( T const * row, int32_t at, int32_t n, float * f )
 }
 
 // Non-temporal: these rows are written whole and not read here again (norm of
-// 16384 x 8192 bf16: 271 -> 256 us; non-temporal loads: 307).
+// 16384 x 8192 bf16: 223 -> 215 us; with non-temporal loads 227, and 4072 x 2048
+// 14.2 -> 19.2).
 template< class T >
 __device__ inline void store_v( T * row, Place< Vec< T >::V > p, int32_t n, float const * f ) {
   if( p.whole( n ) ) {
@@ -357,8 +358,9 @@ void launch_shape( QuantArgs const & a, hipStream_t stream ) {
 // Threads a row by its vectors of 16 bytes: a wave where one vector a lane
 // holds the row (no exchange between waves), else few waves with two vectors a
 // lane, which leaves most of a compute unit's registers to other rows: 4072
-// rows of 256 vectors take 14.7 us so and 16.4 with one vector; 3000 of 126
-// take 10.7 with two vectors in a wave and 8.6 with one in two waves.
+// rows of 256 vectors take 14.2 us so and 15.6 with one vector (a single row 4.1
+// and 3.5); 300 of 88 take 5.8 with two vectors in a wave and 4.2 with one in two
+// waves.
 template< class T, bool NORM >
 void launch_rows( QuantArgs const & a, hipStream_t stream ) {
   // a row of q that starts off a multiple of 4 bytes shifts its vectors

@@ -248,7 +248,7 @@ int etir_hip_permute_execute( etir_plan_t  plan,
  * whose rows and K are multiples of 16 bytes run up to twice as fast as others.
  * A product of any size 0 in C, M or N
  * does nothing; without K the sums are 0.  At most 6 loops of one type that
- * cannot be fused.
+ * cannot be fused, and less than 2^24 blocks of 64 x 64 in C, M and N.
  */
 int etir_hip_contraction_i8_create( int64_t         num_loops,
                                     int32_t const * dim_types,
