@@ -115,17 +115,20 @@ class ContractionI8Plan(_Plan):
     def __init__(self, dim_types, sizes, strides_left, strides_right, strides_out, strides_scale_left=None,
                  strides_scale_right=None, strides_bias=None, dtype_out=FP32, ktype_last_touch=UNDEFINED_KTYPE):
         super().__init__()
-        # the library reads as many entries of each list as there are sizes
-        for name, given in (("dim_types", dim_types), ("strides_left", strides_left), ("strides_right", strides_right),
-                            ("strides_out", strides_out), ("strides_scale_left", strides_scale_left),
-                            ("strides_scale_right", strides_scale_right), ("strides_bias", strides_bias)):
-            if given is not None and len(given) != len(sizes):
-                raise ValueError(f"{name} has {len(given)} entries for {len(sizes)} loops")
-        opt = lambda s: None if s is None else _lib.i64_array(s)  # noqa: E731
-        check(hip_lib().etir_hip_contraction_i8_create(
-            len(sizes), _lib.i32_array(dim_types), _lib.i64_array(sizes), _lib.i64_array(strides_left),
-            _lib.i64_array(strides_right), opt(strides_scale_left), opt(strides_scale_right), opt(strides_bias),
-            _lib.i64_array(strides_out), dtype_out, ktype_last_touch, ctypes.byref(self._handle)))
+        lists = dict(dim_types=dim_types, strides_left=strides_left, strides_right=strides_right,
+                     strides_scale_left=strides_scale_left, strides_scale_right=strides_scale_right,
+                     strides_bias=strides_bias, strides_out=strides_out)
+        for name, given in lists.items():
+            if given is None:
+                continue
+            lists[name] = list(given)
+            # the library reads as many entries of each list as there are sizes
+            if len(lists[name]) != len(sizes):
+                raise ValueError(f"{name} has {len(lists[name])} entries for {len(sizes)} loops")
+        types = _lib.i32_array(lists.pop("dim_types"))
+        strides = [None if v is None else _lib.i64_array(v) for v in lists.values()]
+        check(hip_lib().etir_hip_contraction_i8_create(len(sizes), types, _lib.i64_array(sizes), *strides, dtype_out,
+                                                       ktype_last_touch, ctypes.byref(self._handle)))
 
         self._execute = hip_lib().etir_hip_contraction_i8_execute
 
