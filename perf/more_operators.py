@@ -152,6 +152,11 @@ def _generator(seed):
     return torch.Generator(device="cuda").manual_seed(int(seed))
 
 
+def _power(e):
+    """2^e as fp32, by way of 64 bits, whose exponential is exact there (32 bits' and ldexp are not)."""
+    return torch.exp2(e.double()).float()
+
+
 def _spread(s, block, shape):
     """A scale for each element."""
     s = s.repeat_interleave(block[0], -2)[..., :shape[-2], :]
@@ -167,7 +172,7 @@ def _blocks_f8(shape, block, q, scale, g):
     if scale == "e8m0":
         m, e = torch.frexp(s)
         e = e - (m == 0.5).to(e.dtype)
-        s, bytes_ = torch.ldexp(torch.ones_like(s), e), (e + 127).to(torch.uint8)
+        s, bytes_ = _power(e), (e + 127).to(torch.uint8)
     values = (x / _spread(s, block, shape)).clamp(-_LARGEST[q], _LARGEST[q]).to(_TORCH[q])
     return values, bytes_ if scale == "e8m0" else s
 
@@ -295,8 +300,7 @@ def _plain_quant(case, h):
     a = y.abs().amax((-3, -1), keepdim=True)
     m, e = torch.frexp(a)                     # a = m 2^e, 0.5 <= m < 1; fmax is 0.875 times a power of two
     e = e - int(math.log2(fmax / 0.875)) + (m > 0.875).to(e.dtype)
-    one = torch.ones_like(a)
-    s = torch.where(a > 0, torch.ldexp(one, e), one)
+    s = torch.where(a > 0, _power(e), torch.ones_like(a))
     q = (y / s).to(_TORCH[case["q"]]).float()
     values = (q * s).flatten(-2).flatten(1, 2)[:, :shape[1], :cols]
     return dict(values=values.to(h.dtype), scale=s.squeeze(-1).squeeze(-2))
@@ -307,7 +311,7 @@ def _dequantised(t, s, block):
     if s is None:
         return t.float()
     if s.dtype == torch.uint8:
-        s = torch.ldexp(torch.ones(s.shape, device=s.device), s.int() - 127)
+        s = _power(s.int() - 127)
     return t.float() * _spread(s, block, t.shape)
 
 
