@@ -12,11 +12,12 @@ import ctypes
 from . import _lib
 from ._lib import (SUCCESS, COMPILATION_FAILED, NO_DATA_PTR_PROVIDED, CALLED_BEFORE_COMPILATION,
                    INVALID_ID, INVALID_BACKEND, INVALID_CPX_DIM, INVALID_DTYPE, INVALID_KTYPE, UNDEFINED_ERROR,
-                   FP32, FP64, BF16, INT8, UNDEFINED_DTYPE,
+                   FP32, FP64, BF16, INT8, F8E4M3, F8E5M2, E8M0, UNDEFINED_DTYPE,
                    ZERO, RELU, ADD, COPY, MADD, UNDEFINED_KTYPE, CPX_ZERO, CPX_MADD, SILU,
-                   DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J,
+                   DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J, DIM_G,
                    DTYPE_BYTES, EinsumIrError, hip_lib, check)
-from .loops import binary_loops, contraction_i8_loops, unary_dims, dim_types, row_major_strides  # noqa: F401
+from .loops import (binary_loops, contraction_f8_loops, contraction_i8_loops, dim_types, grouped_loops,  # noqa: F401
+                    row_major_strides, unary_dims)
 
 
 def _ptr(x):
@@ -135,6 +136,98 @@ class ContractionI8Plan(_Plan):
     def execute(self, left, right, out, scale_left=None, scale_right=None, bias=None, stream=None):
         err = self._execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left), _ptr(scale_right), _ptr(bias),
                             _ptr(out), _stream_ptr(stream))
+        if err:
+            check(err)
+
+
+def _loop_lists(sizes, dim_types, **strides):
+    """The arrays of a plan's loop lists, in the order given; an absent one stays None."""
+    given = {"dim_types": dim_types, **strides}
+    for name, values in given.items():
+        if values is None:
+            continue
+        given[name] = list(values)
+        # the library reads as many entries of each list as there are sizes
+        if len(given[name]) != len(sizes):
+            raise ValueError(f"{name} has {len(given[name])} entries for {len(sizes)} loops")
+    types = _lib.i32_array(given.pop("dim_types"))
+    return [len(sizes), types, _lib.i64_array(sizes)] + [None if v is None else _lib.i64_array(v) for v in given.values()]
+
+
+class ContractionF8Plan(_Plan):
+    """Product of 8-bit floating point with a scale for each block of 128
+    (etir_hip_contraction_f8_create):
+
+        out = last(sum_kb scale_left * scale_right * sum_(k in kb) left * right + bias)
+
+    contraction_f8_loops gives the arguments for an einsum string.  A scale or
+    bias without strides is not read."""
+
+    def __init__(self, dim_types, sizes, strides_left, strides_right, strides_out, strides_scale_left=None,
+                 strides_scale_right=None, strides_bias=None, block_left=1, block_right=128, dtype_left=F8E4M3,
+                 dtype_right=F8E4M3, dtype_scale=FP32, dtype_out=FP32, ktype_last_touch=UNDEFINED_KTYPE):
+        super().__init__()
+        lists = _loop_lists(list(sizes), dim_types, strides_left=strides_left, strides_right=strides_right,
+                            strides_scale_left=strides_scale_left, strides_scale_right=strides_scale_right,
+                            strides_bias=strides_bias, strides_out=strides_out)
+        check(hip_lib().etir_hip_contraction_f8_create(*lists, block_left, block_right, dtype_left, dtype_right,
+                                                       dtype_scale, dtype_out, ktype_last_touch,
+                                                       ctypes.byref(self._handle)))
+
+        self._execute = hip_lib().etir_hip_contraction_f8_execute
+
+    def execute(self, left, right, out, scale_left=None, scale_right=None, bias=None, stream=None):
+        err = self._execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left), _ptr(scale_right), _ptr(bias),
+                            _ptr(out), _stream_ptr(stream))
+        if err:
+            check(err)
+
+
+class ContractionGroupedPlan(_Plan):
+    """Product whose ragged loop is cut into groups, each with a matrix of its own
+    (etir_hip_contraction_grouped_create).  grouped_loops gives the arguments for
+    an einsum string; ragged: index of the ragged loop.  offsets: int32 on the
+    GPU, one more than there are groups."""
+
+    def __init__(self, dim_types, sizes, strides_left, strides_right, strides_out, ragged, strides_scale_left=None,
+                 strides_scale_right=None, block_left=1, block_right=128, dtype_left=BF16, dtype_right=None,
+                 dtype_scale=FP32, dtype_out=BF16):
+        super().__init__()
+        if dtype_right is None:
+            dtype_right = BF16 if dtype_left == BF16 else F8E4M3
+        lists = _loop_lists(list(sizes), dim_types, strides_left=strides_left, strides_right=strides_right,
+                            strides_scale_left=strides_scale_left, strides_scale_right=strides_scale_right,
+                            strides_out=strides_out)
+        check(hip_lib().etir_hip_contraction_grouped_create(*lists, ragged, block_left, block_right, dtype_left,
+                                                            dtype_right, dtype_scale, dtype_out,
+                                                            ctypes.byref(self._handle)))
+
+        self._execute = hip_lib().etir_hip_contraction_grouped_execute
+
+    def execute(self, left, right, out, offsets, scale_left=None, scale_right=None, stream=None):
+        err = self._execute(self._handle, _ptr(left), _ptr(right), _ptr(scale_left), _ptr(scale_right), _ptr(offsets),
+                            _ptr(out), _stream_ptr(stream))
+        if err:
+            check(err)
+
+
+class QuantF8Plan(_Plan):
+    """x, f(x) or f(gate) * x rounded to 8-bit floating point with a scale, a power
+    of two, for each block (etir_hip_quant_f8_create).  block: (1, 128), (128, 1)
+    or (128, 128); ktype: UNDEFINED_KTYPE (none), RELU or SILU; ld_*: elements
+    from row to row, cols unless given."""
+
+    def __init__(self, rows, cols, batch=1, dtype=BF16, dtype_q=F8E4M3, block=(1, 128), ktype=UNDEFINED_KTYPE,
+                 dtype_scale=FP32, ld_in=None, ld_gate=None, ld_q=None, ld_values=None):
+        super().__init__()
+        ld = [cols if v is None else v for v in (ld_in, ld_gate, ld_q, ld_values)]
+        check(hip_lib().etir_hip_quant_f8_create(batch, rows, cols, *ld, *block, dtype, dtype_q, dtype_scale, ktype,
+                                                 ctypes.byref(self._handle)))
+
+        self._execute = hip_lib().etir_hip_quant_f8_execute
+
+    def execute(self, x, q, scale, gate=None, values=None, stream=None):
+        err = self._execute(self._handle, _ptr(x), _ptr(gate), _ptr(q), _ptr(scale), _ptr(values), _stream_ptr(stream))
         if err:
             check(err)
 

@@ -23,11 +23,11 @@ INVALID_DTYPE = 9
 INVALID_KTYPE = 10
 UNDEFINED_ERROR = 99
 
-FP32, FP64, BF16, INT8, UNDEFINED_DTYPE = 0, 1, 2, 3, 99
+FP32, FP64, BF16, INT8, F8E4M3, F8E5M2, E8M0, UNDEFINED_DTYPE = 0, 1, 2, 3, 4, 5, 6, 99
 ZERO, RELU, ADD, COPY, MADD, UNDEFINED_KTYPE = 0, 1, 2, 3, 4, 99
 CPX_ZERO, CPX_MADD = 6, 8
 SILU = 20
-DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J = 0, 1, 2, 3, 4, 5, 6
+DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX, DIM_I, DIM_J, DIM_G = 0, 1, 2, 3, 4, 5, 6, 7
 
 DTYPE_BYTES = {FP32: 4, FP64: 8, BF16: 2}
 
@@ -55,6 +55,14 @@ _HIP_SIGS = {
     "etir_hip_act_quant_create": (ctypes.c_int, [ctypes.c_int64] * 6 + [ctypes.c_int32, ctypes.c_int32,
                                                                        ctypes.POINTER(_vp)]),
     "etir_hip_act_quant_execute": (ctypes.c_int, [_vp] * 7),
+    "etir_hip_contraction_f8_create": (ctypes.c_int, [ctypes.c_int64, _i32p] + [_i64p] * 7 + [ctypes.c_int32] * 7
+                                       + [ctypes.POINTER(_vp)]),
+    "etir_hip_contraction_f8_execute": (ctypes.c_int, [_vp] * 8),
+    "etir_hip_contraction_grouped_create": (ctypes.c_int, [ctypes.c_int64, _i32p] + [_i64p] * 6 + [ctypes.c_int64]
+                                            + [ctypes.c_int32] * 6 + [ctypes.POINTER(_vp)]),
+    "etir_hip_contraction_grouped_execute": (ctypes.c_int, [_vp] * 8),
+    "etir_hip_quant_f8_create": (ctypes.c_int, [ctypes.c_int64] * 7 + [ctypes.c_int32] * 6 + [ctypes.POINTER(_vp)]),
+    "etir_hip_quant_f8_execute": (ctypes.c_int, [_vp] * 7),
     "etir_hip_plan_destroy": (ctypes.c_int, [_vp]),
     "etir_hip_plan_describe": (ctypes.c_int, [_vp, ctypes.c_char_p, ctypes.c_int64]),
     "etir_hip_plan_flops": (ctypes.c_int64, [_vp]),

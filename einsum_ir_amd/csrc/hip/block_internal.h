@@ -1,0 +1,135 @@
+// Declarations of the products of 8-bit floating point with a scale for each
+// block of 128, of the products whose rows are grouped by expert (block_plan.cpp,
+// contract_block*.hip) and of the operator that rounds to such blocks
+// (quant_f8.hip).
+#ifndef ETIR_BLOCK_INTERNAL_H
+#define ETIR_BLOCK_INTERNAL_H
+
+#include "etir_internal.h"
+#include <algorithm>
+
+namespace etir {
+
+// k (and, where a side has blocks, rows) that share a scale
+constexpr int kScaleBlock = 128;
+
+// ---------------------------------------------------------------------------
+// products
+//   out[c,m,n] = last( sum_kb sa[c,m,kb] sb[c,n,kb] sum_(k in kb) A[c,m,k] B[c,n,k] + bias[c,n] )
+// A: the left, B: the right tensor; one loop of each type.  Groups: rows of A
+// (GROUP_ROWS) or indices k (GROUP_K) offsets[g] to offsets[g + 1] belong to
+// group g, which is B's or the output's batch index.
+// ---------------------------------------------------------------------------
+struct BlockArgs {
+  void const    * a;
+  void const    * b;
+  void const    * sa;       // null: 1
+  void const    * sb;       // null: 1
+  float const   * bias;     // null: 0
+  int32_t const * offsets;  // groups only
+  void          * out;
+  // elements from index to index; scales: from block to block
+  int64_t a_c, b_c, o_c, sa_c, sb_c, bias_c;
+  int64_t a_row, a_k, b_row, b_k, o_row, o_col, sa_row, sa_k, sb_row, sb_k, bias_col;
+  int32_t M, N, K, C;       // C: batches or groups
+  uint32_t flags;
+
+  enum : uint32_t { OUT_BF16 = 1u, RELU = 2u, GROUP_ROWS = 4u, GROUP_K = 8u, F8 = 16u, A_E5M2 = 32u, E8M0 = 64u,
+                    SA_BLOCKS = 128u, SB_BLOCKS = 256u };   // *_BLOCKS: a scale for 128 rows
+  __host__ __device__ bool has( uint32_t flag ) const { return ( flags & flag ) != 0; }
+};
+
+enum class BlockKernel : int32_t {
+  GENERAL          // any strides, 64 x 64 tiles (contract_block.hip)
+};
+
+struct BlockPlan {
+  BlockKernel kernel = BlockKernel::GENERAL;
+  bool      grouped = false;
+  bool      has_sa = false, has_sb = false, has_bias = false;
+  BlockArgs args{};                    // pointers set at execution
+  int64_t   flops = 0;
+  int64_t   bytes = 0;
+  std::string desc;
+};
+
+int launch_block_general( BlockArgs const & a, hipStream_t stream );
+
+// ---------------------------------------------------------------------------
+// rounding to 8-bit floating point with a scale for each block
+// ---------------------------------------------------------------------------
+struct QuantF8Plan {
+  int64_t batch = 1, rows = 0, cols = 0;
+  int64_t ld_in = 0, ld_gate = 0, ld_q = 0, ld_values = 0;
+  int32_t block_rows = 1, block_cols = kScaleBlock;
+  int32_t dtype = ETIR_BF16, dtype_q = ETIR_F8E4M3, dtype_scale = ETIR_FP32;
+  int32_t ktype = ETIR_KTYPE_UNDEFINED;
+  int64_t bytes = 0;                   // with every optional tensor
+  std::string desc;
+};
+
+int launch_quant_f8( QuantF8Plan const & plan, void const * in, void const * gate, void * q, void * scale, void * values,
+                     hipStream_t stream );
+
+#ifdef __HIPCC__
+// ---------------------------------------------------------------------------
+// device helpers
+// ---------------------------------------------------------------------------
+
+// the number that an e8m0 byte stands for: 2^(byte - 127), 255: NaN
+__device__ inline float e8m0_to_f32( uint8_t v ) {
+  return v == 0 ? 0x1p-127f : v == 255 ? __uint_as_float( 0x7fc00000u ) : __uint_as_float( uint32_t( v ) << 23 );
+}
+
+// Rows (or k) of a group, inside [0, rows] whatever the offsets are.
+struct BlockGroup { int32_t begin, end; };
+__device__ inline BlockGroup block_group( int32_t const * offsets, int32_t g, int32_t rows ) {
+  BlockGroup l_g;
+  l_g.begin = min( max( offsets[g], 0 ), rows );
+  l_g.end   = min( max( offsets[g + 1], l_g.begin ), rows );
+  return l_g;
+}
+
+// Where a workgroup's rows lie: tile `tile` of BM rows, counted through the
+// groups, none of which a tile crosses.
+struct BlockRows { int32_t group, m0, end; };      // group < 0: no such tile
+template< int BM >
+__device__ inline BlockRows block_rows( int32_t const * offsets, int32_t groups, int32_t rows, int32_t tile ) {
+  // every wave looks for itself: 64 groups at a time, the tiles of the groups
+  // up to each lane's by a running sum over the lanes
+  int const l_lane = threadIdx.x % 64;
+  for( int32_t l_g0 = 0; l_g0 < groups; l_g0 += 64 ) {
+    int32_t const l_g = l_g0 + l_lane;
+    BlockGroup l_in = { 0, 0 };
+    if( l_g < groups ) l_in = block_group( offsets, l_g, rows );
+    int32_t const l_tiles = ( l_in.end - l_in.begin + BM - 1 ) / BM;
+    int32_t l_sum = l_tiles;
+#pragma unroll
+    for( int l_d = 1; l_d < 64; l_d *= 2 ) {
+      int32_t const l_v = __shfl_up( l_sum, l_d );
+      if( l_lane >= l_d ) l_sum += l_v;
+    }
+    uint64_t const l_past = __ballot( l_sum > tile );
+    if( l_past != 0 ) {
+      int const l_at = __builtin_ctzll( l_past );
+      int32_t const l_first = __builtin_amdgcn_readlane( l_sum - l_tiles, l_at );
+      BlockRows l_r;
+      l_r.group = l_g0 + l_at;
+      l_r.m0 = __builtin_amdgcn_readlane( l_in.begin, l_at ) + ( tile - l_first ) * BM;
+      l_r.end = __builtin_amdgcn_readlane( l_in.end, l_at );
+      return l_r;
+    }
+    tile -= __builtin_amdgcn_readlane( l_sum, 63 );
+  }
+  return { -1, 0, 0 };
+}
+#endif
+
+// tiles of bm rows that `rows` rows in `groups` groups have at most
+inline int64_t block_most_tiles( int64_t rows, int64_t groups, int64_t bm ) {
+  return rows / bm + std::min( rows, groups );
+}
+
+}  // namespace etir
+
+#endif

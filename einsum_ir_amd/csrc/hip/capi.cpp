@@ -1,6 +1,7 @@
 // extern "C" entry points of libeinsum_ir_hip.so (declared in
 // include/einsum_ir_hip.h).  Thin: argument checks, plan ownership, error
 // strings; planning and kernels live in contract_plan.cpp / permute.hip.
+#include "block_internal.h"
 #include "i8_internal.h"
 #include <cstdio>
 #include <cstdlib>
@@ -147,8 +148,14 @@ int etir_hip_plan_describe( etir_plan_t plan, char * buf, int64_t len ) {
   else if( plan->kind == 3 ) {
     l_s = plan->i8->desc;
   }
-  else if( plan->kind > 3 ) {
+  else if( plan->quant ) {
     l_s = plan->quant->desc;
+  }
+  else if( plan->block ) {
+    l_s = plan->block->desc;
+  }
+  else if( plan->quant_f8 ) {
+    l_s = plan->quant_f8->desc;
   }
   else {
     static char const * l_modes[] = { "fill", "transpose", "copy_vec", "gather", "tiled", "reg4", "rows", "pair" };
@@ -190,6 +197,7 @@ int etir_hip_plan_describe( etir_plan_t plan, char * buf, int64_t len ) {
 
 int64_t etir_hip_plan_flops( etir_plan_t plan ) {
   if( plan != nullptr && plan->kind == 3 ) return plan->i8->flops;
+  if( plan != nullptr && plan->block ) return plan->block->flops;
   if( plan == nullptr || plan->kind != 1 ) return 0;
   return plan->cont.flops;
 }
@@ -198,7 +206,9 @@ int64_t etir_hip_plan_bytes( etir_plan_t plan ) {
   if( plan == nullptr ) return 0;
   if( plan->kind == 1 ) return plan->cont.bytes;
   if( plan->kind == 3 ) return plan->i8->bytes;
-  if( plan->kind > 3 ) return plan->quant->bytes;
+  if( plan->quant ) return plan->quant->bytes;
+  if( plan->block ) return plan->block->bytes;
+  if( plan->quant_f8 ) return plan->quant_f8->bytes;
   etir::PermutePlan const & p = plan->perm;
   int64_t l_rw = ( p.ktype == ETIR_KTYPE_ZERO ) ? 1 : ( p.ktype == ETIR_KTYPE_ADD ? 3 : 2 );
   return l_rw * p.elem_bytes * p.num_elements;

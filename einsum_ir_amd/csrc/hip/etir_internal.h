@@ -471,16 +471,22 @@ int  launch_contraction( ContractionPlan const & plan,
 
 struct I8Plan;
 struct QuantPlan;
+struct BlockPlan;
+struct QuantF8Plan;
 
 }  // namespace etir
 
 struct etir_plan_s {
-  int32_t kind = 0;              // 1 contraction, 2 permutation, 3 8-bit contraction, 4 norm_quant, 5 act_quant
+  // 1 contraction, 2 permutation, 3 8-bit contraction, 4 norm_quant, 5 act_quant,
+  // 6 contraction of 8-bit floating point, 7 grouped contraction, 8 quant_f8
+  int32_t kind = 0;
   int32_t device = 0;
   etir::ContractionPlan cont;
   etir::PermutePlan     perm;
   std::shared_ptr< etir::I8Plan >    i8;
   std::shared_ptr< etir::QuantPlan > quant;
+  std::shared_ptr< etir::BlockPlan > block;
+  std::shared_ptr< etir::QuantF8Plan > quant_f8;
 };
 
 #endif

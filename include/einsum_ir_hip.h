@@ -46,13 +46,19 @@ extern "C" {
 #define ETIR_UNDEFINED_ERROR           99
 
 /* data types: einsum_ir::data_t (reference src/constants.h:48-52) plus the
- * additive values BF16 and INT8 (the reference has neither; 2 and 3 are unused
- * there).  INT8 names the operands of etir_hip_contraction_i8_*; no other call
- * takes it. */
+ * additive values from BF16 on (the reference has none of them; 2 to 6 are
+ * unused there).  INT8 names the operands of etir_hip_contraction_i8_*; no other
+ * call takes it.  F8E4M3 (largest finite value 448, no infinity), F8E5M2 (57344)
+ * and E8M0 (a scale 2^(byte - 127), 255: NaN) belong to
+ * etir_hip_contraction_f8_*, etir_hip_contraction_grouped_* and
+ * etir_hip_quant_f8_*. */
 #define ETIR_FP32                       0
 #define ETIR_FP64                       1
 #define ETIR_BF16                       2
 #define ETIR_INT8                       3
+#define ETIR_F8E4M3                     4
+#define ETIR_F8E5M2                     5
+#define ETIR_E8M0                       6
 #define ETIR_UNDEFINED_DTYPE           99
 
 /* kernel types: einsum_ir::kernel_t (reference src/constants.h:61-77) */
@@ -63,7 +69,7 @@ extern "C" {
 #define ETIR_KTYPE_MADD                 4
 #define ETIR_KTYPE_CPX_ZERO             6
 #define ETIR_KTYPE_CPX_MADD             8
-#define ETIR_KTYPE_SILU                20   /* additive: x / (1 + exp(-x)), etir_hip_act_quant_create only */
+#define ETIR_KTYPE_SILU                20   /* additive: x / (1 + exp(-x)), etir_hip_act_quant_create and etir_hip_quant_f8_create only */
 #define ETIR_KTYPE_UNDEFINED           99
 
 /* dimension types: einsum_ir::dim_t (reference src/constants.h:9-18) */
@@ -74,6 +80,7 @@ extern "C" {
 #define ETIR_DIM_CPX                    4
 #define ETIR_DIM_I                      5
 #define ETIR_DIM_J                      6
+#define ETIR_DIM_G                      7   /* additive: groups, etir_hip_contraction_grouped_create only */
 
 typedef struct etir_plan_s * etir_plan_t;
 
@@ -344,6 +351,149 @@ int etir_hip_act_quant_execute( etir_plan_t  plan,
                                 void       * scale,
                                 void       * values,
                                 void       * stream );
+
+/*
+ * 8-bit floating point with a scale for each block of 128, and products whose
+ * rows are grouped by expert.  No counterpart in the reference.  An expert layer
+ * in 8 bits is
+ *   quant_f8 -> contraction_grouped -> quant_f8 (activation) -> contraction_grouped
+ * and a dense one has contraction_f8 in their place.  The plans own no device
+ * memory: executions overlap freely and may be captured into graphs.
+ *
+ * Product of blocks:
+ *   out[c,m,n] = last( sum_kb scale_left[c,m',kb] * scale_right[c,n',kb]
+ *                      * sum_(k in kb) left[c,m,k] * right[c,n,k] + bias[c,n] )
+ * kb counts blocks of 128 k (the last may be shorter); m' is m / block_left and n'
+ * is n / block_right, each 1 or 128 rows to a scale.  The arguments follow
+ * etir_hip_contraction_i8_create; the strides of a scale are those from block to
+ * block.  left: F8E4M3 or F8E5M2, right: F8E4M3, scales dtype_scale (FP32 or
+ * E8M0), bias fp32, output FP32 or BF16; last touch RELU or UNDEFINED.  The
+ * stride list of a scale or of the bias may be NULL: that tensor is then not read
+ * (a scale of 1, a bias of 0).  Products of two scales are taken in fp32.
+ *
+ * The loops of each type (M, N, C and K) have to fuse to one; a side with a scale
+ * for 128 rows, and K, are one loop from the start.  At most 2^30 indices of one
+ * type.  The output's elements have to lie apart.  A product of any size 0 in C,
+ * M or N does nothing; without K the sums are 0.
+ */
+int etir_hip_contraction_f8_create( int64_t         num_loops,
+                                    int32_t const * dim_types,
+                                    int64_t const * sizes,
+                                    int64_t const * strides_left,
+                                    int64_t const * strides_right,
+                                    int64_t const * strides_scale_left,
+                                    int64_t const * strides_scale_right,
+                                    int64_t const * strides_bias,
+                                    int64_t const * strides_out,
+                                    int32_t         block_left,
+                                    int32_t         block_right,
+                                    int32_t         dtype_left,
+                                    int32_t         dtype_right,
+                                    int32_t         dtype_scale,
+                                    int32_t         dtype_out,
+                                    int32_t         ktype_last_touch,
+                                    etir_plan_t   * plan );
+
+/* Enqueues one product on `stream`.  A scale or bias pointer is needed where
+ * its strides were given.  The output may not overlap an input. */
+int etir_hip_contraction_f8_execute( etir_plan_t  plan,
+                                     void const * left,
+                                     void const * right,
+                                     void const * scale_left,
+                                     void const * scale_right,
+                                     void const * bias,
+                                     void       * out,
+                                     void       * stream );
+
+/*
+ * Products grouped by expert: one loop, the `ragged`-th of the lists, is cut into
+ * groups at offsets that the device holds, and one loop is of type ETIR_DIM_G,
+ * over the groups.  Group g has the ragged indices offsets[g] to
+ * offsets[g + 1] - 1.
+ *   ragged loop of type M:  out[m,n] = sum_k left[m,k] * right[g(m),n,k]
+ *   ragged loop of type K:  out[g,m,n] = sum_(k in g) left[m,k] * right[n,k]
+ * The first is the experts' product, and the gradient of its rows with the
+ * weights read in the other order; the second is the gradient of its weights.
+ * M rows that belong to no group are not written; a group without k gives zeros.
+ *
+ * left and right: BF16, or (ragged M) F8E4M3 / F8E5M2 and F8E4M3 with scales for
+ * blocks as above, where scale_left counts all rows and scale_right has a matrix
+ * for each group; output FP32 or BF16.  Other loops: one of type M (ragged K), N
+ * and K after fusing, none of type C.  At most 2^30 indices of one type.
+ */
+int etir_hip_contraction_grouped_create( int64_t         num_loops,
+                                         int32_t const * dim_types,
+                                         int64_t const * sizes,
+                                         int64_t const * strides_left,
+                                         int64_t const * strides_right,
+                                         int64_t const * strides_scale_left,
+                                         int64_t const * strides_scale_right,
+                                         int64_t const * strides_out,
+                                         int64_t         ragged,
+                                         int32_t         block_left,
+                                         int32_t         block_right,
+                                         int32_t         dtype_left,
+                                         int32_t         dtype_right,
+                                         int32_t         dtype_scale,
+                                         int32_t         dtype_out,
+                                         etir_plan_t   * plan );
+
+/* Enqueues one product on `stream`.  offsets: 32-bit integers on the device, one
+ * more than there are groups, rising from 0 or more to at most the ragged loop's
+ * size; others are cut to that range, so that nothing outside the tensors is
+ * touched, and groups that overlap then write the same rows in any order. */
+int etir_hip_contraction_grouped_execute( etir_plan_t  plan,
+                                          void const * left,
+                                          void const * right,
+                                          void const * scale_left,
+                                          void const * scale_right,
+                                          void const * offsets,
+                                          void       * out,
+                                          void       * stream );
+
+/*
+ * Rounding to 8-bit floating point with a scale for each block of
+ * block_rows x block_cols (1 x 128, 128 x 1 or 128 x 128; blocks at the end of
+ * rows and columns may be smaller) of `batch` matrices of `rows` rows of `cols`:
+ *   y = in, f( in ) or f( gate ) * in  (fp32)       a = max |y| of the block
+ *   scale = 2^e, e the least integer >= -126 with a <= fmax * 2^e
+ *   q = y / scale rounded to dtype_q (to nearest, ties to even)
+ *   values = q * scale, rounded to dtype
+ * fmax: 448 (F8E4M3) or 57344 (F8E5M2).  The quotient is exact, so q is y's own
+ * rounding.  A block of zeros has scale 1; one with an infinity or a NaN has q = 0
+ * and a NaN for its scale.  f: ktype UNDEFINED (identity), RELU or SILU, as for
+ * etir_hip_act_quant_create.
+ * dtype (in, gate, values): ETIR_BF16 or ETIR_FP32; scale: dtype_scale (ETIR_FP32
+ * or ETIR_E8M0), [batch, rows / block_rows, cols / block_cols] rounded up, one
+ * after the other.  Elements of a row are adjacent, row i of matrix b starts at
+ * (b * rows + i) * ld_*; ld_in and ld_gate may be less than cols, the output's
+ * ld_* not.  batch, rows and cols are at most 2^30, less than 2^24 blocks of
+ * 128 x 128 or 2^29 of 1 x 128.
+ */
+int etir_hip_quant_f8_create( int64_t       batch,
+                              int64_t       rows,
+                              int64_t       cols,
+                              int64_t       ld_in,
+                              int64_t       ld_gate,
+                              int64_t       ld_q,
+                              int64_t       ld_values,
+                              int32_t       block_rows,
+                              int32_t       block_cols,
+                              int32_t       dtype,
+                              int32_t       dtype_q,
+                              int32_t       dtype_scale,
+                              int32_t       ktype,
+                              etir_plan_t * plan );
+
+/* Enqueues one rounding on `stream`; gate (none) and values (not wanted) may be
+ * NULL.  No output may overlap an input. */
+int etir_hip_quant_f8_execute( etir_plan_t  plan,
+                               void const * in,
+                               void const * gate,
+                               void       * q,
+                               void       * scale,
+                               void       * values,
+                               void       * stream );
 
 /* Releases a plan of any kind and its device tables. */
 int etir_hip_plan_destroy( etir_plan_t plan );
