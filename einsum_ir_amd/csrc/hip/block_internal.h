@@ -40,11 +40,24 @@ struct BlockArgs {
 };
 
 enum class BlockKernel : int32_t {
-  GENERAL          // any strides, 64 x 64 tiles (contract_block.hip)
+  GENERAL,         // any strides, 64 x 64 tiles (contract_block.hip)
+  TILE_64x64,      // through LDS directly (contract_block_tile.h), both operands at multiples of 16 bytes
+  TILE_128x128,
+  TILE_256x128,
+  TILE_256x256
+};
+
+// How the operands lie for the tiles; rows and k at multiples of 16 bytes.
+enum class BlockLayout : int32_t {
+  NONE,            // any other
+  K_K,             // both unit-stride along k: the product itself
+  K_ROWS,          // B unit-stride along its rows: the gradient of the rows
+  ROWS_ROWS        // both unit-stride along their rows: the gradient of the weights
 };
 
 struct BlockPlan {
   BlockKernel kernel = BlockKernel::GENERAL;
+  BlockLayout layout = BlockLayout::NONE;
   bool      grouped = false;
   bool      has_sa = false, has_sb = false, has_bias = false;
   BlockArgs args{};                    // pointers set at execution
@@ -54,6 +67,10 @@ struct BlockPlan {
 };
 
 int launch_block_general( BlockArgs const & a, hipStream_t stream );
+int launch_block_tile_bf16( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
+int launch_block_tile_f8( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
+int launch_block_tile_exact( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
+int launch_block_tile_e8m0( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 
 // ---------------------------------------------------------------------------
 // rounding to 8-bit floating point with a scale for each block

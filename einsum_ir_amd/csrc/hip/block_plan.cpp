@@ -6,6 +6,7 @@
 // A product's loops are sorted by type and fused where they are contiguous in
 // every tensor; one loop of each type has to be left.
 #include "block_internal.h"
+#include <cstdlib>
 #include <limits>
 #include <vector>
 
@@ -92,6 +93,76 @@ int check_types( Given const & g ) {
     return fail( ETIR_INVALID_KTYPE, l_w + ": the last touch is RELU or UNDEFINED" );
   }
   return ETIR_SUCCESS;
+}
+
+// How the tiles see the operands; pointers count where they are known.
+BlockLayout layout_of( BlockArgs const & a ) {
+  int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2, l_step = 128 / l_item;
+  bool const l_ra = a.a_k != 1, l_rb = a.b_k != 1;
+  if( a.o_col != 1 || a.K == 0 || ( l_ra && ( a.a_row != 1 || a.M < 2 ) ) || ( l_rb && ( a.b_row != 1 || a.N < 2 ) ) || ( l_ra && !l_rb ) ) {
+    return BlockLayout::NONE;
+  }
+  // k (or rows) of 16 bytes start at multiples of 16
+  auto aligned = [&]( void const * p, int64_t c, int64_t stride ) {
+    return uintptr_t( p ) % 16 == 0 && c * l_item % 16 == 0 && stride * l_item % 16 == 0;
+  };
+  int64_t const l_sa = l_ra ? a.a_k : a.a_row, l_sb = l_rb ? a.b_k : a.b_row;
+  if( !aligned( a.a, a.a_c, l_sa ) || !aligned( a.b, a.b_c, l_sb ) ) return BlockLayout::NONE;
+  if( ( !l_ra || !l_rb ) && a.K * l_item % 16 != 0 ) return BlockLayout::NONE;
+  // 31 bits of bytes in a step of a tile, and along k; rows of a k that do not
+  // reach into the next k's, so that k past the end lie past the buffer's end
+  int64_t const l_max = int64_t( 1 ) << 31;
+  if( l_ra ? l_sa * l_item * l_step >= l_max || a.M > l_sa : l_sa * l_item * 256 >= l_max ) return BlockLayout::NONE;
+  if( l_rb ? l_sb * l_item * l_step >= l_max || a.N > l_sb : l_sb * l_item * 256 >= l_max ) return BlockLayout::NONE;
+  if( int64_t( a.K ) * l_item >= l_max - 256 ) return BlockLayout::NONE;
+  // scales: 31 bits along a tile's rows and along k
+  int64_t const l_kb = ( int64_t( a.K ) + kScaleBlock - 1 ) / kScaleBlock;
+  if( a.sa_row * 4 * 256 >= l_max || a.sb_row * 4 * 256 >= l_max || a.sa_k * 4 * l_kb >= l_max || a.sb_k * 4 * l_kb >= l_max ) {
+    return BlockLayout::NONE;
+  }
+  return l_ra ? BlockLayout::ROWS_ROWS : l_rb ? BlockLayout::K_ROWS : BlockLayout::K_K;
+}
+
+struct Tile {
+  BlockKernel  kernel;
+  char const * name;
+  int32_t      rows, cols;
+};
+Tile const kTiles[] = {
+  { BlockKernel::TILE_64x64,   "tile 64x64",   64,  64 },
+  { BlockKernel::TILE_128x128, "tile 128x128", 128, 128 },
+  { BlockKernel::TILE_256x128, "tile 256x128", 256, 128 },
+  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256 }
+};
+
+// rows of tiles in all batches or groups
+int64_t tiles_m( BlockArgs const & a, int64_t rows ) {
+  return a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, rows ) : ( a.M + rows - 1 ) / rows * a.C;
+}
+
+bool exact( BlockArgs const & a ) { return a.has( BlockArgs::F8 ) && !a.has( BlockArgs::OUT_BF16 ); }
+
+char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
+  plan.kernel = BlockKernel::GENERAL;
+  plan.layout = layout_of( a );
+  if( plan.layout == BlockLayout::NONE ) return "general";
+  char const * l_env = std::getenv( "ETIR_BLOCK_TILE" );
+  int const l_forced = l_env ? std::atoi( l_env ) : -1;
+  if( l_forced == 0 ) return "general";
+  Tile const * l_best = nullptr;
+  for( Tile const & l_t : kTiles ) {
+    if( exact( a ) && l_t.kernel == BlockKernel::TILE_256x256 ) continue;
+    double const l_groups = double( tiles_m( a, l_t.rows ) ) * double( ( a.N + l_t.cols - 1 ) / l_t.cols );
+    if( l_groups * 512 >= 4294967296.0 ) continue;
+    if( l_forced == int( l_t.kernel ) ) {
+      l_best = &l_t;
+      break;
+    }
+    if( l_best == nullptr || l_groups >= 256 ) l_best = &l_t;
+  }
+  if( l_best == nullptr ) return "general";
+  plan.kernel = l_best->kernel;
+  return l_best->name;
 }
 
 int plan_block( Given const & g, BlockPlan & plan ) {
@@ -233,7 +304,7 @@ int plan_block( Given const & g, BlockPlan & plan ) {
   if( plan.has_bias ) plan.bytes += 4 * l_c * a.N;
   if( l_grouped ) plan.bytes += 4 * ( int64_t( a.C ) + 1 );
   char const * const l_left = l_f8 ? ( g.dtype_left == ETIR_F8E5M2 ? "e5m2" : "e4m3" ) : "bf16";
-  plan.desc = l_w + " general " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
+  plan.desc = l_w + " " + choose_kernel( a, plan ) + " " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
             + " N=" + std::to_string( a.N ) + " K=" + std::to_string( a.K )
             + ( l_grouped ? ( l_ragged_k ? " ragged K" : " ragged M" ) : "" ) + " " + l_left
             + ( a.has( BlockArgs::OUT_BF16 ) ? " out=bf16" : " out=fp32" );
@@ -260,7 +331,14 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
       || ( plan.has_bias && bias == nullptr ) ) {
     return fail( ETIR_NO_DATA_PTR_PROVIDED, l_w + ": null scale or bias, but its strides were given" );
   }
-  return launch_block_general( a, stream );
+  BlockKernel l_kernel = plan.kernel;
+  // pointers may be less aligned than the strides
+  if( l_kernel != BlockKernel::GENERAL && layout_of( a ) == BlockLayout::NONE ) l_kernel = BlockKernel::GENERAL;
+  if( l_kernel == BlockKernel::GENERAL ) return launch_block_general( a, stream );
+  if( !a.has( BlockArgs::F8 ) )   return launch_block_tile_bf16( a, l_kernel, plan.layout, stream );
+  if( exact( a ) )                return launch_block_tile_exact( a, l_kernel, plan.layout, stream );
+  if( a.has( BlockArgs::E8M0 ) )  return launch_block_tile_e8m0( a, l_kernel, plan.layout, stream );
+  return launch_block_tile_f8( a, l_kernel, plan.layout, stream );
 }
 
 // Runs fn; what it throws (only memory can run out) becomes an error code.

@@ -1,0 +1,631 @@
+// gfx950 product of 8-bit floating point blocks, or of bf16, with or without
+// groups, tiles staged through LDS:
+//
+//   out[c][m][n] = last( sum_kb sa[c][m][kb] sb[c][n][kb] sum_(k in kb) A[c][m][k] B[c][n][k] + bias[c][n] )
+//
+// A workgroup computes a BM x BN tile, a wave a block of TM x TN fragments of
+// 16 x 16.  A step takes 128 bytes of k of every row: one block of 128 8-bit
+// numbers or 64 bf16.
+//
+// Operands go from global memory into LDS directly (buffer_load ... lds), STAGES
+// steps deep, one barrier a step.  An operand that is unit-stride along k lies
+// there as [row][128 bytes], 16-byte piece g of row r at place g ^ swz(r), and a
+// fragment is two 16-byte reads a lane.  One that is unit-stride along its rows
+// lies as [k][row], the pieces of a k likewise exchanged, and a fragment is four
+// transposing reads (ds_read_b64_tr_b8 / _tr_b16).  A lane of either holds row
+// lane % 16 and the pieces lane / 16 and lane / 16 + 4 of its k; which k these
+// are does not matter as long as both operands agree.
+//
+// The columns' side is the first operand of the matrix instruction, so a lane
+// holds one row m and 4 neighbouring columns; the tile goes out through LDS in
+// rows of 16-byte stores.
+//
+// How a block's sum is made (KIND):
+//   BF16    v_mfma_f32_16x16x32_bf16 onto the accumulators.
+//   F8      v_mfma_f32_16x16x128_f8f6f4 from zero, then one fused multiply-add
+//           with the product of the block's scales: 4 for each matrix
+//           instruction of 32 cycles.  The matrix cores add 8-bit products in
+//           groups of 8, cut 13 binary places below the largest (measured), a
+//           relative error of 2^-16 of a sum of normal numbers, which bf16
+//           outputs (2^-9) do not show.
+//   EXACT   fp32 outputs: the 8-bit numbers become bf16 between LDS and the
+//           matrix cores, where products are exact and sums fp32, at half the
+//           rate.
+//   E8M0    as F8, the scales applied by the matrix instruction itself.
+#ifndef ETIR_CONTRACT_BLOCK_TILE_H
+#define ETIR_CONTRACT_BLOCK_TILE_H
+
+#include "block_internal.h"
+#include "contract_dma.h"
+
+namespace etir {
+namespace block {
+
+using kern::i32x4;
+typedef int32_t i32x2 __attribute__( ( ext_vector_type( 2 ) ) );
+typedef int32_t i32x8 __attribute__( ( ext_vector_type( 8 ) ) );
+typedef float   f32x4 __attribute__( ( ext_vector_type( 4 ) ) );
+typedef __bf16  bf16x2 __attribute__( ( ext_vector_type( 2 ) ) );
+typedef __bf16  bf16x8 __attribute__( ( ext_vector_type( 8 ) ) );
+
+enum Kind : int { BF16, F8, EXACT, E8M0 };
+
+constexpr int kStep = 128;      // bytes of k of a step
+
+// Slots of 16 bytes of one k of an operand that lies along its rows, and by what
+// they are exchanged: the 8-byte (f8: of 8 k, bf16: of 4) transposing reads of 16
+// lanes, and of the 16 beside them, touch every bank once.
+template< int ROWS, int ITEM >
+__device__ inline uint32_t swz_rows( int k ) {
+  constexpr int SLOTS = ROWS * ITEM / 16;
+  if constexpr( ITEM == 1 ) {
+    constexpr int P = 16 / SLOTS;                  // k in 256 bytes
+    return uint32_t( k / P % ( 8 / P ) + ( k >> 4 & 1 ) * ( 8 / P ) );
+  }
+  else if constexpr( SLOTS >= 16 ) return uint32_t( 2 * ( k & 3 ) + 8 * ( k >> 3 & 1 ) );
+  else return uint32_t( 2 * ( k >> 1 & 1 ) + 4 * ( k >> 3 & 1 ) );
+}
+
+// One operand's ROWS rows of a step, loaded by WAVES waves, 64 pieces of 16
+// bytes at a time.
+template< int ROWS, int WAVES, bool ALONG_ROWS, int ITEM >
+struct Side {
+  static constexpr int LOADS = ROWS / 8;
+  static constexpr int EACH  = LOADS / WAVES;      // a wave's
+  static constexpr int BYTES = ROWS * kStep;
+  static constexpr int K     = kStep / ITEM;       // k of a step
+  static_assert( LOADS % WAVES == 0, "loads have to divide over the waves" );
+
+  uint32_t     m_off[EACH];      // bytes from the step's first to the lane's piece
+  int          m_k[2];           // along k: the lane's byte of the step in even and odd loads
+  uint32_t     m_first;          // the wave's first load
+  uint8_t const * m_base;
+  int64_t      m_stride;         // along rows: bytes from k to k
+  int32_t      m_extent;         // along rows: bytes of a k from the tile's first row to the tensor's last
+  i32x4        m_rsrc;
+
+  // tile: the first row at k = 0; stride: bytes from row to row, or (along rows)
+  // from k to k; rows: of the tensor from there on
+  __device__ inline void init( uint8_t const * tile, int64_t stride, int32_t rows, int wave, int lane ) {
+    m_first = wave * EACH;
+    m_base = tile;
+    m_stride = stride;
+    if constexpr( ALONG_ROWS ) {
+      constexpr int SLOTS = ROWS * ITEM / 16, PER = 64 / SLOTS;      // k of a load
+      // to the last dword: its bytes past the tensor are in the same dword as the last row
+      m_extent = ( rows * ITEM + 3 ) & ~3;
+#pragma unroll
+      for( int l_i = 0; l_i < EACH; l_i++ ) {
+        int const l_k = ( int( m_first ) + l_i ) * PER + lane / SLOTS;
+        m_off[l_i] = uint32_t( l_k * int32_t( stride ) ) + 16u * ( uint32_t( lane % SLOTS ) ^ swz_rows< ROWS, ITEM >( l_k ) );
+      }
+    }
+    else {
+      m_rsrc = kern::make_rsrc( tile, kern::kDmaOob );
+#pragma unroll
+      for( int l_i = 0; l_i < 2; l_i++ ) m_k[l_i] = 16 * ( ( lane % 8 ) ^ int( kern::swz_k( 8 * l_i + lane / 8 ) ) );
+#pragma unroll
+      for( int l_i = 0; l_i < EACH; l_i++ ) {
+        // rows past the tensor read its last one and are not stored
+        int32_t const l_r = min( int32_t( 8 * ( m_first + l_i ) + lane / 8 ), rows - 1 );
+        m_off[l_i] = uint32_t( l_r * int32_t( stride ) + m_k[( m_first + l_i ) % 2] );
+      }
+    }
+  }
+  // the step of which the next loads are; k: all of the sum's
+  __device__ __attribute__( ( always_inline ) ) inline void at_step( int32_t step, int32_t k ) {
+    if constexpr( ALONG_ROWS ) {
+      // k past the end lie past the buffer's last byte: they load zeros
+      int32_t const l_left = min( k - step * K, K );
+      uint32_t const l_bytes = l_left > 0 ? uint32_t( l_left - 1 ) * uint32_t( m_stride ) + uint32_t( m_extent ) : 0u;
+      m_rsrc = kern::make_rsrc( m_base + int64_t( step ) * K * m_stride, l_bytes );
+    }
+  }
+  // starts the wave's load I of a step into lds
+  template< int I >
+  __device__ __attribute__( ( always_inline ) ) inline void issue( uint32_t lds, int32_t step, int32_t k ) {
+    uint32_t l_off = m_off[I], l_soff = 0;
+    if constexpr( !ALONG_ROWS ) {
+      // k is a multiple of 16 bytes, so a lane's piece is inside or outside; outside: zeros
+      int32_t const l_at = step * kStep, l_bytes = k * ITEM;
+      if( l_at + kStep > l_bytes && l_at + m_k[( m_first + I ) % 2] >= l_bytes ) l_off = kern::kDmaOob;
+      l_soff = uint32_t( l_at );
+    }
+    kern::set_m0( lds + ( m_first + I ) * 1024 );
+    kern::dma16_so< 0 >( m_rsrc, l_off, l_soff );
+  }
+};
+
+// 16 rows x 128 bytes of k: a lane's two pieces of 16 bytes
+struct Frag { i32x4 v[2]; };
+
+// Reads fragments of an operand's side.
+template< int ROWS, bool ALONG_ROWS, int ITEM >
+struct Reader {
+  typedef short v4i16 __attribute__( ( ext_vector_type( 4 ) ) );
+  typedef __attribute__( ( address_space( 3 ) ) ) v4i16 lds_v4i16;
+  typedef __attribute__( ( address_space( 3 ) ) ) i32x2 lds_v2i32;
+  int      m_lane;
+  uint32_t m_k[4];          // along rows: bytes to the k of the lane's four reads
+  uint32_t m_swz[4];
+
+  __device__ inline void init( int lane ) {
+    m_lane = lane;
+    if constexpr( ALONG_ROWS ) {
+#pragma unroll
+      for( int l_i = 0; l_i < 4; l_i++ ) {
+        // piece lane / 16 (+ 4) has 16 / ITEM k, read 8 / ITEM at a time
+        int const l_piece = lane / 16 + 4 * ( l_i / 2 );
+        int const l_k = l_piece * ( 16 / ITEM ) + ( l_i % 2 ) * ( 8 / ITEM ) + lane % 16 / ( ITEM == 1 ? 2 : 4 );
+        m_k[l_i] = uint32_t( l_k * ROWS * ITEM );
+        m_swz[l_i] = swz_rows< ROWS, ITEM >( l_k );
+      }
+    }
+  }
+  // the fragment of rows row .. row + 15 (a multiple of 16)
+  __device__ __attribute__( ( always_inline ) ) inline Frag read( char const * lds, int row ) const {
+    Frag l_f;
+    if constexpr( !ALONG_ROWS ) {
+      int const l_r = row + m_lane % 16;
+      uint32_t const l_swz = kern::swz_k( m_lane % 16 );      // of rows 16 apart: the same
+#pragma unroll
+      for( int l_i = 0; l_i < 2; l_i++ ) {
+        l_f.v[l_i] = *reinterpret_cast< i32x4 const * >( lds + l_r * kStep + ( ( uint32_t( m_lane / 16 + 4 * l_i ) ^ l_swz ) << 4 ) );
+      }
+    }
+    else {
+#pragma unroll
+      for( int l_i = 0; l_i < 4; l_i++ ) {
+        // f8: lanes 2 j and 2 j + 1 read the 16 rows of k j; bf16: lanes 4 j to 4 j + 3
+        i32x2 l_v;
+        if constexpr( ITEM == 1 ) {
+          char const * l_p = lds + m_k[l_i] + ( ( uint32_t( row / 16 ) ^ m_swz[l_i] ) << 4 ) + 8 * ( m_lane & 1 );
+          l_v = __builtin_amdgcn_ds_read_tr8_b64_v2i32( (lds_v2i32 *) l_p );
+        }
+        else {
+          char const * l_p = lds + m_k[l_i] + ( ( uint32_t( row / 8 + ( m_lane >> 1 & 1 ) ) ^ m_swz[l_i] ) << 4 ) + 8 * ( m_lane & 1 );
+          l_v = __builtin_bit_cast( i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16( (lds_v4i16 *) l_p ) );
+        }
+        l_f.v[l_i / 2][2 * ( l_i % 2 )] = l_v[0];
+        l_f.v[l_i / 2][2 * ( l_i % 2 ) + 1] = l_v[1];
+      }
+    }
+    return l_f;
+  }
+};
+
+// 32 8-bit numbers as four operands of 8 bf16
+struct Wide { bf16x8 v[4]; };
+template< bool E5M2 >
+__device__ __attribute__( ( always_inline ) ) inline Wide widen( Frag const & f ) {
+  Wide l_w;
+#pragma unroll
+  for( int l_i = 0; l_i < 8; l_i++ ) {
+    int const l_d = f.v[l_i / 4][l_i % 4];
+    bf16x2 l_lo, l_hi;
+    if constexpr( E5M2 ) {
+      l_lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8( l_d, 1.0f, false );
+      l_hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8( l_d, 1.0f, true );
+    }
+    else {
+      l_lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8( l_d, 1.0f, false );
+      l_hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8( l_d, 1.0f, true );
+    }
+    l_w.v[l_i / 2][4 * ( l_i % 2 )] = l_lo[0];
+    l_w.v[l_i / 2][4 * ( l_i % 2 ) + 1] = l_lo[1];
+    l_w.v[l_i / 2][4 * ( l_i % 2 ) + 2] = l_hi[0];
+    l_w.v[l_i / 2][4 * ( l_i % 2 ) + 3] = l_hi[1];
+  }
+  return l_w;
+}
+
+// What a workgroup computes: tile of BM x BN of batch or group c.
+struct Where {
+  int32_t c, m0, m_end, n0;
+  int32_t k_begin, K;
+  bool    any;
+};
+
+// Neighbouring tiles on one XCD (workgroups go to the 8 XCDs in turn), and there
+// in bands of 8 tile rows, so that its cache serves both operands.
+template< int BM, int BN >
+__device__ inline Where where( BlockArgs const & a ) {
+  bool const l_grouped = a.has( BlockArgs::GROUP_ROWS );
+  int32_t const l_tiles_n = ( a.N + BN - 1 ) / BN;
+  // rows of tiles: as many as the grid has
+  int32_t const l_tiles_m = l_grouped ? a.M / BM + min( a.M, a.C ) : ( a.M + BM - 1 ) / BM;
+  int32_t const l_per_c = l_tiles_m * l_tiles_n, l_each = l_per_c / 8;
+  Where l_w;
+  l_w.c = int32_t( blockIdx.x / uint32_t( l_per_c ) );
+  int32_t l_r = int32_t( blockIdx.x % uint32_t( l_per_c ) );
+  if( l_r < 8 * l_each ) l_r = l_r % 8 * l_each + l_r / 8;
+  int32_t const l_band = l_r / ( 8 * l_tiles_n ) * 8;
+  int32_t const l_high = min( 8, l_tiles_m - l_band );
+  int32_t const l_tile_m = l_band + l_r % ( 8 * l_tiles_n ) % l_high;
+  l_w.n0 = ( l_r % ( 8 * l_tiles_n ) / l_high ) * BN;
+  l_w.m0 = l_tile_m * BM;
+  l_w.m_end = a.M;
+  l_w.k_begin = 0;
+  l_w.K = a.K;
+  l_w.any = true;
+  if( l_grouped ) {
+    BlockRows const l_rows = block_rows< BM >( a.offsets, a.C, a.M, l_tile_m );
+    l_w.any = l_rows.group >= 0;
+    l_w.c = l_rows.group;
+    l_w.m0 = l_rows.m0;
+    l_w.m_end = l_rows.end;
+  }
+  else if( a.has( BlockArgs::GROUP_K ) ) {
+    BlockGroup const l_g = block_group( a.offsets, l_w.c, a.K );
+    l_w.k_begin = l_g.begin;
+    l_w.K = l_g.end - l_g.begin;
+  }
+  return l_w;
+}
+
+// The scales of a step: BM of A's rows, then BN of B's, a dword each in LDS
+// (E8M0: the byte).  64 of them a load; every wave has EACH loads, those past the
+// last one load zeros.
+template< int BM, int BN, int WAVES >
+struct Scales {
+  static constexpr int LOADS = ( BM + BN ) / 64;
+  static constexpr int EACH  = ( LOADS + WAVES - 1 ) / WAVES;
+  static constexpr int BYTES = EACH * WAVES * 256;
+  uint32_t m_off[EACH];      // bytes from block kb = 0 to the lane's scale
+  uint32_t m_k[EACH];        // bytes from block to block of k
+  i32x4    m_rsrc[EACH];
+  uint32_t m_first;
+
+  __device__ inline void init( BlockArgs const & a, Where const & w, int wave, int lane ) {
+    int const l_item = a.has( BlockArgs::E8M0 ) ? 1 : 4;
+    m_first = wave * EACH;
+#pragma unroll
+    for( int l_i = 0; l_i < EACH; l_i++ ) {
+      int const l_load = int( m_first ) + l_i;
+      bool const l_a = l_load < BM / 64;
+      int32_t const l_at = 64 * ( l_a ? l_load : l_load - BM / 64 ) + lane;
+      // rows past the tensor take the last one's scale and are not stored; the
+      // tile's first row or block is in the base
+      int32_t const l_first = l_a ? w.m0 : w.n0;
+      int32_t const l_row = min( l_first + l_at, ( l_a ? w.m_end : a.N ) - 1 );
+      bool const l_blocks = a.has( l_a ? BlockArgs::SA_BLOCKS : BlockArgs::SB_BLOCKS );
+      int32_t const l_b0 = l_blocks ? l_first / kScaleBlock : l_first, l_b = l_blocks ? l_row / kScaleBlock : l_row;
+      int64_t const l_stride = l_a ? a.sa_row : a.sb_row;
+      void const * const l_s = l_a ? a.sa : a.sb;
+      m_off[l_i] = l_s != nullptr && l_load < LOADS ? uint32_t( ( l_b - l_b0 ) * int32_t( l_stride ) * l_item ) : kern::kDmaOob;
+      m_k[l_i] = uint32_t( ( l_a ? a.sa_k : a.sb_k ) * l_item );
+      m_rsrc[l_i] = kern::make_rsrc( static_cast< uint8_t const * >( l_s ) + ( w.c * ( l_a ? a.sa_c : a.sb_c ) + l_b0 * l_stride ) * l_item,
+                                     kern::kDmaOob );
+    }
+  }
+  template< int I >
+  __device__ __attribute__( ( always_inline ) ) inline void issue( uint32_t lds, int32_t step, int32_t blocks, bool e8m0 ) {
+    uint32_t const l_off = step < blocks ? m_off[I] : kern::kDmaOob;
+    uint32_t const l_soff = step < blocks ? uint32_t( step ) * m_k[I] : 0u;
+    kern::set_m0( lds + ( m_first + I ) * 256 );
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    if( e8m0 ) asm volatile( "buffer_load_ubyte %0, %1, %2 offen lds" :: "v"( l_off ), "s"( m_rsrc[I] ), "s"( l_soff ) );
+    else       asm volatile( "buffer_load_dword %0, %1, %2 offen lds" :: "v"( l_off ), "s"( m_rsrc[I] ), "s"( l_soff ) );
+#pragma clang diagnostic pop
+  }
+};
+
+// elements from row to row of a wave's output slab in LDS
+template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T ) );
+
+// Stores 16 rows x COLS columns of a wave's slab, 16 bytes a lane, non-temporal:
+// the output is not read here again.
+template< int COLS, class T >
+__device__ inline void store_slab( BlockArgs const & a, T const * slab, T * out, int32_t m1, int32_t m_end, int32_t n1, int lane ) {
+  constexpr int V = 16 / sizeof( T ), LANES = COLS / V, PITCH = kPitch< T, COLS >;
+  typedef T v __attribute__( ( ext_vector_type( V ) ) );
+  typedef v v_any __attribute__( ( aligned( sizeof( T ) ) ) );
+#pragma unroll
+  for( int l_p = 0; l_p < ( 16 * LANES + 63 ) / 64; l_p++ ) {
+    int const l_i = l_p * 64 + lane;
+    int const l_r = l_i / LANES, l_c = l_i % LANES * V;
+    if( l_r >= 16 || m1 + l_r >= m_end ) continue;
+    v const l_v = *reinterpret_cast< v const * >( slab + l_r * PITCH + l_c );
+    T * const l_o = out + int64_t( m1 + l_r ) * a.o_row + n1 + l_c;
+    int32_t const l_left = a.N - n1 - l_c;       // columns from this lane's first on
+    if( l_left >= V ) __builtin_nontemporal_store( l_v, reinterpret_cast< v_any * >( l_o ) );
+    else {
+#pragma unroll
+      for( int l_e = 0; l_e < V; l_e++ ) if( l_e < l_left ) l_o[l_e] = l_v[l_e];
+    }
+  }
+}
+
+// KIND: see above.  RA, RB: A (B) is unit-stride along its rows, else along k.
+// SB_ROWS: B has a scale for every row (F8 and EXACT), else one for 128.
+template< int KIND, int BM, int BN, int WM, int WN, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
+__global__ __launch_bounds__( 64 * WM * WN )
+void contract_block_tile_kernel( BlockArgs a ) {
+  constexpr int  ITEM = KIND == BF16 ? 2 : 1;
+  constexpr bool SCALED = KIND != BF16;
+  constexpr int  WAVES = WM * WN;
+  constexpr int  TM = BM / WM / 16, TN = BN / WN / 16;       // fragments of a wave
+  constexpr int  COLS = BN / WN;
+  static_assert( TN % 2 == 0 && ( KIND == BF16 || KIND == E8M0 || SB_ROWS || COLS <= kScaleBlock ), "wave tile" );
+  typedef Side< BM, WAVES, RA, ITEM > SideA;
+  typedef Side< BN, WAVES, RB, ITEM > SideB;
+  typedef Scales< BM, BN, WAVES > SideS;
+  constexpr int EACH = SideA::EACH + SideB::EACH + ( SCALED ? SideS::EACH : 0 );      // a wave's loads of a step
+  constexpr int STAGE = SideA::BYTES + SideB::BYTES + ( SCALED ? SideS::BYTES : 0 );
+  constexpr int SLAB = 16 * kPitch< float, COLS > * 4;
+  constexpr int BYTES = STAGES * STAGE > WAVES * SLAB ? STAGES * STAGE : WAVES * SLAB;
+  __shared__ __align__( 16 ) char l_lds[BYTES];
+
+  int const l_lane = threadIdx.x % 64;
+  int const l_wave = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
+  int const l_wm = l_wave / WN * ( BM / WM ), l_wn = l_wave % WN * COLS;
+  Where const w = where< BM, BN >( a );
+  if( !w.any ) return;
+
+  uint8_t const * const l_at_a = static_cast< uint8_t const * >( a.a ) + ( w.c * a.a_c + w.m0 * a.a_row + w.k_begin * a.a_k ) * ITEM;
+  uint8_t const * const l_at_b = static_cast< uint8_t const * >( a.b ) + ( w.c * a.b_c + w.n0 * a.b_row + w.k_begin * a.b_k ) * ITEM;
+  SideA l_a;
+  SideB l_b;
+  SideS l_s;
+  l_a.init( l_at_a, ( RA ? a.a_k : a.a_row ) * ITEM, w.m_end - w.m0, l_wave, l_lane );
+  l_b.init( l_at_b, ( RB ? a.b_k : a.b_row ) * ITEM, a.N - w.n0, l_wave, l_lane );
+  if constexpr( SCALED ) l_s.init( a, w, l_wave, l_lane );
+  Reader< BM, RA, ITEM > l_ra;
+  Reader< BN, RB, ITEM > l_rb;
+  l_ra.init( l_lane );
+  l_rb.init( l_lane );
+
+  int32_t const l_steps = int32_t( ( int64_t( w.K ) * ITEM + kStep - 1 ) / kStep );
+  uint32_t const l_lds_at = kern::lds_addr( l_lds );
+  // the wave's load i of a step, those of both sides and the scales counted through
+  auto issue = [&]( auto ic, int stage, int32_t step ) __attribute__( ( always_inline ) ) {
+    constexpr int l_i = decltype( ic )::value;
+    uint32_t const l_to = l_lds_at + stage * STAGE;
+    if constexpr( l_i < SideA::EACH ) {
+      if constexpr( l_i == 0 ) l_a.at_step( step, w.K );
+      l_a.template issue< l_i >( l_to, step, w.K );
+    }
+    else if constexpr( l_i < SideA::EACH + SideB::EACH ) {
+      if constexpr( l_i == SideA::EACH ) l_b.at_step( step, w.K );
+      l_b.template issue< l_i - SideA::EACH >( l_to + SideA::BYTES, step, w.K );
+    }
+    else if constexpr( SCALED ) {
+      l_s.template issue< l_i - SideA::EACH - SideB::EACH >( l_to + SideA::BYTES + SideB::BYTES, step, l_steps,
+                                                             KIND == E8M0 || ( KIND == EXACT && a.has( BlockArgs::E8M0 ) ) );
+    }
+  };
+  // loads of step 1 (two buffers) that are issued in front of the loop
+  constexpr int EARLY = ( EACH + 1 ) / 2;
+  kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, 0 ); } );
+  if constexpr( STAGES > 2 ) {
+    kern::static_for< STAGES - 2 >( [&]( auto sc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_st = decltype( sc )::value + 1;
+      kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, l_st, l_st ); } );
+    } );
+    kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+  }
+  else {
+    kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, 1 ); } );
+    kern::wait_vmcnt< EARLY >();
+  }
+  kern::barrier_lds();
+
+  f32x4 l_acc[TN][TM];
+#pragma unroll
+  for( int l_i = 0; l_i < TN * TM; l_i++ ) l_acc[l_i / TM][l_i % TM] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
+  Frag l_fa[TM], l_fb[2];
+  // scales: a row's of each fragment of A, and B's: of the 128 columns, or of a
+  // lane's 4 columns (E8M0: of the lane's row) of two fragments
+  int32_t l_sa[TM], l_sb1 = 0;
+  i32x4 l_sb[2];
+  auto scale_value = [&]( int32_t bits, bool have ) __attribute__( ( always_inline ) ) -> float {
+    if( !have ) return 1.0f;
+    return KIND == EXACT && a.has( BlockArgs::E8M0 ) ? e8m0_to_f32( uint8_t( bits ) ) : __uint_as_float( uint32_t( bits ) );
+  };
+  auto read_a = [&]( auto ic, int stage ) __attribute__( ( always_inline ) ) {
+    constexpr int l_i = decltype( ic )::value;
+    l_fa[l_i] = l_ra.read( l_lds + stage * STAGE, l_wm + 16 * l_i );
+  };
+  auto read_b = [&]( auto jc, int stage ) __attribute__( ( always_inline ) ) {
+    constexpr int l_j = decltype( jc )::value;
+    l_fb[l_j % 2] = l_rb.read( l_lds + stage * STAGE + SideA::BYTES, l_wn + 16 * l_j );
+    char const * const l_sc = l_lds + stage * STAGE + SideA::BYTES + SideB::BYTES + 4 * BM;
+    if constexpr( SCALED && KIND != E8M0 && SB_ROWS ) {
+      l_sb[l_j % 2] = *reinterpret_cast< i32x4 const * >( l_sc + 4 * ( l_wn + 16 * l_j + 4 * ( l_lane / 16 ) ) );
+    }
+    if constexpr( KIND == E8M0 ) l_sb[l_j % 2][0] = *reinterpret_cast< int32_t const * >( l_sc + 4 * ( l_wn + 16 * l_j + l_lane % 16 ) );
+  };
+  // the scales of A's rows (and of the 128 columns) of a step
+  auto read_s = [&]( int stage ) __attribute__( ( always_inline ) ) {
+    if constexpr( SCALED ) {
+      char const * const l_sc = l_lds + stage * STAGE + SideA::BYTES + SideB::BYTES;
+#pragma unroll
+      for( int l_i = 0; l_i < TM; l_i++ ) l_sa[l_i] = *reinterpret_cast< int32_t const * >( l_sc + 4 * ( l_wm + 16 * l_i + l_lane % 16 ) );
+      if constexpr( KIND != E8M0 && !SB_ROWS ) l_sb1 = *reinterpret_cast< int32_t const * >( l_sc + 4 * ( BM + l_wn ) );
+    }
+  };
+
+  // One step in TN parts, each a fragment of B against all of A's.  During a
+  // part the next fragment of B is read; the barrier stands in front of the last
+  // part, when every wave has read all of this step and the next one has landed,
+  // and behind it A's fragments of the next step replace this one's as they
+  // fall free.  Two buffers: the step after that is loaded over this one from
+  // there on, half of it in the last part, half in the next step's first.  More:
+  // the step STAGES - 1 ahead is loaded over the last one, spread over the parts
+  // in front of the barrier.
+  auto step = [&]( int l_st, int l_next, int l_free, int32_t s ) __attribute__( ( always_inline ) ) {
+    float l_scale[TM];
+    if constexpr( KIND == F8 || KIND == EXACT ) {
+      float const l_b1 = SB_ROWS ? 1.0f : scale_value( l_sb1, a.sb != nullptr );
+#pragma unroll
+      for( int l_i = 0; l_i < TM; l_i++ ) l_scale[l_i] = scale_value( l_sa[l_i], a.sa != nullptr ) * l_b1;
+    }
+    constexpr int RING = 3;
+    f32x4 l_part[KIND == F8 ? RING : TM];
+    f32x4 l_of_b[2];        // SB_ROWS: the scales of the columns of this part and the last
+    Wide l_wa[KIND == EXACT ? TM : 1];
+    if constexpr( KIND == EXACT ) {
+#pragma unroll
+      for( int l_i = 0; l_i < TM; l_i++ ) l_wa[l_i] = widen< A_E5M2 >( l_fa[l_i] );
+    }
+    auto add = [&]( auto mc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_j = decltype( mc )::value / TM, l_i = decltype( mc )::value % TM;
+      f32x4 const & l_p = l_part[KIND == F8 ? decltype( mc )::value % RING : l_i];
+#pragma unroll
+      for( int l_e = 0; l_e < 4; l_e++ ) {
+        float const l_f = SB_ROWS ? l_scale[l_i] * l_of_b[l_j % 2][l_e] : l_scale[l_i];
+        l_acc[l_j][l_i][l_e] = fmaf( l_p[l_e], l_f, l_acc[l_j][l_i][l_e] );
+      }
+    };
+    kern::static_for< TN >( [&]( auto jc ) __attribute__( ( always_inline ) ) {
+      constexpr int l_j = decltype( jc )::value;
+      constexpr bool LAST = l_j == TN - 1;
+      if constexpr( LAST ) {
+        kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+        kern::wait_lgkmcnt0();
+        kern::barrier_lds();
+      }
+      Frag const & l_f = l_fb[l_j % 2];
+      int32_t l_bits_b = 0;
+      if constexpr( KIND == E8M0 ) l_bits_b = a.sb != nullptr ? l_sb[l_j % 2][0] : 127;
+      if constexpr( ( KIND == F8 || KIND == EXACT ) && SB_ROWS ) {
+#pragma unroll
+        for( int l_e = 0; l_e < 4; l_e++ ) l_of_b[l_j % 2][l_e] = scale_value( l_sb[l_j % 2][l_e], a.sb != nullptr );
+      }
+      Wide l_wb;
+      if constexpr( KIND == EXACT ) l_wb = widen< false >( l_f );
+      if constexpr( !LAST ) read_b( std::integral_constant< int, l_j + 1 >(), l_st );
+      else                  read_b( std::integral_constant< int, 0 >(), l_next );
+      kern::static_for< TM >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
+        constexpr int l_i = decltype( ic )::value, l_m = l_j * TM + l_i;
+        if constexpr( KIND == BF16 ) {
+          l_acc[l_j][l_i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16( __builtin_bit_cast( bf16x8, l_f.v[0] ),
+                                                                     __builtin_bit_cast( bf16x8, l_fa[l_i].v[0] ), l_acc[l_j][l_i], 0, 0, 0 );
+          l_acc[l_j][l_i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16( __builtin_bit_cast( bf16x8, l_f.v[1] ),
+                                                                     __builtin_bit_cast( bf16x8, l_fa[l_i].v[1] ), l_acc[l_j][l_i], 0, 0, 0 );
+        }
+        else if constexpr( KIND == EXACT ) {
+          f32x4 l_p = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+          for( int l_q = 0; l_q < 4; l_q++ ) l_p = __builtin_amdgcn_mfma_f32_16x16x32_bf16( l_wb.v[l_q], l_wa[l_i].v[l_q], l_p, 0, 0, 0 );
+          l_part[l_i] = l_p;
+          if constexpr( l_i > 0 ) add( std::integral_constant< int, l_m - 1 >() );
+        }
+        else {
+          i32x8 const l_vb = __builtin_shufflevector( l_f.v[0], l_f.v[1], 0, 1, 2, 3, 4, 5, 6, 7 );
+          i32x8 const l_va = __builtin_shufflevector( l_fa[l_i].v[0], l_fa[l_i].v[1], 0, 1, 2, 3, 4, 5, 6, 7 );
+          constexpr int FORMAT = A_E5M2 ? 1 : 0;
+          if constexpr( KIND == E8M0 ) {
+            l_acc[l_j][l_i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, l_acc[l_j][l_i], 0, FORMAT, 0, l_bits_b, 0,
+                                                                                a.sa != nullptr ? l_sa[l_i] : 127 );
+          }
+          else {
+            l_part[l_m % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, FORMAT,
+                                                                                   0, 0, 0, 0 );
+            if constexpr( l_m >= RING - 1 ) add( std::integral_constant< int, l_m - RING + 1 >() );
+          }
+        }
+        if constexpr( LAST ) read_a( ic, l_next );
+        if constexpr( STAGES > 2 && !LAST ) {
+          constexpr int l_from = EACH * l_m / ( ( TN - 1 ) * TM ), l_to = EACH * ( l_m + 1 ) / ( ( TN - 1 ) * TM );
+          kern::static_for< l_to - l_from >( [&]( auto dc ) __attribute__( ( always_inline ) ) {
+            issue( std::integral_constant< int, l_from + decltype( dc )::value >(), l_free, s + STAGES - 1 );
+          } );
+        }
+        if constexpr( STAGES == 2 && ( LAST || l_j == 0 ) ) {
+          constexpr int l_p0 = LAST ? 0 : EARLY, l_n = LAST ? EARLY : EACH - EARLY;
+          constexpr int l_from = l_p0 + l_n * l_i / TM, l_to = l_p0 + l_n * ( l_i + 1 ) / TM;
+          kern::static_for< l_to - l_from >( [&]( auto dc ) __attribute__( ( always_inline ) ) {
+            issue( std::integral_constant< int, l_from + decltype( dc )::value >(), LAST ? l_st : l_next, LAST ? s + 2 : s + 1 );
+          } );
+        }
+        __builtin_amdgcn_sched_barrier( 0 );
+      } );
+      if constexpr( KIND == EXACT ) add( std::integral_constant< int, l_j * TM + TM - 1 >() );
+    } );
+    if constexpr( KIND == F8 ) {
+      kern::static_for< RING - 1 >( [&]( auto rc ) __attribute__( ( always_inline ) ) {
+        add( std::integral_constant< int, TN * TM - ( RING - 1 ) + decltype( rc )::value >() );
+      } );
+    }
+    read_s( l_next );
+  };
+  if( l_steps > 0 ) {
+    kern::static_for< TM >( [&]( auto ic ) __attribute__( ( always_inline ) ) { read_a( ic, 0 ); } );
+    read_b( std::integral_constant< int, 0 >(), 0 );
+    read_s( 0 );
+  }
+  int l_st = 0, l_free = STAGES - 1;
+  for( int32_t l_step = 0; l_step < l_steps; l_step++ ) {
+    int const l_next = l_st == STAGES - 1 ? 0 : l_st + 1;
+    step( l_st, l_next, l_free, l_step );
+    l_free = l_st;
+    l_st = l_next;
+  }
+  kern::wait_vmcnt< 0 >();
+  __syncthreads();           // nothing is on its way into LDS, all fragments are read
+
+  // 16 rows at a time through this wave's slab
+  auto finish = [&]( auto zero ) __attribute__( ( always_inline ) ) {
+    typedef decltype( zero ) T;
+    typedef T t4 __attribute__( ( ext_vector_type( 4 ) ) );
+    T * const l_slab = reinterpret_cast< T * >( l_lds + l_wave * SLAB );
+    T * const l_out = static_cast< T * >( a.out ) + w.c * a.o_c;
+#pragma unroll
+    for( int l_i = 0; l_i < TM; l_i++ ) {
+#pragma unroll
+      for( int l_j = 0; l_j < TN; l_j++ ) {
+        int const l_n = 16 * l_j + 4 * ( l_lane / 16 );
+        t4 l_v;
+#pragma unroll
+        for( int l_e = 0; l_e < 4; l_e++ ) {
+          float l_f = l_acc[l_j][l_i][l_e];
+          if( a.bias ) l_f += a.bias[w.c * a.bias_c + min( w.n0 + l_wn + l_n + l_e, a.N - 1 ) * a.bias_col];
+          if( a.has( BlockArgs::RELU ) && l_f < 0.0f ) l_f = 0.0f;         // a NaN stays
+          l_v[l_e] = static_cast< T >( l_f );
+        }
+        *reinterpret_cast< t4 * >( l_slab + ( l_lane % 16 ) * kPitch< T, COLS > + l_n ) = l_v;
+      }
+      // the slab is this wave's own, and its LDS operations are in order
+      __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
+      store_slab< COLS, T >( a, l_slab, l_out, w.m0 + l_wm + 16 * l_i, w.m_end, w.n0 + l_wn, l_lane );
+      __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
+    }
+  };
+  if( a.has( BlockArgs::OUT_BF16 ) ) finish( __bf16( 0.0f ) );
+  else                               finish( 0.0f );
+}
+
+template< int KIND, int BM, int BN, int WM, int WN, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
+int launch_shape( BlockArgs const & a, hipStream_t stream ) {
+  int64_t const l_tiles_n = ( int64_t( a.N ) + BN - 1 ) / BN;
+  int64_t const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, BM ) : ( int64_t( a.M ) + BM - 1 ) / BM * a.C;
+  hipLaunchKernelGGL( ( contract_block_tile_kernel< KIND, BM, BN, WM, WN, STAGES, RA, RB, A_E5M2, SB_ROWS > ),
+                      dim3( uint32_t( l_tiles_m * l_tiles_n ) ), dim3( 64 * WM * WN ), 0, stream, a );
+  hipError_t const l_e = hipGetLastError();
+  if( l_e != hipSuccess ) {
+    return fail( ETIR_UNDEFINED_ERROR, std::string( "contraction launch failed: " ) + hipGetErrorString( l_e ) );
+  }
+  return ETIR_SUCCESS;
+}
+
+// the tiles of one kind and layout
+template< int KIND, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
+int launch_tiles( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
+  switch( kernel ) {
+    case BlockKernel::TILE_64x64:   return launch_shape< KIND, 64, 64, 2, 2, 4, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+    case BlockKernel::TILE_128x128: return launch_shape< KIND, 128, 128, 2, 2, 2, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+    case BlockKernel::TILE_256x128: return launch_shape< KIND, 256, 128, 4, 2, 3, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+    case BlockKernel::TILE_256x256:
+      // the widened operands of EXACT leave no registers for it
+      if constexpr( KIND != EXACT ) return launch_shape< KIND, 256, 256, 4, 2, 2, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+      [[fallthrough]];
+    default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown tile" );
+  }
+}
+
+}  // namespace block
+}  // namespace etir
+
+#endif

@@ -1,0 +1,25 @@
+// The tiles of contract_block_tile.h: 8-bit products on the matrix cores, which apply the e8m0 scales.
+#include "contract_block_tile.h"
+
+namespace etir {
+
+namespace {
+
+template< bool A_E5M2 >
+int launch_type( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
+  using namespace block;
+  switch( layout ) {
+    case BlockLayout::K_K:       return launch_tiles< block::E8M0, false, false, A_E5M2, true >( a, kernel, stream );
+    case BlockLayout::K_ROWS:    return launch_tiles< block::E8M0, false, true, A_E5M2, true >( a, kernel, stream );
+    case BlockLayout::ROWS_ROWS: return launch_tiles< block::E8M0, true, true, A_E5M2, true >( a, kernel, stream );
+    default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown layout" );
+  }
+}
+
+}  // namespace
+
+int launch_block_tile_e8m0( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
+  return a.has( BlockArgs::A_E5M2 ) ? launch_type< true >( a, kernel, layout, stream ) : launch_type< false >( a, kernel, layout, stream );
+}
+
+}  // namespace etir
