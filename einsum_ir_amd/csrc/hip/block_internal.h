@@ -41,6 +41,9 @@ struct BlockArgs {
 
 enum class BlockKernel : int32_t {
   GENERAL,         // any strides, 64 x 64 tiles (contract_block.hip)
+  FEW_4,           // few rows of A, K over the waves and in 4 parts (contract_block_few.hip)
+  FEW_16,          // the same, 16 rows at a time, K over the waves
+  FEW_32,          // 32 rows at a time
   TILE_64x64,      // through LDS directly (contract_block_tile.h), both operands at multiples of 16 bytes
   TILE_128x128,
   TILE_256x128,
@@ -67,6 +70,7 @@ struct BlockPlan {
 };
 
 int launch_block_general( BlockArgs const & a, hipStream_t stream );
+int launch_block_few( BlockArgs const & a, BlockKernel kernel, hipStream_t stream );
 int launch_block_tile_bf16( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 int launch_block_tile_f8( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 int launch_block_tile_exact( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );

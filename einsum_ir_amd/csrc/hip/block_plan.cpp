@@ -129,6 +129,9 @@ struct Tile {
   int32_t      rows, cols;
 };
 Tile const kTiles[] = {
+  { BlockKernel::FEW_4,        "few 4",        4,   4 },
+  { BlockKernel::FEW_16,       "few 16",       16,  16 },
+  { BlockKernel::FEW_32,       "few 32",       32,  16 },
   { BlockKernel::TILE_64x64,   "tile 64x64",   64,  64 },
   { BlockKernel::TILE_128x128, "tile 128x128", 128, 128 },
   { BlockKernel::TILE_256x128, "tile 256x128", 256, 128 },
@@ -142,15 +145,21 @@ int64_t tiles_m( BlockArgs const & a, int64_t rows ) {
 
 bool exact( BlockArgs const & a ) { return a.has( BlockArgs::F8 ) && !a.has( BlockArgs::OUT_BF16 ); }
 
+// operands that the kernel of few rows reads: unit-stride along k, at any address
+bool few_fits( BlockArgs const & a ) {
+  return a.a_k == 1 && a.b_k == 1 && a.K * ( a.has( BlockArgs::F8 ) ? int64_t( 1 ) : int64_t( 2 ) ) >= 16 && !a.has( BlockArgs::GROUP_K );
+}
+
 char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
   plan.kernel = BlockKernel::GENERAL;
   plan.layout = layout_of( a );
-  if( plan.layout == BlockLayout::NONE ) return "general";
   char const * l_env = std::getenv( "ETIR_BLOCK_TILE" );
   int const l_forced = l_env ? std::atoi( l_env ) : -1;
   if( l_forced == 0 ) return "general";
   Tile const * l_best = nullptr;
   for( Tile const & l_t : kTiles ) {
+    bool const l_few = l_t.kernel <= BlockKernel::FEW_32;
+    if( l_few ? !few_fits( a ) : plan.layout == BlockLayout::NONE ) continue;
     if( exact( a ) && l_t.kernel == BlockKernel::TILE_256x256 ) continue;
     double const l_groups = double( tiles_m( a, l_t.rows ) ) * double( ( a.N + l_t.cols - 1 ) / l_t.cols );
     if( l_groups * 512 >= 4294967296.0 ) continue;
@@ -158,7 +167,9 @@ char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
       l_best = &l_t;
       break;
     }
-    if( l_best == nullptr || l_groups >= 256 ) l_best = &l_t;
+    if( l_few && l_t.rows < ( a.has( BlockArgs::GROUP_ROWS ) ? 2 * a.M / a.C : a.M ) ) continue;
+    if( l_few && l_best ) continue;
+    if( l_best == nullptr || ( l_best->kernel > BlockKernel::FEW_32 && l_groups >= 256 ) ) l_best = &l_t;
   }
   if( l_best == nullptr ) return "general";
   plan.kernel = l_best->kernel;
@@ -333,8 +344,9 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
   }
   BlockKernel l_kernel = plan.kernel;
   // pointers may be less aligned than the strides
-  if( l_kernel != BlockKernel::GENERAL && layout_of( a ) == BlockLayout::NONE ) l_kernel = BlockKernel::GENERAL;
+  if( l_kernel >= BlockKernel::TILE_64x64 && layout_of( a ) == BlockLayout::NONE ) l_kernel = BlockKernel::GENERAL;
   if( l_kernel == BlockKernel::GENERAL ) return launch_block_general( a, stream );
+  if( l_kernel <= BlockKernel::FEW_32 )  return launch_block_few( a, l_kernel, stream );
   if( !a.has( BlockArgs::F8 ) )   return launch_block_tile_bf16( a, l_kernel, plan.layout, stream );
   if( exact( a ) )                return launch_block_tile_exact( a, l_kernel, plan.layout, stream );
   if( a.has( BlockArgs::E8M0 ) )  return launch_block_tile_e8m0( a, l_kernel, plan.layout, stream );

@@ -356,6 +356,8 @@ void contract_block_tile_kernel( BlockArgs a ) {
   constexpr int SLAB = 16 * kPitch< float, COLS > * 4;
   constexpr int BYTES = STAGES * STAGE > WAVES * SLAB ? STAGES * STAGE : WAVES * SLAB;
   __shared__ __align__( 16 ) char l_lds[BYTES];
+  __shared__ __align__( 16 ) float l_bias[BN];
+  static_assert( BN <= 64 * WAVES, "a thread a column" );
 
   int const l_lane = threadIdx.x % 64;
   int const l_wave = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
@@ -375,6 +377,10 @@ void contract_block_tile_kernel( BlockArgs a ) {
   Reader< BN, RB, ITEM > l_rb;
   l_ra.init( l_lane );
   l_rb.init( l_lane );
+
+  // the bias, needed after the loop
+  float l_bias_r = 0.0f;
+  if( a.bias && threadIdx.x < BN ) l_bias_r = a.bias[w.c * a.bias_c + min( w.n0 + int32_t( threadIdx.x ), a.N - 1 ) * a.bias_col];
 
   int32_t const l_steps = int32_t( ( int64_t( w.K ) * ITEM + kStep - 1 ) / kStep );
   uint32_t const l_lds_at = kern::lds_addr( l_lds );
@@ -461,8 +467,9 @@ void contract_block_tile_kernel( BlockArgs a ) {
 #pragma unroll
       for( int l_i = 0; l_i < TM; l_i++ ) l_scale[l_i] = scale_value( l_sa[l_i], a.sa != nullptr ) * l_b1;
     }
-    constexpr int RING = 3;
-    f32x4 l_part[KIND == F8 ? RING : TM];
+    // F8, EXACT: the sums of a pair of fragments are added RING - 1 pairs later
+    constexpr int RING = KIND == EXACT ? 2 : 3;
+    f32x4 l_part[RING];
     f32x4 l_of_b[2];        // SB_ROWS: the scales of the columns of this part and the last
     Wide l_wa[KIND == EXACT ? TM : 1];
     if constexpr( KIND == EXACT ) {
@@ -471,7 +478,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
     }
     auto add = [&]( auto mc ) __attribute__( ( always_inline ) ) {
       constexpr int l_j = decltype( mc )::value / TM, l_i = decltype( mc )::value % TM;
-      f32x4 const & l_p = l_part[KIND == F8 ? decltype( mc )::value % RING : l_i];
+      f32x4 const & l_p = l_part[decltype( mc )::value % RING];
 #pragma unroll
       for( int l_e = 0; l_e < 4; l_e++ ) {
         float const l_f = SB_ROWS ? l_scale[l_i] * l_of_b[l_j % 2][l_e] : l_scale[l_i];
@@ -499,18 +506,20 @@ void contract_block_tile_kernel( BlockArgs a ) {
       else                  read_b( std::integral_constant< int, 0 >(), l_next );
       kern::static_for< TM >( [&]( auto ic ) __attribute__( ( always_inline ) ) {
         constexpr int l_i = decltype( ic )::value, l_m = l_j * TM + l_i;
+        constexpr f32x4 ZERO = { 0.0f, 0.0f, 0.0f, 0.0f };
         if constexpr( KIND == BF16 ) {
-          l_acc[l_j][l_i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16( __builtin_bit_cast( bf16x8, l_f.v[0] ),
-                                                                     __builtin_bit_cast( bf16x8, l_fa[l_i].v[0] ), l_acc[l_j][l_i], 0, 0, 0 );
-          l_acc[l_j][l_i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16( __builtin_bit_cast( bf16x8, l_f.v[1] ),
-                                                                     __builtin_bit_cast( bf16x8, l_fa[l_i].v[1] ), l_acc[l_j][l_i], 0, 0, 0 );
+#pragma unroll
+          for( int l_q = 0; l_q < 2; l_q++ ) {
+            l_acc[l_j][l_i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16( __builtin_bit_cast( bf16x8, l_f.v[l_q] ),
+                                                                       __builtin_bit_cast( bf16x8, l_fa[l_i].v[l_q] ), l_acc[l_j][l_i], 0, 0, 0 );
+          }
         }
         else if constexpr( KIND == EXACT ) {
-          f32x4 l_p = { 0.0f, 0.0f, 0.0f, 0.0f };
+          f32x4 l_p = ZERO;
 #pragma unroll
           for( int l_q = 0; l_q < 4; l_q++ ) l_p = __builtin_amdgcn_mfma_f32_16x16x32_bf16( l_wb.v[l_q], l_wa[l_i].v[l_q], l_p, 0, 0, 0 );
-          l_part[l_i] = l_p;
-          if constexpr( l_i > 0 ) add( std::integral_constant< int, l_m - 1 >() );
+          l_part[l_m % RING] = l_p;
+          if constexpr( l_m > 0 ) add( std::integral_constant< int, l_m - 1 >() );
         }
         else {
           i32x8 const l_vb = __builtin_shufflevector( l_f.v[0], l_f.v[1], 0, 1, 2, 3, 4, 5, 6, 7 );
@@ -521,8 +530,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
                                                                                 a.sa != nullptr ? l_sa[l_i] : 127 );
           }
           else {
-            l_part[l_m % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, FORMAT,
-                                                                                   0, 0, 0, 0 );
+            l_part[l_m % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, ZERO, 0, FORMAT, 0, 0, 0, 0 );
             if constexpr( l_m >= RING - 1 ) add( std::integral_constant< int, l_m - RING + 1 >() );
           }
         }
@@ -542,9 +550,8 @@ void contract_block_tile_kernel( BlockArgs a ) {
         }
         __builtin_amdgcn_sched_barrier( 0 );
       } );
-      if constexpr( KIND == EXACT ) add( std::integral_constant< int, l_j * TM + TM - 1 >() );
     } );
-    if constexpr( KIND == F8 ) {
+    if constexpr( KIND == F8 || KIND == EXACT ) {
       kern::static_for< RING - 1 >( [&]( auto rc ) __attribute__( ( always_inline ) ) {
         add( std::integral_constant< int, TN * TM - ( RING - 1 ) + decltype( rc )::value >() );
       } );
@@ -564,6 +571,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
     l_st = l_next;
   }
   kern::wait_vmcnt< 0 >();
+  if( threadIdx.x < BN ) l_bias[threadIdx.x] = l_bias_r;
   __syncthreads();           // nothing is on its way into LDS, all fragments are read
 
   // 16 rows at a time through this wave's slab
@@ -577,15 +585,14 @@ void contract_block_tile_kernel( BlockArgs a ) {
 #pragma unroll
       for( int l_j = 0; l_j < TN; l_j++ ) {
         int const l_n = 16 * l_j + 4 * ( l_lane / 16 );
-        t4 l_v;
+        f32x4 l_f = l_acc[l_j][l_i];
+        if( a.bias ) l_f += *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
+        if( a.has( BlockArgs::RELU ) ) {
 #pragma unroll
-        for( int l_e = 0; l_e < 4; l_e++ ) {
-          float l_f = l_acc[l_j][l_i][l_e];
-          if( a.bias ) l_f += a.bias[w.c * a.bias_c + min( w.n0 + l_wn + l_n + l_e, a.N - 1 ) * a.bias_col];
-          if( a.has( BlockArgs::RELU ) && l_f < 0.0f ) l_f = 0.0f;         // a NaN stays
-          l_v[l_e] = static_cast< T >( l_f );
+          for( int l_e = 0; l_e < 4; l_e++ ) l_f[l_e] = l_f[l_e] < 0.0f ? 0.0f : l_f[l_e];      // a NaN stays
         }
-        *reinterpret_cast< t4 * >( l_slab + ( l_lane % 16 ) * kPitch< T, COLS > + l_n ) = l_v;
+        *reinterpret_cast< t4 * >( l_slab + ( l_lane % 16 ) * kPitch< T, COLS > + l_n )
+            = t4{ static_cast< T >( l_f[0] ), static_cast< T >( l_f[1] ), static_cast< T >( l_f[2] ), static_cast< T >( l_f[3] ) };
       }
       // the slab is this wave's own, and its LDS operations are in order
       __builtin_amdgcn_fence( __ATOMIC_ACQ_REL, "wavefront" );
