@@ -13,8 +13,8 @@
 // fragment is two 16-byte reads a lane.  One that is unit-stride along its rows
 // lies as [k][row], the pieces of a k likewise exchanged, and a fragment is four
 // transposing reads (ds_read_b64_tr_b8 / _tr_b16).  A lane of either holds row
-// lane % 16 and the pieces lane / 16 and lane / 16 + 4 of its k; which k these
-// are does not matter as long as both operands agree.
+// lane % 16 and two pieces of its k; which these are does not matter as long as
+// both operands agree.
 //
 // The columns' side is the first operand of the matrix instruction, so a lane
 // holds one row m and 4 neighbouring columns; the tile goes out through LDS in
@@ -60,10 +60,10 @@ __device__ inline uint32_t swz_rows( int k ) {
   constexpr int SLOTS = ROWS * ITEM / 16;
   if constexpr( ITEM == 1 ) {
     constexpr int P = 16 / SLOTS;                  // k in 256 bytes
-    return uint32_t( k / P % ( 8 / P ) + ( k >> 4 & 1 ) * ( 8 / P ) );
+    return uint32_t( k / P % ( 8 / P ) + ( k >> 5 & 1 ) * ( 8 / P ) );
   }
-  else if constexpr( SLOTS >= 16 ) return uint32_t( 2 * ( k & 3 ) + 8 * ( k >> 3 & 1 ) );
-  else return uint32_t( 2 * ( k >> 1 & 1 ) + 4 * ( k >> 3 & 1 ) );
+  else if constexpr( SLOTS >= 16 ) return uint32_t( 2 * ( k & 3 ) + 8 * ( k >> 4 & 1 ) );
+  else return uint32_t( 2 * ( k >> 1 & 1 ) + 4 * ( k >> 4 & 1 ) );
 }
 
 // One operand's ROWS rows of a step, loaded by WAVES waves, 64 pieces of 16
@@ -136,6 +136,12 @@ struct Side {
   }
 };
 
+// The first of the two pieces (the other is 4 further) of a lane.  16-byte reads
+// take lanes 0-3, 12-15 and 20-27 together, then 4-11, 16-19 and 28-31: pieces 0
+// and 2 of lanes next to each other then touch every bank once, pieces 0 and 1
+// half of them twice.
+__device__ inline int first_piece( int lane ) { return ( lane >> 5 & 1 ) + 2 * ( lane >> 4 & 1 ); }
+
 // 16 rows x 128 bytes of k: a lane's two pieces of 16 bytes
 struct Frag { i32x4 v[2]; };
 
@@ -154,8 +160,8 @@ struct Reader {
     if constexpr( ALONG_ROWS ) {
 #pragma unroll
       for( int l_i = 0; l_i < 4; l_i++ ) {
-        // piece lane / 16 (+ 4) has 16 / ITEM k, read 8 / ITEM at a time
-        int const l_piece = lane / 16 + 4 * ( l_i / 2 );
+        // a piece has 16 / ITEM k, read 8 / ITEM at a time
+        int const l_piece = first_piece( lane ) + 4 * ( l_i / 2 );
         int const l_k = l_piece * ( 16 / ITEM ) + ( l_i % 2 ) * ( 8 / ITEM ) + lane % 16 / ( ITEM == 1 ? 2 : 4 );
         m_k[l_i] = uint32_t( l_k * ROWS * ITEM );
         m_swz[l_i] = swz_rows< ROWS, ITEM >( l_k );
@@ -170,7 +176,7 @@ struct Reader {
       uint32_t const l_swz = kern::swz_k( m_lane % 16 );      // of rows 16 apart: the same
 #pragma unroll
       for( int l_i = 0; l_i < 2; l_i++ ) {
-        l_f.v[l_i] = *reinterpret_cast< i32x4 const * >( lds + l_r * kStep + ( ( uint32_t( m_lane / 16 + 4 * l_i ) ^ l_swz ) << 4 ) );
+        l_f.v[l_i] = *reinterpret_cast< i32x4 const * >( lds + l_r * kStep + ( ( uint32_t( first_piece( m_lane ) + 4 * l_i ) ^ l_swz ) << 4 ) );
       }
     }
     else {
