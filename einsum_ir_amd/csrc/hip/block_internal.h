@@ -44,13 +44,20 @@ enum class BlockKernel : int32_t {
   FEW_4,           // few rows of A, K over the waves and in 4 parts (contract_block_few.hip)
   FEW_16,          // the same, 16 rows at a time, K over the waves
   FEW_32,          // 32 rows at a time
-  TILE_64x64,      // through LDS directly (contract_block_tile.h), both operands at multiples of 16 bytes
+  // through LDS directly (contract_block_tile.h), both operands at multiples of 16 bytes
+  TILE_32x32,      // K in 8 groups of waves
+  TILE_64x64_K,    // K in 4 groups of waves
+  TILE_64x64,
   TILE_128x128,
   TILE_256x128,
-  TILE_256x256
+  TILE_256x256,
+  // the same through registers, operands at any address
+  STAGED_64x64_K,  // K in 2 groups of waves
+  STAGED_64x64,
+  STAGED_128x128
 };
 
-// How the operands lie for the tiles; rows and k at multiples of 16 bytes.
+// How the operands lie for the tiles.
 enum class BlockLayout : int32_t {
   NONE,            // any other
   K_K,             // both unit-stride along k: the product itself
@@ -71,6 +78,7 @@ struct BlockPlan {
 
 int launch_block_general( BlockArgs const & a, hipStream_t stream );
 int launch_block_few( BlockArgs const & a, BlockKernel kernel, hipStream_t stream );
+int launch_block_staged( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 int launch_block_tile_bf16( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 int launch_block_tile_f8( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );
 int launch_block_tile_exact( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream );

@@ -95,32 +95,37 @@ int check_types( Given const & g ) {
   return ETIR_SUCCESS;
 }
 
-// How the tiles see the operands; pointers count where they are known.
+// How the tiles see the operands.
 BlockLayout layout_of( BlockArgs const & a ) {
-  int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2, l_step = 128 / l_item;
   bool const l_ra = a.a_k != 1, l_rb = a.b_k != 1;
   if( a.o_col != 1 || a.K == 0 || ( l_ra && ( a.a_row != 1 || a.M < 2 ) ) || ( l_rb && ( a.b_row != 1 || a.N < 2 ) ) || ( l_ra && !l_rb ) ) {
     return BlockLayout::NONE;
   }
+  return l_ra ? BlockLayout::ROWS_ROWS : l_rb ? BlockLayout::K_ROWS : BlockLayout::K_K;
+}
+
+// Whether the loads into LDS directly take the operands; pointers count where
+// they are known.
+bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
+  if( layout == BlockLayout::NONE ) return false;
+  int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2, l_step = 128 / l_item;
+  bool const l_ra = layout == BlockLayout::ROWS_ROWS, l_rb = layout != BlockLayout::K_K;
   // k (or rows) of 16 bytes start at multiples of 16
   auto aligned = [&]( void const * p, int64_t c, int64_t stride ) {
     return uintptr_t( p ) % 16 == 0 && c * l_item % 16 == 0 && stride * l_item % 16 == 0;
   };
   int64_t const l_sa = l_ra ? a.a_k : a.a_row, l_sb = l_rb ? a.b_k : a.b_row;
-  if( !aligned( a.a, a.a_c, l_sa ) || !aligned( a.b, a.b_c, l_sb ) ) return BlockLayout::NONE;
-  if( ( !l_ra || !l_rb ) && a.K * l_item % 16 != 0 ) return BlockLayout::NONE;
+  if( !aligned( a.a, a.a_c, l_sa ) || !aligned( a.b, a.b_c, l_sb ) ) return false;
+  if( ( !l_ra || !l_rb ) && a.K * l_item % 16 != 0 ) return false;
   // 31 bits of bytes in a step of a tile, and along k; rows of a k that do not
   // reach into the next k's, so that k past the end lie past the buffer's end
   int64_t const l_max = int64_t( 1 ) << 31;
-  if( l_ra ? l_sa * l_item * l_step >= l_max || a.M > l_sa : l_sa * l_item * 256 >= l_max ) return BlockLayout::NONE;
-  if( l_rb ? l_sb * l_item * l_step >= l_max || a.N > l_sb : l_sb * l_item * 256 >= l_max ) return BlockLayout::NONE;
-  if( int64_t( a.K ) * l_item >= l_max - 256 ) return BlockLayout::NONE;
+  if( l_ra ? l_sa * l_item * l_step >= l_max || a.M > l_sa : l_sa * l_item * 256 >= l_max ) return false;
+  if( l_rb ? l_sb * l_item * l_step >= l_max || a.N > l_sb : l_sb * l_item * 256 >= l_max ) return false;
+  if( int64_t( a.K ) * l_item >= l_max - 2048 ) return false;
   // scales: 31 bits along a tile's rows and along k
   int64_t const l_kb = ( int64_t( a.K ) + kScaleBlock - 1 ) / kScaleBlock;
-  if( a.sa_row * 4 * 256 >= l_max || a.sb_row * 4 * 256 >= l_max || a.sa_k * 4 * l_kb >= l_max || a.sb_k * 4 * l_kb >= l_max ) {
-    return BlockLayout::NONE;
-  }
-  return l_ra ? BlockLayout::ROWS_ROWS : l_rb ? BlockLayout::K_ROWS : BlockLayout::K_K;
+  return a.sa_row * 4 * 256 < l_max && a.sb_row * 4 * 256 < l_max && a.sa_k * 4 * l_kb < l_max && a.sb_k * 4 * l_kb < l_max;
 }
 
 struct Tile {
@@ -132,10 +137,15 @@ Tile const kTiles[] = {
   { BlockKernel::FEW_4,        "few 4",        4,   4 },
   { BlockKernel::FEW_16,       "few 16",       16,  16 },
   { BlockKernel::FEW_32,       "few 32",       32,  16 },
+  { BlockKernel::TILE_32x32,   "tile 32x32",   32,  32 },
+  { BlockKernel::TILE_64x64_K, "tile 64x64 K", 64,  64 },
   { BlockKernel::TILE_64x64,   "tile 64x64",   64,  64 },
   { BlockKernel::TILE_128x128, "tile 128x128", 128, 128 },
   { BlockKernel::TILE_256x128, "tile 256x128", 256, 128 },
-  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256 }
+  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256 },
+  { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64 },
+  { BlockKernel::STAGED_64x64,   "staged 64x64",   64, 64 },
+  { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128 }
 };
 
 // rows of tiles in all batches or groups
@@ -159,10 +169,11 @@ char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
   Tile const * l_best = nullptr;
   for( Tile const & l_t : kTiles ) {
     bool const l_few = l_t.kernel <= BlockKernel::FEW_32;
-    if( l_few ? !few_fits( a ) : plan.layout == BlockLayout::NONE ) continue;
+    bool const l_staged = l_t.kernel >= BlockKernel::STAGED_64x64_K;
+    if( l_few ? !few_fits( a ) : l_staged ? plan.layout == BlockLayout::NONE : !direct_fits( a, plan.layout ) ) continue;
     if( exact( a ) && l_t.kernel == BlockKernel::TILE_256x256 ) continue;
     double const l_groups = double( tiles_m( a, l_t.rows ) ) * double( ( a.N + l_t.cols - 1 ) / l_t.cols );
-    if( l_groups * 512 >= 4294967296.0 ) continue;
+    if( l_groups * 1024 >= 4294967296.0 ) continue;
     if( l_forced == int( l_t.kernel ) ) {
       l_best = &l_t;
       break;
@@ -344,9 +355,11 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
   }
   BlockKernel l_kernel = plan.kernel;
   // pointers may be less aligned than the strides
-  if( l_kernel >= BlockKernel::TILE_64x64 && layout_of( a ) == BlockLayout::NONE ) l_kernel = BlockKernel::GENERAL;
+  bool const l_staged = l_kernel >= BlockKernel::STAGED_64x64_K;
+  if( !l_staged && l_kernel > BlockKernel::FEW_32 && !direct_fits( a, plan.layout ) ) l_kernel = BlockKernel::STAGED_64x64;
   if( l_kernel == BlockKernel::GENERAL ) return launch_block_general( a, stream );
   if( l_kernel <= BlockKernel::FEW_32 )  return launch_block_few( a, l_kernel, stream );
+  if( l_kernel >= BlockKernel::STAGED_64x64_K ) return launch_block_staged( a, l_kernel, plan.layout, stream );
   if( !a.has( BlockArgs::F8 ) )   return launch_block_tile_bf16( a, l_kernel, plan.layout, stream );
   if( exact( a ) )                return launch_block_tile_exact( a, l_kernel, plan.layout, stream );
   if( a.has( BlockArgs::E8M0 ) )  return launch_block_tile_e8m0( a, l_kernel, plan.layout, stream );

@@ -4,14 +4,13 @@
 //   out[c][m][n] = last( sum_kb sa[c][m][kb] sb[c][n][kb] sum_(k in kb) A[c][m][k] B[c][n][k] + bias[c][n] )
 //
 // One workgroup of 4 waves computes a 64 x 64 tile with
-// v_mfma_f32_32x32x16_bf16 (a wave a 32 x 32 block), 64 k at a time through LDS.
-// 8-bit numbers become bf16 on their way into LDS, which holds all of them
-// exactly, so products are exact and sums are fp32.  Both 64-k halves of a block
-// of 128 are summed before its scales are applied.  An operand that is
+// v_mfma_f32_32x32x16_bf16 (a wave a 32 x 32 block), 128 k at a time through LDS,
+// the next 128 on their way in registers meanwhile (509 x 1001 x 333 in 5 groups
+// 19.5 -> XX us).  8-bit numbers become bf16 on their way into LDS, which holds
+// all of them exactly, so products are exact and sums are fp32.  An operand that is
 // unit-stride along k, or along its rows, is read in 16-byte pieces at any
 // address, any other element by element with neighbouring lanes on neighbouring
-// rows.  It is the kernel for layouts that the others do not take; the waits of
-// its single buffer bound it.
+// rows.  It is the kernel for layouts that the others do not take.
 #include "block_internal.h"
 #include "contract_kernel.h"
 
@@ -25,16 +24,11 @@ typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
 typedef u32x4    u32x4_u __attribute__( ( aligned( 1 ) ) );
 
 constexpr int kTile  = 64;
-constexpr int kBk    = 64;
-constexpr int kPitch = kBk + 8;    // bf16 elements a row: 144 bytes, 16-byte reads of 16 rows over all banks
+constexpr int kBk    = 128;        // of 8-bit numbers: one block
+constexpr int kPitch = kBk + 8;    // bf16 elements a row: 272 bytes, 16-byte reads of 16 rows over all banks
 
 // how an operand lies
 enum Lie : int { ALONG_K, ALONG_ROWS, APART };
-
-// 16 elements as bf16 bits, two a dword
-struct Piece { uint32_t w[8]; };
-
-__device__ inline void put( Piece & p, int i, uint32_t bits ) { p.w[i / 2] |= bits << ( 16 * ( i % 2 ) ); }
 
 // four 8-bit numbers to bf16
 template< bool E5M2 >
@@ -52,69 +46,97 @@ __device__ inline void widen4( uint32_t v, uint32_t * to ) {
   to[1] = __builtin_bit_cast( uint32_t, l_hi );
 }
 
+// 16 elements as they lie in memory
+template< bool F8 > struct Piece { uint32_t w[F8 ? 4 : 8]; };
+
 // 16 elements from p on with the given stride, of which the first n exist
-template< bool F8, bool E5M2 >
-__device__ inline Piece load16( uint8_t const * p, int64_t stride, int n ) {
-  Piece l_p = {};
-  if constexpr( F8 ) {
-    uint32_t l_v[4] = { 0, 0, 0, 0 };
-    if( stride == 1 && n >= 16 ) {
-      u32x4 const l_r = *reinterpret_cast< u32x4_u const * >( p );
+template< bool F8 >
+__device__ inline Piece< F8 > load16( uint8_t const * p, int64_t stride, int n ) {
+  constexpr int WORDS = F8 ? 4 : 8;
+  Piece< F8 > l_p = {};
+  if( stride == 1 && n >= 16 ) {
 #pragma unroll
-      for( int l_i = 0; l_i < 4; l_i++ ) l_v[l_i] = l_r[l_i];
+    for( int l_h = 0; l_h < WORDS / 4; l_h++ ) {
+      u32x4 const l_r = *reinterpret_cast< u32x4_u const * >( p + 16 * l_h );
+#pragma unroll
+      for( int l_i = 0; l_i < 4; l_i++ ) l_p.w[4 * l_h + l_i] = l_r[l_i];
     }
-    else {
-#pragma unroll
-      for( int l_i = 0; l_i < 16; l_i++ ) if( l_i < n ) l_v[l_i / 4] |= uint32_t( p[l_i * stride] ) << ( 8 * ( l_i % 4 ) );
-    }
-#pragma unroll
-    for( int l_i = 0; l_i < 4; l_i++ ) widen4< E5M2 >( l_v[l_i], l_p.w + 2 * l_i );
+    return l_p;
   }
-  else {
-    uint16_t const * l_q = reinterpret_cast< uint16_t const * >( p );
-    if( stride == 1 && n >= 16 ) {
 #pragma unroll
-      for( int l_h = 0; l_h < 2; l_h++ ) {
-        u32x4 const l_r = *reinterpret_cast< u32x4_u const * >( p + 16 * l_h );
-#pragma unroll
-        for( int l_i = 0; l_i < 4; l_i++ ) l_p.w[4 * l_h + l_i] = l_r[l_i];
-      }
-    }
-    else {
-#pragma unroll
-      for( int l_i = 0; l_i < 16; l_i++ ) if( l_i < n ) put( l_p, l_i, l_q[l_i * stride] );
-    }
+  for( int l_i = 0; l_i < 16; l_i++ ) {
+    if( l_i >= n ) continue;
+    if constexpr( F8 ) l_p.w[l_i / 4] |= uint32_t( p[l_i * stride] ) << ( 8 * ( l_i % 4 ) );
+    else l_p.w[l_i / 2] |= uint32_t( reinterpret_cast< uint16_t const * >( p )[l_i * stride] ) << ( 16 * ( l_i % 2 ) );
   }
   return l_p;
 }
 
-// One operand's 64 rows x 64 k of a step into LDS as [row][k] of bf16, 16
-// elements a thread.  base: the tile's first row at k = 0; rows and k past the
-// tensor's count as zeros.
+// One operand's 64 rows x 128 k of a step: 32 elements a thread, from global
+// memory into registers and from there into LDS as [row][k] of bf16.  Rows and k
+// past the tensor's count as zeros.
 template< bool F8, bool E5M2 >
-__device__ inline void stage( uint16_t * lds, uint8_t const * base, int64_t row, int64_t k, int rows, int32_t k0, int32_t K ) {
-  constexpr int ITEM = F8 ? 1 : 2;
-  int const l_t = threadIdx.x;
-  Lie const l_lie = k == 1 ? ALONG_K : row == 1 ? ALONG_ROWS : APART;
-  if( l_lie != ALONG_ROWS ) {
-    int const l_r = l_lie == ALONG_K ? l_t / 4 : l_t % 64;
-    int const l_k = 16 * ( l_lie == ALONG_K ? l_t % 4 : l_t / 64 );
-    int const l_n = l_r < rows ? max( min( K - k0 - l_k, 16 ), 0 ) : 0;
-    Piece l_p = {};
-    if( l_n > 0 ) l_p = load16< F8, E5M2 >( base + ( l_r * row + int64_t( k0 + l_k ) * k ) * ITEM, k, l_n );
-    u32x4 * const l_to = reinterpret_cast< u32x4 * >( lds + l_r * kPitch + l_k );
-    l_to[0] = u32x4{ l_p.w[0], l_p.w[1], l_p.w[2], l_p.w[3] };
-    l_to[1] = u32x4{ l_p.w[4], l_p.w[5], l_p.w[6], l_p.w[7] };
+struct Side {
+  static constexpr int ITEM = F8 ? 1 : 2;
+  uint8_t const * m_base;      // the tile's first row at k = 0
+  int64_t m_row, m_k;
+  int     m_rows;
+  Lie     m_lie;
+  Piece< F8 > m_p[2];
+
+  __device__ inline void init( uint8_t const * base, int64_t row, int64_t k, int rows ) {
+    m_base = base;
+    m_row = row;
+    m_k = k;
+    m_rows = rows;
+    m_lie = k == 1 ? ALONG_K : row == 1 ? ALONG_ROWS : APART;
   }
-  else {
-    int const l_k = l_t / 4, l_r = 16 * ( l_t % 4 );
-    int const l_n = k0 + l_k < K ? max( min( rows - l_r, 16 ), 0 ) : 0;
-    Piece l_p = {};
-    if( l_n > 0 ) l_p = load16< F8, E5M2 >( base + ( l_r + int64_t( k0 + l_k ) * k ) * ITEM, 1, l_n );
+  __device__ inline void load( int32_t k0, int32_t K ) {
+    int const l_t = threadIdx.x;
 #pragma unroll
-    for( int l_i = 0; l_i < 16; l_i++ ) lds[( l_r + l_i ) * kPitch + l_k] = uint16_t( l_p.w[l_i / 2] >> ( 16 * ( l_i % 2 ) ) );
+    for( int l_h = 0; l_h < 2; l_h++ ) {
+      int l_r, l_k, l_n;
+      if( m_lie == ALONG_ROWS ) {
+        l_k = l_t / 2;
+        l_r = 32 * ( l_t % 2 ) + 16 * l_h;
+        l_n = k0 + l_k < K ? min( m_rows - l_r, 16 ) : 0;
+      }
+      else {
+        l_r = m_lie == ALONG_K ? l_t / 4 : l_t % 64;
+        l_k = 32 * ( m_lie == ALONG_K ? l_t % 4 : l_t / 64 ) + 16 * l_h;
+        l_n = l_r < m_rows ? min( K - k0 - l_k, 16 ) : 0;
+      }
+      m_p[l_h] = Piece< F8 >{};
+      if( l_n > 0 ) {
+        m_p[l_h] = load16< F8 >( m_base + ( l_r * m_row + int64_t( k0 + l_k ) * m_k ) * ITEM, m_lie == ALONG_ROWS ? 1 : m_k, l_n );
+      }
+    }
   }
-}
+  __device__ inline void store( uint16_t * lds ) const {
+    int const l_t = threadIdx.x;
+#pragma unroll
+    for( int l_h = 0; l_h < 2; l_h++ ) {
+      uint32_t l_w[8];
+#pragma unroll
+      for( int l_i = 0; l_i < ( F8 ? 4 : 8 ); l_i++ ) {
+        if constexpr( F8 ) widen4< E5M2 >( m_p[l_h].w[l_i], l_w + 2 * l_i );
+        else               l_w[l_i] = m_p[l_h].w[l_i];
+      }
+      if( m_lie == ALONG_ROWS ) {
+        int const l_k = l_t / 2, l_r = 32 * ( l_t % 2 ) + 16 * l_h;
+#pragma unroll
+        for( int l_i = 0; l_i < 16; l_i++ ) lds[( l_r + l_i ) * kPitch + l_k] = uint16_t( l_w[l_i / 2] >> ( 16 * ( l_i % 2 ) ) );
+      }
+      else {
+        int const l_r = m_lie == ALONG_K ? l_t / 4 : l_t % 64;
+        int const l_k = 32 * ( m_lie == ALONG_K ? l_t % 4 : l_t / 64 ) + 16 * l_h;
+        u32x4 * const l_to = reinterpret_cast< u32x4 * >( lds + l_r * kPitch + l_k );
+        l_to[0] = u32x4{ l_w[0], l_w[1], l_w[2], l_w[3] };
+        l_to[1] = u32x4{ l_w[4], l_w[5], l_w[6], l_w[7] };
+      }
+    }
+  }
+};
 
 __device__ inline float scale_at( void const * s, bool e8m0, int64_t at ) {
   return e8m0 ? e8m0_to_f32( static_cast< uint8_t const * >( s )[at] ) : static_cast< float const * >( s )[at];
@@ -132,7 +154,7 @@ void contract_block_general_kernel( BlockArgs a ) {
 
   int const l_t = threadIdx.x;
   int32_t const l_tiles_n = ( a.N + kTile - 1 ) / kTile;
-  int64_t const l_id = blockIdx.x;
+  uint32_t const l_id = blockIdx.x;
   int32_t const l_n0 = int32_t( l_id % l_tiles_n ) * kTile;
   int32_t l_c, l_m0, l_m_end = a.M, l_k_begin = 0, l_K = a.K;
   if( a.has( BlockArgs::GROUP_ROWS ) ) {
@@ -159,30 +181,41 @@ void contract_block_general_kernel( BlockArgs a ) {
 
   int const l_wave = l_t / 64, l_lane = l_t % 64;
   int const l_wm = 32 * ( l_wave / 2 ), l_wn = 32 * ( l_wave % 2 );
-  f32x16 l_acc = { 0 }, l_part = { 0 };
-  for( int32_t l_k0 = 0; l_k0 < l_K; l_k0 += kBk ) {
-    stage< F8, A_E5M2 >( l_lds_a, l_a, a.a_row, a.a_k, l_rows, l_k0, l_K );
-    stage< F8, false >( l_lds_b, l_b, a.b_row, a.b_k, l_cols, l_k0, l_K );
-    bool const l_first = l_k0 % kScaleBlock == 0;
-    if( F8 && l_first && l_t < 2 * kTile ) {
-      // rows past the tensor take the last one's scale and are not stored
-      int32_t const l_kb = l_k0 / kScaleBlock;
-      if( l_t < kTile ) {
-        int64_t const l_m = l_m0 + min( l_t, l_rows - 1 );
-        l_sa[l_t] = a.sa == nullptr ? 1.0f : scale_at( a.sa, a.has( BlockArgs::E8M0 ), l_c * a.sa_c + l_kb * a.sa_k
-                                       + ( a.has( BlockArgs::SA_BLOCKS ) ? l_m / kScaleBlock : l_m ) * a.sa_row );
-      }
-      else {
-        int64_t const l_n = l_n0 + min( l_t - kTile, l_cols - 1 );
-        l_sb[l_t - kTile] = a.sb == nullptr ? 1.0f : scale_at( a.sb, a.has( BlockArgs::E8M0 ), l_c * a.sb_c + l_kb * a.sb_k
-                                       + ( a.has( BlockArgs::SB_BLOCKS ) ? l_n / kScaleBlock : l_n ) * a.sb_row );
-      }
+  Side< F8, A_E5M2 > l_side_a;
+  Side< F8, false > l_side_b;
+  l_side_a.init( l_a, a.a_row, a.a_k, l_rows );
+  l_side_b.init( l_b, a.b_row, a.b_k, l_cols );
+  // the scale of a row or column of the tile, by a thread of its own
+  float l_scale = 1.0f;
+  auto load = [&]( int32_t k0 ) {
+    l_side_a.load( k0, l_K );
+    l_side_b.load( k0, l_K );
+    if( !F8 || l_t >= 2 * kTile ) return;
+    // rows past the tensor take the last one's scale and are not stored
+    int32_t const l_kb = k0 / kScaleBlock;
+    if( l_t < kTile ) {
+      int64_t const l_m = l_m0 + min( l_t, l_rows - 1 );
+      if( a.sa != nullptr ) l_scale = scale_at( a.sa, a.has( BlockArgs::E8M0 ), l_c * a.sa_c + l_kb * a.sa_k
+                                               + ( a.has( BlockArgs::SA_BLOCKS ) ? l_m / kScaleBlock : l_m ) * a.sa_row );
     }
+    else {
+      int64_t const l_n = l_n0 + min( l_t - kTile, l_cols - 1 );
+      if( a.sb != nullptr ) l_scale = scale_at( a.sb, a.has( BlockArgs::E8M0 ), l_c * a.sb_c + l_kb * a.sb_k
+                                               + ( a.has( BlockArgs::SB_BLOCKS ) ? l_n / kScaleBlock : l_n ) * a.sb_row );
+    }
+  };
+  f32x16 l_acc = { 0 };
+  if( l_K > 0 ) load( 0 );
+  for( int32_t l_k0 = 0; l_k0 < l_K; l_k0 += kBk ) {
+    __syncthreads();         // the last step's fragments are read
+    l_side_a.store( l_lds_a );
+    l_side_b.store( l_lds_b );
+    if( F8 && l_t < 2 * kTile ) ( l_t < kTile ? l_sa : l_sb - kTile )[l_t] = l_scale;
     __syncthreads();
+    if( l_K - l_k0 > kBk ) load( l_k0 + kBk );
     // the columns' side first: a lane holds one row m and 16 columns
     f32x16 l_sum = { 0 };
     if( !F8 ) l_sum = l_acc;
-    else if( !l_first ) l_sum = l_part;
 #pragma unroll
     for( int l_s = 0; l_s < kBk / 16; l_s++ ) {
       int const l_k = 16 * l_s + 8 * ( l_lane / 32 );
@@ -192,17 +225,14 @@ void contract_block_general_kernel( BlockArgs a ) {
     }
     if( !F8 ) l_acc = l_sum;
     else {
-      l_part = l_sum;
-      if( !l_first || l_k0 + kBk >= l_K ) {
-        float const l_s = l_sa[l_wm + l_lane % 32];
+      float const l_s = l_sa[l_wm + l_lane % 32];
 #pragma unroll
-        for( int l_i = 0; l_i < 16; l_i++ ) {
-          l_acc[l_i] += l_part[l_i] * ( l_s * l_sb[l_wn + 8 * ( l_i / 4 ) + 4 * ( l_lane / 32 ) + l_i % 4] );
-        }
+      for( int l_i = 0; l_i < 16; l_i++ ) {
+        l_acc[l_i] += l_sum[l_i] * ( l_s * l_sb[l_wn + 8 * ( l_i / 4 ) + 4 * ( l_lane / 32 ) + l_i % 4] );
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
 
   // out through LDS, neighbouring lanes on the output's shorter stride
   float * const l_out = reinterpret_cast< float * >( l_lds );

@@ -1,0 +1,28 @@
+// The tiles of contract_block_tile.h for operands at any address: bf16, and 8-bit
+// numbers multiplied as bf16.
+#include "contract_block_tile.h"
+
+namespace etir {
+
+namespace {
+
+template< int KIND, bool A_E5M2 >
+int launch_type( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
+  using namespace block;
+  switch( layout ) {
+    case BlockLayout::K_K:       return launch_staged< KIND, false, false, A_E5M2 >( a, kernel, stream );
+    case BlockLayout::K_ROWS:    return launch_staged< KIND, false, true, A_E5M2 >( a, kernel, stream );
+    case BlockLayout::ROWS_ROWS: return launch_staged< KIND, true, true, A_E5M2 >( a, kernel, stream );
+    default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown layout" );
+  }
+}
+
+}  // namespace
+
+int launch_block_staged( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
+  if( !a.has( BlockArgs::F8 ) ) return launch_type< block::BF16, false >( a, kernel, layout, stream );
+  return a.has( BlockArgs::A_E5M2 ) ? launch_type< block::EXACT, true >( a, kernel, layout, stream )
+                                    : launch_type< block::EXACT, false >( a, kernel, layout, stream );
+}
+
+}  // namespace etir

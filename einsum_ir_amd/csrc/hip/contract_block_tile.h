@@ -63,10 +63,11 @@ __device__ inline uint32_t swz_rows( int k ) {
     return uint32_t( k / P % ( 8 / P ) + ( k >> 5 & 1 ) * ( 8 / P ) );
   }
   else if constexpr( SLOTS >= 16 ) return uint32_t( 2 * ( k & 3 ) + 8 * ( k >> 4 & 1 ) );
-  else return uint32_t( 2 * ( k >> 1 & 1 ) + 4 * ( k >> 4 & 1 ) );
+  else if constexpr( SLOTS == 8 ) return uint32_t( 2 * ( k >> 1 & 1 ) + 4 * ( k >> 4 & 1 ) );
+  else return uint32_t( 2 * ( k >> 4 & 1 ) );
 }
 
-// One operand's ROWS rows of a step, loaded by WAVES waves, 64 pieces of 16
+// One operand's ROWS rows of a step, loaded directly by WAVES waves, 64 pieces of 16
 // bytes at a time.
 template< int ROWS, int WAVES, bool ALONG_ROWS, int ITEM >
 struct Side {
@@ -269,14 +270,15 @@ __device__ inline Where where( BlockArgs const & a ) {
   return l_w;
 }
 
-// The scales of a step: BM of A's rows, then BN of B's, a dword each in LDS
-// (E8M0: the byte).  64 of them a load; every wave has EACH loads, those past the
-// last one load zeros.
+// The scales of a step: those of A's rows, then of B's, a dword each in LDS
+// (E8M0: the byte), 64 a load; a side of 32 rows has a load of its own.  Every
+// wave has EACH loads, those past the last one load zeros.
 template< int BM, int BN, int WAVES >
 struct Scales {
-  static constexpr int LOADS = ( BM + BN ) / 64;
-  static constexpr int EACH  = ( LOADS + WAVES - 1 ) / WAVES;
+  static constexpr int LOADS_A = ( BM + 63 ) / 64, LOADS_B = ( BN + 63 ) / 64;
+  static constexpr int EACH  = ( LOADS_A + LOADS_B + WAVES - 1 ) / WAVES;
   static constexpr int BYTES = EACH * WAVES * 256;
+  static constexpr int AT_B  = LOADS_A * 256;
   uint32_t m_off[EACH];      // bytes from block kb = 0 to the lane's scale
   uint32_t m_k[EACH];        // bytes from block to block of k
   i32x4    m_rsrc[EACH];
@@ -288,8 +290,8 @@ struct Scales {
 #pragma unroll
     for( int l_i = 0; l_i < EACH; l_i++ ) {
       int const l_load = int( m_first ) + l_i;
-      bool const l_a = l_load < BM / 64;
-      int32_t const l_at = 64 * ( l_a ? l_load : l_load - BM / 64 ) + lane;
+      bool const l_a = l_load < LOADS_A;
+      int32_t const l_at = 64 * ( l_a ? l_load : l_load - LOADS_A ) + lane;
       // rows past the tensor take the last one's scale and are not stored; the
       // tile's first row or block is in the base
       int32_t const l_first = l_a ? w.m0 : w.n0;
@@ -298,7 +300,7 @@ struct Scales {
       int32_t const l_b0 = l_blocks ? l_first / kScaleBlock : l_first, l_b = l_blocks ? l_row / kScaleBlock : l_row;
       int64_t const l_stride = l_a ? a.sa_row : a.sb_row;
       void const * const l_s = l_a ? a.sa : a.sb;
-      m_off[l_i] = l_s != nullptr && l_load < LOADS ? uint32_t( ( l_b - l_b0 ) * int32_t( l_stride ) * l_item ) : kern::kDmaOob;
+      m_off[l_i] = l_s != nullptr && l_load < LOADS_A + LOADS_B ? uint32_t( ( l_b - l_b0 ) * int32_t( l_stride ) * l_item ) : kern::kDmaOob;
       m_k[l_i] = uint32_t( ( l_a ? a.sa_k : a.sb_k ) * l_item );
       m_rsrc[l_i] = kern::make_rsrc( static_cast< uint8_t const * >( l_s ) + ( w.c * ( l_a ? a.sa_c : a.sb_c ) + l_b0 * l_stride ) * l_item,
                                      kern::kDmaOob );
@@ -314,6 +316,69 @@ struct Scales {
     if( e8m0 ) asm volatile( "buffer_load_ubyte %0, %1, %2 offen lds" :: "v"( l_off ), "s"( m_rsrc[I] ), "s"( l_soff ) );
     else       asm volatile( "buffer_load_dword %0, %1, %2 offen lds" :: "v"( l_off ), "s"( m_rsrc[I] ), "s"( l_soff ) );
 #pragma clang diagnostic pop
+  }
+};
+
+// The same operand and scales through registers, for rows at any address: a
+// step's pieces are loaded while the one in front of it is multiplied, and
+// written to the places in LDS that the direct loads would give them.
+template< int ROWS, int WAVES, bool ALONG_ROWS, int ITEM >
+struct Staged {
+  static constexpr int EACH = ROWS / 8 / WAVES, BYTES = ROWS * kStep, K = kStep / ITEM;
+  static_assert( ROWS / 8 % WAVES == 0, "loads have to divide over the waves" );
+  typedef i32x4 i32x4_any __attribute__( ( aligned( 1 ) ) );
+
+  uint8_t const * m_base;
+  int64_t  m_stride;
+  int32_t  m_rows;
+  int      m_wave, m_lane;
+  i32x4    m_v[EACH];
+
+  __device__ inline void init( uint8_t const * tile, int64_t stride, int32_t rows, int wave, int lane ) {
+    m_base = tile;
+    m_stride = stride;
+    m_rows = rows;
+    m_wave = wave;
+    m_lane = lane;
+  }
+  __device__ __attribute__( ( always_inline ) ) inline void load( int32_t step, int32_t k ) {
+#pragma unroll
+    for( int l_i = 0; l_i < EACH; l_i++ ) {
+      int const l_load = m_wave * EACH + l_i;
+      uint8_t const * l_p;
+      int64_t l_left;           // bytes from there to the end of the row (or, along rows, of the k's rows)
+      if constexpr( ALONG_ROWS ) {
+        constexpr int SLOTS = ROWS * ITEM / 16;
+        int const l_k = l_load * ( 64 / SLOTS ) + m_lane / SLOTS;
+        int const l_at = 16 * int( uint32_t( m_lane % SLOTS ) ^ swz_rows< ROWS, ITEM >( l_k ) );
+        l_p = m_base + ( int64_t( step ) * K + l_k ) * m_stride + l_at;
+        l_left = int64_t( step ) * K + l_k < k ? int64_t( m_rows ) * ITEM - l_at : 0;
+      }
+      else {
+        // rows past the tensor read its last one and are not stored
+        int const l_r = 8 * l_load + m_lane / 8;
+        int64_t const l_at = int64_t( step ) * kStep + 16 * ( ( m_lane % 8 ) ^ int( kern::swz_k( l_r ) ) );
+        l_p = m_base + min( l_r, m_rows - 1 ) * m_stride + l_at;
+        l_left = int64_t( k ) * ITEM - l_at;
+      }
+      m_v[l_i] = i32x4{ 0, 0, 0, 0 };
+      if( l_left >= 16 ) m_v[l_i] = *reinterpret_cast< i32x4_any const * >( l_p );
+      else if( l_left > 0 ) {
+        // the end of a row, byte by byte (bf16: two)
+#pragma unroll
+        for( int l_e = 0; l_e < 16 / ITEM; l_e++ ) {
+          if( l_e * ITEM >= l_left ) continue;
+          uint32_t const l_x = ITEM == 1 ? uint32_t( l_p[l_e] ) : uint32_t( reinterpret_cast< uint16_t const * >( l_p )[l_e] );
+          m_v[l_i][l_e * ITEM / 4] |= int32_t( l_x << ( 8 * ( l_e * ITEM % 4 ) ) );
+        }
+      }
+    }
+  }
+  __device__ __attribute__( ( always_inline ) ) inline void store( char * lds ) const {
+#pragma unroll
+    for( int l_i = 0; l_i < EACH; l_i++ ) {
+      *reinterpret_cast< i32x4 * >( lds + ( m_wave * EACH + l_i ) * 1024 + 16 * m_lane ) = m_v[l_i];
+    }
   }
 };
 
@@ -344,29 +409,37 @@ __device__ inline void store_slab( BlockArgs const & a, T const * slab, T * out,
 }
 
 // KIND: see above.  RA, RB: A (B) is unit-stride along its rows, else along k.
-// SB_ROWS: B has a scale for every row (F8 and EXACT), else one for 128.
-template< int KIND, int BM, int BN, int WM, int WN, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
-__global__ __launch_bounds__( 64 * WM * WN )
+// SB_ROWS: B has a scale for every row (F8 and EXACT), else one for 128.  KG
+// groups of WM x WN waves take the steps in turn, each with STAGES buffers of its
+// own, and add their sums in LDS at the end, in the groups' order: few tiles with
+// a long K keep more loads and waves on a compute unit.  REG: operands at any
+// address, through registers (two buffers).
+template< int KIND, int BM, int BN, int WM, int WN, int KG, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS, bool REG >
+__global__ __launch_bounds__( 64 * WM * WN * KG )
 void contract_block_tile_kernel( BlockArgs a ) {
   constexpr int  ITEM = KIND == BF16 ? 2 : 1;
   constexpr bool SCALED = KIND != BF16;
-  constexpr int  WAVES = WM * WN;
+  constexpr int  WAVES = WM * WN;                            // of a group
   constexpr int  TM = BM / WM / 16, TN = BN / WN / 16;       // fragments of a wave
   constexpr int  COLS = BN / WN;
   static_assert( TN % 2 == 0 && ( KIND == BF16 || KIND == E8M0 || SB_ROWS || COLS <= kScaleBlock ), "wave tile" );
-  typedef Side< BM, WAVES, RA, ITEM > SideA;
-  typedef Side< BN, WAVES, RB, ITEM > SideB;
+  static_assert( !REG || STAGES == 2, "two buffers" );
+  typedef std::conditional_t< REG, Staged< BM, WAVES, RA, ITEM >, Side< BM, WAVES, RA, ITEM > > SideA;
+  typedef std::conditional_t< REG, Staged< BN, WAVES, RB, ITEM >, Side< BN, WAVES, RB, ITEM > > SideB;
   typedef Scales< BM, BN, WAVES > SideS;
   constexpr int EACH = SideA::EACH + SideB::EACH + ( SCALED ? SideS::EACH : 0 );      // a wave's loads of a step
   constexpr int STAGE = SideA::BYTES + SideB::BYTES + ( SCALED ? SideS::BYTES : 0 );
   constexpr int SLAB = 16 * kPitch< float, COLS > * 4;
-  constexpr int BYTES = STAGES * STAGE > WAVES * SLAB ? STAGES * STAGE : WAVES * SLAB;
-  __shared__ __align__( 16 ) char l_lds[BYTES];
+  constexpr int SLABS = WAVES * SLAB, PARTS = ( KG - 1 ) * BM * BN * 4;
+  constexpr int BYTES = KG * STAGES * STAGE > SLABS + PARTS ? KG * STAGES * STAGE : SLABS + PARTS;
+  __shared__ __align__( 16 ) char l_all[BYTES];
   __shared__ __align__( 16 ) float l_bias[BN];
-  static_assert( BN <= 64 * WAVES, "a thread a column" );
+  static_assert( BN <= 64 * WAVES * KG, "a thread a column" );
 
   int const l_lane = threadIdx.x % 64;
-  int const l_wave = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
+  int const l_w = __builtin_amdgcn_readfirstlane( threadIdx.x / 64 );
+  int const l_group = l_w / WAVES, l_wave = l_w % WAVES;
+  char * const l_lds = l_all + l_group * ( STAGES * STAGE );      // the group's buffers
   int const l_wm = l_wave / WN * ( BM / WM ), l_wn = l_wave % WN * COLS;
   Where const w = where< BM, BN >( a );
   if( !w.any ) return;
@@ -378,7 +451,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
   SideS l_s;
   l_a.init( l_at_a, ( RA ? a.a_k : a.a_row ) * ITEM, w.m_end - w.m0, l_wave, l_lane );
   l_b.init( l_at_b, ( RB ? a.b_k : a.b_row ) * ITEM, a.N - w.n0, l_wave, l_lane );
-  if constexpr( SCALED ) l_s.init( a, w, l_wave, l_lane );
+  if constexpr( SCALED && !REG ) l_s.init( a, w, l_wave, l_lane );
   Reader< BM, RA, ITEM > l_ra;
   Reader< BN, RB, ITEM > l_rb;
   l_ra.init( l_lane );
@@ -388,38 +461,88 @@ void contract_block_tile_kernel( BlockArgs a ) {
   float l_bias_r = 0.0f;
   if( a.bias && threadIdx.x < BN ) l_bias_r = a.bias[w.c * a.bias_c + min( w.n0 + int32_t( threadIdx.x ), a.N - 1 ) * a.bias_col];
 
-  int32_t const l_steps = int32_t( ( int64_t( w.K ) * ITEM + kStep - 1 ) / kStep );
+  int32_t const l_blocks = int32_t( ( int64_t( w.K ) * ITEM + kStep - 1 ) / kStep );
+  // A group's steps; past the last block nothing is in range and zeros are
+  // loaded, so that all groups take as many.
+  int32_t const l_steps = ( l_blocks + KG - 1 ) / KG;
   uint32_t const l_lds_at = kern::lds_addr( l_lds );
+
+  // REG: the thread's scale (of the first threads of a group) of the step that is on its way
+  int32_t l_scale_r = 0;
+  int const l_gt = l_wave * 64 + l_lane;
+  auto load_regs = [&]( int32_t s ) __attribute__( ( always_inline ) ) {
+    if constexpr( REG ) {
+      int32_t const l_step = s * KG + l_group;
+      l_a.load( l_step, w.K );
+      l_b.load( l_step, w.K );
+      if constexpr( SCALED ) {
+        static_assert( BM + BN <= 64 * WAVES, "a thread a scale" );
+        bool const l_is_a = l_gt < BM;
+        void const * const l_p = l_is_a ? a.sa : a.sb;
+        l_scale_r = 0;
+        if( l_p != nullptr && l_gt < BM + BN && l_step < l_blocks ) {
+          int32_t const l_row = l_is_a ? min( w.m0 + l_gt, w.m_end - 1 ) : min( w.n0 + l_gt - BM, a.N - 1 );
+          bool const l_by = a.has( BlockArgs::SA_BLOCKS ) && l_is_a ? true : a.has( BlockArgs::SB_BLOCKS ) && !l_is_a;
+          int64_t const l_i = w.c * ( l_is_a ? a.sa_c : a.sb_c ) + int64_t( l_step ) * ( l_is_a ? a.sa_k : a.sb_k )
+                            + int64_t( l_by ? l_row / kScaleBlock : l_row ) * ( l_is_a ? a.sa_row : a.sb_row );
+          l_scale_r = a.has( BlockArgs::E8M0 ) ? int32_t( static_cast< uint8_t const * >( l_p )[l_i] ) : static_cast< int32_t const * >( l_p )[l_i];
+        }
+      }
+    }
+  };
+  auto store_regs = [&]( int stage ) __attribute__( ( always_inline ) ) {
+    if constexpr( REG ) {
+      char * const l_to = l_lds + stage * STAGE;
+      l_a.store( l_to );
+      l_b.store( l_to + SideA::BYTES );
+      if constexpr( SCALED ) {
+        if( l_gt < BM + BN ) {
+          *reinterpret_cast< int32_t * >( l_to + SideA::BYTES + SideB::BYTES + ( l_gt < BM ? 4 * l_gt : SideS::AT_B + 4 * ( l_gt - BM ) ) ) = l_scale_r;
+        }
+      }
+    }
+  };
   // the wave's load i of a step, those of both sides and the scales counted through
-  auto issue = [&]( auto ic, int stage, int32_t step ) __attribute__( ( always_inline ) ) {
-    constexpr int l_i = decltype( ic )::value;
-    uint32_t const l_to = l_lds_at + stage * STAGE;
-    if constexpr( l_i < SideA::EACH ) {
-      if constexpr( l_i == 0 ) l_a.at_step( step, w.K );
-      l_a.template issue< l_i >( l_to, step, w.K );
-    }
-    else if constexpr( l_i < SideA::EACH + SideB::EACH ) {
-      if constexpr( l_i == SideA::EACH ) l_b.at_step( step, w.K );
-      l_b.template issue< l_i - SideA::EACH >( l_to + SideA::BYTES, step, w.K );
-    }
-    else if constexpr( SCALED ) {
-      l_s.template issue< l_i - SideA::EACH - SideB::EACH >( l_to + SideA::BYTES + SideB::BYTES, step, l_steps,
-                                                             KIND == E8M0 || ( KIND == EXACT && a.has( BlockArgs::E8M0 ) ) );
+  auto issue = [&]( auto ic, int stage, int32_t s ) __attribute__( ( always_inline ) ) {
+    if constexpr( !REG ) {
+      constexpr int l_i = decltype( ic )::value;
+      int32_t const l_step = s * KG + l_group;
+      uint32_t const l_to = l_lds_at + stage * STAGE;
+      if constexpr( l_i < SideA::EACH ) {
+        if constexpr( l_i == 0 ) l_a.at_step( l_step, w.K );
+        l_a.template issue< l_i >( l_to, l_step, w.K );
+      }
+      else if constexpr( l_i < SideA::EACH + SideB::EACH ) {
+        if constexpr( l_i == SideA::EACH ) l_b.at_step( l_step, w.K );
+        l_b.template issue< l_i - SideA::EACH >( l_to + SideA::BYTES, l_step, w.K );
+      }
+      else if constexpr( SCALED ) {
+        l_s.template issue< l_i - SideA::EACH - SideB::EACH >( l_to + SideA::BYTES + SideB::BYTES, l_step, l_blocks,
+                                                               KIND == E8M0 || ( KIND == EXACT && a.has( BlockArgs::E8M0 ) ) );
+      }
     }
   };
   // loads of step 1 (two buffers) that are issued in front of the loop
   constexpr int EARLY = ( EACH + 1 ) / 2;
-  kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, 0 ); } );
-  if constexpr( STAGES > 2 ) {
-    kern::static_for< STAGES - 2 >( [&]( auto sc ) __attribute__( ( always_inline ) ) {
-      constexpr int l_st = decltype( sc )::value + 1;
-      kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, l_st, l_st ); } );
-    } );
-    kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+  if constexpr( REG ) {
+    load_regs( 0 );
+    store_regs( 0 );
+    load_regs( 1 );
+    kern::wait_lgkmcnt0();
   }
   else {
-    kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, 1 ); } );
-    kern::wait_vmcnt< EARLY >();
+    kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 0, 0 ); } );
+    if constexpr( STAGES > 2 ) {
+      kern::static_for< STAGES - 2 >( [&]( auto sc ) __attribute__( ( always_inline ) ) {
+        constexpr int l_st = decltype( sc )::value + 1;
+        kern::static_for< EACH >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, l_st, l_st ); } );
+      } );
+      kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+    }
+    else {
+      kern::static_for< EARLY >( [&]( auto ic ) __attribute__( ( always_inline ) ) { issue( ic, 1, 1 ); } );
+      kern::wait_vmcnt< EARLY >();
+    }
   }
   kern::barrier_lds();
 
@@ -442,7 +565,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
   auto read_b = [&]( auto jc, int stage ) __attribute__( ( always_inline ) ) {
     constexpr int l_j = decltype( jc )::value;
     l_fb[l_j % 2] = l_rb.read( l_lds + stage * STAGE + SideA::BYTES, l_wn + 16 * l_j );
-    char const * const l_sc = l_lds + stage * STAGE + SideA::BYTES + SideB::BYTES + 4 * BM;
+    char const * const l_sc = l_lds + stage * STAGE + SideA::BYTES + SideB::BYTES + SideS::AT_B;
     if constexpr( SCALED && KIND != E8M0 && SB_ROWS ) {
       l_sb[l_j % 2] = *reinterpret_cast< i32x4 const * >( l_sc + 4 * ( l_wn + 16 * l_j + 4 * ( l_lane / 16 ) ) );
     }
@@ -454,7 +577,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
       char const * const l_sc = l_lds + stage * STAGE + SideA::BYTES + SideB::BYTES;
 #pragma unroll
       for( int l_i = 0; l_i < TM; l_i++ ) l_sa[l_i] = *reinterpret_cast< int32_t const * >( l_sc + 4 * ( l_wm + 16 * l_i + l_lane % 16 ) );
-      if constexpr( KIND != E8M0 && !SB_ROWS ) l_sb1 = *reinterpret_cast< int32_t const * >( l_sc + 4 * ( BM + l_wn ) );
+      if constexpr( KIND != E8M0 && !SB_ROWS ) l_sb1 = *reinterpret_cast< int32_t const * >( l_sc + SideS::AT_B + 4 * l_wn );
     }
   };
 
@@ -494,8 +617,13 @@ void contract_block_tile_kernel( BlockArgs a ) {
     kern::static_for< TN >( [&]( auto jc ) __attribute__( ( always_inline ) ) {
       constexpr int l_j = decltype( jc )::value;
       constexpr bool LAST = l_j == TN - 1;
+      // REG: the next step over the last one, which every wave has read
+      if constexpr( REG && l_j == 0 ) {
+        store_regs( l_next );
+        load_regs( s + 2 );
+      }
       if constexpr( LAST ) {
-        kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
+        if constexpr( !REG ) kern::wait_vmcnt< ( STAGES - 2 ) * EACH >();
         kern::wait_lgkmcnt0();
         kern::barrier_lds();
       }
@@ -541,13 +669,13 @@ void contract_block_tile_kernel( BlockArgs a ) {
           }
         }
         if constexpr( LAST ) read_a( ic, l_next );
-        if constexpr( STAGES > 2 && !LAST ) {
+        if constexpr( !REG && STAGES > 2 && !LAST ) {
           constexpr int l_from = EACH * l_m / ( ( TN - 1 ) * TM ), l_to = EACH * ( l_m + 1 ) / ( ( TN - 1 ) * TM );
           kern::static_for< l_to - l_from >( [&]( auto dc ) __attribute__( ( always_inline ) ) {
             issue( std::integral_constant< int, l_from + decltype( dc )::value >(), l_free, s + STAGES - 1 );
           } );
         }
-        if constexpr( STAGES == 2 && ( LAST || l_j == 0 ) ) {
+        if constexpr( !REG && STAGES == 2 && ( LAST || l_j == 0 ) ) {
           constexpr int l_p0 = LAST ? 0 : EARLY, l_n = LAST ? EARLY : EACH - EARLY;
           constexpr int l_from = l_p0 + l_n * l_i / TM, l_to = l_p0 + l_n * ( l_i + 1 ) / TM;
           kern::static_for< l_to - l_from >( [&]( auto dc ) __attribute__( ( always_inline ) ) {
@@ -580,11 +708,28 @@ void contract_block_tile_kernel( BlockArgs a ) {
   if( threadIdx.x < BN ) l_bias[threadIdx.x] = l_bias_r;
   __syncthreads();           // nothing is on its way into LDS, all fragments are read
 
+  // the other groups' sums to the first one
+  if constexpr( KG > 1 ) {
+    f32x4 * const l_parts = reinterpret_cast< f32x4 * >( l_all + SLABS );
+    if( l_group > 0 ) {
+#pragma unroll
+      for( int l_i = 0; l_i < TN * TM; l_i++ ) {
+        l_parts[( ( ( l_group - 1 ) * WAVES + l_wave ) * TN * TM + l_i ) * 64 + l_lane] = l_acc[l_i / TM][l_i % TM];
+      }
+    }
+    __syncthreads();
+    if( l_group > 0 ) return;
+    for( int l_g = 0; l_g < KG - 1; l_g++ ) {
+#pragma unroll
+      for( int l_i = 0; l_i < TN * TM; l_i++ ) l_acc[l_i / TM][l_i % TM] += l_parts[( ( l_g * WAVES + l_wave ) * TN * TM + l_i ) * 64 + l_lane];
+    }
+  }
+
   // 16 rows at a time through this wave's slab
   auto finish = [&]( auto zero ) __attribute__( ( always_inline ) ) {
     typedef decltype( zero ) T;
     typedef T t4 __attribute__( ( ext_vector_type( 4 ) ) );
-    T * const l_slab = reinterpret_cast< T * >( l_lds + l_wave * SLAB );
+    T * const l_slab = reinterpret_cast< T * >( l_all + l_wave * SLAB );
     T * const l_out = static_cast< T * >( a.out ) + w.c * a.o_c;
 #pragma unroll
     for( int l_i = 0; l_i < TM; l_i++ ) {
@@ -610,12 +755,12 @@ void contract_block_tile_kernel( BlockArgs a ) {
   else                               finish( 0.0f );
 }
 
-template< int KIND, int BM, int BN, int WM, int WN, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
+template< int KIND, int BM, int BN, int WM, int WN, int KG, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS, bool REG >
 int launch_shape( BlockArgs const & a, hipStream_t stream ) {
   int64_t const l_tiles_n = ( int64_t( a.N ) + BN - 1 ) / BN;
   int64_t const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, BM ) : ( int64_t( a.M ) + BM - 1 ) / BM * a.C;
-  hipLaunchKernelGGL( ( contract_block_tile_kernel< KIND, BM, BN, WM, WN, STAGES, RA, RB, A_E5M2, SB_ROWS > ),
-                      dim3( uint32_t( l_tiles_m * l_tiles_n ) ), dim3( 64 * WM * WN ), 0, stream, a );
+  hipLaunchKernelGGL( ( contract_block_tile_kernel< KIND, BM, BN, WM, WN, KG, STAGES, RA, RB, A_E5M2, SB_ROWS, REG > ),
+                      dim3( uint32_t( l_tiles_m * l_tiles_n ) ), dim3( 64 * WM * WN * KG ), 0, stream, a );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
     return fail( ETIR_UNDEFINED_ERROR, std::string( "contraction launch failed: " ) + hipGetErrorString( l_e ) );
@@ -623,17 +768,30 @@ int launch_shape( BlockArgs const & a, hipStream_t stream ) {
   return ETIR_SUCCESS;
 }
 
-// the tiles of one kind and layout
+// the tiles of one kind and layout, through LDS directly
 template< int KIND, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
 int launch_tiles( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
   switch( kernel ) {
-    case BlockKernel::TILE_64x64:   return launch_shape< KIND, 64, 64, 2, 2, 4, RA, RB, A_E5M2, SB_ROWS >( a, stream );
-    case BlockKernel::TILE_128x128: return launch_shape< KIND, 128, 128, 2, 2, 2, RA, RB, A_E5M2, SB_ROWS >( a, stream );
-    case BlockKernel::TILE_256x128: return launch_shape< KIND, 256, 128, 4, 2, 3, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+    case BlockKernel::TILE_32x32:   return launch_shape< KIND, 32, 32, 1, 1, 8, 2, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
+    case BlockKernel::TILE_64x64_K: return launch_shape< KIND, 64, 64, 2, 2, 4, 2, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
+    case BlockKernel::TILE_64x64:   return launch_shape< KIND, 64, 64, 2, 2, 1, 4, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
+    case BlockKernel::TILE_128x128: return launch_shape< KIND, 128, 128, 2, 2, 1, 2, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
+    case BlockKernel::TILE_256x128: return launch_shape< KIND, 256, 128, 4, 2, 1, 3, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
     case BlockKernel::TILE_256x256:
       // the widened operands of EXACT leave no registers for it
-      if constexpr( KIND != EXACT ) return launch_shape< KIND, 256, 256, 4, 2, 2, RA, RB, A_E5M2, SB_ROWS >( a, stream );
+      if constexpr( KIND != EXACT ) return launch_shape< KIND, 256, 256, 4, 2, 1, 2, RA, RB, A_E5M2, SB_ROWS, false >( a, stream );
       [[fallthrough]];
+    default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown tile" );
+  }
+}
+
+// the tiles of one kind and layout, through registers
+template< int KIND, bool RA, bool RB, bool A_E5M2 >
+int launch_staged( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
+  switch( kernel ) {
+    case BlockKernel::STAGED_64x64_K:  return launch_shape< KIND, 64, 64, 2, 2, 2, 2, RA, RB, A_E5M2, true, true >( a, stream );
+    case BlockKernel::STAGED_64x64:    return launch_shape< KIND, 64, 64, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
+    case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown tile" );
   }
 }
