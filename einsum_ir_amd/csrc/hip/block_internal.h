@@ -42,6 +42,7 @@ struct BlockArgs {
 enum class BlockKernel : int32_t {
   GENERAL,         // any strides, 64 x 64 tiles (contract_block.hip)
   FEW_4,           // few rows of A, K over the waves and in 4 parts (contract_block_few.hip)
+  FEW_8_PARTS,     // the same, 8 rows at a time
   FEW_16,          // the same, 16 rows at a time, K over the waves
   FEW_32,          // 32 rows at a time
   // through LDS directly (contract_block_tile.h), both operands at multiples of 16 bytes
@@ -52,6 +53,7 @@ enum class BlockKernel : int32_t {
   TILE_256x128,
   TILE_256x256,
   // the same through registers, operands at any address
+  STAGED_32x32,    // K in 8 groups of waves
   STAGED_64x64_K,  // K in 2 groups of waves
   STAGED_64x64,
   STAGED_128x128

@@ -135,6 +135,7 @@ struct Tile {
 };
 Tile const kTiles[] = {
   { BlockKernel::FEW_4,        "few 4",        4,   4 },
+  { BlockKernel::FEW_8_PARTS,  "few 8 parts",  8,   4 },
   { BlockKernel::FEW_16,       "few 16",       16,  16 },
   { BlockKernel::FEW_32,       "few 32",       32,  16 },
   { BlockKernel::TILE_32x32,   "tile 32x32",   32,  32 },
@@ -143,6 +144,7 @@ Tile const kTiles[] = {
   { BlockKernel::TILE_128x128, "tile 128x128", 128, 128 },
   { BlockKernel::TILE_256x128, "tile 256x128", 256, 128 },
   { BlockKernel::TILE_256x256, "tile 256x256", 256, 256 },
+  { BlockKernel::STAGED_32x32,   "staged 32x32",   32, 32 },
   { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64 },
   { BlockKernel::STAGED_64x64,   "staged 64x64",   64, 64 },
   { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128 }
@@ -169,7 +171,7 @@ char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
   Tile const * l_best = nullptr;
   for( Tile const & l_t : kTiles ) {
     bool const l_few = l_t.kernel <= BlockKernel::FEW_32;
-    bool const l_staged = l_t.kernel >= BlockKernel::STAGED_64x64_K;
+    bool const l_staged = l_t.kernel >= BlockKernel::STAGED_32x32;
     if( l_few ? !few_fits( a ) : l_staged ? plan.layout == BlockLayout::NONE : !direct_fits( a, plan.layout ) ) continue;
     if( exact( a ) && l_t.kernel == BlockKernel::TILE_256x256 ) continue;
     double const l_groups = double( tiles_m( a, l_t.rows ) ) * double( ( a.N + l_t.cols - 1 ) / l_t.cols );
@@ -355,11 +357,11 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
   }
   BlockKernel l_kernel = plan.kernel;
   // pointers may be less aligned than the strides
-  bool const l_staged = l_kernel >= BlockKernel::STAGED_64x64_K;
+  bool const l_staged = l_kernel >= BlockKernel::STAGED_32x32;
   if( !l_staged && l_kernel > BlockKernel::FEW_32 && !direct_fits( a, plan.layout ) ) l_kernel = BlockKernel::STAGED_64x64;
   if( l_kernel == BlockKernel::GENERAL ) return launch_block_general( a, stream );
   if( l_kernel <= BlockKernel::FEW_32 )  return launch_block_few( a, l_kernel, stream );
-  if( l_kernel >= BlockKernel::STAGED_64x64_K ) return launch_block_staged( a, l_kernel, plan.layout, stream );
+  if( l_kernel >= BlockKernel::STAGED_32x32 ) return launch_block_staged( a, l_kernel, plan.layout, stream );
   if( !a.has( BlockArgs::F8 ) )   return launch_block_tile_bf16( a, l_kernel, plan.layout, stream );
   if( exact( a ) )                return launch_block_tile_exact( a, l_kernel, plan.layout, stream );
   if( a.has( BlockArgs::E8M0 ) )  return launch_block_tile_e8m0( a, l_kernel, plan.layout, stream );

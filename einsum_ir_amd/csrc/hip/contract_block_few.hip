@@ -22,7 +22,7 @@ namespace {
 
 typedef float    f32x4 __attribute__( ( ext_vector_type( 4 ) ) );
 typedef uint32_t u32x4 __attribute__( ( ext_vector_type( 4 ) ) );
-typedef u32x4    u32x4_any __attribute__( ( aligned( 1 ) ) );
+typedef u32x4    u32x4_dword __attribute__( ( aligned( 4 ) ) );
 typedef __bf16   bf16x2 __attribute__( ( ext_vector_type( 2 ) ) );
 typedef __bf16   bf16x8 __attribute__( ( ext_vector_type( 8 ) ) );
 
@@ -30,20 +30,48 @@ constexpr int kWaves = 8;       // of a workgroup, over K
 constexpr int kLoads = 4;       // of 64 bytes of a row, in flight together
 constexpr int kPiece = 64 * kLoads;
 
-// 16 bytes of a row where K ends inside or before them: the row's last 16 are
-// loaded in their place, and those that belong to an earlier piece, or to none,
-// count as zeros.  bytes: of the row, at least 16.
-__device__ inline u32x4 load_piece( uint8_t const * row, int64_t at, int64_t bytes ) {
-  int64_t const l_at = min( at, bytes - 16 );
-  u32x4 l_v = *reinterpret_cast< u32x4_any const * >( row + l_at );
-  int const l_skip = int( min( at - l_at, int64_t( 16 ) ) );      // leading bytes that do not count
-#pragma unroll
-  for( int l_d = 0; l_d < 4; l_d++ ) {
-    int const l_z = l_skip - 4 * l_d;
-    l_v[l_d] &= l_z <= 0 ? 0xffffffffu : l_z >= 4 ? 0u : 0xffffffffu << ( 8 * l_z );
+// 16 bytes of a row on their way.  OFF: at any address, read as the five aligned
+// dwords that hold them (of which only those with a byte of the 16 are read) and
+// shifted into place: 16-byte loads off a 4-byte boundary run at a third of the
+// rate.  Else: at a multiple of 4.
+// MASKED: K may end inside or before them; the row's last 16 bytes are then loaded
+// in their place, and those that belong to an earlier piece, or to none, count as
+// zeros.  bytes: of the row, at least 16.
+template< bool OFF >
+struct Load {
+  u32x4    m_v;
+  uint32_t m_w;
+  int      m_shift, m_skip;
+
+  template< bool MASKED >
+  __device__ __attribute__( ( always_inline ) ) inline void load( uint8_t const * row, int64_t at, int64_t bytes ) {
+    int64_t const l_at = MASKED ? min( at, bytes - 16 ) : at;
+    m_skip = MASKED ? int( min( at - l_at, int64_t( 16 ) ) ) : 0;      // leading bytes that do not count
+    uintptr_t const l_p = reinterpret_cast< uintptr_t >( row + l_at );
+    if constexpr( OFF ) {
+      m_v = *reinterpret_cast< u32x4_dword const * >( l_p & ~uintptr_t( 3 ) );
+      m_w = *reinterpret_cast< uint32_t const * >( ( l_p + 15 ) & ~uintptr_t( 3 ) );
+      m_shift = int( l_p & 3 );
+    }
+    else m_v = *reinterpret_cast< u32x4_dword const * >( l_p );
   }
-  return l_v;
-}
+  template< bool MASKED >
+  __device__ __attribute__( ( always_inline ) ) inline u32x4 value() const {
+    u32x4 l_v = m_v;
+    if constexpr( OFF ) {
+      l_v = u32x4{ __builtin_amdgcn_alignbyte( m_v[1], m_v[0], m_shift ), __builtin_amdgcn_alignbyte( m_v[2], m_v[1], m_shift ),
+                   __builtin_amdgcn_alignbyte( m_v[3], m_v[2], m_shift ), __builtin_amdgcn_alignbyte( m_w, m_v[3], m_shift ) };
+    }
+    if constexpr( MASKED ) {
+#pragma unroll
+      for( int l_d = 0; l_d < 4; l_d++ ) {
+        int const l_z = m_skip - 4 * l_d;
+        l_v[l_d] &= l_z <= 0 ? 0xffffffffu : l_z >= 4 ? 0u : 0xffffffffu << ( 8 * l_z );
+      }
+    }
+    return l_v;
+  }
+};
 
 // half H of 16 8-bit numbers as bf16
 template< bool E5M2, int H >
@@ -73,7 +101,7 @@ __device__ inline float scale_at( void const * s, bool e8m0, int64_t at ) {
   return e8m0 ? e8m0_to_f32( static_cast< uint8_t const * >( s )[at] ) : static_cast< float const * >( s )[at];
 }
 
-template< bool F8, bool A_E5M2, int FB, int PARTS >
+template< bool F8, bool A_E5M2, int FB, int PARTS, bool OFF >
 __global__ __launch_bounds__( 64 * kWaves )
 void contract_block_few_kernel( BlockArgs a ) {
   constexpr int ITEM = F8 ? 1 : 2;
@@ -121,22 +149,25 @@ void contract_block_few_kernel( BlockArgs a ) {
   auto step = [&]( int32_t piece, auto masked ) __attribute__( ( always_inline ) ) {
     // the lane's first byte: its part of K, its 16 of 64 bytes
     int64_t const l_at = ( int64_t( l_of ) * l_pieces + piece ) * kPiece + 16 * ( l_lane / 16 );
-    u32x4 l_vb[kLoads], l_va[kLoads][FB];
+    constexpr bool MASKED = decltype( masked )::value;
+    Load< OFF > l_lb[kLoads], l_la[kLoads][FB];
 #pragma unroll
     for( int l_s = 0; l_s < kLoads; l_s++ ) {
-      int64_t const l_k = l_at + 64 * l_s;
-      if constexpr( decltype( masked )::value ) {
-        l_vb[l_s] = load_piece( l_b, l_k, l_bytes );
+      l_lb[l_s].template load< MASKED >( l_b, l_at + 64 * l_s, l_bytes );
 #pragma unroll
-        for( int l_i = 0; l_i < FB; l_i++ ) l_va[l_s][l_i] = load_piece( l_a[l_i], l_k, l_bytes );
-      }
-      else {
-        l_vb[l_s] = *reinterpret_cast< u32x4_any const * >( l_b + l_k );
-#pragma unroll
-        for( int l_i = 0; l_i < FB; l_i++ ) l_va[l_s][l_i] = *reinterpret_cast< u32x4_any const * >( l_a[l_i] + l_k );
-      }
+      for( int l_i = 0; l_i < FB; l_i++ ) l_la[l_s][l_i].template load< MASKED >( l_a[l_i], l_at + 64 * l_s, l_bytes );
     }
+    u32x4 l_vb[kLoads], l_va[kLoads][FB];
+    auto values = [&]() __attribute__( ( always_inline ) ) {
+#pragma unroll
+      for( int l_s = 0; l_s < kLoads; l_s++ ) {
+        l_vb[l_s] = l_lb[l_s].template value< MASKED >();
+#pragma unroll
+        for( int l_i = 0; l_i < FB; l_i++ ) l_va[l_s][l_i] = l_la[l_s][l_i].template value< MASKED >();
+      }
+    };
     if constexpr( !F8 ) {
+      values();
 #pragma unroll
       for( int l_s = 0; l_s < kLoads; l_s++ ) {
 #pragma unroll
@@ -155,7 +186,7 @@ void contract_block_few_kernel( BlockArgs a ) {
 #pragma unroll
       for( int l_k = 0; l_k < kPiece / kScaleBlock; l_k++ ) {
         int64_t const l_kb = min( l_first + l_k, int64_t( l_last ) );
-        bool const l_past = decltype( masked )::value && l_first + l_k > l_last;
+        bool const l_past = MASKED && l_first + l_k > l_last;
 #pragma unroll
         for( int l_i = 0; l_i < FB; l_i++ ) {
           l_sa[l_k][l_i] = a.sa == nullptr ? 1.0f : scale_at( a.sa, l_e8m0, l_c * a.sa_c + l_kb * a.sa_k
@@ -180,6 +211,7 @@ void contract_block_few_kernel( BlockArgs a ) {
           for( int l_e = 0; l_e < 4; l_e++ ) l_sb[l_k][l_e] = 0.0f;
         }
       }
+      values();
 #pragma unroll
       for( int l_k = 0; l_k < kPiece / kScaleBlock; l_k++ ) {
 #pragma unroll
@@ -231,21 +263,22 @@ void contract_block_few_kernel( BlockArgs a ) {
   }
 }
 
-template< bool F8, bool A_E5M2, int FB, int PARTS >
+template< bool F8, bool A_E5M2, int FB, int PARTS, bool OFF >
 void launch_shape( BlockArgs const & a, hipStream_t stream ) {
   constexpr int MANY = 16 / PARTS, FEW = MANY * FB;
   int64_t const l_tiles_n = ( int64_t( a.N ) + MANY - 1 ) / MANY;
   int64_t const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, FEW ) : ( int64_t( a.M ) + FEW - 1 ) / FEW * a.C;
-  hipLaunchKernelGGL( ( contract_block_few_kernel< F8, A_E5M2, FB, PARTS > ), dim3( uint32_t( l_tiles_m * l_tiles_n ) ),
+  hipLaunchKernelGGL( ( contract_block_few_kernel< F8, A_E5M2, FB, PARTS, OFF > ), dim3( uint32_t( l_tiles_m * l_tiles_n ) ),
                       dim3( 64 * kWaves ), 0, stream, a );
 }
 
-template< bool F8, bool A_E5M2 >
+template< bool F8, bool A_E5M2, bool OFF >
 int launch_type( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
   switch( kernel ) {
-    case BlockKernel::FEW_4:  launch_shape< F8, A_E5M2, 1, 4 >( a, stream ); break;
-    case BlockKernel::FEW_16: launch_shape< F8, A_E5M2, 1, 1 >( a, stream ); break;
-    default:                  launch_shape< F8, A_E5M2, 2, 1 >( a, stream ); break;
+    case BlockKernel::FEW_4:       launch_shape< F8, A_E5M2, 1, 4, OFF >( a, stream ); break;
+    case BlockKernel::FEW_8_PARTS: launch_shape< F8, A_E5M2, 2, 4, OFF >( a, stream ); break;
+    case BlockKernel::FEW_16:      launch_shape< F8, A_E5M2, 1, 1, OFF >( a, stream ); break;
+    default:                       launch_shape< F8, A_E5M2, 2, 1, OFF >( a, stream ); break;
   }
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
@@ -257,9 +290,14 @@ int launch_type( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
 }  // namespace
 
 int launch_block_few( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
-  if( !a.has( BlockArgs::F8 ) )     return launch_type< false, false >( a, kernel, stream );
-  if( a.has( BlockArgs::A_E5M2 ) )  return launch_type< true, true >( a, kernel, stream );
-  return launch_type< true, false >( a, kernel, stream );
+  int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2;
+  auto off = [&]( void const * p, int64_t c, int64_t row ) { return ( uintptr_t( p ) | uintptr_t( c * l_item ) | uintptr_t( row * l_item ) ) % 4 != 0; };
+  if( off( a.a, a.a_c, a.a_row ) || off( a.b, a.b_c, a.b_row ) || a.K * l_item % 4 != 0 ) {
+    if( !a.has( BlockArgs::F8 ) ) return launch_type< false, false, true >( a, kernel, stream );
+    return a.has( BlockArgs::A_E5M2 ) ? launch_type< true, true, true >( a, kernel, stream ) : launch_type< true, false, true >( a, kernel, stream );
+  }
+  if( !a.has( BlockArgs::F8 ) ) return launch_type< false, false, false >( a, kernel, stream );
+  return a.has( BlockArgs::A_E5M2 ) ? launch_type< true, true, false >( a, kernel, stream ) : launch_type< true, false, false >( a, kernel, stream );
 }
 
 }  // namespace etir

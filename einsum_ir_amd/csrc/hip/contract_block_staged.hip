@@ -1,5 +1,6 @@
-// The tiles of contract_block_tile.h for operands at any address: bf16, and 8-bit
-// numbers multiplied as bf16.
+// The tiles of contract_block_tile.h for operands at any address: bf16, 8-bit
+// products on the matrix cores with scales of either type, and 8-bit numbers
+// multiplied as bf16.
 #include "contract_block_tile.h"
 
 namespace etir {
@@ -21,6 +22,10 @@ int launch_type( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hi
 
 int launch_block_staged( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
   if( !a.has( BlockArgs::F8 ) ) return launch_type< block::BF16, false >( a, kernel, layout, stream );
+  if( a.has( BlockArgs::OUT_BF16 ) ) {
+    return a.has( BlockArgs::A_E5M2 ) ? launch_type< block::F8, true >( a, kernel, layout, stream )
+                                      : launch_type< block::F8, false >( a, kernel, layout, stream );
+  }
   return a.has( BlockArgs::A_E5M2 ) ? launch_type< block::EXACT, true >( a, kernel, layout, stream )
                                     : launch_type< block::EXACT, false >( a, kernel, layout, stream );
 }

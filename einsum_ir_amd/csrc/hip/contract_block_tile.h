@@ -346,13 +346,16 @@ struct Staged {
     for( int l_i = 0; l_i < EACH; l_i++ ) {
       int const l_load = m_wave * EACH + l_i;
       uint8_t const * l_p;
-      int64_t l_left;           // bytes from there to the end of the row (or, along rows, of the k's rows)
+      // Bytes from there on: to the end of the row, or, along rows, to the end of
+      // the last k's rows, as what follows a k's rows is not stored.
+      int64_t l_left;
       if constexpr( ALONG_ROWS ) {
         constexpr int SLOTS = ROWS * ITEM / 16;
         int const l_k = l_load * ( 64 / SLOTS ) + m_lane / SLOTS;
         int const l_at = 16 * int( uint32_t( m_lane % SLOTS ) ^ swz_rows< ROWS, ITEM >( l_k ) );
         l_p = m_base + ( int64_t( step ) * K + l_k ) * m_stride + l_at;
-        l_left = int64_t( step ) * K + l_k < k ? int64_t( m_rows ) * ITEM - l_at : 0;
+        int64_t const l_ks = int64_t( k ) - 1 - ( int64_t( step ) * K + l_k );      // k behind this one
+        l_left = l_ks >= 0 ? int64_t( m_rows ) * ITEM - l_at + l_ks * m_stride : 0;
       }
       else {
         // rows past the tensor read its last one and are not stored
@@ -364,7 +367,7 @@ struct Staged {
       m_v[l_i] = i32x4{ 0, 0, 0, 0 };
       if( l_left >= 16 ) m_v[l_i] = *reinterpret_cast< i32x4_any const * >( l_p );
       else if( l_left > 0 ) {
-        // the end of a row, byte by byte (bf16: two)
+        // the end, byte by byte (bf16: two)
 #pragma unroll
         for( int l_e = 0; l_e < 16 / ITEM; l_e++ ) {
           if( l_e * ITEM >= l_left ) continue;
@@ -556,7 +559,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
   i32x4 l_sb[2];
   auto scale_value = [&]( int32_t bits, bool have ) __attribute__( ( always_inline ) ) -> float {
     if( !have ) return 1.0f;
-    return KIND == EXACT && a.has( BlockArgs::E8M0 ) ? e8m0_to_f32( uint8_t( bits ) ) : __uint_as_float( uint32_t( bits ) );
+    return ( KIND == EXACT || REG ) && a.has( BlockArgs::E8M0 ) ? e8m0_to_f32( uint8_t( bits ) ) : __uint_as_float( uint32_t( bits ) );
   };
   auto read_a = [&]( auto ic, int stage ) __attribute__( ( always_inline ) ) {
     constexpr int l_i = decltype( ic )::value;
@@ -789,6 +792,7 @@ int launch_tiles( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) 
 template< int KIND, bool RA, bool RB, bool A_E5M2 >
 int launch_staged( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
   switch( kernel ) {
+    case BlockKernel::STAGED_32x32:    return launch_shape< KIND, 32, 32, 1, 1, 8, 2, RA, RB, A_E5M2, true, true >( a, stream );
     case BlockKernel::STAGED_64x64_K:  return launch_shape< KIND, 64, 64, 2, 2, 2, 2, RA, RB, A_E5M2, true, true >( a, stream );
     case BlockKernel::STAGED_64x64:    return launch_shape< KIND, 64, 64, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
     case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
