@@ -332,38 +332,49 @@ struct Staged {
   int64_t  m_stride;
   int32_t  m_rows;
   int      m_wave, m_lane;
+  int64_t  m_at[EACH];           // bytes from the step's first to the lane's piece
   i32x4    m_v[EACH];
 
+  // along rows: the k and the byte of it of the wave's load i; along k: the byte of the step
+  __device__ inline int k_of( int i ) const {
+    constexpr int SLOTS = ROWS * ITEM / 16;
+    return ( m_wave * EACH + i ) * ( 64 / SLOTS ) + m_lane / SLOTS;
+  }
+  __device__ inline int byte_of( int i ) const {
+    if constexpr( ALONG_ROWS ) return 16 * int( uint32_t( m_lane % ( ROWS * ITEM / 16 ) ) ^ swz_rows< ROWS, ITEM >( k_of( i ) ) );
+    else return 16 * ( ( m_lane % 8 ) ^ int( kern::swz_k( 8 * ( m_wave * EACH + i ) + m_lane / 8 ) ) );
+  }
   __device__ inline void init( uint8_t const * tile, int64_t stride, int32_t rows, int wave, int lane ) {
     m_base = tile;
     m_stride = stride;
     m_rows = rows;
     m_wave = wave;
     m_lane = lane;
-  }
-  __device__ __attribute__( ( always_inline ) ) inline void load( int32_t step, int32_t k ) {
 #pragma unroll
     for( int l_i = 0; l_i < EACH; l_i++ ) {
-      int const l_load = m_wave * EACH + l_i;
-      uint8_t const * l_p;
-      // Bytes from there on: to the end of the row, or, along rows, to the end of
-      // the last k's rows, as what follows a k's rows is not stored.
-      int64_t l_left;
+      // along k: rows past the tensor read its last one and are not stored
+      m_at[l_i] = ( ALONG_ROWS ? k_of( l_i ) : min( 8 * ( wave * EACH + l_i ) + lane / 8, rows - 1 ) ) * stride + byte_of( l_i );
+    }
+  }
+  __device__ __attribute__( ( always_inline ) ) inline void load( int32_t step, int32_t k ) {
+    uint8_t const * const l_base = m_base + int64_t( step ) * ( ALONG_ROWS ? K * m_stride : int64_t( kStep ) );
+    // Whether all 16 bytes of every piece are there; what follows a k's rows is
+    // not stored and may be read, up to the end of the last k's.
+    int64_t const l_after = int64_t( k ) - int64_t( step + 1 ) * K;      // k behind this step's
+    if( ALONG_ROWS ? l_after >= 0 && l_after * m_stride + int64_t( m_rows ) * ITEM >= ROWS * ITEM : l_after >= 0 ) {
+#pragma unroll
+      for( int l_i = 0; l_i < EACH; l_i++ ) m_v[l_i] = *reinterpret_cast< i32x4_any const * >( l_base + m_at[l_i] );
+      return;
+    }
+#pragma unroll
+    for( int l_i = 0; l_i < EACH; l_i++ ) {
+      int64_t l_left;            // bytes that are there
       if constexpr( ALONG_ROWS ) {
-        constexpr int SLOTS = ROWS * ITEM / 16;
-        int const l_k = l_load * ( 64 / SLOTS ) + m_lane / SLOTS;
-        int const l_at = 16 * int( uint32_t( m_lane % SLOTS ) ^ swz_rows< ROWS, ITEM >( l_k ) );
-        l_p = m_base + ( int64_t( step ) * K + l_k ) * m_stride + l_at;
-        int64_t const l_ks = int64_t( k ) - 1 - ( int64_t( step ) * K + l_k );      // k behind this one
-        l_left = l_ks >= 0 ? int64_t( m_rows ) * ITEM - l_at + l_ks * m_stride : 0;
+        int64_t const l_ks = l_after + K - 1 - k_of( l_i );      // k behind this one
+        l_left = l_ks >= 0 ? int64_t( m_rows ) * ITEM - byte_of( l_i ) + l_ks * m_stride : 0;
       }
-      else {
-        // rows past the tensor read its last one and are not stored
-        int const l_r = 8 * l_load + m_lane / 8;
-        int64_t const l_at = int64_t( step ) * kStep + 16 * ( ( m_lane % 8 ) ^ int( kern::swz_k( l_r ) ) );
-        l_p = m_base + min( l_r, m_rows - 1 ) * m_stride + l_at;
-        l_left = int64_t( k ) * ITEM - l_at;
-      }
+      else l_left = ( l_after + K ) * ITEM - byte_of( l_i );
+      uint8_t const * const l_p = l_base + m_at[l_i];
       m_v[l_i] = i32x4{ 0, 0, 0, 0 };
       if( l_left >= 16 ) m_v[l_i] = *reinterpret_cast< i32x4_any const * >( l_p );
       else if( l_left > 0 ) {
@@ -795,7 +806,7 @@ int launch_staged( BlockArgs const & a, BlockKernel kernel, hipStream_t stream )
     case BlockKernel::STAGED_32x32:    return launch_shape< KIND, 32, 32, 1, 1, 8, 2, RA, RB, A_E5M2, true, true >( a, stream );
     case BlockKernel::STAGED_64x64_K:  return launch_shape< KIND, 64, 64, 2, 2, 2, 2, RA, RB, A_E5M2, true, true >( a, stream );
     case BlockKernel::STAGED_64x64:    return launch_shape< KIND, 64, 64, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
-    case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
+    case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 4, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown tile" );
   }
 }
