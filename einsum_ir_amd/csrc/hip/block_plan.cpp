@@ -6,6 +6,7 @@
 // A product's loops are sorted by type and fused where they are contiguous in
 // every tensor; one loop of each type has to be left.
 #include "block_internal.h"
+#include <cmath>
 #include <cstdlib>
 #include <limits>
 #include <vector>
@@ -128,63 +129,101 @@ bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
   return a.sa_row * 4 * 256 < l_max && a.sb_row * 4 * 256 < l_max && a.sa_k * 4 * l_kb < l_max && a.sb_k * 4 * l_kb < l_max;
 }
 
-struct Tile {
+// What choose_kernel knows of a kernel: rows and columns of a workgroup, groups of
+// waves (few rows: parts of a fragment) that K is split over, workgroups on a
+// compute unit, and microseconds for bf16, 8-bit products on the matrix cores and
+// 8-bit numbers multiplied as bf16:
+//   fixed, a step of 128 bytes of k alone, a step of each workgroup beside others,
+//   a workgroup's beginning and end, factor of rows off 4 bytes (few rows)
+// Few rows: fixed, 2 KiB (8 KiB in parts) of k of a workgroup, a workgroup beside
+// others, and 1 KiB of k of one beside others.
+// Fitted to 1200 products of 1 to 16384 rows, 64 to 12288 columns and k, up to 64
+// groups, multiples of 16 and odd: the times that follow are off by 6 to 15 %
+// (root mean square), the kernel chosen is 3 % slower than the best of all on
+// average (64 x 64 tiles everywhere: XX %) and twice as slow at most.
+struct Candidate {
   BlockKernel  kernel;
   char const * name;
-  int32_t      rows, cols;
+  int32_t      rows, cols, split, slots;
+  float        us[3][5];
 };
-Tile const kTiles[] = {
-  { BlockKernel::FEW_4,        "few 4",        4,   4 },
-  { BlockKernel::FEW_8_PARTS,  "few 8 parts",  8,   4 },
-  { BlockKernel::FEW_16,       "few 16",       16,  16 },
-  { BlockKernel::FEW_32,       "few 32",       32,  16 },
-  { BlockKernel::TILE_32x32,   "tile 32x32",   32,  32 },
-  { BlockKernel::TILE_64x64_K, "tile 64x64 K", 64,  64 },
-  { BlockKernel::TILE_64x64,   "tile 64x64",   64,  64 },
-  { BlockKernel::TILE_128x128, "tile 128x128", 128, 128 },
-  { BlockKernel::TILE_256x128, "tile 256x128", 256, 128 },
-  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256 },
-  { BlockKernel::STAGED_32x32,   "staged 32x32",   32, 32 },
-  { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64 },
-  { BlockKernel::STAGED_64x64,   "staged 64x64",   64, 64 },
-  { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128 }
+Candidate const kCandidates[] = {
+  { BlockKernel::GENERAL, "general", 64, 64, 1, 4, { { 4.39f, 1.22f, 0.85f, 0.74f, 1.00f }, { 3.66f, 1.67f, 0.71f, 1.40f, 1.00f }, { 3.66f, 1.67f, 0.71f, 1.40f, 1.00f } } },
+  { BlockKernel::FEW_4, "few 4", 4, 4, 4, 1, { { 4.11f, 0.09f, 0.71f, 0.13f, 2.87f }, { 3.69f, 0.89f, 1.44f, 0.23f, 1.32f }, { 3.69f, 0.89f, 1.44f, 0.23f, 1.32f } } },
+  { BlockKernel::FEW_8_PARTS, "few 8 parts", 8, 4, 4, 1, { { 4.13f, 0.21f, 1.11f, 0.22f, 1.42f }, { 3.94f, 0.95f, 1.66f, 0.35f, 1.98f }, { 3.94f, 0.95f, 1.66f, 0.35f, 1.98f } } },
+  { BlockKernel::FEW_16, "few 16", 16, 16, 1, 1, { { 3.23f, 0.83f, 0.50f, 0.73f, 2.44f }, { 3.04f, 1.34f, 1.40f, 0.91f, 1.54f }, { 3.04f, 1.34f, 1.40f, 0.91f, 1.54f } } },
+  { BlockKernel::FEW_32, "few 32", 32, 16, 1, 1, { { 3.00f, 1.11f, 0.73f, 1.14f, 2.20f }, { 2.77f, 1.90f, 1.81f, 1.53f, 1.72f }, { 2.77f, 1.90f, 1.81f, 1.53f, 1.72f } } },
+  { BlockKernel::TILE_32x32, "tile 32x32", 32, 32, 8, 1, { { 0.21f, 0.60f, 1.01f, 3.86f, 1.00f }, { 0.40f, 0.50f, 0.87f, 4.10f, 1.00f }, { 0.20f, 0.50f, 1.30f, 4.31f, 1.00f } } },
+  { BlockKernel::TILE_64x64_K, "tile 64x64 K", 64, 64, 4, 1, { { 0.26f, 0.50f, 1.05f, 4.46f, 1.00f }, { 0.04f, 0.50f, 0.98f, 4.92f, 1.00f }, { 0.08f, 0.50f, 1.54f, 5.16f, 1.00f } } },
+  { BlockKernel::TILE_64x64, "tile 64x64", 64, 64, 1, 2, { { 2.99f, 0.28f, 0.26f, 1.05f, 1.00f }, { 2.58f, 0.34f, 0.27f, 1.26f, 1.00f }, { 2.35f, 0.75f, 0.50f, 1.47f, 1.00f } } },
+  { BlockKernel::TILE_128x128, "tile 128x128", 128, 128, 1, 2, { { 4.09f, 0.57f, 0.64f, 1.70f, 1.00f }, { 2.34f, 0.80f, 0.55f, 2.69f, 1.00f }, { 2.40f, 1.51f, 1.13f, 3.10f, 1.00f } } },
+  { BlockKernel::TILE_256x128, "tile 256x128", 256, 128, 1, 1, { { 0.85f, 0.41f, 0.76f, 4.83f, 1.00f }, { 0.02f, 0.50f, 0.86f, 5.53f, 1.00f }, { 0.04f, 0.50f, 1.93f, 6.58f, 1.00f } } },
+  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256, 1, 1, { { 0.40f, 0.71f, 1.29f, 7.72f, 1.00f }, { 0.02f, 0.50f, 1.39f, 8.18f, 1.00f }, { 0.0f } } },
+  { BlockKernel::STAGED_32x32, "staged 32x32", 32, 32, 8, 1, { { 0.04f, 0.71f, 1.10f, 6.03f, 1.00f }, { 0.13f, 0.50f, 2.20f, 5.81f, 1.00f }, { 0.21f, 2.51f, 0.40f, 5.69f, 1.00f } } },
+  { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64, 2, 2, { { 3.29f, 0.48f, 0.51f, 2.10f, 1.00f }, { 2.56f, 1.20f, 1.00f, 3.06f, 1.00f }, { 1.20f, 0.50f, 1.53f, 4.37f, 1.00f } } },
+  { BlockKernel::STAGED_64x64, "staged 64x64", 64, 64, 1, 4, { { 4.01f, 0.46f, 0.27f, 0.85f, 1.00f }, { 3.26f, 1.13f, 0.49f, 1.68f, 1.00f }, { 3.46f, 1.28f, 0.67f, 1.54f, 1.00f } } },
+  { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128, 1, 2, { { 1.39f, 0.70f, 0.74f, 4.08f, 1.00f }, { 0.06f, 0.50f, 1.33f, 6.39f, 1.00f }, { 0.14f, 0.50f, 1.82f, 6.55f, 1.00f } } }
 };
 
-// rows of tiles in all batches or groups
-int64_t tiles_m( BlockArgs const & a, int64_t rows ) {
+// rows of tiles in all batches or groups at most
+int64_t most_tiles_m( BlockArgs const & a, int64_t rows ) {
   return a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, rows ) : ( a.M + rows - 1 ) / rows * a.C;
 }
 
 bool exact( BlockArgs const & a ) { return a.has( BlockArgs::F8 ) && !a.has( BlockArgs::OUT_BF16 ); }
 
-// operands that the kernel of few rows reads: unit-stride along k, at any address
+// operands that the kernels of few rows read: unit-stride along k, at any address
 bool few_fits( BlockArgs const & a ) {
   return a.a_k == 1 && a.b_k == 1 && a.K * ( a.has( BlockArgs::F8 ) ? int64_t( 1 ) : int64_t( 2 ) ) >= 16 && !a.has( BlockArgs::GROUP_K );
 }
 
-char const * choose_kernel( BlockArgs const & a, BlockPlan & plan ) {
-  plan.kernel = BlockKernel::GENERAL;
-  plan.layout = layout_of( a );
-  char const * l_env = std::getenv( "ETIR_BLOCK_TILE" );
-  int const l_forced = l_env ? std::atoi( l_env ) : -1;
-  if( l_forced == 0 ) return "general";
-  Tile const * l_best = nullptr;
-  for( Tile const & l_t : kTiles ) {
-    bool const l_few = l_t.kernel <= BlockKernel::FEW_32;
-    bool const l_staged = l_t.kernel >= BlockKernel::STAGED_32x32;
-    if( l_few ? !few_fits( a ) : l_staged ? plan.layout == BlockLayout::NONE : !direct_fits( a, plan.layout ) ) continue;
-    if( exact( a ) && l_t.kernel == BlockKernel::TILE_256x256 ) continue;
-    double const l_groups = double( tiles_m( a, l_t.rows ) ) * double( ( a.N + l_t.cols - 1 ) / l_t.cols );
-    if( l_groups * 1024 >= 4294967296.0 ) continue;
-    if( l_forced == int( l_t.kernel ) ) {
-      l_best = &l_t;
-      break;
-    }
-    if( l_few && l_t.rows < ( a.has( BlockArgs::GROUP_ROWS ) ? 2 * a.M / a.C : a.M ) ) continue;
-    if( l_few && l_best ) continue;
-    if( l_best == nullptr || ( l_best->kernel > BlockKernel::FEW_32 && l_groups >= 256 ) ) l_best = &l_t;
+bool fits( Candidate const & c, BlockArgs const & a, BlockLayout layout ) {
+  // a grid's threads are counted in 32 bits
+  if( double( most_tiles_m( a, c.rows ) ) * double( ( int64_t( a.N ) + c.cols - 1 ) / c.cols ) * 1024 >= 4294967296.0 ) return false;
+  if( c.kernel == BlockKernel::GENERAL ) return true;
+  if( c.kernel <= BlockKernel::FEW_32 ) return few_fits( a );
+  if( c.kernel >= BlockKernel::STAGED_32x32 ) return layout != BlockLayout::NONE;
+  return direct_fits( a, layout ) && !( exact( a ) && c.kernel == BlockKernel::TILE_256x256 );
+}
+
+// the time that a kernel should take on 256 compute units
+double estimate( Candidate const & c, BlockArgs const & a, BlockLayout layout, double bytes ) {
+  float const * const l_us = c.us[exact( a ) ? 2 : a.has( BlockArgs::F8 ) ? 1 : 0];
+  bool const l_rows = a.has( BlockArgs::GROUP_ROWS ), l_ragged_k = a.has( BlockArgs::GROUP_K );
+  int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2;
+  // half of every group's last tile is empty; a group's K is the average one, the longest twice that
+  double const l_tiles_m = l_rows ? double( a.M ) / c.rows + 0.5 * std::min( a.M, a.C ) : double( most_tiles_m( a, c.rows ) );
+  double const l_groups = std::max( l_tiles_m, 1.0 ) * double( ( int64_t( a.N ) + c.cols - 1 ) / c.cols ), l_each = l_groups / 256;
+  double const l_k = double( a.K ) * l_item / ( l_ragged_k ? a.C : 1 );
+  double const l_least = bytes / 5.3e6;
+  if( c.kernel != BlockKernel::GENERAL && c.kernel <= BlockKernel::FEW_32 ) {
+    double const l_off = l_k != std::floor( l_k / 4 ) * 4 ? l_us[4] : 1.0;
+    double const l_turns = std::ceil( std::ceil( l_k / ( 256 * c.split ) ) / 8 );
+    return std::max( { l_us[0] + l_turns * l_us[1] * l_off, 0.5 * l_us[0] + l_each * ( l_us[2] + l_k / 1024 * l_us[3] * l_off ), l_least + 2 } );
   }
-  if( l_best == nullptr ) return "general";
+  double const l_layout = layout == BlockLayout::ROWS_ROWS ? 1.3 : layout == BlockLayout::K_ROWS ? 1.2 : 1.0;
+  double const l_steps = c.kernel == BlockKernel::GENERAL ? std::ceil( l_k / l_item / 128 ) : std::ceil( std::ceil( l_k / 128 ) / c.split );
+  double const l_rounds = l_rows || l_ragged_k ? std::max( 1.0, l_each > c.slots ? l_each / c.slots + 0.4 : 1.0 ) : std::ceil( l_each / c.slots );
+  double const l_beside = l_rows || l_ragged_k ? std::max( 1.0, l_each + 0.4 ) : std::ceil( l_each );
+  return std::max( { l_us[0] + l_rounds * ( l_steps * ( l_ragged_k ? 2 : 1 ) * l_us[1] * l_layout + l_us[3] ),
+                     l_us[0] + l_beside * ( l_steps * l_us[2] * l_layout + l_us[3] ), l_least + 2.5 } );
+}
+
+// ETIR_BLOCK_KERNEL forces a kernel, by its place in BlockKernel, where it fits.
+char const * choose_kernel( BlockArgs const & a, double bytes, BlockPlan & plan ) {
+  plan.layout = layout_of( a );
+  char const * const l_env = std::getenv( "ETIR_BLOCK_KERNEL" );
+  int const l_forced = l_env ? std::atoi( l_env ) : -1;
+  Candidate const * l_best = nullptr;
+  double l_least = 0.0;
+  for( Candidate const & l_c : kCandidates ) {
+    if( !fits( l_c, a, plan.layout ) ) continue;
+    double const l_us = l_forced == int( l_c.kernel ) ? -1.0 : estimate( l_c, a, plan.layout, bytes );
+    if( l_best == nullptr || l_us < l_least ) {
+      l_best = &l_c;
+      l_least = l_us;
+    }
+  }
   plan.kernel = l_best->kernel;
   return l_best->name;
 }
@@ -328,7 +367,7 @@ int plan_block( Given const & g, BlockPlan & plan ) {
   if( plan.has_bias ) plan.bytes += 4 * l_c * a.N;
   if( l_grouped ) plan.bytes += 4 * ( int64_t( a.C ) + 1 );
   char const * const l_left = l_f8 ? ( g.dtype_left == ETIR_F8E5M2 ? "e5m2" : "e4m3" ) : "bf16";
-  plan.desc = l_w + " " + choose_kernel( a, plan ) + " " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
+  plan.desc = l_w + " " + choose_kernel( a, double( plan.bytes ), plan ) + " " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
             + " N=" + std::to_string( a.N ) + " K=" + std::to_string( a.K )
             + ( l_grouped ? ( l_ragged_k ? " ragged K" : " ragged M" ) : "" ) + " " + l_left
             + ( a.has( BlockArgs::OUT_BF16 ) ? " out=bf16" : " out=fp32" );
