@@ -35,7 +35,8 @@ struct BlockArgs {
   uint32_t flags;
 
   enum : uint32_t { OUT_BF16 = 1u, RELU = 2u, GROUP_ROWS = 4u, GROUP_K = 8u, F8 = 16u, A_E5M2 = 32u, E8M0 = 64u,
-                    SA_BLOCKS = 128u, SB_BLOCKS = 256u };   // *_BLOCKS: a scale for 128 rows
+                    SA_BLOCKS = 128u, SB_BLOCKS = 256u,     // a scale for 128 rows
+                    SCALES = 512u };                        // both operands have scales
   __host__ __device__ bool has( uint32_t flag ) const { return ( flags & flag ) != 0; }
 };
 
@@ -108,8 +109,11 @@ int launch_quant_f8( QuantF8Plan const & plan, void const * in, void const * gat
 // ---------------------------------------------------------------------------
 
 // the number that an e8m0 byte stands for: 2^(byte - 127), 255: NaN
-__device__ inline float e8m0_to_f32( uint8_t v ) {
-  return v == 0 ? 0x1p-127f : v == 255 ? __uint_as_float( 0x7fc00000u ) : __uint_as_float( uint32_t( v ) << 23 );
+__device__ __attribute__( ( always_inline ) ) inline float e8m0_to_f32( uint32_t v ) {
+  uint32_t l_bits = v << 23;
+  l_bits |= v == 0 ? 0x00400000u : 0u;          // 2^-127
+  l_bits |= v == 255 ? 0x00400000u : 0u;        // the infinity's bits so far
+  return __uint_as_float( l_bits );
 }
 
 // Rows (or k) of a group, inside [0, rows] whatever the offsets are.

@@ -108,7 +108,7 @@ BlockLayout layout_of( BlockArgs const & a ) {
 // Whether the loads into LDS directly take the operands; pointers count where
 // they are known.
 bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
-  if( layout == BlockLayout::NONE ) return false;
+  if( layout == BlockLayout::NONE || ( a.has( BlockArgs::F8 ) && !a.has( BlockArgs::SCALES ) ) ) return false;
   int64_t const l_item = a.has( BlockArgs::F8 ) ? 1 : 2, l_step = 128 / l_item;
   bool const l_ra = layout == BlockLayout::ROWS_ROWS, l_rb = layout != BlockLayout::K_K;
   // k (or rows) of 16 bytes start at multiples of 16
@@ -344,7 +344,8 @@ int plan_block( Given const & g, BlockPlan & plan ) {
           | ( l_f8 ? BlockArgs::F8 : 0u ) | ( g.dtype_left == ETIR_F8E5M2 ? BlockArgs::A_E5M2 : 0u )
           | ( l_f8 && g.dtype_scale == ETIR_E8M0 ? BlockArgs::E8M0 : 0u )
           | ( g.block_left == kScaleBlock ? BlockArgs::SA_BLOCKS : 0u )
-          | ( g.block_right == kScaleBlock ? BlockArgs::SB_BLOCKS : 0u );
+          | ( g.block_right == kScaleBlock ? BlockArgs::SB_BLOCKS : 0u )
+          | ( g.strides[T_SA] != nullptr && g.strides[T_SB] != nullptr ? BlockArgs::SCALES : 0u );
   plan.grouped = l_grouped;
   plan.has_sa = g.strides[T_SA] != nullptr;
   plan.has_sb = g.strides[T_SB] != nullptr;

@@ -10,10 +10,16 @@ namespace {
 template< int KIND, bool A_E5M2 >
 int launch_type( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
   using namespace block;
+  // without scales there is one, 1, for 128 rows, too
+  bool const l_rows = KIND != BF16 && a.sb != nullptr && !a.has( BlockArgs::SB_BLOCKS );
   switch( layout ) {
-    case BlockLayout::K_K:       return launch_staged< KIND, false, false, A_E5M2 >( a, kernel, stream );
-    case BlockLayout::K_ROWS:    return launch_staged< KIND, false, true, A_E5M2 >( a, kernel, stream );
-    case BlockLayout::ROWS_ROWS: return launch_staged< KIND, true, true, A_E5M2 >( a, kernel, stream );
+    case BlockLayout::K_K:
+      return l_rows ? launch_staged< KIND, false, false, A_E5M2, KIND != BF16 >( a, kernel, stream )
+                    : launch_staged< KIND, false, false, A_E5M2, false >( a, kernel, stream );
+    case BlockLayout::K_ROWS:
+      return l_rows ? launch_staged< KIND, false, true, A_E5M2, KIND != BF16 >( a, kernel, stream )
+                    : launch_staged< KIND, false, true, A_E5M2, false >( a, kernel, stream );
+    case BlockLayout::ROWS_ROWS: return launch_staged< KIND, true, true, A_E5M2, KIND != BF16 >( a, kernel, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown layout" );
   }
 }

@@ -481,8 +481,9 @@ void contract_block_tile_kernel( BlockArgs a ) {
   int32_t const l_steps = ( l_blocks + KG - 1 ) / KG;
   uint32_t const l_lds_at = kern::lds_addr( l_lds );
 
-  // REG: the thread's scale (of the first threads of a group) of the step that is on its way
-  int32_t l_scale_r = 0;
+  // REG: the thread's scale (of the first threads of a group) of the step that
+  // is on its way, as fp32; without scales 1
+  float l_scale_r = 1.0f;
   int const l_gt = l_wave * 64 + l_lane;
   auto load_regs = [&]( int32_t s ) __attribute__( ( always_inline ) ) {
     if constexpr( REG ) {
@@ -493,13 +494,13 @@ void contract_block_tile_kernel( BlockArgs a ) {
         static_assert( BM + BN <= 64 * WAVES, "a thread a scale" );
         bool const l_is_a = l_gt < BM;
         void const * const l_p = l_is_a ? a.sa : a.sb;
-        l_scale_r = 0;
         if( l_p != nullptr && l_gt < BM + BN && l_step < l_blocks ) {
           int32_t const l_row = l_is_a ? min( w.m0 + l_gt, w.m_end - 1 ) : min( w.n0 + l_gt - BM, a.N - 1 );
           bool const l_by = a.has( BlockArgs::SA_BLOCKS ) && l_is_a ? true : a.has( BlockArgs::SB_BLOCKS ) && !l_is_a;
           int64_t const l_i = w.c * ( l_is_a ? a.sa_c : a.sb_c ) + int64_t( l_step ) * ( l_is_a ? a.sa_k : a.sb_k )
                             + int64_t( l_by ? l_row / kScaleBlock : l_row ) * ( l_is_a ? a.sa_row : a.sb_row );
-          l_scale_r = a.has( BlockArgs::E8M0 ) ? int32_t( static_cast< uint8_t const * >( l_p )[l_i] ) : static_cast< int32_t const * >( l_p )[l_i];
+          if( a.has( BlockArgs::E8M0 ) ) l_scale_r = e8m0_to_f32( static_cast< uint8_t const * >( l_p )[l_i] );
+          else                           l_scale_r = static_cast< float const * >( l_p )[l_i];
         }
       }
     }
@@ -511,7 +512,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
       l_b.store( l_to + SideA::BYTES );
       if constexpr( SCALED ) {
         if( l_gt < BM + BN ) {
-          *reinterpret_cast< int32_t * >( l_to + SideA::BYTES + SideB::BYTES + ( l_gt < BM ? 4 * l_gt : SideS::AT_B + 4 * ( l_gt - BM ) ) ) = l_scale_r;
+          *reinterpret_cast< float * >( l_to + SideA::BYTES + SideB::BYTES + ( l_gt < BM ? 4 * l_gt : SideS::AT_B + 4 * ( l_gt - BM ) ) ) = l_scale_r;
         }
       }
     }
@@ -568,9 +569,8 @@ void contract_block_tile_kernel( BlockArgs a ) {
   // lane's 4 columns (E8M0: of the lane's row) of two fragments
   int32_t l_sa[TM], l_sb1 = 0;
   i32x4 l_sb[2];
-  auto scale_value = [&]( int32_t bits, bool have ) __attribute__( ( always_inline ) ) -> float {
-    if( !have ) return 1.0f;
-    return ( KIND == EXACT || REG ) && a.has( BlockArgs::E8M0 ) ? e8m0_to_f32( uint8_t( bits ) ) : __uint_as_float( uint32_t( bits ) );
+  auto scale_value = [&]( int32_t bits ) __attribute__( ( always_inline ) ) -> float {
+    return KIND == EXACT && !REG && a.has( BlockArgs::E8M0 ) ? e8m0_to_f32( uint32_t( bits ) ) : __uint_as_float( uint32_t( bits ) );
   };
   auto read_a = [&]( auto ic, int stage ) __attribute__( ( always_inline ) ) {
     constexpr int l_i = decltype( ic )::value;
@@ -606,9 +606,9 @@ void contract_block_tile_kernel( BlockArgs a ) {
   auto step = [&]( int l_st, int l_next, int l_free, int32_t s ) __attribute__( ( always_inline ) ) {
     float l_scale[TM];
     if constexpr( KIND == F8 || KIND == EXACT ) {
-      float const l_b1 = SB_ROWS ? 1.0f : scale_value( l_sb1, a.sb != nullptr );
+      float const l_b1 = SB_ROWS ? 1.0f : scale_value( l_sb1 );
 #pragma unroll
-      for( int l_i = 0; l_i < TM; l_i++ ) l_scale[l_i] = scale_value( l_sa[l_i], a.sa != nullptr ) * l_b1;
+      for( int l_i = 0; l_i < TM; l_i++ ) l_scale[l_i] = scale_value( l_sa[l_i] ) * l_b1;
     }
     // F8, EXACT: the sums of a pair of fragments are added RING - 1 pairs later
     constexpr int RING = KIND == EXACT ? 2 : 3;
@@ -643,10 +643,10 @@ void contract_block_tile_kernel( BlockArgs a ) {
       }
       Frag const & l_f = l_fb[l_j % 2];
       int32_t l_bits_b = 0;
-      if constexpr( KIND == E8M0 ) l_bits_b = a.sb != nullptr ? l_sb[l_j % 2][0] : 127;
+      if constexpr( KIND == E8M0 ) l_bits_b = l_sb[l_j % 2][0];
       if constexpr( ( KIND == F8 || KIND == EXACT ) && SB_ROWS ) {
 #pragma unroll
-        for( int l_e = 0; l_e < 4; l_e++ ) l_of_b[l_j % 2][l_e] = scale_value( l_sb[l_j % 2][l_e], a.sb != nullptr );
+        for( int l_e = 0; l_e < 4; l_e++ ) l_of_b[l_j % 2][l_e] = scale_value( l_sb[l_j % 2][l_e] );
       }
       Wide l_wb;
       if constexpr( KIND == EXACT ) l_wb = widen< false >( l_f );
@@ -675,7 +675,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
           constexpr int FORMAT = A_E5M2 ? 1 : 0;
           if constexpr( KIND == E8M0 ) {
             l_acc[l_j][l_i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, l_acc[l_j][l_i], 0, FORMAT, 0, l_bits_b, 0,
-                                                                                a.sa != nullptr ? l_sa[l_i] : 127 );
+                                                                                l_sa[l_i] );
           }
           else {
             l_part[l_m % RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( l_vb, l_va, ZERO, 0, FORMAT, 0, 0, 0, 0 );
@@ -800,13 +800,13 @@ int launch_tiles( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) 
 }
 
 // the tiles of one kind and layout, through registers
-template< int KIND, bool RA, bool RB, bool A_E5M2 >
+template< int KIND, bool RA, bool RB, bool A_E5M2, bool SB_ROWS >
 int launch_staged( BlockArgs const & a, BlockKernel kernel, hipStream_t stream ) {
   switch( kernel ) {
-    case BlockKernel::STAGED_32x32:    return launch_shape< KIND, 32, 32, 1, 1, 8, 2, RA, RB, A_E5M2, true, true >( a, stream );
-    case BlockKernel::STAGED_64x64_K:  return launch_shape< KIND, 64, 64, 2, 2, 2, 2, RA, RB, A_E5M2, true, true >( a, stream );
-    case BlockKernel::STAGED_64x64:    return launch_shape< KIND, 64, 64, 2, 2, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
-    case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 4, 1, 2, RA, RB, A_E5M2, true, true >( a, stream );
+    case BlockKernel::STAGED_32x32:    return launch_shape< KIND, 32, 32, 1, 1, 8, 2, RA, RB, A_E5M2, SB_ROWS, true >( a, stream );
+    case BlockKernel::STAGED_64x64_K:  return launch_shape< KIND, 64, 64, 2, 2, 2, 2, RA, RB, A_E5M2, SB_ROWS, true >( a, stream );
+    case BlockKernel::STAGED_64x64:    return launch_shape< KIND, 64, 64, 2, 2, 1, 2, RA, RB, A_E5M2, SB_ROWS, true >( a, stream );
+    case BlockKernel::STAGED_128x128:  return launch_shape< KIND, 128, 128, 2, 4, 1, 2, RA, RB, A_E5M2, SB_ROWS, true >( a, stream );
     default: return fail( ETIR_COMPILATION_FAILED, "contraction: unknown tile" );
   }
 }

@@ -8,8 +8,7 @@ namespace {
 template< bool A_E5M2 >
 int launch_type( BlockArgs const & a, BlockKernel kernel, BlockLayout layout, hipStream_t stream ) {
   using namespace block;
-  // a B without scales has one for 128 rows, too
-  bool const l_rows = a.sb != nullptr && !a.has( BlockArgs::SB_BLOCKS );
+  bool const l_rows = !a.has( BlockArgs::SB_BLOCKS );
   switch( layout ) {
     case BlockLayout::K_K:
       return l_rows ? launch_tiles< EXACT, false, false, A_E5M2, true >( a, kernel, stream )
