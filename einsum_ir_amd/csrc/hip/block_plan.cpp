@@ -181,6 +181,7 @@ bool fits( Candidate const & c, BlockArgs const & a, BlockLayout layout ) {
   // a grid's threads are counted in 32 bits
   if( double( most_tiles_m( a, c.rows ) ) * double( ( int64_t( a.N ) + c.cols - 1 ) / c.cols ) * 1024 >= 4294967296.0 ) return false;
   if( c.kernel == BlockKernel::GENERAL ) return true;
+  if( !BlockFast::fits( a ) ) return false;
   if( c.kernel <= BlockKernel::FEW_32 ) return few_fits( a );
   if( c.kernel >= BlockKernel::STAGED_32x32 ) return layout != BlockLayout::NONE;
   return direct_fits( a, layout ) && !( exact( a ) && c.kernel == BlockKernel::TILE_256x256 );
@@ -345,7 +346,8 @@ int plan_block( Given const & g, BlockPlan & plan ) {
           | ( l_f8 && g.dtype_scale == ETIR_E8M0 ? BlockArgs::E8M0 : 0u )
           | ( g.block_left == kScaleBlock ? BlockArgs::SA_BLOCKS : 0u )
           | ( g.block_right == kScaleBlock ? BlockArgs::SB_BLOCKS : 0u )
-          | ( g.strides[T_SA] != nullptr && g.strides[T_SB] != nullptr ? BlockArgs::SCALES : 0u );
+          | ( g.strides[T_SA] != nullptr && g.strides[T_SB] != nullptr ? BlockArgs::SCALES : 0u )
+          | ( g.strides[T_BIAS] != nullptr ? BlockArgs::BIAS : 0u );
   plan.grouped = l_grouped;
   plan.has_sa = g.strides[T_SA] != nullptr;
   plan.has_sb = g.strides[T_SB] != nullptr;
@@ -379,7 +381,9 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
                   void const * bias, void const * offsets, void * out, hipStream_t stream ) {
   BlockArgs a = plan.args;
   if( a.C == 0 || a.N == 0 || a.M == 0 ) return ETIR_SUCCESS;
-  std::string const l_w( plan.grouped ? "contraction_grouped" : "contraction_f8" );
+  auto l_missing = [&]( char const * what ) {
+    return fail( ETIR_NO_DATA_PTR_PROVIDED, std::string( plan.grouped ? "contraction_grouped" : "contraction_f8" ) + what );
+  };
   a.a = left;
   a.b = right;
   a.sa = plan.has_sa ? scale_left : nullptr;
@@ -388,12 +392,12 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
   a.offsets = static_cast< int32_t const * >( offsets );
   a.out = out;
   if( out == nullptr || ( a.K > 0 && ( left == nullptr || right == nullptr ) ) ) {
-    return fail( ETIR_NO_DATA_PTR_PROVIDED, l_w + ": null tensor pointer" );
+    return l_missing( ": null tensor pointer" );
   }
-  if( plan.grouped && offsets == nullptr ) return fail( ETIR_NO_DATA_PTR_PROVIDED, l_w + ": null offsets" );
+  if( plan.grouped && offsets == nullptr ) return l_missing( ": null offsets" );
   if( ( plan.has_sa && scale_left == nullptr && a.K > 0 ) || ( plan.has_sb && scale_right == nullptr && a.K > 0 )
       || ( plan.has_bias && bias == nullptr ) ) {
-    return fail( ETIR_NO_DATA_PTR_PROVIDED, l_w + ": null scale or bias, but its strides were given" );
+    return l_missing( ": null scale or bias, but its strides were given" );
   }
   BlockKernel l_kernel = plan.kernel;
   // pointers may be less aligned than the strides

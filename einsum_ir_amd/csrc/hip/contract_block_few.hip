@@ -103,7 +103,7 @@ __device__ inline float scale_at( void const * s, bool e8m0, int64_t at ) {
 
 template< bool F8, bool A_E5M2, int FB, int PARTS, bool OFF >
 __global__ __launch_bounds__( 64 * kWaves )
-void contract_block_few_kernel( BlockArgs a ) {
+void contract_block_few_kernel( BlockFast a ) {
   constexpr int ITEM = F8 ? 1 : 2;
   constexpr int MANY = 16 / PARTS, EACH = 16 / PARTS, FEW = EACH * FB;      // rows of B, of a fragment of A, of A
   constexpr int PITCH = MANY + 4;
@@ -116,7 +116,7 @@ void contract_block_few_kernel( BlockArgs a ) {
   int32_t const l_n0 = int32_t( blockIdx.x % uint32_t( l_tiles_n ) ) * MANY;
   int32_t l_c, l_m0, l_m_end = a.M;
   if( a.has( BlockArgs::GROUP_ROWS ) ) {
-    BlockRows const l_r = block_rows< FEW >( a.offsets, a.C, a.M, int32_t( l_cm ) );
+    BlockRows const l_r = block_rows< FEW >( a.offsets(), a.groups(), a.M, int32_t( l_cm ) );
     if( l_r.group < 0 ) return;
     l_c = l_r.group;
     l_m0 = l_r.m0;
@@ -132,13 +132,13 @@ void contract_block_few_kernel( BlockArgs a ) {
   int64_t const l_bytes = int64_t( a.K ) * ITEM;
   int32_t const l_pieces = int32_t( ( l_bytes + kPiece * PARTS - 1 ) / ( kPiece * PARTS ) );      // of a part of K
   int32_t const l_n = min( l_n0 + l_row, a.N - 1 );
-  uint8_t const * const l_b = static_cast< uint8_t const * >( a.b ) + ( l_c * a.b_c + l_n * a.b_row ) * ITEM;
+  uint8_t const * const l_b = static_cast< uint8_t const * >( a.b ) + ( l_c * int64_t( a.b_c ) + l_n * int64_t( a.b_ld ) ) * ITEM;
   uint8_t const * l_a[FB];
   int32_t l_m[FB];
 #pragma unroll
   for( int l_i = 0; l_i < FB; l_i++ ) {
     l_m[l_i] = min( l_m0 + EACH * l_i + l_row, l_m_end - 1 );
-    l_a[l_i] = static_cast< uint8_t const * >( a.a ) + ( l_c * a.a_c + l_m[l_i] * a.a_row ) * ITEM;
+    l_a[l_i] = static_cast< uint8_t const * >( a.a ) + ( l_c * a.a_batch() + l_m[l_i] * int64_t( a.a_ld ) ) * ITEM;
   }
 
   f32x4 l_acc[FB];
@@ -189,19 +189,19 @@ void contract_block_few_kernel( BlockArgs a ) {
         bool const l_past = MASKED && l_first + l_k > l_last;
 #pragma unroll
         for( int l_i = 0; l_i < FB; l_i++ ) {
-          l_sa[l_k][l_i] = a.sa == nullptr ? 1.0f : scale_at( a.sa, l_e8m0, l_c * a.sa_c + l_kb * a.sa_k
+          l_sa[l_k][l_i] = a.sa == nullptr ? 1.0f : scale_at( a.sa, l_e8m0, l_c * int64_t( a.sa_c ) + l_kb * a.sa_k
                                                   + int64_t( a.has( BlockArgs::SA_BLOCKS ) ? l_m[l_i] / kScaleBlock : l_m[l_i] ) * a.sa_row );
         }
         if( a.sb == nullptr || a.has( BlockArgs::SB_BLOCKS ) ) {
           // a workgroup's rows of B are in one block
-          l_sb[l_k][0] = a.sb == nullptr ? 1.0f : scale_at( a.sb, l_e8m0, l_c * a.sb_c + l_kb * a.sb_k + int64_t( l_n0 / kScaleBlock ) * a.sb_row );
+          l_sb[l_k][0] = a.sb == nullptr ? 1.0f : scale_at( a.sb, l_e8m0, l_c * int64_t( a.sb_c ) + l_kb * a.sb_k + int64_t( l_n0 / kScaleBlock ) * a.sb_row );
           l_sb[l_k][1] = l_sb[l_k][2] = l_sb[l_k][3] = l_sb[l_k][0];
         }
         else {
 #pragma unroll
           for( int l_e = 0; l_e < 4; l_e++ ) {
             int32_t const l_r = min( l_n0 + ( PARTS > 1 ? l_e : 4 * ( l_lane / 16 ) + l_e ), a.N - 1 );
-            l_sb[l_k][l_e] = scale_at( a.sb, l_e8m0, l_c * a.sb_c + l_kb * a.sb_k + l_r * a.sb_row );
+            l_sb[l_k][l_e] = scale_at( a.sb, l_e8m0, l_c * int64_t( a.sb_c ) + l_kb * a.sb_k + l_r * int64_t( a.sb_row ) );
           }
         }
         if( l_past ) {
@@ -255,9 +255,9 @@ void contract_block_few_kernel( BlockArgs a ) {
     float l_v = 0.0f;
 #pragma unroll
     for( int l_w = 0; l_w < kWaves * PARTS; l_w++ ) l_v += l_part[l_w][l_f * PITCH + l_i];
-    if( a.bias ) l_v += a.bias[l_c * a.bias_c + l_ng * a.bias_col];
+    if( a.bias() ) l_v += a.bias()[l_ng];
     if( a.has( BlockArgs::RELU ) && l_v < 0.0f ) l_v = 0.0f;         // a NaN stays
-    int64_t const l_o = l_c * a.o_c + l_mg * a.o_row + l_ng * a.o_col;
+    int64_t const l_o = l_c * int64_t( a.o_c ) + l_mg * int64_t( a.o_row ) + l_ng;
     if( a.has( BlockArgs::OUT_BF16 ) ) static_cast< uint16_t * >( a.out )[l_o] = kern::f32_to_bf16_rne( l_v );
     else                               static_cast< float * >( a.out )[l_o] = l_v;
   }
@@ -269,7 +269,7 @@ void launch_shape( BlockArgs const & a, hipStream_t stream ) {
   int64_t const l_tiles_n = ( int64_t( a.N ) + MANY - 1 ) / MANY;
   int64_t const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, FEW ) : ( int64_t( a.M ) + FEW - 1 ) / FEW * a.C;
   hipLaunchKernelGGL( ( contract_block_few_kernel< F8, A_E5M2, FB, PARTS, OFF > ), dim3( uint32_t( l_tiles_m * l_tiles_n ) ),
-                      dim3( 64 * kWaves ), 0, stream, a );
+                      dim3( 64 * kWaves ), 0, stream, BlockFast::of( a, false, false ) );
 }
 
 template< bool F8, bool A_E5M2, bool OFF >

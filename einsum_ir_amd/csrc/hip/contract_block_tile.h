@@ -236,11 +236,11 @@ struct Where {
 // Neighbouring tiles on one XCD (workgroups go to the 8 XCDs in turn), and there
 // in bands of 8 tile rows, so that its cache serves both operands.
 template< int BM, int BN >
-__device__ inline Where where( BlockArgs const & a ) {
+__device__ inline Where where( BlockFast const & a ) {
   bool const l_grouped = a.has( BlockArgs::GROUP_ROWS );
   int32_t const l_tiles_n = ( a.N + BN - 1 ) / BN;
   // rows of tiles: as many as the grid has
-  int32_t const l_tiles_m = l_grouped ? a.M / BM + min( a.M, a.C ) : ( a.M + BM - 1 ) / BM;
+  int32_t const l_tiles_m = l_grouped ? a.M / BM + min( a.M, a.groups() ) : ( a.M + BM - 1 ) / BM;
   int32_t const l_per_c = l_tiles_m * l_tiles_n, l_each = l_per_c / 8;
   Where l_w;
   l_w.c = int32_t( blockIdx.x / uint32_t( l_per_c ) );
@@ -256,14 +256,14 @@ __device__ inline Where where( BlockArgs const & a ) {
   l_w.K = a.K;
   l_w.any = true;
   if( l_grouped ) {
-    BlockRows const l_rows = block_rows< BM >( a.offsets, a.C, a.M, l_tile_m );
+    BlockRows const l_rows = block_rows< BM >( a.offsets(), a.groups(), a.M, l_tile_m );
     l_w.any = l_rows.group >= 0;
     l_w.c = l_rows.group;
     l_w.m0 = l_rows.m0;
     l_w.m_end = l_rows.end;
   }
   else if( a.has( BlockArgs::GROUP_K ) ) {
-    BlockGroup const l_g = block_group( a.offsets, l_w.c, a.K );
+    BlockGroup const l_g = block_group( a.offsets(), l_w.c, a.K );
     l_w.k_begin = l_g.begin;
     l_w.K = l_g.end - l_g.begin;
   }
@@ -284,7 +284,7 @@ struct Scales {
   i32x4    m_rsrc[EACH];
   uint32_t m_first;
 
-  __device__ inline void init( BlockArgs const & a, Where const & w, int wave, int lane ) {
+  __device__ inline void init( BlockFast const & a, Where const & w, int wave, int lane ) {
     int const l_item = a.has( BlockArgs::E8M0 ) ? 1 : 4;
     m_first = wave * EACH;
 #pragma unroll
@@ -302,7 +302,7 @@ struct Scales {
       void const * const l_s = l_a ? a.sa : a.sb;
       m_off[l_i] = l_s != nullptr && l_load < LOADS_A + LOADS_B ? uint32_t( ( l_b - l_b0 ) * int32_t( l_stride ) * l_item ) : kern::kDmaOob;
       m_k[l_i] = uint32_t( ( l_a ? a.sa_k : a.sb_k ) * l_item );
-      m_rsrc[l_i] = kern::make_rsrc( static_cast< uint8_t const * >( l_s ) + ( w.c * ( l_a ? a.sa_c : a.sb_c ) + l_b0 * l_stride ) * l_item,
+      m_rsrc[l_i] = kern::make_rsrc( static_cast< uint8_t const * >( l_s ) + ( int64_t( w.c ) * ( l_a ? a.sa_c : a.sb_c ) + l_b0 * l_stride ) * l_item,
                                      kern::kDmaOob );
     }
   }
@@ -402,7 +402,7 @@ template< class T, int COLS > constexpr int kPitch = COLS + 16 / int( sizeof( T 
 // Stores 16 rows x COLS columns of a wave's slab, 16 bytes a lane, non-temporal:
 // the output is not read here again.
 template< int COLS, class T >
-__device__ inline void store_slab( BlockArgs const & a, T const * slab, T * out, int32_t m1, int32_t m_end, int32_t n1, int lane ) {
+__device__ inline void store_slab( BlockFast const & a, T const * slab, T * out, int32_t m1, int32_t m_end, int32_t n1, int lane ) {
   constexpr int V = 16 / sizeof( T ), LANES = COLS / V, PITCH = kPitch< T, COLS >;
   typedef T v __attribute__( ( ext_vector_type( V ) ) );
   typedef v v_any __attribute__( ( aligned( sizeof( T ) ) ) );
@@ -430,7 +430,7 @@ __device__ inline void store_slab( BlockArgs const & a, T const * slab, T * out,
 // address, through registers (two buffers).
 template< int KIND, int BM, int BN, int WM, int WN, int KG, int STAGES, bool RA, bool RB, bool A_E5M2, bool SB_ROWS, bool REG >
 __global__ __launch_bounds__( 64 * WM * WN * KG )
-void contract_block_tile_kernel( BlockArgs a ) {
+void contract_block_tile_kernel( BlockFast a ) {
   constexpr int  ITEM = KIND == BF16 ? 2 : 1;
   constexpr bool SCALED = KIND != BF16;
   constexpr int  WAVES = WM * WN;                            // of a group
@@ -458,13 +458,13 @@ void contract_block_tile_kernel( BlockArgs a ) {
   Where const w = where< BM, BN >( a );
   if( !w.any ) return;
 
-  uint8_t const * const l_at_a = static_cast< uint8_t const * >( a.a ) + ( w.c * a.a_c + w.m0 * a.a_row + w.k_begin * a.a_k ) * ITEM;
-  uint8_t const * const l_at_b = static_cast< uint8_t const * >( a.b ) + ( w.c * a.b_c + w.n0 * a.b_row + w.k_begin * a.b_k ) * ITEM;
+  uint8_t const * const l_at_a = static_cast< uint8_t const * >( a.a ) + ( w.c * a.a_batch() + ( RA ? w.m0 + w.k_begin * int64_t( a.a_ld ) : w.m0 * int64_t( a.a_ld ) + w.k_begin ) ) * ITEM;
+  uint8_t const * const l_at_b = static_cast< uint8_t const * >( a.b ) + ( w.c * int64_t( a.b_c ) + ( RB ? w.n0 + w.k_begin * int64_t( a.b_ld ) : w.n0 * int64_t( a.b_ld ) + w.k_begin ) ) * ITEM;
   SideA l_a;
   SideB l_b;
   SideS l_s;
-  l_a.init( l_at_a, ( RA ? a.a_k : a.a_row ) * ITEM, w.m_end - w.m0, l_wave, l_lane );
-  l_b.init( l_at_b, ( RB ? a.b_k : a.b_row ) * ITEM, a.N - w.n0, l_wave, l_lane );
+  l_a.init( l_at_a, int64_t( a.a_ld ) * ITEM, w.m_end - w.m0, l_wave, l_lane );
+  l_b.init( l_at_b, int64_t( a.b_ld ) * ITEM, a.N - w.n0, l_wave, l_lane );
   if constexpr( SCALED && !REG ) l_s.init( a, w, l_wave, l_lane );
   Reader< BM, RA, ITEM > l_ra;
   Reader< BN, RB, ITEM > l_rb;
@@ -473,7 +473,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
 
   // the bias, needed after the loop
   float l_bias_r = 0.0f;
-  if( a.bias && threadIdx.x < BN ) l_bias_r = a.bias[w.c * a.bias_c + min( w.n0 + int32_t( threadIdx.x ), a.N - 1 ) * a.bias_col];
+  if( a.bias() && threadIdx.x < BN ) l_bias_r = a.bias()[min( w.n0 + int32_t( threadIdx.x ), a.N - 1 )];
 
   int32_t const l_blocks = int32_t( ( int64_t( w.K ) * ITEM + kStep - 1 ) / kStep );
   // A group's steps; past the last block nothing is in range and zeros are
@@ -497,7 +497,7 @@ void contract_block_tile_kernel( BlockArgs a ) {
         if( l_p != nullptr && l_gt < BM + BN && l_step < l_blocks ) {
           int32_t const l_row = l_is_a ? min( w.m0 + l_gt, w.m_end - 1 ) : min( w.n0 + l_gt - BM, a.N - 1 );
           bool const l_by = a.has( BlockArgs::SA_BLOCKS ) && l_is_a ? true : a.has( BlockArgs::SB_BLOCKS ) && !l_is_a;
-          int64_t const l_i = w.c * ( l_is_a ? a.sa_c : a.sb_c ) + int64_t( l_step ) * ( l_is_a ? a.sa_k : a.sb_k )
+          int64_t const l_i = int64_t( w.c ) * ( l_is_a ? a.sa_c : a.sb_c ) + int64_t( l_step ) * ( l_is_a ? a.sa_k : a.sb_k )
                             + int64_t( l_by ? l_row / kScaleBlock : l_row ) * ( l_is_a ? a.sa_row : a.sb_row );
           if( a.has( BlockArgs::E8M0 ) ) l_scale_r = e8m0_to_f32( static_cast< uint8_t const * >( l_p )[l_i] );
           else                           l_scale_r = static_cast< float const * >( l_p )[l_i];
@@ -744,14 +744,14 @@ void contract_block_tile_kernel( BlockArgs a ) {
     typedef decltype( zero ) T;
     typedef T t4 __attribute__( ( ext_vector_type( 4 ) ) );
     T * const l_slab = reinterpret_cast< T * >( l_all + l_wave * SLAB );
-    T * const l_out = static_cast< T * >( a.out ) + w.c * a.o_c;
+    T * const l_out = static_cast< T * >( a.out ) + int64_t( w.c ) * a.o_c;
 #pragma unroll
     for( int l_i = 0; l_i < TM; l_i++ ) {
 #pragma unroll
       for( int l_j = 0; l_j < TN; l_j++ ) {
         int const l_n = 16 * l_j + 4 * ( l_lane / 16 );
         f32x4 l_f = l_acc[l_j][l_i];
-        if( a.bias ) l_f += *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
+        if( a.bias() ) l_f += *reinterpret_cast< f32x4 const * >( l_bias + l_wn + l_n );
         if( a.has( BlockArgs::RELU ) ) {
 #pragma unroll
           for( int l_e = 0; l_e < 4; l_e++ ) l_f[l_e] = l_f[l_e] < 0.0f ? 0.0f : l_f[l_e];      // a NaN stays
@@ -774,7 +774,8 @@ int launch_shape( BlockArgs const & a, hipStream_t stream ) {
   int64_t const l_tiles_n = ( int64_t( a.N ) + BN - 1 ) / BN;
   int64_t const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? block_most_tiles( a.M, a.C, BM ) : ( int64_t( a.M ) + BM - 1 ) / BM * a.C;
   hipLaunchKernelGGL( ( contract_block_tile_kernel< KIND, BM, BN, WM, WN, KG, STAGES, RA, RB, A_E5M2, SB_ROWS, REG > ),
-                      dim3( uint32_t( l_tiles_m * l_tiles_n ) ), dim3( 64 * WM * WN * KG ), 0, stream, a );
+                      dim3( uint32_t( l_tiles_m * l_tiles_n ) ), dim3( 64 * WM * WN * KG ), 0, stream,
+                      BlockFast::of( a, RA, RB ) );
   hipError_t const l_e = hipGetLastError();
   if( l_e != hipSuccess ) {
     return fail( ETIR_UNDEFINED_ERROR, std::string( "contraction launch failed: " ) + hipGetErrorString( l_e ) );
