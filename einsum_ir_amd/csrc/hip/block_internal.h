@@ -187,6 +187,19 @@ __device__ inline BlockGroup block_group( int32_t const * offsets, int32_t g, in
   return l_g;
 }
 
+// tiles of BM rows in all groups
+template< int BM >
+__device__ inline int32_t block_tiles( int32_t const * offsets, int32_t groups, int32_t rows ) {
+  int32_t l_sum = 0;
+  for( int32_t l_g = threadIdx.x % 64; l_g < groups; l_g += 64 ) {
+    BlockGroup const l_in = block_group( offsets, l_g, rows );
+    l_sum += ( l_in.end - l_in.begin + BM - 1 ) / BM;
+  }
+#pragma unroll
+  for( int l_d = 32; l_d > 0; l_d /= 2 ) l_sum += __shfl_xor( l_sum, l_d );
+  return __builtin_amdgcn_readfirstlane( l_sum );
+}
+
 // Where a workgroup's rows lie: tile `tile` of BM rows, counted through the
 // groups, none of which a tile crosses.
 struct BlockRows { int32_t group, m0, end; };      // group < 0: no such tile

@@ -239,10 +239,15 @@ template< int BM, int BN >
 __device__ inline Where where( BlockFast const & a ) {
   bool const l_grouped = a.has( BlockArgs::GROUP_ROWS );
   int32_t const l_tiles_n = ( a.N + BN - 1 ) / BN;
-  // rows of tiles: as many as the grid has
-  int32_t const l_tiles_m = l_grouped ? a.M / BM + min( a.M, a.groups() ) : ( a.M + BM - 1 ) / BM;
+  // rows of tiles: the groups may have fewer than the grid, whose last ones
+  // would else all be missing on the same XCD (with offsets that do not rise
+  // they may have more, which are left out)
+  int32_t const l_tiles_m = l_grouped ? min( block_tiles< BM >( a.offsets(), a.groups(), a.M ), a.M / BM + min( a.M, a.groups() ) )
+                                      : ( a.M + BM - 1 ) / BM;
   int32_t const l_per_c = l_tiles_m * l_tiles_n, l_each = l_per_c / 8;
   Where l_w;
+  l_w.any = !l_grouped || int64_t( blockIdx.x ) < l_per_c;
+  if( !l_w.any ) return l_w;
   l_w.c = int32_t( blockIdx.x / uint32_t( l_per_c ) );
   int32_t l_r = int32_t( blockIdx.x % uint32_t( l_per_c ) );
   if( l_r < 8 * l_each ) l_r = l_r % 8 * l_each + l_r / 8;
@@ -254,7 +259,6 @@ __device__ inline Where where( BlockFast const & a ) {
   l_w.m_end = a.M;
   l_w.k_begin = 0;
   l_w.K = a.K;
-  l_w.any = true;
   if( l_grouped ) {
     BlockRows const l_rows = block_rows< BM >( a.offsets(), a.groups(), a.M, l_tile_m );
     l_w.any = l_rows.group >= 0;
