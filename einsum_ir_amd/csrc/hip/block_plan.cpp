@@ -140,7 +140,7 @@ bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
 // Fitted to 1400 products of 1 to 16384 rows, 64 to 12288 columns and k, up to 64
 // groups, multiples of 16 and odd: the times that follow are off by 7 to 17 %
 // (root mean square), the kernel chosen is 3 % slower than the best of all on
-// average (64 x 64 tiles everywhere: 42 %) and 64 % slower at most.
+// average (64 x 64 tiles everywhere: 41 %) and twice as slow at most.
 struct Candidate {
   BlockKernel  kernel;
   char const * name;
@@ -148,21 +148,21 @@ struct Candidate {
   float        us[3][5];
 };
 Candidate const kCandidates[] = {
-  { BlockKernel::GENERAL, "general", 64, 64, 1, 4, { { 4.24f, 1.22f, 0.85f, 0.67f, 1.00f }, { 3.87f, 1.53f, 0.76f, 1.21f, 1.00f }, { 3.87f, 1.53f, 0.76f, 1.21f, 1.00f } } },
-  { BlockKernel::FEW_4, "few 4", 4, 4, 4, 1, { { 3.60f, 0.50f, 0.76f, 0.11f, 2.22f }, { 3.61f, 0.81f, 1.37f, 0.22f, 1.62f }, { 3.61f, 0.81f, 1.37f, 0.22f, 1.62f } } },
-  { BlockKernel::FEW_8_PARTS, "few 8 parts", 8, 4, 4, 1, { { 3.46f, 0.69f, 1.20f, 0.17f, 2.20f }, { 4.00f, 0.61f, 1.55f, 0.32f, 2.57f }, { 4.00f, 0.61f, 1.55f, 0.32f, 2.57f } } },
-  { BlockKernel::FEW_16, "few 16", 16, 16, 1, 1, { { 3.39f, 0.74f, 0.51f, 0.63f, 1.97f }, { 2.94f, 1.31f, 1.26f, 0.84f, 1.49f }, { 2.94f, 1.31f, 1.26f, 0.84f, 1.49f } } },
-  { BlockKernel::FEW_32, "few 32", 32, 16, 1, 1, { { 3.01f, 1.16f, 0.77f, 0.98f, 1.73f }, { 2.22f, 2.16f, 3.06f, 1.55f, 1.39f }, { 2.22f, 2.16f, 3.06f, 1.55f, 1.39f } } },
-  { BlockKernel::TILE_32x32, "tile 32x32", 32, 32, 8, 1, { { 1.26f, 0.91f, 0.35f, 3.17f, 1.00f }, { 0.42f, 0.50f, 0.91f, 3.76f, 1.00f }, { 0.23f, 0.50f, 1.09f, 4.06f, 1.00f } } },
-  { BlockKernel::TILE_64x64_K, "tile 64x64 K", 64, 64, 4, 1, { { 0.92f, 0.50f, 1.00f, 3.80f, 1.00f }, { 0.21f, 0.50f, 0.99f, 4.53f, 1.00f }, { 0.45f, 0.50f, 1.38f, 4.68f, 1.00f } } },
-  { BlockKernel::TILE_64x64, "tile 64x64", 64, 64, 1, 2, { { 2.92f, 0.26f, 0.23f, 1.12f, 1.00f }, { 2.66f, 0.31f, 0.26f, 1.09f, 1.00f }, { 2.36f, 0.58f, 0.41f, 1.29f, 1.00f } } },
-  { BlockKernel::TILE_128x128, "tile 128x128", 128, 128, 1, 2, { { 3.88f, 0.61f, 0.56f, 1.71f, 1.00f }, { 2.37f, 0.77f, 0.57f, 2.37f, 1.00f }, { 2.46f, 1.28f, 0.98f, 2.51f, 1.00f } } },
-  { BlockKernel::TILE_256x128, "tile 256x128", 256, 128, 1, 1, { { 0.82f, 0.40f, 0.70f, 4.72f, 1.00f }, { 0.02f, 0.50f, 0.83f, 5.17f, 1.00f }, { 0.05f, 0.50f, 1.79f, 5.99f, 1.00f } } },
-  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256, 1, 1, { { 0.69f, 0.73f, 1.28f, 7.18f, 1.00f }, { 0.02f, 1.38f, 0.40f, 7.44f, 1.00f }, { 0.0f } } },
-  { BlockKernel::STAGED_32x32, "staged 32x32", 32, 32, 8, 1, { { 1.50f, 0.99f, 0.09f, 5.02f, 1.00f }, { 0.39f, 1.69f, 1.59f, 5.05f, 1.00f }, { 0.07f, 1.92f, 1.84f, 5.42f, 1.00f } } },
-  { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64, 2, 2, { { 3.58f, 0.41f, 0.47f, 1.93f, 1.00f }, { 2.48f, 0.87f, 0.77f, 2.52f, 1.00f }, { 1.39f, 0.50f, 1.20f, 3.65f, 1.00f } } },
-  { BlockKernel::STAGED_64x64, "staged 64x64", 64, 64, 1, 4, { { 3.87f, 0.46f, 0.25f, 0.86f, 1.00f }, { 3.67f, 0.66f, 0.35f, 0.99f, 1.00f }, { 3.54f, 0.82f, 0.51f, 1.20f, 1.00f } } },
-  { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128, 1, 2, { { 1.69f, 0.68f, 0.66f, 3.91f, 1.00f }, { 0.07f, 0.50f, 0.92f, 5.53f, 1.00f }, { 0.17f, 0.50f, 1.40f, 5.64f, 1.00f } } }
+  { BlockKernel::GENERAL, "general", 64, 64, 1, 4, { { 4.36f, 1.20f, 0.87f, 0.68f, 1.00f }, { 3.74f, 1.55f, 0.78f, 1.22f, 1.00f }, { 3.74f, 1.55f, 0.78f, 1.22f, 1.00f } } },
+  { BlockKernel::FEW_4, "few 4", 4, 4, 4, 1, { { 3.94f, 0.37f, 0.67f, 0.13f, 2.63f }, { 3.01f, 1.43f, 1.58f, 0.20f, 1.11f }, { 3.01f, 1.43f, 1.58f, 0.20f, 1.11f } } },
+  { BlockKernel::FEW_8_PARTS, "few 8 parts", 8, 4, 4, 1, { { 3.81f, 0.58f, 1.02f, 0.21f, 2.39f }, { 3.28f, 1.34f, 1.81f, 0.33f, 1.56f }, { 3.28f, 1.34f, 1.81f, 0.33f, 1.56f } } },
+  { BlockKernel::FEW_16, "few 16", 16, 16, 1, 1, { { 3.32f, 0.81f, 0.46f, 0.75f, 2.68f }, { 2.99f, 1.32f, 1.29f, 0.90f, 1.46f }, { 2.99f, 1.32f, 1.29f, 0.90f, 1.46f } } },
+  { BlockKernel::FEW_32, "few 32", 32, 16, 1, 1, { { 2.80f, 1.34f, 0.78f, 1.05f, 2.02f }, { 2.05f, 2.34f, 3.33f, 1.51f, 1.33f }, { 2.05f, 2.34f, 3.33f, 1.51f, 1.33f } } },
+  { BlockKernel::TILE_32x32, "tile 32x32", 32, 32, 8, 1, { { 0.74f, 0.52f, 0.98f, 3.48f, 1.00f }, { 0.66f, 0.50f, 0.91f, 3.55f, 1.00f }, { 0.38f, 0.50f, 1.04f, 3.73f, 1.00f } } },
+  { BlockKernel::TILE_64x64_K, "tile 64x64 K", 64, 64, 4, 1, { { 0.75f, 0.47f, 0.93f, 4.14f, 1.00f }, { 0.18f, 0.50f, 0.98f, 4.56f, 1.00f }, { 0.44f, 0.50f, 1.37f, 4.52f, 1.00f } } },
+  { BlockKernel::TILE_64x64, "tile 64x64", 64, 64, 1, 2, { { 2.80f, 0.28f, 0.23f, 1.14f, 1.00f }, { 2.63f, 0.31f, 0.27f, 1.13f, 1.00f }, { 2.40f, 0.51f, 0.38f, 1.25f, 1.00f } } },
+  { BlockKernel::TILE_128x128, "tile 128x128", 128, 128, 1, 2, { { 3.73f, 0.66f, 0.54f, 1.87f, 1.00f }, { 2.25f, 0.77f, 0.56f, 2.34f, 1.00f }, { 2.15f, 1.21f, 0.95f, 2.53f, 1.00f } } },
+  { BlockKernel::TILE_256x128, "tile 256x128", 256, 128, 1, 1, { { 0.82f, 0.42f, 0.69f, 4.83f, 1.00f }, { 0.01f, 0.50f, 0.84f, 4.98f, 1.00f }, { 0.03f, 0.50f, 1.69f, 5.59f, 1.00f } } },
+  { BlockKernel::TILE_256x256, "tile 256x256", 256, 256, 1, 1, { { 0.35f, 0.71f, 1.31f, 7.30f, 1.00f }, { 0.02f, 0.50f, 1.41f, 7.07f, 1.00f }, { 0.0f } } },
+  { BlockKernel::STAGED_32x32, "staged 32x32", 32, 32, 8, 1, { { 0.83f, 0.63f, 1.07f, 5.32f, 1.00f }, { 0.07f, 1.65f, 1.45f, 5.63f, 1.00f }, { 0.31f, 0.50f, 1.88f, 5.25f, 1.00f } } },
+  { BlockKernel::STAGED_64x64_K, "staged 64x64 K", 64, 64, 2, 2, { { 3.47f, 0.47f, 0.45f, 2.02f, 1.00f }, { 2.82f, 0.89f, 0.81f, 2.36f, 1.00f }, { 1.24f, 0.50f, 1.15f, 3.88f, 1.00f } } },
+  { BlockKernel::STAGED_64x64, "staged 64x64", 64, 64, 1, 4, { { 3.84f, 0.48f, 0.23f, 0.91f, 1.00f }, { 3.86f, 0.68f, 0.35f, 0.94f, 1.00f }, { 3.30f, 0.83f, 0.46f, 1.44f, 1.00f } } },
+  { BlockKernel::STAGED_128x128, "staged 128x128", 128, 128, 1, 2, { { 1.88f, 0.67f, 0.67f, 3.83f, 1.00f }, { 0.71f, 0.50f, 0.92f, 5.08f, 1.00f }, { 0.15f, 0.50f, 1.35f, 5.88f, 1.00f } } }
 };
 
 // rows of tiles in all batches or groups at most
