@@ -176,3 +176,33 @@ def test_far_rows_are_rounded(torch_cuda):
         eir.QuantF8Plan(rows, cols, block=block).execute(near, near_q, near_s)
         torch.cuda.synchronize()
         assert torch.equal(q.contiguous().view(torch.uint8), near_q.view(torch.uint8)) and torch.equal(s, near_s)
+
+
+@pytest.mark.parametrize("left", [eir.F8E4M3, eir.F8E5M2])
+@pytest.mark.parametrize("out", [eir.FP32, eir.BF16])
+@pytest.mark.parametrize("expr", ["tk,ok->to", "to,ok->tk", "to,tk->ok"])
+def test_ends_of_byte_scales(torch_cuda, forced, left, out, expr):
+    """Bytes 0 (2^-127) and 254 (2^127), one of each in every block's pair, so that each pair's product is 1."""
+    torch = torch_cuda
+    import block_products as bp
+    g = torch.Generator(device="cuda").manual_seed(11)
+    sizes = dict(t=272, k=400, o=304)
+    ins, res = expr.split("->")
+    l, r = ins.split(",")
+    contracted = [d for d in l if d in r and d not in res][0]
+    block = [(1, 128) if d[-1] == contracted else (128, 1) for d in (l, r)]
+    x, sx, _ = bp.blocks_f8([sizes[d] for d in l], block[0], left, eir.E8M0, g)
+    w, sw, _ = bp.blocks_f8([sizes[d] for d in r], block[1], eir.F8E4M3, eir.E8M0, g)
+    ends = torch.tensor([0, 254, 1, 253], dtype=torch.uint8, device="cuda")
+    for s, dims, turn in ((sx, l, ends), (sw, r, 254 - ends)):
+        n = s.shape[-1] if dims[-1] == contracted else s.shape[-2]
+        s.copy_(turn[:n] if dims[-1] == contracted else turn[:n, None])
+    plan = eir.ContractionF8Plan(**eir.contraction_f8_loops(expr, sizes, block_right=1), dtype_left=left,
+                                 dtype_scale=eir.E8M0, dtype_out=out)
+    y = torch.zeros([sizes[d] for d in res], device="cuda", dtype=bp.TORCH[out])
+    torch.cuda.synchronize()
+    plan.execute(x, w, y, scale_left=sx, scale_right=sw)
+    torch.cuda.synchronize()
+    vx, vw = x.cpu().float().double(), w.cpu().float().double()
+    want, mag = torch.einsum(expr, vx, vw).cuda(), torch.einsum(expr, vx.abs(), vw.abs()).cuda()
+    bp.within(y, want, bp.tolerance(mag, want, sizes[contracted], out == eir.BF16, out, True), plan.describe())
