@@ -233,6 +233,21 @@ __device__ inline BlockRows block_rows( int32_t const * offsets, int32_t groups,
   }
   return { -1, 0, 0 };
 }
+
+// The nth-longest group, the first of equal ones first; up to 64 groups, nth one of
+// them.  A lane holds a group's length and counts those in front of it.
+__device__ inline int32_t block_nth_longest( int32_t const * offsets, int32_t groups, int32_t rows, int32_t nth ) {
+  int32_t const l_lane = threadIdx.x % 64;
+  BlockGroup const l_in = block_group( offsets, min( l_lane, groups - 1 ), rows );
+  int32_t const l_length = l_lane < groups ? l_in.end - l_in.begin : -1;
+  int32_t l_front = 0;
+  for( int32_t l_g = 0; l_g < groups; l_g++ ) {
+    int32_t const l_other = __builtin_amdgcn_readlane( l_length, l_g );
+    l_front += l_other > l_length || ( l_other == l_length && l_g < l_lane ) ? 1 : 0;
+  }
+  // the places of the groups are 0 to groups - 1, each once; lanes past them come after
+  return __builtin_ctzll( __ballot( l_front == nth ) );
+}
 #endif
 
 // tiles of bm rows that `rows` rows in `groups` groups have at most

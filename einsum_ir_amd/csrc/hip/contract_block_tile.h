@@ -277,6 +277,12 @@ __device__ inline Where where( BlockFast const & a ) {
     l_w.m_end = l_rows.end;
   }
   else if( a.has( BlockArgs::GROUP_K ) ) {
+    // The longest groups first, so that none is begun last (16 groups of 8192 rows,
+    // 2048 x 2048 each 98 -> 94 us).  Every workgroup ranks the groups, so for large
+    // tiles and up to 32 groups only: more of them are short against a launch (64:
+    // 65.7 -> 66.2 us), and small tiles lose more than they gain (64 x 64 of 32 groups
+    // 269 -> 337 us).
+    if( BM * BN >= 256 * 256 && a.groups() <= 32 ) l_w.c = block_nth_longest( a.offsets(), a.groups(), a.K, l_w.c );
     BlockGroup const l_g = block_group( a.offsets(), l_w.c, a.K );
     l_w.k_begin = l_g.begin;
     l_w.K = l_g.end - l_g.begin;
