@@ -118,6 +118,9 @@ bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
   int64_t const l_sa = l_ra ? a.a_k : a.a_row, l_sb = l_rb ? a.b_k : a.b_row;
   if( !aligned( a.a, a.a_c, l_sa ) || !aligned( a.b, a.b_c, l_sb ) ) return false;
   if( ( !l_ra || !l_rb ) && a.K * l_item % 16 != 0 ) return false;
+  // a group's k start and end anywhere: pieces of 16 bytes along k would not, and
+  // the last of them would hold the next group's first k
+  if( ( !l_ra || !l_rb ) && a.has( BlockArgs::GROUP_K ) ) return false;
   // 31 bits of bytes in a step of a tile, and along k; rows of a k that do not
   // reach into the next k's, so that k past the end lie past the buffer's end
   int64_t const l_max = int64_t( 1 ) << 31;
