@@ -121,6 +121,8 @@ bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
   // a group's k start and end anywhere: pieces of 16 bytes along k would not, and
   // the last of them would hold the next group's first k
   if( ( !l_ra || !l_rb ) && a.has( BlockArgs::GROUP_K ) ) return false;
+  // and a group's rows start at any row, also within 16 bytes along them
+  if( l_ra && a.has( BlockArgs::GROUP_ROWS ) ) return false;
   // 31 bits of bytes in a step of a tile, and along k; rows of a k that do not
   // reach into the next k's, so that k past the end lie past the buffer's end
   int64_t const l_max = int64_t( 1 ) << 31;

@@ -35,3 +35,22 @@ def test_a_ragged_k_along_no_operand_is(program):
     lines = [block_plans.grouped_line(eir.grouped_loops("to,tk->eok", s, "e", "t")) for s in SIZES]
     for desc in block_plans.describe(program, lines):
         assert " tile " in desc, desc
+
+
+@pytest.mark.parametrize("expr", ["kt,eko->to", "ot,eok->tk"])
+def test_ragged_rows_along_the_left_operand_are_not_loaded_in_pieces(program, expr):
+    """A group's rows start at any row: neither a tile's address nor its extent is a multiple of 4 bytes."""
+    lines = [block_plans.grouped_line(eir.grouped_loops(expr, s, "e", "t"), out=out) for s in SIZES for out in (eir.BF16, eir.FP32)]
+    for s in SIZES:
+        loops = eir.grouped_loops(expr, s, "e", "t", scales=True)
+        lines += [block_plans.grouped_line(loops, left=left, scale=scale, out=out) for left in (eir.F8E4M3, eir.F8E5M2)
+                  for scale in (eir.FP32, eir.E8M0) for out in (eir.BF16, eir.FP32)]
+    for desc in _all(program, lines):
+        assert desc.startswith("contraction_grouped ") and " tile " not in desc, desc
+
+
+def test_ragged_rows_of_k_are(program):
+    for expr in ("tk,eok->to", "to,eok->tk"):
+        lines = [block_plans.grouped_line(eir.grouped_loops(expr, s, "e", "t")) for s in SIZES]
+        for desc in block_plans.describe(program, lines, env=dict(ETIR_BLOCK_KERNEL="7")):
+            assert " tile 64x64 " in desc, desc

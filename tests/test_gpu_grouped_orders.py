@@ -29,12 +29,15 @@ def run(torch, expr, groups, k, o, spare=0, first=0, left=eir.BF16, scale=eir.FP
 
     def operand(dims, dtype, block, shift):
         """Its buffer, address and scales, and the values that it stands for, 0 in place of NaN."""
-        shape = [sizes[d] for d in dims]
+        # blocks are along the contracted dimension and the operand's other one, wherever they lie
+        order = sorted(dims, key=lambda d: (d != "e", d == contracted))
+        shape = [sizes[d] for d in order]
         if f8:
-            q, s, v = bp.blocks_f8(shape, (block, 128) if dims[-1] == contracted else (128, block), dtype, scale, g)
+            q, s, v = bp.blocks_f8(shape, (block, 128), dtype, scale, g)
         else:
             q, s = torch.randn(shape, device="cuda", generator=g).to(torch.bfloat16), None
             v = q.double()
+        q, s, v = (None if x is None else x.permute([order.index(d) for d in dims]).contiguous() for x in (q, s, v))
         if "t" in dims:
             for a, b in unknown:
                 q.view(torch.uint8 if f8 else torch.int16).movedim(dims.index("t"), 0)[a:b] = 0x7f if f8 else 0x7fc0
@@ -133,3 +136,45 @@ def test_every_kernel_on_a_ragged_k(torch_cuda, monkeypatch, kernel, expr, k, o)
     for groups in ([5, 0, 150, 33, 1], [300, 2, 0, 257]):
         for out in (eir.FP32, eir.BF16):
             run(torch_cuda, expr, groups, k, o, spare=-(2 + sum(groups)) % 8, first=2, out=out, nan_group=0, seed=k)
+
+
+RAGGED_ROWS = ["kt,eko->to", "kt,eok->to", "tk,eko->to", "ot,eok->tk"]
+LEFTS = [(eir.BF16, None), (eir.F8E4M3, eir.FP32), (eir.F8E5M2, eir.E8M0), (eir.F8E4M3, None)]
+
+
+@pytest.mark.parametrize("expr", RAGGED_ROWS)
+@pytest.mark.parametrize("left,scale", LEFTS)
+@pytest.mark.parametrize("out", [eir.FP32, eir.BF16])
+@pytest.mark.parametrize("groups", GROUPS, ids=lambda g: "-".join(map(str, g[:6])))
+def test_ragged_rows(torch_cuda, expr, left, scale, groups, out):
+    """The rows' number is made a multiple of 16: only the groups lie anywhere."""
+    longest = max(range(len(groups)), key=lambda e: groups[e])
+    run(torch_cuda, expr, groups, 272, 400, spare=-(3 + sum(groups)) % 16, first=3, left=left, scale=scale, out=out,
+        nan_group=longest, seed=sum(groups))
+
+
+@pytest.mark.parametrize("expr", RAGGED_ROWS + ["kt,oek->to", "kt,eko->ot", "tk,eok->ot"])
+@pytest.mark.parametrize("left,scale", LEFTS)
+@pytest.mark.parametrize("k,o", [(1, 1), (8, 8), (1, 64), (64, 1), (17, 33), (129, 127), (512, 512), (257, 640)])
+def test_sizes_of_ragged_rows(torch_cuda, expr, left, scale, k, o):
+    run(torch_cuda, expr, [5, 0, 150, 33], k, o, spare=1, first=3, left=left, scale=scale, block_left=128 if k == 17 else 1,
+        block_right=1 if k == 129 else 128, nan_group=3, seed=k + o)
+
+
+@pytest.mark.parametrize("expr", RAGGED_ROWS)
+@pytest.mark.parametrize("left,scale", LEFTS[:2])
+@pytest.mark.parametrize("shift", [(1, 0, 0), (0, 3, 0), (8, 8, 1), (5, 2, 3)])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_views_of_ragged_rows(torch_cuda, expr, left, scale, shift, pad):
+    run(torch_cuda, expr, [9, 0, 140, 33], 144, 272, spare=2, left=left, scale=scale, pad=pad, shift=shift, nan_group=0, seed=pad)
+
+
+@pytest.mark.parametrize("kernel", range(15))
+@pytest.mark.parametrize("expr", RAGGED_ROWS)
+@pytest.mark.parametrize("left,scale", LEFTS[:3])
+@pytest.mark.parametrize("k,o", [(272, 400), (131, 77)])
+def test_every_kernel_on_ragged_rows(torch_cuda, monkeypatch, kernel, expr, left, scale, k, o):
+    monkeypatch.setenv("ETIR_BLOCK_KERNEL", str(kernel))
+    for groups in ([5, 0, 150, 33, 1], [300, 2, 0, 257]):
+        run(torch_cuda, expr, groups, k, o, spare=-(2 + sum(groups)) % 16, first=2, left=left, scale=scale,
+            out=eir.FP32 if kernel % 2 else eir.BF16, nan_group=0, seed=k)
