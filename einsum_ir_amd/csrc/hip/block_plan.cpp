@@ -182,9 +182,25 @@ bool few_fits( BlockArgs const & a ) {
   return a.a_k == 1 && a.b_k == 1 && a.K * ( a.has( BlockArgs::F8 ) ? int64_t( 1 ) : int64_t( 2 ) ) >= 16 && !a.has( BlockArgs::GROUP_K );
 }
 
+// threads of a workgroup
+int64_t threads( BlockKernel kernel ) {
+  switch( kernel ) {
+    case BlockKernel::GENERAL:
+    case BlockKernel::TILE_64x64:
+    case BlockKernel::TILE_128x128:
+    case BlockKernel::STAGED_64x64: return 256;
+    case BlockKernel::TILE_64x64_K: return 1024;
+    default:                        return 512;
+  }
+}
+
+// A grid's threads are counted in 32 bits.
+bool grid_fits( BlockArgs const & a, int64_t rows, int64_t cols, int64_t threads ) {
+  return double( most_tiles_m( a, rows ) ) * double( ( int64_t( a.N ) + cols - 1 ) / cols ) * double( threads ) < 4294967296.0;
+}
+
 bool fits( Candidate const & c, BlockArgs const & a, BlockLayout layout ) {
-  // a grid's threads are counted in 32 bits
-  if( double( most_tiles_m( a, c.rows ) ) * double( ( int64_t( a.N ) + c.cols - 1 ) / c.cols ) * 1024 >= 4294967296.0 ) return false;
+  if( !grid_fits( a, c.rows, c.cols, threads( c.kernel ) ) ) return false;
   if( c.kernel == BlockKernel::GENERAL ) return true;
   if( !BlockFast::fits( a ) ) return false;
   if( c.kernel <= BlockKernel::FEW_32 ) return few_fits( a );
@@ -271,7 +287,7 @@ int plan_block( Given const & g, BlockPlan & plan ) {
     int64_t const l_sz = g.sizes[l_i];
     if( l_sz < 0 ) return fail( ETIR_COMPILATION_FAILED, l_w + ": negative loop size" );
     if( l_sz != 0 && l_total[l_to] > kMaxIndex / 2 / l_sz ) {
-      return fail( ETIR_COMPILATION_FAILED, l_w + ": more than 2^30 indices of one type" );
+      return fail( ETIR_COMPILATION_FAILED, l_w + ": 2^30 indices of one type, or more" );
     }
     l_total[l_to] *= l_sz;
     if( l_sz < 2 ) continue;
@@ -357,12 +373,8 @@ int plan_block( Given const & g, BlockPlan & plan ) {
   plan.has_sa = g.strides[T_SA] != nullptr;
   plan.has_sb = g.strides[T_SB] != nullptr;
   plan.has_bias = g.strides[T_BIAS] != nullptr;
-  // a grid's threads are counted in 32 bits
-  double const l_tiles_m = a.has( BlockArgs::GROUP_ROWS ) ? double( block_most_tiles( a.M, a.C, 64 ) )
-                                                          : double( ( int64_t( a.M ) + 63 ) / 64 ) * a.C;
-  if( l_tiles_m * double( ( int64_t( a.N ) + 63 ) / 64 ) >= 4294967296.0 / 256 ) {
-    return fail( ETIR_COMPILATION_FAILED, l_w + ": grid too large" );
-  }
+  // the kernels that take any operands have 64 x 64 tiles: less than 2^24 of them
+  if( !grid_fits( a, 64, 64, threads( BlockKernel::GENERAL ) ) ) return fail( ETIR_COMPILATION_FAILED, l_w + ": grid too large" );
 
   // a group of rows: one pass over all of them, and all weights
   int64_t const l_c = l_grouped ? 1 : int64_t( a.C ), l_item = l_f8 ? 1 : 2, l_out = g.dtype_out == ETIR_BF16 ? 2 : 4;

@@ -372,8 +372,9 @@ int etir_hip_act_quant_execute( etir_plan_t  plan,
  * (a scale of 1, a bias of 0).  Products of two scales are taken in fp32.
  *
  * The loops of each type (M, N, C and K) have to fuse to one; a side with a scale
- * for 128 rows, and K, are one loop from the start.  At most 2^30 indices of one
- * type.  The output's elements have to lie apart.  A product of any size 0 in C,
+ * for 128 rows, and K, are one loop from the start.  Less than 2^30 indices of one
+ * type, and less than 2^24 blocks of 64 x 64 of the output in all batches (each
+ * batch has its own).  The output's elements have to lie apart.  A product of any size 0 in C,
  * M or N does nothing; without K the sums are 0.
  */
 int etir_hip_contraction_f8_create( int64_t         num_loops,
@@ -419,7 +420,9 @@ int etir_hip_contraction_f8_execute( etir_plan_t  plan,
  * left and right: BF16, or (ragged M) F8E4M3 / F8E5M2 and F8E4M3 with scales for
  * blocks as above, where scale_left counts all rows and scale_right has a matrix
  * for each group; output FP32 or BF16.  Other loops: one of type M (ragged K), N
- * and K after fusing, none of type C.  At most 2^30 indices of one type.
+ * and K after fusing, none of type C.  Less than 2^30 indices of one type, and blocks
+ * of 64 x 64 as above: with a ragged M, M / 64 and one for each group (or row, if
+ * they are fewer) along M.
  */
 int etir_hip_contraction_grouped_create( int64_t         num_loops,
                                          int32_t const * dim_types,

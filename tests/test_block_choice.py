@@ -54,3 +54,41 @@ def test_ragged_rows_of_k_are(program):
         lines = [block_plans.grouped_line(eir.grouped_loops(expr, s, "e", "t")) for s in SIZES]
         for desc in block_plans.describe(program, lines, env=dict(ETIR_BLOCK_KERNEL="7")):
             assert " tile 64x64 " in desc, desc
+
+
+def _batches(c, m, n, k, expr="cmk,cnk->cmn", **kinds):
+    return block_plans.f8_line(eir.contraction_f8_loops(expr, dict(c=c, m=m, n=n, k=k), **kinds))
+
+
+@pytest.mark.parametrize("c", [(1 << 22) - 1, 1 << 22, 5000000, 1 << 23, (1 << 24) - 1])
+def test_many_batches_have_a_kernel(program, c):
+    """More tiles than workgroups of 1024 threads can be launched, none larger that would do with fewer."""
+    lines = [_batches(c, 2, 2, 16), _batches(c, 2, 2, 16, scales=False), _batches(c, 1, 1, 8), _batches(c, 33, 64, 40, "ckm,cnk->cnm")]
+    for desc in block_plans.describe(program, lines):
+        assert desc.startswith("contraction_f8 ") and f" C={c} " in desc, desc
+
+
+def test_large_outputs_have_a_kernel(program):
+    for n in ((1 << 17) - 64, 1 << 17, 1 << 18):
+        sizes = dict(m=(1 << 18) - 64, n=n, k=32)
+        lines = [block_plans.f8_line(eir.contraction_f8_loops(e, sizes)) for e in ("mk,nk->mn", "km,nk->mn", "mk,nk->nm")]
+        # a group more than there are blocks of rows
+        lines.append(block_plans.grouped_line(eir.grouped_loops("mk,enk->mn", dict(sizes, e=1, m=sizes["m"] - 64), "e", "m")))
+        for desc in block_plans.describe(program, lines):
+            assert desc.startswith("contraction_"), desc
+
+
+def test_many_groups_have_a_kernel(program):
+    for e in (1 << 22, 5000000, (1 << 23) - 1):
+        line = block_plans.grouped_line(eir.grouped_loops("to,tk->eok", dict(t=1 << 23, e=e, o=3, k=5), "e", "t"))
+        desc, = block_plans.describe(program, [line])
+        assert desc.startswith("contraction_grouped ") and f" groups={e} " in desc, desc
+
+
+def test_grids_that_are_too_large_are_refused(program):
+    lines = [_batches(1 << 24, 2, 2, 16), _batches((1 << 30) - 1, 1, 1, 1),
+             block_plans.f8_line(eir.contraction_f8_loops("mk,nk->mn", dict(m=1 << 18, n=1 << 18, k=32))),
+             block_plans.grouped_line(eir.grouped_loops("to,tk->eok", dict(t=1 << 24, e=1 << 24, o=3, k=5), "e", "t")),
+             block_plans.grouped_line(eir.grouped_loops("tk,eok->to", dict(t=1 << 18, e=4, o=1 << 18, k=5), "e", "t"))]
+    for desc in block_plans.describe(program, lines):
+        assert desc.startswith(f"{eir.COMPILATION_FAILED} ") and desc.endswith(": grid too large"), desc
