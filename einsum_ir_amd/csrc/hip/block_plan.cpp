@@ -194,13 +194,24 @@ int64_t threads( BlockKernel kernel ) {
   }
 }
 
+double tiles_of( BlockArgs const & a, int64_t rows, int64_t cols ) {
+  return double( most_tiles_m( a, rows ) ) * double( ( int64_t( a.N ) + cols - 1 ) / cols );
+}
+
 // A grid's threads are counted in 32 bits.
 bool grid_fits( BlockArgs const & a, int64_t rows, int64_t cols, int64_t threads ) {
-  return double( most_tiles_m( a, rows ) ) * double( ( int64_t( a.N ) + cols - 1 ) / cols ) * double( threads ) < 4294967296.0;
+  return tiles_of( a, rows, cols ) * double( threads ) < 4294967296.0;
+}
+
+// With groups of rows every workgroup looks through the offsets, 64 in about a
+// nanosecond of the whole card (65536 groups of one row: 37 ms): 2^36 of them would
+// take a second.
+bool groups_fit( BlockArgs const & a, int64_t rows, int64_t cols ) {
+  return !a.has( BlockArgs::GROUP_ROWS ) || tiles_of( a, rows, cols ) * a.C < 68719476736.0;
 }
 
 bool fits( Candidate const & c, BlockArgs const & a, BlockLayout layout ) {
-  if( !grid_fits( a, c.rows, c.cols, threads( c.kernel ) ) ) return false;
+  if( !grid_fits( a, c.rows, c.cols, threads( c.kernel ) ) || !groups_fit( a, c.rows, c.cols ) ) return false;
   if( c.kernel == BlockKernel::GENERAL ) return true;
   if( !BlockFast::fits( a ) ) return false;
   if( c.kernel <= BlockKernel::FEW_32 ) return few_fits( a );
@@ -375,6 +386,7 @@ int plan_block( Given const & g, BlockPlan & plan ) {
   plan.has_bias = g.strides[T_BIAS] != nullptr;
   // the kernels that take any operands have 64 x 64 tiles: less than 2^24 of them
   if( !grid_fits( a, 64, 64, threads( BlockKernel::GENERAL ) ) ) return fail( ETIR_COMPILATION_FAILED, l_w + ": grid too large" );
+  if( !groups_fit( a, 64, 64 ) ) return fail( ETIR_COMPILATION_FAILED, l_w + ": too many groups for as many blocks" );
 
   // a group of rows: one pass over all of them, and all weights
   int64_t const l_c = l_grouped ? 1 : int64_t( a.C ), l_item = l_f8 ? 1 : 2, l_out = g.dtype_out == ETIR_BF16 ? 2 : 4;

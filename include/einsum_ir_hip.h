@@ -422,7 +422,8 @@ int etir_hip_contraction_f8_execute( etir_plan_t  plan,
  * for each group; output FP32 or BF16.  Other loops: one of type M (ragged K), N
  * and K after fusing, none of type C.  Less than 2^30 indices of one type, and blocks
  * of 64 x 64 as above: with a ragged M, M / 64 and one for each group (or row, if
- * they are fewer) along M.
+ * they are fewer) along M, and less than 2^36 blocks times groups, because every
+ * workgroup looks through the offsets (1024 groups of one row take 20 us, 65536 37 ms).
  */
 int etir_hip_contraction_grouped_create( int64_t         num_loops,
                                          int32_t const * dim_types,

@@ -92,3 +92,20 @@ def test_grids_that_are_too_large_are_refused(program):
              block_plans.grouped_line(eir.grouped_loops("tk,eok->to", dict(t=1 << 18, e=4, o=1 << 18, k=5), "e", "t"))]
     for desc in block_plans.describe(program, lines):
         assert desc.startswith(f"{eir.COMPILATION_FAILED} ") and desc.endswith(": grid too large"), desc
+
+
+def _groups(e, t, o):
+    return block_plans.grouped_line(eir.grouped_loops("tk,eok->to", dict(t=t, e=e, o=o, k=64), "e", "t"))
+
+
+def test_groups_of_rows_that_take_seconds_to_find_are_refused(program):
+    """Every workgroup looks through the offsets: groups times workgroups are bounded, for every kernel."""
+    many = [_groups(1 << 22, 1 << 22, 64), _groups(4500000, 4500000, 3), _groups(1 << 18, 1 << 18, 64), _groups(1 << 16, 1 << 27, 1)]
+    for desc in _all(program, many) + block_plans.describe(program, many, env=dict(ETIR_BLOCK_KERNEL="1")):
+        assert desc.startswith(f"{eir.COMPILATION_FAILED} ") and desc.endswith(": too many groups for as many blocks"), desc
+    some = [_groups(1 << 17, 1 << 17, 64), _groups(1 << 16, 1 << 24, 1), _groups(4096, 1 << 29, 1)]
+    for desc in block_plans.describe(program, some):
+        assert desc.startswith("contraction_grouped "), desc
+    # 32 times as many workgroups
+    desc, = block_plans.describe(program, some[:1], env=dict(ETIR_BLOCK_KERNEL="1"))
+    assert " few 4 " not in desc, desc

@@ -60,3 +60,26 @@ def test_groups_of_k(torch_cuda, monkeypatch, kernel):
     plan.execute(a, b, y, at)
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_groups_of_rows(torch_cuda, monkeypatch, kernel):
+    """20000 groups of 0 to 2 rows, whole numbers."""
+    torch = torch_cuda
+    if kernel is not None:
+        monkeypatch.setenv("ETIR_BLOCK_KERNEL", str(kernel))
+    e, k, o = 20000, 16, 5
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rows = torch.arange(e, device="cuda") % 3
+    off = torch.cat([torch.zeros(1, device="cuda", dtype=torch.int64), rows.cumsum(0)]).int()
+    t = int(off[-1])
+    of = torch.repeat_interleave(torch.arange(e, device="cuda"), rows)
+    x, w = (torch.randint(-8, 9, s, device="cuda", generator=g).to(torch.bfloat16) for s in ((t, k), (e, o, k)))
+    want = torch.stack([(x.float() * w[:, j].float()[of]).sum(-1) for j in range(o)], -1)
+    plan = eir.ContractionGroupedPlan(**eir.grouped_loops("tk,eok->to", dict(t=t, e=e, o=o, k=k), "e", "t"), dtype_out=eir.FP32)
+    print(plan.describe(), flush=True)
+    y = torch.empty(t, o, device="cuda")
+    torch.cuda.synchronize()
+    plan.execute(x, w, y, off)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
