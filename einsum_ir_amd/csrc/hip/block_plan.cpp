@@ -326,9 +326,10 @@ int plan_block( Given const & g, BlockPlan & plan ) {
     l_loops[l_to].push_back( l_l );
   }
   if( l_grouped && l_groups != 1 ) return fail( ETIR_COMPILATION_FAILED, l_w + ": one loop is over the groups" );
-  // one scale a block of 128 is counted along one loop
-  if( ( g.block_left == kScaleBlock && l_loops[ETIR_DIM_M].size() > 1 )
-      || ( g.block_right == kScaleBlock && l_loops[ETIR_DIM_N].size() > 1 ) || ( l_f8 && l_loops[ETIR_DIM_K].size() > 1 ) ) {
+  // one scale a block of 128 is counted along one loop; a side without scales has no blocks
+  if( ( g.block_left == kScaleBlock && g.strides[T_SA] != nullptr && l_loops[ETIR_DIM_M].size() > 1 )
+      || ( g.block_right == kScaleBlock && g.strides[T_SB] != nullptr && l_loops[ETIR_DIM_N].size() > 1 )
+      || ( l_f8 && l_loops[ETIR_DIM_K].size() > 1 ) ) {
     return fail( ETIR_COMPILATION_FAILED, l_w + ": blocks of 128 run along one loop" );
   }
   // the ragged loop is alone, also where it is shorter than 2

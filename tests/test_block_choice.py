@@ -109,3 +109,19 @@ def test_groups_of_rows_that_take_seconds_to_find_are_refused(program):
     # 32 times as many workgroups
     desc, = block_plans.describe(program, some[:1], env=dict(ETIR_BLOCK_KERNEL="1"))
     assert " few 4 " not in desc, desc
+
+
+def test_a_side_without_scales_may_have_several_loops(program):
+    """Blocks of 128 rows are said of a side whose scales are not given; its loops fuse."""
+    s = dict(t=40, a=3, b=50, k=144, e=4)
+    lines = [block_plans.f8_line(eir.contraction_f8_loops("tk,abk->tab", s, scales=False)),
+             block_plans.f8_line(eir.contraction_f8_loops("abk,tk->abt", s, block_left=128, scales=False)),
+             block_plans.grouped_line(eir.grouped_loops("tk,eabk->tab", s, "e", "t"))]
+    for desc, mn in zip(block_plans.describe(program, lines), ("M=40 N=150", "M=150 N=40", "M=40 N=150")):
+        assert desc.startswith("contraction_") and f" {mn} K=144" in desc, desc
+    one = eir.contraction_f8_loops("tk,abk->tab", s)
+    refused = [block_plans.f8_line(one), block_plans.f8_line(dict(one, strides_scale_left=None)),
+               block_plans.f8_line(eir.contraction_f8_loops("abk,tk->abt", s, block_left=128)),
+               block_plans.grouped_line(eir.grouped_loops("tk,eabk->tab", s, "e", "t", scales=True), left=eir.F8E4M3)]
+    for desc in block_plans.describe(program, refused):
+        assert desc.endswith(": blocks of 128 run along one loop"), desc
