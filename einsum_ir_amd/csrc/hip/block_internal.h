@@ -132,6 +132,7 @@ enum class BlockLayout : int32_t {
 
 struct BlockPlan {
   BlockKernel kernel = BlockKernel::GENERAL;
+  BlockKernel kernel_off = BlockKernel::GENERAL;      // for pointers off 16 bytes
   BlockLayout layout = BlockLayout::NONE;
   bool      grouped = false;
   bool      has_sa = false, has_sb = false, has_bias = false;

@@ -242,23 +242,37 @@ double estimate( Candidate const & c, BlockArgs const & a, BlockLayout layout, d
                      l_us[0] + l_beside * ( l_steps * l_us[2] * l_layout + l_us[3] ), l_least + 2.5 } );
 }
 
-// ETIR_BLOCK_KERNEL forces a kernel, by its place in BlockKernel, where it fits.
-char const * choose_kernel( BlockArgs const & a, double bytes, BlockPlan & plan ) {
+// Whether a kernel loads into LDS directly.
+bool direct( BlockKernel kernel ) { return kernel > BlockKernel::FEW_32 && kernel < BlockKernel::STAGED_32x32; }
+
+// The kernel for operands as their strides say, and for a direct one another that
+// takes pointers off 16 bytes at a call.  ETIR_BLOCK_KERNEL forces the first, by its
+// place in BlockKernel, where it fits.
+struct Choice { char const * name, * name_off; };      // name_off: null where it is the same
+Choice choose_kernel( BlockArgs const & a, double bytes, BlockPlan & plan ) {
   plan.layout = layout_of( a );
   char const * const l_env = std::getenv( "ETIR_BLOCK_KERNEL" );
   int const l_forced = l_env ? std::atoi( l_env ) : -1;
-  Candidate const * l_best = nullptr;
-  double l_least = 0.0;
+  Candidate const * l_best = nullptr, * l_off = nullptr;
+  double l_least = 0.0, l_least_off = 0.0;
   for( Candidate const & l_c : kCandidates ) {
     if( !fits( l_c, a, plan.layout ) ) continue;
-    double const l_us = l_forced == int( l_c.kernel ) ? -1.0 : estimate( l_c, a, plan.layout, bytes );
-    if( l_best == nullptr || l_us < l_least ) {
+    double const l_us = estimate( l_c, a, plan.layout, bytes );
+    if( l_c.kernel >= BlockKernel::STAGED_32x32 && ( l_off == nullptr || l_us < l_least_off ) ) {
+      l_off = &l_c;
+      l_least_off = l_us;
+    }
+    bool const l_force = l_forced == int( l_c.kernel );
+    if( l_best == nullptr || l_force || l_us < l_least ) {
       l_best = &l_c;
-      l_least = l_us;
+      l_least = l_force ? -1.0 : l_us;
     }
   }
-  plan.kernel = l_best->kernel;
-  return l_best->name;
+  plan.kernel = plan.kernel_off = l_best->kernel;
+  if( !direct( plan.kernel ) ) return { l_best->name, nullptr };
+  // where a direct kernel fits, STAGED_64x64 does
+  plan.kernel_off = l_off->kernel;
+  return { l_best->name, l_off->name };
 }
 
 int plan_block( Given const & g, BlockPlan & plan ) {
@@ -400,10 +414,12 @@ int plan_block( Given const & g, BlockPlan & plan ) {
   if( plan.has_bias ) plan.bytes += 4 * l_c * a.N;
   if( l_grouped ) plan.bytes += 4 * ( int64_t( a.C ) + 1 );
   char const * const l_left = l_f8 ? ( g.dtype_left == ETIR_F8E5M2 ? "e5m2" : "e4m3" ) : "bf16";
-  plan.desc = l_w + " " + choose_kernel( a, double( plan.bytes ), plan ) + " " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
+  Choice const l_choice = choose_kernel( a, double( plan.bytes ), plan );
+  plan.desc = l_w + " " + l_choice.name + " " + ( l_grouped ? "groups=" : "C=" ) + std::to_string( a.C ) + " M=" + std::to_string( a.M )
             + " N=" + std::to_string( a.N ) + " K=" + std::to_string( a.K )
             + ( l_grouped ? ( l_ragged_k ? " ragged K" : " ragged M" ) : "" ) + " " + l_left
-            + ( a.has( BlockArgs::OUT_BF16 ) ? " out=bf16" : " out=fp32" );
+            + ( a.has( BlockArgs::OUT_BF16 ) ? " out=bf16" : " out=fp32" )
+            + ( l_choice.name_off ? std::string( " off 16 bytes=" ) + l_choice.name_off : std::string() );
   return ETIR_SUCCESS;
 }
 
@@ -429,10 +445,8 @@ int launch_block( BlockPlan const & plan, void const * left, void const * right,
       || ( plan.has_bias && bias == nullptr ) ) {
     return l_missing( ": null scale or bias, but its strides were given" );
   }
-  BlockKernel l_kernel = plan.kernel;
   // pointers may be less aligned than the strides
-  bool const l_staged = l_kernel >= BlockKernel::STAGED_32x32;
-  if( !l_staged && l_kernel > BlockKernel::FEW_32 && !direct_fits( a, plan.layout ) ) l_kernel = BlockKernel::STAGED_64x64;
+  BlockKernel const l_kernel = direct( plan.kernel ) && !direct_fits( a, plan.layout ) ? plan.kernel_off : plan.kernel;
   if( l_kernel == BlockKernel::GENERAL ) return launch_block_general( a, stream );
   if( l_kernel <= BlockKernel::FEW_32 )  return launch_block_few( a, l_kernel, stream );
   if( l_kernel >= BlockKernel::STAGED_32x32 ) return launch_block_staged( a, l_kernel, plan.layout, stream );

@@ -125,3 +125,27 @@ def test_a_side_without_scales_may_have_several_loops(program):
                block_plans.grouped_line(eir.grouped_loops("tk,eabk->tab", s, "e", "t", scales=True), left=eir.F8E4M3)]
     for desc in block_plans.describe(program, refused):
         assert desc.endswith(": blocks of 128 run along one loop"), desc
+
+
+def test_pointers_off_16_bytes_have_a_kernel_chosen_by_size(program):
+    """A plan of direct tiles names the kernel of calls whose pointers are less aligned than its strides: the one through
+    registers with the least estimated time, as for strides that are."""
+    seen = set()
+    for t, k, o in ((32, 4096, 256), (256, 1024, 512), (300, 4096, 1024), (1024, 1024, 1024), (4096, 4096, 4096), (8192, 8192, 8192)):
+        s = dict(t=t, k=k, o=o)
+        for f, kinds in ((eir.contraction_f8_loops, {}), (eir.grouped_loops, dict(group="e", ragged="t"))):
+            expr = "tk,ok->to" if f is eir.contraction_f8_loops else "tk,eok->to"
+            line = block_plans.f8_line if f is eir.contraction_f8_loops else block_plans.grouped_line
+            loops = f(expr, dict(s, e=4), **kinds)
+            # rows one element apart from that: no direct kernel, and hardly any other size
+            off = f(expr, dict(s, e=4), sizes_outer_left=dict(t=t, k=k + 1), **kinds)
+            forced, = block_plans.describe(program, [line(loops)], env=dict(ETIR_BLOCK_KERNEL="7"))
+            assert " tile 64x64 " in forced and " off 16 bytes=staged " in forced, forced
+            chosen, other = block_plans.describe(program, [line(loops), line(off)])
+            assert (" off 16 bytes=" in chosen) == (" tile " in chosen), chosen
+            assert " tile " not in other and " off 16 bytes=" not in other, other
+            name = forced.split(" off 16 bytes=")[1]
+            if " staged " in other:
+                assert f" {name} " in other, (forced, other)
+            seen.add(name)
+    assert len(seen) > 1, seen
