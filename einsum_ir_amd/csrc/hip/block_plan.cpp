@@ -143,9 +143,10 @@ bool direct_fits( BlockArgs const & a, BlockLayout layout ) {
 // Few rows: fixed, 2 KiB (8 KiB in parts) of k of a workgroup, a workgroup beside
 // others, and 1 KiB of k of one beside others.
 // Fitted to 1400 products of 1 to 16384 rows, 64 to 12288 columns and k, up to 64
-// groups, multiples of 16 and odd: the times that follow are off by 7 to 17 %
-// (root mean square), the kernel chosen is 3 % slower than the best of all on
-// average (64 x 64 tiles everywhere: 41 %) and twice as slow at most.
+// groups, multiples of 16 and odd (profiles/block_choice.txt): the times that follow
+// are off by 7 to 17 % (root mean square), the kernel chosen is 3 % slower than the
+// best of all on average (64 x 64 tiles everywhere: 41 %), more than 20 % slower in
+// one of 20 and 2.7 times at most (2 rows in 23 groups).
 struct Candidate {
   BlockKernel  kernel;
   char const * name;

@@ -2,8 +2,10 @@
 // products on the matrix cores with scales of either type, and 8-bit numbers
 // multiplied as bf16.  What is not at multiples of 16 bytes cannot go to LDS
 // directly; a step waits in registers while the last one is multiplied, and a
-// deeper store of steps costs more waves than it hides.  4096^3 off 16 bytes: 148 us,
-// on them 65.
+// deeper store of steps costs more waves than it hides.  4096^3 one byte off: 130 us,
+// with 4097 k 150, at multiples of 16 bytes 64.  Operands whose groups start and end
+// inside a piece of 16 bytes come here too: groups of k with an operand along k,
+// groups of rows with A along them.
 #include "contract_block_tile.h"
 
 namespace etir {

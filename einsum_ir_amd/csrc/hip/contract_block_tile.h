@@ -36,10 +36,11 @@
 //           gradient of weights 8192 x 4096 x 2048 164 -> 134 us without it).
 //   E8M0    as F8, the scales applied by the matrix instruction itself.
 //
-// Bound by the matrix cores' power where the tiles are many: 8192^3 takes 420 us
-// with E8M0 (2.6 PFLOP/s, matrix cores busy 61 % at 1.9 of 2.4 GHz), 456 with F8,
-// 924 with EXACT; bf16, 16384 rows in 8 groups times 4096 x 4096, 470 us (1.17
-// PFLOP/s).  Large tiles read LDS least for a product, small ones fill the
+// Bound by the matrix cores' power where the tiles are many: 8192^3 with inputs
+// that change from call to call takes 446 us with E8M0 (2.5 PFLOP/s, matrix cores
+// busy 61 % at 1.9 of 2.4 GHz), 487 with F8, 972 with EXACT; bf16, 16384 rows in 8
+// groups times 4096 x 4096, 491 us (1.12 PFLOP/s).  With the same inputs again and
+// again: 428, 462, 949 and 470.  Large tiles read LDS least for a product, small ones fill the
 // compute units: 4072 x 2048 x 2048 takes 39 us with 64 x 64, 24 with 128 x 128, 21
 // with 256 x 128 (one round of 256 tiles) and 29 with 256 x 256 (half of one).
 #ifndef ETIR_CONTRACT_BLOCK_TILE_H
